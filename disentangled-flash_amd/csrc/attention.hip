@@ -376,7 +376,7 @@ const char* dflash_error_string(int code) {
     case DFLASH_ERR_TOO_LARGE:
       return "launch grid exceeds the device limit";
     case DFLASH_ERR_WORKSPACE:
-      return "workspace smaller than dflash_attention_rel_split_plan reports";
+      return "workspace smaller than the call's plan or workspace_bytes function reports";
     case DFLASH_ERR_BUSY:
       return "the static scratch is in use by a call on another stream that has not "
              "completed (dflash_attention_rel_fwd_noalloc)";

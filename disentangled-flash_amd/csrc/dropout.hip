@@ -1,0 +1,76 @@
+// Dropout whose mask is drawn again wherever it is needed and never stored.
+//
+//   y = x / P(kept) where the element's 16 bits of the generator are at least 65536 p, else 0
+//
+// Forward and backward are the same kernel (dx is the same function of dy).  A dropped element
+// is 0 whatever it held (infinities and NaN too): it is selected, not multiplied by 0.
+// One 16-byte chunk a lane: n * sizeof(T) bytes read and written, and one generator block
+// for 8 elements.
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "dflash.h"
+#include "training.h"
+
+namespace dflash {
+namespace {
+
+// WIDE: x and y lie on 16-byte boundaries; otherwise element accesses.
+template <typename T, bool WIDE>
+__global__ __launch_bounds__(256) void dropout_kernel(const T* __restrict__ x, T* __restrict__ y,
+                                                      int64_t n, Dropout d) {
+  constexpr int N = Chunk<T>::N;
+  const int64_t first = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) * N;
+  if (first >= n) return;
+  const DropoutKey key = dropout_key(d);
+  const int live = n - first < N ? static_cast<int>(n - first) : N;
+  float v[N];
+  if (WIDE && live == N)
+    load_floats<T, N, true>(x + first, N, v);
+  else
+    load_floats<T, N, false>(x + first, live, v);
+  const uint32_t dropped = dropped_from<N, true>(d, key, first);
+#pragma unroll
+  for (int e = 0; e < N; ++e) v[e] = (dropped >> e) & 1 ? 0.0f : v[e] * d.scale;
+  if (WIDE && live == N)
+    store_floats<T, N, true>(y + first, N, v);
+  else
+    store_floats<T, N, false>(y + first, live, v);
+}
+
+template <typename T>
+int launch_dropout(const void* x, void* y, int64_t n, const Dropout& d, hipStream_t stream) {
+  const int64_t per_block = 256 * Chunk<T>::N;
+  const int64_t blocks = (n + per_block - 1) / per_block;
+  if (blocks > kMaxBlocks256) return DFLASH_ERR_TOO_LARGE;
+  const bool wide = (reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(y)) % 16 == 0;
+  hipLaunchKernelGGL((wide ? &dropout_kernel<T, true> : &dropout_kernel<T, false>),
+                     dim3(static_cast<uint32_t>(blocks)), dim3(256), 0, stream,
+                     static_cast<const T*>(x), static_cast<T*>(y), n, d);
+  return static_cast<int>(hipGetLastError());
+}
+
+}  // namespace
+}  // namespace dflash
+
+using namespace dflash;
+
+extern "C" int dflash_dropout(const void* x, void* y, int64_t n, double p, const int64_t* rng,
+                              uint32_t site, int dtype, void* stream) {
+  Dropout d;
+  if (n < 0 || !make_dropout(p, rng, site, d)) return DFLASH_ERR_SHAPE;
+  if (dtype < DFLASH_DTYPE_FP16 || dtype > DFLASH_DTYPE_FP32) return DFLASH_ERR_DTYPE;
+  if (n == 0) return DFLASH_OK;
+  if (!x || !y || (d.active && !rng)) return DFLASH_ERR_NULL;
+  const uintptr_t element = dtype == DFLASH_DTYPE_FP32 ? 4 : 2;
+  if ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(y)) % element != 0 ||
+      reinterpret_cast<uintptr_t>(rng) % 8 != 0)
+    return DFLASH_ERR_ALIGN;
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  switch (dtype) {
+    case DFLASH_DTYPE_FP16: return launch_dropout<_Float16>(x, y, n, d, s);
+    case DFLASH_DTYPE_BF16: return launch_dropout<__bf16>(x, y, n, d, s);
+    default: return launch_dropout<float>(x, y, n, d, s);
+  }
+}

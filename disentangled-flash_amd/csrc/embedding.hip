@@ -1,0 +1,514 @@
+// Embedding lookup with scaling, and the dense gradient of its table.
+//
+//   out[i] = T(scale * table[id_i])
+//   dtable[v] = T(scale * sum over i with id_i = v of dout[i]),  0 for padding and unused rows
+//
+// The gradient sorts the tokens by id (stably), so that the rows of one id lie together and
+// their fp32 sum is taken in an order that depends on the ids alone: no floating-point
+// atomics, the same bits on every call.  Its kernels:
+//
+//   sort   one workgroup per kSortTokens tokens, a radix sort in LDS.  The other workgroups of
+//          the launch write the zeros of dtable, which for a vocabulary is most of the bytes.
+//   merge  (more than one sorted range) each token's place by binary searches in the others.
+//   sum    kTile sorted tokens per group of lanes; an id whose tokens all lie in the tile is
+//          written, one that crosses a tile's edge leaves an fp32 partial row.
+//   join   the partial rows of ids that cross edges, added in order.
+//
+// Ids outside [0, rows): the lookup returns NaN for them, the gradient leaves them out.
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "device_common.h"
+#include "dflash.h"
+#include "training.h"
+
+namespace dflash {
+namespace {
+
+// ---- lookup ------------------------------------------------------------------
+
+// `lanes` (a power of two, at most 64) lanes a row; V elements an access (a chunk or 1).
+template <typename T, typename I, int V>
+__global__ __launch_bounds__(256) void embedding_fwd_kernel(
+    const I* __restrict__ ids, const T* __restrict__ table, T* __restrict__ out, int64_t n,
+    int rows, int hidden, float scale, int lanes_log2) {
+  const int lanes = 1 << lanes_log2;
+  const int64_t token = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) >> lanes_log2;
+  if (token >= n) return;
+  const int64_t id = static_cast<int64_t>(ids[token]);
+  const bool known = id >= 0 && id < rows;
+  const T* from = table + (known ? id : 0) * hidden;
+  T* to = out + token * hidden;
+  for (int col = (threadIdx.x & (lanes - 1)) * V; col < hidden; col += lanes * V) {
+    float v[V];
+    if (known) {
+      load_floats<T, V, (V > 1)>(from + col, V, v);
+#pragma unroll
+      for (int e = 0; e < V; ++e) v[e] *= scale;
+    } else {
+#pragma unroll
+      for (int e = 0; e < V; ++e) v[e] = __builtin_nanf("");
+    }
+    store_floats<T, V, (V > 1)>(to + col, V, v);
+  }
+}
+
+// ---- sort --------------------------------------------------------------------
+
+constexpr int kSortTokens = 16384;   // per workgroup; a place in the range is 16 bits
+constexpr int kSortThreads = 1024;
+constexpr int kSortWaves = kSortThreads / 64;
+constexpr int kSortRounds = kSortTokens / kSortThreads;  // tokens a lane
+constexpr int kDigitBits = 9;
+constexpr int kBins = 1 << kDigitBits;
+// keys, places, counters of every wavefront, and the sums of the scan's wavefronts
+constexpr int kSortLds =
+    kSortTokens * 4 + kSortTokens * 2 + kSortWaves * kBins * 4 + kSortWaves * 4;
+
+// Wavefront-local order of LDS accesses: a wavefront's LDS instructions execute in order.
+__device__ inline void wave_order() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+
+// Stable radix sort of one range.  Ids that take no gradient become `rows`, past every other.
+// Each wavefront owns a contiguous part of the range and ranks 64 keys a round: the lanes of
+// equal digits are found with one ballot a bit, the digit's count so far is the
+// wavefront's counter.  A scan over (digit, wavefront) gives the places.
+template <typename I>
+__device__ void sort_range(const I* __restrict__ ids, int64_t first, int count, int rows,
+                           int64_t padding, int bits, int32_t* __restrict__ sorted_ids,
+                           int32_t* __restrict__ sorted_tokens, char* lds) {
+  uint32_t* keys = reinterpret_cast<uint32_t*>(lds);
+  uint32_t* counters = keys + kSortTokens;
+  uint32_t* wave_sums = counters + kSortWaves * kBins;
+  uint16_t* places = reinterpret_cast<uint16_t*>(wave_sums + kSortWaves);
+  const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+  const int rounds = (count + kSortThreads - 1) / kSortThreads;
+  const int mine = wave * rounds * 64 + lane;  // + 64 a round
+  const uint32_t last = bits < 32 ? (1u << bits) - 1 : ~0u;  // at least `rows`
+
+  uint32_t key[kSortRounds], place[kSortRounds], rank[kSortRounds];
+#pragma unroll
+  for (int j = 0; j < kSortRounds; ++j) {
+    key[j] = last;  // past the end: stays behind every token, by its value and its place
+    place[j] = mine + 64 * j;
+    if (j < rounds && mine + 64 * j < count) {
+      const int64_t id = static_cast<int64_t>(ids[first + mine + 64 * j]);
+      key[j] = id >= 0 && id < rows && id != padding ? static_cast<uint32_t>(id)
+                                                     : static_cast<uint32_t>(rows);
+    }
+  }
+  const int passes = (bits + kDigitBits - 1) / kDigitBits;
+  const int digit_bits = (bits + passes - 1) / passes;
+  const int bins = 1 << digit_bits;
+  for (int pass = 0; pass < passes; ++pass) {
+    const int shift = pass * digit_bits;
+    uint32_t* counter = counters + wave * kBins;
+    for (int b = lane; b < bins; b += 64) counter[b] = 0;
+    wave_order();
+#pragma unroll
+    for (int j = 0; j < kSortRounds; ++j) {
+      if (j < rounds) {
+        const uint32_t digit = (key[j] >> shift) & (bins - 1);
+        uint64_t same = ~0ull;
+        for (int b = 0; b < digit_bits; ++b) {
+          const uint64_t ones = __ballot((digit >> b) & 1);
+          same &= (digit >> b) & 1 ? ones : ~ones;
+        }
+        const uint32_t before = counter[digit];
+        const uint32_t ahead = __popcll(same & ((1ull << lane) - 1));
+        rank[j] = before + ahead;
+        wave_order();  // every lane has read the count
+        if (ahead == 0) counter[digit] = before + __popcll(same);
+        wave_order();
+      }
+    }
+    __syncthreads();
+    // Exclusive scan over (digit, wavefront): thread b owns digit b.
+    uint32_t total = 0;
+    if (threadIdx.x < bins) {
+      for (int w = 0; w < kSortWaves; ++w) {
+        const uint32_t c = counters[w * kBins + threadIdx.x];
+        counters[w * kBins + threadIdx.x] = total;
+        total += c;
+      }
+    }
+    uint32_t upto = total;
+#pragma unroll
+    for (int m = 1; m < 64; m <<= 1) {
+      const uint32_t other = __shfl_up(upto, m);
+      if (lane >= m) upto += other;
+    }
+    if (lane == 63) wave_sums[wave] = upto;
+    __syncthreads();
+    if (threadIdx.x < bins) {
+      uint32_t base = upto - total;
+      for (int w = 0; w < wave; ++w) base += wave_sums[w];
+      for (int w = 0; w < kSortWaves; ++w) counters[w * kBins + threadIdx.x] += base;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < kSortRounds; ++j) {
+      if (j < rounds) {
+        const uint32_t at = counter[(key[j] >> shift) & (bins - 1)] + rank[j];
+        keys[at] = key[j];
+        places[at] = static_cast<uint16_t>(place[j]);
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < kSortRounds; ++j) {
+      if (j < rounds) {
+        key[j] = keys[mine + 64 * j];
+        place[j] = places[mine + 64 * j];
+      }
+    }
+    __syncthreads();
+  }
+#pragma unroll
+  for (int j = 0; j < kSortRounds; ++j) {
+    const int at = mine + 64 * j;
+    if (j < rounds && at < count) {
+      sorted_ids[first + at] = static_cast<int32_t>(key[j]);
+      sorted_tokens[first + at] = static_cast<int32_t>(first + place[j]);
+    }
+  }
+}
+
+template <typename I>
+__global__ __launch_bounds__(kSortThreads) void embedding_sort_kernel(
+    const I* __restrict__ ids, int64_t n, int rows, int64_t padding, int bits, int ranges,
+    int32_t* __restrict__ sorted_ids, int32_t* __restrict__ sorted_tokens,
+    u32x4_t* __restrict__ table, int64_t table_bytes) {
+  extern __shared__ char lds[];
+  if (blockIdx.x < ranges) {
+    const int64_t first = static_cast<int64_t>(blockIdx.x) * kSortTokens;
+    const int count = n - first < kSortTokens ? static_cast<int>(n - first) : kSortTokens;
+    sort_range(ids, first, count, rows, padding, bits, sorted_ids, sorted_tokens, lds);
+    return;
+  }
+  const int64_t chunks = table_bytes / 16;
+  const int64_t step = static_cast<int64_t>(gridDim.x - ranges) * kSortThreads;
+  const int64_t at = static_cast<int64_t>(blockIdx.x - ranges) * kSortThreads + threadIdx.x;
+  for (int64_t i = at; i < chunks; i += step) table[i] = u32x4_t{0, 0, 0, 0};
+  // The last bytes of a table that is not whole chunks (elements are 2 or 4 bytes).
+  const int64_t rest = (table_bytes - chunks * 16) / 2;
+  if (at < rest) reinterpret_cast<uint16_t*>(table + chunks)[at] = 0;
+}
+
+// ---- merge -------------------------------------------------------------------
+
+// A token's place among all: its place in its own range, and in every other range the
+// number of ids before it (equal ids of earlier ranges come first).
+__global__ __launch_bounds__(256) void embedding_merge_kernel(
+    const int32_t* __restrict__ ids, const int32_t* __restrict__ tokens, int64_t n,
+    int32_t* __restrict__ merged_ids, int32_t* __restrict__ merged_tokens) {
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  if (i >= n) return;
+  const int32_t id = ids[i];
+  const int64_t own = i / kSortTokens;
+  const int64_t ranges = (n + kSortTokens - 1) / kSortTokens;
+  int64_t place = i - own * kSortTokens;
+  for (int64_t r = 0; r < ranges; ++r) {
+    if (r == own) continue;
+    const int32_t* range = ids + r * kSortTokens;
+    int low = 0, high = n - r * kSortTokens < kSortTokens ? static_cast<int>(n - r * kSortTokens)
+                                                          : kSortTokens;
+    while (low < high) {
+      const int middle = (low + high) / 2;
+      if (range[middle] < id || (r < own && range[middle] == id))
+        low = middle + 1;
+      else
+        high = middle;
+    }
+    place += low;
+  }
+  merged_ids[place] = id;
+  merged_tokens[place] = tokens[i];
+}
+
+// ---- sum and join --------------------------------------------------------------
+
+constexpr int kTile = 32;    // sorted tokens of a group of lanes
+constexpr int kAhead = 8;    // rows of dout in flight
+
+// A group of `lanes` lanes sums one tile over lanes * V columns (blockIdx.y: which).
+// partials[tile][0]: what the tile holds of an id that began in an earlier tile;
+// partials[tile][1]: of an id that begins here and goes on in the next tile.
+template <typename T, int V>
+__global__ __launch_bounds__(256) void embedding_sum_kernel(
+    const int32_t* __restrict__ ids, const int32_t* __restrict__ tokens, int64_t n, int rows,
+    const T* __restrict__ dout, T* __restrict__ dtable, int hidden, float scale,
+    float* __restrict__ partials, int lanes_log2) {
+  const int lanes = 1 << lanes_log2;
+  const int64_t tile = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) >> lanes_log2;
+  const int64_t begin = tile * kTile;
+  const int col = (static_cast<int>(blockIdx.y) * lanes + (threadIdx.x & (lanes - 1))) * V;
+  if (begin >= n || col >= hidden) return;
+  const int count = n - begin < kTile ? static_cast<int>(n - begin) : kTile;
+  ids += begin;
+  tokens += begin;
+  float* partial = partials + tile * 2 * hidden + col;
+  const bool from_before = begin > 0 && ids[-1] == ids[0];
+  const bool goes_on = begin + count < n && ids[count - 1] == ids[count];
+
+  float acc[V];
+#pragma unroll
+  for (int e = 0; e < V; ++e) acc[e] = 0.0f;
+  int32_t current = ids[0];
+  bool first = from_before;  // the sum in acc belongs to partials[tile][0]
+  for (int i0 = 0; i0 < count; i0 += kAhead) {
+    float row[kAhead][V];
+    int32_t id[kAhead];
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) {
+      id[j] = rows;
+      if (i0 + j < count) {
+        id[j] = ids[i0 + j];
+        if (id[j] < rows)
+          load_floats<T, V, (V > 1)>(dout + static_cast<int64_t>(tokens[i0 + j]) * hidden + col, V,
+                                     row[j]);
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) {
+      if (i0 + j >= count) break;
+      if (id[j] != current) {
+        if (first) {
+          store_floats<float, V, false>(partial, V, acc);
+        } else {
+#pragma unroll
+          for (int e = 0; e < V; ++e) acc[e] *= scale;
+          store_floats<T, V, (V > 1)>(dtable + static_cast<int64_t>(current) * hidden + col, V,
+                                      acc);
+        }
+#pragma unroll
+        for (int e = 0; e < V; ++e) acc[e] = 0.0f;
+        current = id[j];
+        first = false;
+      }
+      if (current >= rows) return;  // the ids without a gradient come last
+#pragma unroll
+      for (int e = 0; e < V; ++e) acc[e] += row[j][e];
+    }
+  }
+  if (first) {
+    store_floats<float, V, false>(partial, V, acc);
+  } else if (goes_on) {
+    store_floats<float, V, false>(partial + hidden, V, acc);
+  } else {
+#pragma unroll
+    for (int e = 0; e < V; ++e) acc[e] *= scale;
+    store_floats<T, V, (V > 1)>(dtable + static_cast<int64_t>(current) * hidden + col, V, acc);
+  }
+}
+
+// One workgroup per tile and 64 columns.  If an id begins in the tile and goes on, its partial
+// rows are added: four wavefronts each take a contiguous quarter, added in order.
+template <typename T>
+__global__ __launch_bounds__(256) void embedding_join_kernel(const int32_t* __restrict__ ids,
+                                                             int64_t n, int rows,
+                                                             T* __restrict__ dtable, int hidden,
+                                                             float scale,
+                                                             const float* __restrict__ partials) {
+  __shared__ float lds[4][64];
+  const int64_t tile = blockIdx.x;
+  const int64_t begin = tile * kTile;
+  const int64_t end = begin + kTile;
+  if (end >= n) return;  // (the last tile goes nowhere)
+  const int32_t id = ids[end - 1];
+  if (id >= rows || ids[end] != id) return;
+  if (ids[begin] == id && begin > 0 && ids[begin - 1] == id) return;  // began earlier
+  // Tiles whose first token is of the id: [tile + 1, low).
+  int64_t low = tile + 2, high = (n + kTile - 1) / kTile;
+  while (low < high) {
+    const int64_t middle = (low + high) / 2;
+    if (ids[middle * kTile] == id)
+      low = middle + 1;
+    else
+      high = middle;
+  }
+  const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+  const int col = blockIdx.y * 64 + lane;
+  const int64_t count = low - tile;  // partial rows, this tile's among them
+  const int64_t per = (count + 3) / 4;
+  const int64_t from = wave * per;
+  const int64_t to = from + per < count ? from + per : count;
+  float v = 0.0f;
+  if (col < hidden) {
+#pragma unroll 8
+    for (int64_t i = from; i < to; ++i)
+      v += partials[((tile + i) * 2 + (i == 0)) * hidden + col];
+  }
+  lds[wave][lane] = v;
+  __syncthreads();
+  if (wave == 0 && col < hidden) {
+#pragma unroll
+    for (int w = 1; w < 4; ++w) v += lds[w][lane];
+    dtable[static_cast<int64_t>(id) * hidden + col] = static_cast<T>(v * scale);
+  }
+}
+
+// ---- host --------------------------------------------------------------------
+
+int lanes_log2_for(int accesses, int most) {
+  int log2 = 0;
+  while ((1 << log2) < accesses && log2 < most) ++log2;
+  return log2;
+}
+
+uintptr_t address(const void* p) { return reinterpret_cast<uintptr_t>(p); }
+
+template <typename T, typename I>
+int launch_fwd(const void* ids, const void* table, void* out, int64_t n, int rows, int hidden,
+               float scale, hipStream_t stream) {
+  constexpr int N = Chunk<T>::N;
+  const bool wide = hidden % N == 0 && (address(table) | address(out)) % 16 == 0;
+  const int log2 = lanes_log2_for(wide ? hidden / N : hidden, 6);
+  if (n > (kMaxBlocks256 * 256) >> log2) return DFLASH_ERR_TOO_LARGE;
+  const int64_t blocks = ((n << log2) + 255) / 256;
+  hipLaunchKernelGGL(
+      (wide ? &embedding_fwd_kernel<T, I, N> : &embedding_fwd_kernel<T, I, 1>),
+      dim3(static_cast<uint32_t>(blocks)), dim3(256), 0, stream, static_cast<const I*>(ids),
+      static_cast<const T*>(table), static_cast<T*>(out), n, rows, hidden, scale, log2);
+  return static_cast<int>(hipGetLastError());
+}
+
+constexpr int64_t kMaxTokens = int64_t{1} << 26;
+constexpr int kMaxHidden = 1 << 20;
+
+int64_t tiles_of(int64_t n) { return (n + kTile - 1) / kTile; }
+int64_t ranges_of(int64_t n) { return (n + kSortTokens - 1) / kSortTokens; }
+int64_t aligned(int64_t bytes) { return (bytes + 255) / 256 * 256; }
+
+struct Workspace {
+  int64_t index_bytes, partial_bytes, total;
+};
+
+Workspace workspace_of(int64_t n, int hidden) {
+  Workspace w;
+  w.index_bytes = aligned(n * 4);
+  w.partial_bytes = tiles_of(n) > 1 ? aligned(tiles_of(n) * 2 * hidden * 4) : 0;
+  w.total = (ranges_of(n) > 1 ? 4 : 2) * w.index_bytes + w.partial_bytes;
+  return w;
+}
+
+template <typename T, typename I>
+int launch_bwd(const void* ids_in, const void* dout_in, void* dtable_in, int64_t n, int rows,
+               int hidden, float scale, int64_t padding, char* workspace, hipStream_t stream) {
+  const Workspace w = workspace_of(n, hidden);
+  const int ranges = static_cast<int>(ranges_of(n));
+  int32_t* ids = reinterpret_cast<int32_t*>(workspace);
+  int32_t* tokens = reinterpret_cast<int32_t*>(workspace + w.index_bytes);
+  float* partials = reinterpret_cast<float*>(workspace + w.total - w.partial_bytes);
+  int bits = 1;
+  while (bits < 32 && (int64_t{1} << bits) - 1 < rows) ++bits;
+  const int64_t table_bytes = static_cast<int64_t>(rows) * hidden * sizeof(T);
+  // Zeros: 64 bytes a thread at least, one workgroup a CU at most (their LDS holds one a CU).
+  const int64_t fill = (table_bytes / 16 + 4 * kSortThreads - 1) / (4 * kSortThreads);
+  const int fill_blocks = fill < 1 ? 1 : fill > 256 ? 256 : static_cast<int>(fill);
+  auto* sort = &embedding_sort_kernel<I>;
+  const hipError_t err = ensure_dynamic_lds<&embedding_sort_kernel<I>>(kSortLds);
+  if (err != hipSuccess) return static_cast<int>(err);
+  hipLaunchKernelGGL(sort, dim3(ranges + fill_blocks), dim3(kSortThreads), kSortLds, stream,
+                     static_cast<const I*>(ids_in), n, rows, padding, bits, ranges, ids, tokens,
+                     static_cast<u32x4_t*>(dtable_in), table_bytes);
+  int rc = static_cast<int>(hipGetLastError());
+  if (rc != DFLASH_OK || n == 0) return rc;
+  if (ranges > 1) {
+    int32_t* merged = reinterpret_cast<int32_t*>(workspace + 2 * w.index_bytes);
+    int32_t* merged_tokens = reinterpret_cast<int32_t*>(workspace + 3 * w.index_bytes);
+    hipLaunchKernelGGL(embedding_merge_kernel, dim3(static_cast<uint32_t>((n + 255) / 256)),
+                       dim3(256), 0, stream, ids, tokens, n, merged, merged_tokens);
+    rc = static_cast<int>(hipGetLastError());
+    if (rc != DFLASH_OK) return rc;
+    ids = merged;
+    tokens = merged_tokens;
+  }
+  constexpr int N = Chunk<T>::N;
+  const T* dout = static_cast<const T*>(dout_in);
+  T* dtable = static_cast<T*>(dtable_in);
+  const bool wide = hidden % N == 0 && (address(dout) | address(dtable)) % 16 == 0;
+  const int accesses = wide ? hidden / N : hidden;
+  const int log2 = lanes_log2_for(accesses, 5);
+  const int64_t tiles = tiles_of(n);
+  hipLaunchKernelGGL((wide ? &embedding_sum_kernel<T, N> : &embedding_sum_kernel<T, 1>),
+                     dim3(static_cast<uint32_t>(((tiles << log2) + 255) / 256),
+                          (accesses + (1 << log2) - 1) >> log2),
+                     dim3(256), 0, stream, ids, tokens, n, rows, dout, dtable, hidden, scale,
+                     partials, log2);
+  rc = static_cast<int>(hipGetLastError());
+  if (rc != DFLASH_OK || tiles == 1) return rc;
+  hipLaunchKernelGGL((embedding_join_kernel<T>),
+                     dim3(static_cast<uint32_t>(tiles), (hidden + 63) / 64), dim3(256), 0, stream,
+                     ids, n, rows, dtable, hidden, scale, partials);
+  return static_cast<int>(hipGetLastError());
+}
+
+// Calls f(T, I) with the element types of the codes.
+template <typename F>
+int with_types(int dtype, int id_bytes, F f) {
+  if (id_bytes != 4 && id_bytes != 8) return DFLASH_ERR_DTYPE;
+  auto with_ids = [&](auto t) {
+    return id_bytes == 4 ? f(t, int32_t()) : f(t, int64_t());
+  };
+  switch (dtype) {
+    case DFLASH_DTYPE_FP16: return with_ids(_Float16());
+    case DFLASH_DTYPE_BF16: return with_ids(__bf16());
+    case DFLASH_DTYPE_FP32: return with_ids(float());
+    default: return DFLASH_ERR_DTYPE;
+  }
+}
+
+bool shape_taken(int64_t n, int rows, int hidden) {
+  return n >= 0 && n <= kMaxTokens && rows >= 1 && rows < INT32_MAX && hidden >= 1 &&
+         hidden <= kMaxHidden;
+}
+
+}  // namespace
+}  // namespace dflash
+
+using namespace dflash;
+
+extern "C" int dflash_embedding_fwd(const void* ids, const void* table, void* out, int64_t n,
+                                    int rows, int hidden, float scale, int id_bytes, int dtype,
+                                    void* stream) {
+  if (!shape_taken(n, rows, hidden)) return DFLASH_ERR_SHAPE;
+  return with_types(dtype, id_bytes, [&](auto t, auto i) {
+    using T = decltype(t);
+    using I = decltype(i);
+    if (n == 0) return static_cast<int>(DFLASH_OK);
+    if (!ids || !table || !out) return static_cast<int>(DFLASH_ERR_NULL);
+    if (address(ids) % sizeof(I) != 0 || (address(table) | address(out)) % sizeof(T) != 0)
+      return static_cast<int>(DFLASH_ERR_ALIGN);
+    return launch_fwd<T, I>(ids, table, out, n, rows, hidden, scale,
+                            static_cast<hipStream_t>(stream));
+  });
+}
+
+extern "C" size_t dflash_embedding_bwd_workspace_bytes(int64_t n, int hidden) {
+  if (!shape_taken(n, 1, hidden)) return 0;
+  return static_cast<size_t>(workspace_of(n, hidden).total);
+}
+
+extern "C" int dflash_embedding_bwd(const void* ids, const void* dout, void* dtable, int64_t n,
+                                    int rows, int hidden, float scale, int64_t padding,
+                                    int id_bytes, int dtype, void* workspace,
+                                    size_t workspace_bytes, void* stream) {
+  if (!shape_taken(n, rows, hidden)) return DFLASH_ERR_SHAPE;
+  return with_types(dtype, id_bytes, [&](auto t, auto i) {
+    using T = decltype(t);
+    using I = decltype(i);
+    if (!dtable || (n > 0 && (!ids || !dout || !workspace)))
+      return static_cast<int>(DFLASH_ERR_NULL);
+    if (address(ids) % sizeof(I) != 0 || address(dout) % sizeof(T) != 0 ||
+        address(dtable) % 16 != 0 || address(workspace) % 16 != 0)
+      return static_cast<int>(DFLASH_ERR_ALIGN);
+    if (workspace_bytes < static_cast<size_t>(workspace_of(n, hidden).total))
+      return static_cast<int>(DFLASH_ERR_WORKSPACE);
+    return launch_bwd<T, I>(ids, dout, dtable, n, rows, hidden, scale, padding,
+                            static_cast<char*>(workspace), static_cast<hipStream_t>(stream));
+  });
+}

@@ -3,7 +3,8 @@
 Drop-in for the reference package's public API (``__init__.py:3-19``):
 ``optimize_deberta``, ``enable_deberta_inference``, ``compile_deberta_buckets``,
 ``DebertaV2InferenceEncoder`` and the ``DisentangledFlashAttention`` module,
-plus ``capture_deberta_buckets`` (HIP-graph replay of prepared buckets).
+plus ``capture_deberta_buckets`` (HIP-graph replay of prepared buckets) and
+``enable_deberta_training`` (the operators of a training step, ``training``).
 """
 
 from .deberta import (
@@ -14,6 +15,7 @@ from .deberta import (
 )
 from .graphs import DebertaGraphBucket, capture_deberta_buckets
 from .kernel import DisentangledFlashAttention
+from .training import enable_deberta_training
 
 __version__ = "0.1.0"
 
@@ -24,5 +26,6 @@ __all__ = [
     "DisentangledFlashAttention",
     "compile_deberta_buckets",
     "enable_deberta_inference",
+    "enable_deberta_training",
     "optimize_deberta",
 ]

@@ -20,7 +20,7 @@ from pathlib import Path
 import torch  # noqa: F401  (load torch's HIP runtime first)
 
 LIBRARY_NAME = "libdflash.so"
-ABI_VERSION = 7
+ABI_VERSION = 8
 
 ERR_WORKSPACE = -7  # DFLASH_ERR_WORKSPACE
 
@@ -34,6 +34,8 @@ _c_void_p = ctypes.c_void_p
 _c_int = ctypes.c_int
 _c_int64 = ctypes.c_int64
 _c_float = ctypes.c_float
+_c_double = ctypes.c_double
+_c_uint32 = ctypes.c_uint32
 
 
 class EncoderLayer(ctypes.Structure):
@@ -135,6 +137,47 @@ def _bind(lib: ctypes.CDLL) -> None:
     lib.dflash_encoder_layer_fwd.argtypes = [
         ctypes.POINTER(EncoderLayer), _c_void_p, _c_void_p, _c_void_p,  # layer, x, mask, out
         _c_int, _c_int,                                          # B, L
+        _c_void_p, ctypes.c_size_t, _c_void_p,                   # workspace, bytes, stream
+    ]
+    lib.dflash_dropout.restype = _c_int
+    lib.dflash_dropout.argtypes = [
+        _c_void_p, _c_void_p, _c_int64,                          # x, y, n
+        _c_double, _c_void_p, _c_uint32,                         # p, rng, site
+        _c_int, _c_void_p,                                       # dtype, stream
+    ]
+    lib.dflash_dropout_layernorm_fwd.restype = _c_int
+    lib.dflash_dropout_layernorm_fwd.argtypes = [
+        _c_void_p, _c_void_p, _c_void_p, _c_void_p,              # x, residual, gamma, beta
+        _c_void_p, _c_void_p, _c_void_p,                         # y, mean, rstd
+        _c_int64, _c_int, _c_float,                              # rows, hidden, eps
+        _c_double, _c_void_p, _c_uint32,                         # p, rng, site
+        _c_int, _c_int, _c_void_p,                               # dtype, weight dtype, stream
+    ]
+    lib.dflash_dropout_layernorm_bwd_workspace_bytes.restype = ctypes.c_size_t
+    lib.dflash_dropout_layernorm_bwd_workspace_bytes.argtypes = [_c_int64, _c_int]
+    lib.dflash_dropout_layernorm_bwd.restype = _c_int
+    lib.dflash_dropout_layernorm_bwd.argtypes = [
+        _c_void_p, _c_void_p, _c_void_p, _c_void_p,              # dy, x, residual, gamma
+        _c_void_p, _c_void_p,                                    # mean, rstd
+        _c_void_p, _c_void_p, _c_void_p, _c_void_p,              # dx, dresidual, dgamma, dbeta
+        _c_int64, _c_int,                                        # rows, hidden
+        _c_double, _c_void_p, _c_uint32,                         # p, rng, site
+        _c_int, _c_int,                                          # dtype, weight dtype
+        _c_void_p, ctypes.c_size_t, _c_void_p,                   # workspace, bytes, stream
+    ]
+    lib.dflash_embedding_fwd.restype = _c_int
+    lib.dflash_embedding_fwd.argtypes = [
+        _c_void_p, _c_void_p, _c_void_p,                         # ids, table, out
+        _c_int64, _c_int, _c_int, _c_float,                      # n, rows, hidden, scale
+        _c_int, _c_int, _c_void_p,                               # id bytes, dtype, stream
+    ]
+    lib.dflash_embedding_bwd_workspace_bytes.restype = ctypes.c_size_t
+    lib.dflash_embedding_bwd_workspace_bytes.argtypes = [_c_int64, _c_int]
+    lib.dflash_embedding_bwd.restype = _c_int
+    lib.dflash_embedding_bwd.argtypes = [
+        _c_void_p, _c_void_p, _c_void_p,                         # ids, dout, dtable
+        _c_int64, _c_int, _c_int, _c_float, _c_int64,            # n, rows, hidden, scale, padding
+        _c_int, _c_int,                                          # id bytes, dtype
         _c_void_p, ctypes.c_size_t, _c_void_p,                   # workspace, bytes, stream
     ]
     lib.dflash_error_string.restype = ctypes.c_char_p

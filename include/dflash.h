@@ -25,7 +25,7 @@ extern "C" {
 
 #define DFLASH_API __attribute__((visibility("default")))
 
-#define DFLASH_ABI_VERSION 7
+#define DFLASH_ABI_VERSION 8
 
 #define DFLASH_DTYPE_FP16 0
 #define DFLASH_DTYPE_BF16 1
@@ -336,6 +336,76 @@ DFLASH_API size_t dflash_encoder_layer_workspace_bytes(const dflash_encoder_laye
 DFLASH_API int dflash_encoder_layer_fwd(const dflash_encoder_layer* layer, const void* x,
                                         const uint8_t* mask, void* out, int B, int L,
                                         void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * Training operators: dropout, LayerNorm with dropout and residual, embedding.
+ *
+ * The generator: p is rounded to a multiple of 2^-16 (to 0 and 1 only where it is 0 or 1).
+ * Element i of the flattened tensor belongs to block i / 8; Philox4x32 with 7 rounds of the
+ * counter (block low, block high, site, step) under the 64-bit key seed gives the block four
+ * words, element e of it the low (e even) or high 16 bits of word e / 2.  It is kept where they
+ * are at least 65536 p, and then divided by the rounded 1 - p; otherwise it is 0
+ * whatever it held.
+ *   rng  : device int64 [2] = seed, step (the step's low 32 bits are used); read by the kernels;
+ *          may be NULL when p is 0
+ *   site : numbers the places of a model that drop elements
+ * Pointers need the alignment of their element type only; rows of whole 16-byte chunks on
+ * 16-byte boundaries are faster.  Outputs must not overlap inputs.  The workspaces' contents
+ * need not outlive the kernels; calls that share one must not overlap.
+ */
+
+/* y = drop(x) over n elements; also the backward pass (dx = drop(dy)). */
+DFLASH_API int dflash_dropout(const void* x, void* y, int64_t n, double p, const int64_t* rng,
+                              uint32_t site, int dtype, void* stream);
+
+/*
+ * y = LayerNorm(drop(x) + residual), the tail of DebertaV2SelfOutput / DebertaV2Output in
+ * training (/root/reference/src/disentangled_flash/_reference.py:101-112, 474-485).
+ *   x, residual, y : [rows, hidden], dtype `dtype`; residual may be NULL; hidden 1 to 8192
+ *   gamma, beta    : [hidden], `weight_dtype`: `dtype` or fp32
+ *   mean, rstd     : fp32 [rows], kept for the backward pass; both may be NULL
+ * All in fp32, y rounded once (dflash_add_layernorm_fwd rounds the sum too).
+ */
+DFLASH_API int dflash_dropout_layernorm_fwd(const void* x, const void* residual, const void* gamma,
+                                            const void* beta, void* y, float* mean, float* rstd,
+                                            int64_t rows, int hidden, float eps, double p,
+                                            const int64_t* rng, uint32_t site, int dtype,
+                                            int weight_dtype, void* stream);
+
+/*
+ * Its backward pass, from the same x, residual, p, rng and site.
+ *   dx, dresidual  : [rows, hidden], `dtype`; each may be NULL (with p = 0 they are equal)
+ *   dgamma, dbeta  : [hidden], `weight_dtype`; both may be NULL, then no workspace is needed
+ *   workspace      : dflash_dropout_layernorm_bwd_workspace_bytes(rows, hidden) bytes
+ * The sums over rows are taken in an order that depends on rows and hidden alone.
+ */
+DFLASH_API size_t dflash_dropout_layernorm_bwd_workspace_bytes(int64_t rows, int hidden);
+DFLASH_API int dflash_dropout_layernorm_bwd(
+    const void* dy, const void* x, const void* residual, const void* gamma, const float* mean,
+    const float* rstd, void* dx, void* dresidual, void* dgamma, void* dbeta, int64_t rows,
+    int hidden, double p, const int64_t* rng, uint32_t site, int dtype, int weight_dtype,
+    void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * out[i] = scale * table[ids[i]], rounded once; NaN for an id outside [0, rows).
+ *   ids   : int32 (id_bytes 4) or int64 (8), n of them, at most 2^26
+ *   table : [rows, hidden], out: [n, hidden], dtype `dtype`; hidden at most 2^20
+ */
+DFLASH_API int dflash_embedding_fwd(const void* ids, const void* table, void* out, int64_t n,
+                                    int rows, int hidden, float scale, int id_bytes, int dtype,
+                                    void* stream);
+
+/*
+ * The table's dense gradient: dtable[v] = scale * (sum of dout[i] over ids[i] = v), 0 for
+ * v = padding (-1: none) and for rows that no id names; every row is written.  Ids outside
+ * [0, rows) are left out.  fp32 sums in an order that depends on the ids alone.
+ *   dtable, workspace : 16-byte aligned; dflash_embedding_bwd_workspace_bytes(n, hidden) bytes
+ */
+DFLASH_API size_t dflash_embedding_bwd_workspace_bytes(int64_t n, int hidden);
+DFLASH_API int dflash_embedding_bwd(const void* ids, const void* dout, void* dtable, int64_t n,
+                                    int rows, int hidden, float scale, int64_t padding,
+                                    int id_bytes, int dtype, void* workspace,
+                                    size_t workspace_bytes, void* stream);
 
 /* Text for a return code of any dflash_* entry point. */
 DFLASH_API const char* dflash_error_string(int code);
