@@ -24,19 +24,25 @@ __global__ __launch_bounds__(256) void dropout_kernel(const T* __restrict__ x, T
   const int64_t first = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) * N;
   if (first >= n) return;
   const DropoutKey key = dropout_key(d);
+  // The last chunk may be a part of one.
   const int live = n - first < N ? static_cast<int>(n - first) : N;
-  float v[N];
-  if (WIDE && live == N)
-    load_floats<T, N, true>(x + first, N, v);
-  else
-    load_floats<T, N, false>(x + first, live, v);
-  const uint32_t dropped = dropped_from<N, true>(d, key, first);
-#pragma unroll
-  for (int e = 0; e < N; ++e) v[e] = (dropped >> e) & 1 ? 0.0f : v[e] * d.scale;
-  if (WIDE && live == N)
-    store_floats<T, N, true>(y + first, N, v);
-  else
-    store_floats<T, N, false>(y + first, live, v);
+  if (WIDE && live == N) {
+    RowChunk<T, N, true> chunk;
+    chunk.load(x + first, 0, N);  // in flight while the mask is drawn
+    const uint32_t dropped = dropped_from<N, true>(d, key, first);
+    float v[N];
+    chunk.floats(0, N, v);
+    apply_dropout(d, dropped, v);
+    store_chunk<T, N, true>(y + first, 0, N, v);
+  } else {
+    RowChunk<T, N, false> chunk;
+    chunk.load(x + first, 0, live);
+    const uint32_t dropped = dropped_from<N, true>(d, key, first);
+    float v[N];
+    chunk.floats(0, live, v);
+    apply_dropout(d, dropped, v);
+    store_chunk<T, N, false>(y + first, 0, live, v);
+  }
 }
 
 template <typename T>

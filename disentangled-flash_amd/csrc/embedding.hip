@@ -43,28 +43,32 @@ __global__ __launch_bounds__(256) void embedding_fwd_kernel(
   for (int col = (threadIdx.x & (lanes - 1)) * V; col < hidden; col += lanes * V) {
     float v[V];
     if (known) {
-      load_floats<T, V, (V > 1)>(from + col, V, v);
+      load_floats<T, V>(from + col, v);
 #pragma unroll
       for (int e = 0; e < V; ++e) v[e] *= scale;
     } else {
 #pragma unroll
       for (int e = 0; e < V; ++e) v[e] = __builtin_nanf("");
     }
-    store_floats<T, V, (V > 1)>(to + col, V, v);
+    store_floats<T, V>(to + col, v);
   }
 }
 
 // ---- sort --------------------------------------------------------------------
 
-constexpr int kSortTokens = 16384;   // per workgroup; a place in the range is 16 bits
-constexpr int kSortThreads = 1024;
+constexpr int kSortTokens = 2048;    // per workgroup; a place in the range is 16 bits
+constexpr int kSortThreads = 512;
 constexpr int kSortWaves = kSortThreads / 64;
 constexpr int kSortRounds = kSortTokens / kSortThreads;  // tokens a lane
 constexpr int kDigitBits = 9;
 constexpr int kBins = 1 << kDigitBits;
-// keys, places, counters of every wavefront, and the sums of the scan's wavefronts
-constexpr int kSortLds =
-    kSortTokens * 4 + kSortTokens * 2 + kSortWaves * kBins * 4 + kSortWaves * 4;
+
+struct SortLds {
+  uint32_t keys[kSortTokens];
+  uint32_t counters[kSortWaves][kBins];
+  uint32_t wave_sums[kSortWaves];
+  uint16_t places[kSortTokens];
+};
 
 // Wavefront-local order of LDS accesses: a wavefront's LDS instructions execute in order.
 __device__ inline void wave_order() {
@@ -79,11 +83,7 @@ __device__ inline void wave_order() {
 template <typename I>
 __device__ void sort_range(const I* __restrict__ ids, int64_t first, int count, int rows,
                            int64_t padding, int bits, int32_t* __restrict__ sorted_ids,
-                           int32_t* __restrict__ sorted_tokens, char* lds) {
-  uint32_t* keys = reinterpret_cast<uint32_t*>(lds);
-  uint32_t* counters = keys + kSortTokens;
-  uint32_t* wave_sums = counters + kSortWaves * kBins;
-  uint16_t* places = reinterpret_cast<uint16_t*>(wave_sums + kSortWaves);
+                           int32_t* __restrict__ sorted_tokens, SortLds& lds) {
   const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
   const int rounds = (count + kSortThreads - 1) / kSortThreads;
   const int mine = wave * rounds * 64 + lane;  // + 64 a round
@@ -105,7 +105,7 @@ __device__ void sort_range(const I* __restrict__ ids, int64_t first, int count, 
   const int bins = 1 << digit_bits;
   for (int pass = 0; pass < passes; ++pass) {
     const int shift = pass * digit_bits;
-    uint32_t* counter = counters + wave * kBins;
+    uint32_t* counter = lds.counters[wave];
     for (int b = lane; b < bins; b += 64) counter[b] = 0;
     wave_order();
 #pragma unroll
@@ -113,9 +113,12 @@ __device__ void sort_range(const I* __restrict__ ids, int64_t first, int count, 
       if (j < rounds) {
         const uint32_t digit = (key[j] >> shift) & (bins - 1);
         uint64_t same = ~0ull;
-        for (int b = 0; b < digit_bits; ++b) {
-          const uint64_t ones = __ballot((digit >> b) & 1);
-          same &= (digit >> b) & 1 ? ones : ~ones;
+#pragma unroll
+        for (int b = 0; b < kDigitBits; ++b) {
+          if (b < digit_bits) {
+            const uint64_t ones = __ballot((digit >> b) & 1);
+            same &= (digit >> b) & 1 ? ones : ~ones;
+          }
         }
         const uint32_t before = counter[digit];
         const uint32_t ahead = __popcll(same & ((1ull << lane) - 1));
@@ -129,9 +132,10 @@ __device__ void sort_range(const I* __restrict__ ids, int64_t first, int count, 
     // Exclusive scan over (digit, wavefront): thread b owns digit b.
     uint32_t total = 0;
     if (threadIdx.x < bins) {
+#pragma unroll
       for (int w = 0; w < kSortWaves; ++w) {
-        const uint32_t c = counters[w * kBins + threadIdx.x];
-        counters[w * kBins + threadIdx.x] = total;
+        const uint32_t c = lds.counters[w][threadIdx.x];
+        lds.counters[w][threadIdx.x] = total;
         total += c;
       }
     }
@@ -141,28 +145,29 @@ __device__ void sort_range(const I* __restrict__ ids, int64_t first, int count, 
       const uint32_t other = __shfl_up(upto, m);
       if (lane >= m) upto += other;
     }
-    if (lane == 63) wave_sums[wave] = upto;
+    if (lane == 63) lds.wave_sums[wave] = upto;
     __syncthreads();
     if (threadIdx.x < bins) {
       uint32_t base = upto - total;
-      for (int w = 0; w < wave; ++w) base += wave_sums[w];
-      for (int w = 0; w < kSortWaves; ++w) counters[w * kBins + threadIdx.x] += base;
+      for (int w = 0; w < wave; ++w) base += lds.wave_sums[w];
+#pragma unroll
+      for (int w = 0; w < kSortWaves; ++w) lds.counters[w][threadIdx.x] += base;
     }
     __syncthreads();
 #pragma unroll
     for (int j = 0; j < kSortRounds; ++j) {
       if (j < rounds) {
         const uint32_t at = counter[(key[j] >> shift) & (bins - 1)] + rank[j];
-        keys[at] = key[j];
-        places[at] = static_cast<uint16_t>(place[j]);
+        lds.keys[at] = key[j];
+        lds.places[at] = static_cast<uint16_t>(place[j]);
       }
     }
     __syncthreads();
 #pragma unroll
     for (int j = 0; j < kSortRounds; ++j) {
       if (j < rounds) {
-        key[j] = keys[mine + 64 * j];
-        place[j] = places[mine + 64 * j];
+        key[j] = lds.keys[mine + 64 * j];
+        place[j] = lds.places[mine + 64 * j];
       }
     }
     __syncthreads();
@@ -182,8 +187,8 @@ __global__ __launch_bounds__(kSortThreads) void embedding_sort_kernel(
     const I* __restrict__ ids, int64_t n, int rows, int64_t padding, int bits, int ranges,
     int32_t* __restrict__ sorted_ids, int32_t* __restrict__ sorted_tokens,
     u32x4_t* __restrict__ table, int64_t table_bytes) {
-  extern __shared__ char lds[];
-  if (blockIdx.x < ranges) {
+  __shared__ SortLds lds;
+  if (static_cast<int>(blockIdx.x) < ranges) {
     const int64_t first = static_cast<int64_t>(blockIdx.x) * kSortTokens;
     const int count = n - first < kSortTokens ? static_cast<int>(n - first) : kSortTokens;
     sort_range(ids, first, count, rows, padding, bits, sorted_ids, sorted_tokens, lds);
@@ -192,7 +197,8 @@ __global__ __launch_bounds__(kSortThreads) void embedding_sort_kernel(
   const int64_t chunks = table_bytes / 16;
   const int64_t step = static_cast<int64_t>(gridDim.x - ranges) * kSortThreads;
   const int64_t at = static_cast<int64_t>(blockIdx.x - ranges) * kSortThreads + threadIdx.x;
-  for (int64_t i = at; i < chunks; i += step) table[i] = u32x4_t{0, 0, 0, 0};
+  for (int64_t i = at; i < chunks; i += step)
+    __builtin_nontemporal_store(u32x4_t{0, 0, 0, 0}, table + i);
   // The last bytes of a table that is not whole chunks (elements are 2 or 4 bytes).
   const int64_t rest = (table_bytes - chunks * 16) / 2;
   if (at < rest) reinterpret_cast<uint16_t*>(table + chunks)[at] = 0;
@@ -201,119 +207,155 @@ __global__ __launch_bounds__(kSortThreads) void embedding_sort_kernel(
 // ---- merge -------------------------------------------------------------------
 
 // A token's place among all: its place in its own range, and in every other range the
-// number of ids before it (equal ids of earlier ranges come first).
-__global__ __launch_bounds__(256) void embedding_merge_kernel(
+// number of ids before it (equal ids of earlier ranges come first).  The ranges pass through
+// LDS kMergeRanges at a time, where each search takes 11 steps and the searches of one
+// token are independent; from L2 the steps alone would take their latency 11 times over.
+constexpr int kMergeRanges = 8;
+constexpr int kMergeThreads = 512;
+constexpr int kMergeLds = kMergeRanges * kSortTokens * 4;
+
+__global__ __launch_bounds__(kMergeThreads) void embedding_merge_kernel(
     const int32_t* __restrict__ ids, const int32_t* __restrict__ tokens, int64_t n,
     int32_t* __restrict__ merged_ids, int32_t* __restrict__ merged_tokens) {
-  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-  if (i >= n) return;
-  const int32_t id = ids[i];
+  extern __shared__ int32_t lds[];
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * kMergeThreads + threadIdx.x;
+  const int32_t id = i < n ? ids[i] : 0;
   const int64_t own = i / kSortTokens;
-  const int64_t ranges = (n + kSortTokens - 1) / kSortTokens;
   int64_t place = i - own * kSortTokens;
-  for (int64_t r = 0; r < ranges; ++r) {
-    if (r == own) continue;
-    const int32_t* range = ids + r * kSortTokens;
-    int low = 0, high = n - r * kSortTokens < kSortTokens ? static_cast<int>(n - r * kSortTokens)
-                                                          : kSortTokens;
-    while (low < high) {
-      const int middle = (low + high) / 2;
-      if (range[middle] < id || (r < own && range[middle] == id))
-        low = middle + 1;
-      else
-        high = middle;
+  const int64_t ranges = (n + kSortTokens - 1) / kSortTokens;
+  for (int64_t r0 = 0; r0 < ranges; r0 += kMergeRanges) {
+    const int64_t first = r0 * kSortTokens;
+    const int64_t held = n - first < kMergeRanges * kSortTokens ? n - first
+                                                               : kMergeRanges * kSortTokens;
+    __syncthreads();  // the ranges before have been searched
+    for (int j = threadIdx.x * 4; j < kMergeRanges * kSortTokens; j += kMergeThreads * 4) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        lds[j + e] = j + e < held ? ids[first + j + e] : INT32_MAX;  // past the end: above all
     }
-    place += low;
+    __syncthreads();
+    int before[kMergeRanges];
+#pragma unroll
+    for (int r = 0; r < kMergeRanges; ++r) before[r] = 0;
+    for (int step = kSortTokens / 2; step >= 1; step /= 2) {
+#pragma unroll
+      for (int r = 0; r < kMergeRanges; ++r) {
+        const int32_t other = lds[r * kSortTokens + before[r] + step - 1];
+        before[r] += other < id || (other == id && r0 + r < own) ? step : 0;
+      }
+    }
+#pragma unroll
+    for (int r = 0; r < kMergeRanges; ++r) {
+      // (The steps add up to kSortTokens - 1: the last id is still to be compared.)
+      const int32_t other = lds[r * kSortTokens + before[r]];
+      before[r] += other < id || (other == id && r0 + r < own) ? 1 : 0;
+      if (r0 + r != own) place += before[r];
+    }
   }
-  merged_ids[place] = id;
-  merged_tokens[place] = tokens[i];
+  if (i < n) {
+    merged_ids[place] = id;
+    merged_tokens[place] = tokens[i];
+  }
 }
 
 // ---- sum and join --------------------------------------------------------------
 
-constexpr int kTile = 32;    // sorted tokens of a group of lanes
-constexpr int kAhead = 8;    // rows of dout in flight
+constexpr int kTile = 32;      // sorted tokens of a group of lanes
+constexpr int kAhead = 16;     // rows of dout in flight
+constexpr int kMinLanes = 8;   // of a group, so that its workgroup's tokens fit LDS
+
+template <int V>
+__device__ inline void store_partial(float* p, const float (&v)[V]) {
+#pragma unroll
+  for (int e = 0; e < V; ++e) p[e] = v[e];
+}
 
 // A group of `lanes` lanes sums one tile over lanes * V columns (blockIdx.y: which).
 // partials[tile][0]: what the tile holds of an id that began in an earlier tile;
 // partials[tile][1]: of an id that begins here and goes on in the next tile.
+// Bound by the latency of rows gathered from HBM: the tile's ids and tokens come through LDS
+// first, so that the loads of kAhead rows depend on nothing else and are in flight together.
 template <typename T, int V>
 __global__ __launch_bounds__(256) void embedding_sum_kernel(
     const int32_t* __restrict__ ids, const int32_t* __restrict__ tokens, int64_t n, int rows,
     const T* __restrict__ dout, T* __restrict__ dtable, int hidden, float scale,
     float* __restrict__ partials, int lanes_log2) {
+  typedef T Access __attribute__((ext_vector_type(V)));
+  constexpr int kMost = 256 / kMinLanes * kTile;
+  __shared__ int32_t lds_ids[kMost + 2];  // with the neighbours on both sides, -1 past the ends
+  __shared__ int32_t lds_tokens[kMost];
   const int lanes = 1 << lanes_log2;
-  const int64_t tile = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) >> lanes_log2;
+  const int tiles = 256 >> lanes_log2;
+  const int64_t start = static_cast<int64_t>(blockIdx.x) * tiles * kTile;
+  for (int i = threadIdx.x; i < tiles * kTile + 2; i += 256) {
+    const int64_t at = start + i - 1;
+    lds_ids[i] = at >= 0 && at < n ? ids[at] : -1;
+    if (i < tiles * kTile) lds_tokens[i] = start + i < n ? tokens[start + i] : 0;
+  }
+  __syncthreads();
+  const int group = threadIdx.x >> lanes_log2;
+  const int64_t tile = static_cast<int64_t>(blockIdx.x) * tiles + group;
   const int64_t begin = tile * kTile;
   const int col = (static_cast<int>(blockIdx.y) * lanes + (threadIdx.x & (lanes - 1))) * V;
   if (begin >= n || col >= hidden) return;
   const int count = n - begin < kTile ? static_cast<int>(n - begin) : kTile;
-  ids += begin;
-  tokens += begin;
+  const int32_t* id = lds_ids + 1 + group * kTile;
+  const int32_t* token = lds_tokens + group * kTile;
   float* partial = partials + tile * 2 * hidden + col;
-  const bool from_before = begin > 0 && ids[-1] == ids[0];
-  const bool goes_on = begin + count < n && ids[count - 1] == ids[count];
 
   float acc[V];
 #pragma unroll
   for (int e = 0; e < V; ++e) acc[e] = 0.0f;
-  int32_t current = ids[0];
-  bool first = from_before;  // the sum in acc belongs to partials[tile][0]
+  int32_t current = id[0];
+  bool first = id[-1] == current;  // the sum in acc belongs to partials[tile][0]
   for (int i0 = 0; i0 < count; i0 += kAhead) {
-    float row[kAhead][V];
-    int32_t id[kAhead];
+    Access row[kAhead];
 #pragma unroll
-    for (int j = 0; j < kAhead; ++j) {
-      id[j] = rows;
-      if (i0 + j < count) {
-        id[j] = ids[i0 + j];
-        if (id[j] < rows)
-          load_floats<T, V, (V > 1)>(dout + static_cast<int64_t>(tokens[i0 + j]) * hidden + col, V,
-                                     row[j]);
-      }
-    }
+    for (int j = 0; j < kAhead; ++j)  // (past the tile's end its last row again)
+      row[j] = *reinterpret_cast<const Access*>(
+          dout + static_cast<int64_t>(token[min(i0 + j, count - 1)]) * hidden + col);
 #pragma unroll
     for (int j = 0; j < kAhead; ++j) {
       if (i0 + j >= count) break;
-      if (id[j] != current) {
+      const int32_t next = id[i0 + j];
+      if (next != current) {
         if (first) {
-          store_floats<float, V, false>(partial, V, acc);
+          store_partial(partial, acc);
         } else {
 #pragma unroll
           for (int e = 0; e < V; ++e) acc[e] *= scale;
-          store_floats<T, V, (V > 1)>(dtable + static_cast<int64_t>(current) * hidden + col, V,
-                                      acc);
+          store_floats<T, V>(dtable + static_cast<int64_t>(current) * hidden + col, acc);
         }
 #pragma unroll
         for (int e = 0; e < V; ++e) acc[e] = 0.0f;
-        current = id[j];
+        current = next;
         first = false;
       }
       if (current >= rows) return;  // the ids without a gradient come last
 #pragma unroll
-      for (int e = 0; e < V; ++e) acc[e] += row[j][e];
+      for (int e = 0; e < V; ++e) acc[e] += static_cast<float>(row[j][e]);
     }
   }
   if (first) {
-    store_floats<float, V, false>(partial, V, acc);
-  } else if (goes_on) {
-    store_floats<float, V, false>(partial + hidden, V, acc);
+    store_partial(partial, acc);
+  } else if (id[count] == current) {
+    store_partial(partial + hidden, acc);
   } else {
 #pragma unroll
     for (int e = 0; e < V; ++e) acc[e] *= scale;
-    store_floats<T, V, (V > 1)>(dtable + static_cast<int64_t>(current) * hidden + col, V, acc);
+    store_floats<T, V>(dtable + static_cast<int64_t>(current) * hidden + col, acc);
   }
 }
 
-// One workgroup per tile and 64 columns.  If an id begins in the tile and goes on, its partial
-// rows are added: four wavefronts each take a contiguous quarter, added in order.
+// One workgroup per tile and 256 columns.  If an id begins in the tile and goes on, its partial
+// rows are added: kJoinWaves wavefronts take a contiguous part each, added in order.
+constexpr int kJoinWaves = 8;
+
 template <typename T>
-__global__ __launch_bounds__(256) void embedding_join_kernel(const int32_t* __restrict__ ids,
-                                                             int64_t n, int rows,
-                                                             T* __restrict__ dtable, int hidden,
-                                                             float scale,
-                                                             const float* __restrict__ partials) {
-  __shared__ float lds[4][64];
+__global__ __launch_bounds__(64 * kJoinWaves) void embedding_join_kernel(
+    const int32_t* __restrict__ ids, int64_t n, int rows, T* __restrict__ dtable, int hidden,
+    float scale, const float* __restrict__ partials) {
+  __shared__ float lds[kJoinWaves][256];
   const int64_t tile = blockIdx.x;
   const int64_t begin = tile * kTile;
   const int64_t end = begin + kTile;
@@ -331,30 +373,35 @@ __global__ __launch_bounds__(256) void embedding_join_kernel(const int32_t* __re
       high = middle;
   }
   const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
-  const int col = blockIdx.y * 64 + lane;
   const int64_t count = low - tile;  // partial rows, this tile's among them
-  const int64_t per = (count + 3) / 4;
+  const int64_t per = (count + kJoinWaves - 1) / kJoinWaves;
   const int64_t from = wave * per;
   const int64_t to = from + per < count ? from + per : count;
-  float v = 0.0f;
-  if (col < hidden) {
-#pragma unroll 8
-    for (int64_t i = from; i < to; ++i)
-      v += partials[((tile + i) * 2 + (i == 0)) * hidden + col];
-  }
-  lds[wave][lane] = v;
-  __syncthreads();
-  if (wave == 0 && col < hidden) {
 #pragma unroll
-    for (int w = 1; w < 4; ++w) v += lds[w][lane];
+  for (int c = 0; c < 4; ++c) {
+    const int col = blockIdx.y * 256 + c * 64 + lane;
+    float v = 0.0f;
+    if (col < hidden) {
+#pragma unroll 8
+      for (int64_t i = from; i < to; ++i)
+        v += partials[((tile + i) * 2 + (i == 0)) * hidden + col];
+    }
+    lds[wave][c * 64 + lane] = v;
+  }
+  __syncthreads();
+  const int col = blockIdx.y * 256 + threadIdx.x;
+  if (threadIdx.x < 256 && col < hidden) {
+    float v = lds[0][threadIdx.x];
+#pragma unroll
+    for (int w = 1; w < kJoinWaves; ++w) v += lds[w][threadIdx.x];
     dtable[static_cast<int64_t>(id) * hidden + col] = static_cast<T>(v * scale);
   }
 }
 
 // ---- host --------------------------------------------------------------------
 
-int lanes_log2_for(int accesses, int most) {
-  int log2 = 0;
+int lanes_log2_for(int accesses, int least, int most) {
+  int log2 = least;
   while ((1 << log2) < accesses && log2 < most) ++log2;
   return log2;
 }
@@ -366,7 +413,7 @@ int launch_fwd(const void* ids, const void* table, void* out, int64_t n, int row
                float scale, hipStream_t stream) {
   constexpr int N = Chunk<T>::N;
   const bool wide = hidden % N == 0 && (address(table) | address(out)) % 16 == 0;
-  const int log2 = lanes_log2_for(wide ? hidden / N : hidden, 6);
+  const int log2 = lanes_log2_for(wide ? hidden / N : hidden, 0, 6);
   if (n > (kMaxBlocks256 * 256) >> log2) return DFLASH_ERR_TOO_LARGE;
   const int64_t blocks = ((n << log2) + 255) / 256;
   hipLaunchKernelGGL(
@@ -376,6 +423,7 @@ int launch_fwd(const void* ids, const void* table, void* out, int64_t n, int row
   return static_cast<int>(hipGetLastError());
 }
 
+constexpr int kFillBlocks = 2048;  // workgroups that write zeros
 constexpr int64_t kMaxTokens = int64_t{1} << 26;
 constexpr int kMaxHidden = 1 << 20;
 
@@ -406,22 +454,21 @@ int launch_bwd(const void* ids_in, const void* dout_in, void* dtable_in, int64_t
   int bits = 1;
   while (bits < 32 && (int64_t{1} << bits) - 1 < rows) ++bits;
   const int64_t table_bytes = static_cast<int64_t>(rows) * hidden * sizeof(T);
-  // Zeros: 64 bytes a thread at least, one workgroup a CU at most (their LDS holds one a CU).
+  // Zeros: 64 bytes a thread at least, kFillBlocks workgroups at most.
   const int64_t fill = (table_bytes / 16 + 4 * kSortThreads - 1) / (4 * kSortThreads);
-  const int fill_blocks = fill < 1 ? 1 : fill > 256 ? 256 : static_cast<int>(fill);
-  auto* sort = &embedding_sort_kernel<I>;
-  const hipError_t err = ensure_dynamic_lds<&embedding_sort_kernel<I>>(kSortLds);
-  if (err != hipSuccess) return static_cast<int>(err);
-  hipLaunchKernelGGL(sort, dim3(ranges + fill_blocks), dim3(kSortThreads), kSortLds, stream,
-                     static_cast<const I*>(ids_in), n, rows, padding, bits, ranges, ids, tokens,
-                     static_cast<u32x4_t*>(dtable_in), table_bytes);
+  const int fill_blocks = fill < 1 ? 1 : fill > kFillBlocks ? kFillBlocks : static_cast<int>(fill);
+  hipLaunchKernelGGL((embedding_sort_kernel<I>), dim3(ranges + fill_blocks), dim3(kSortThreads), 0,
+                     stream, static_cast<const I*>(ids_in), n, rows, padding, bits, ranges, ids,
+                     tokens, static_cast<u32x4_t*>(dtable_in), table_bytes);
   int rc = static_cast<int>(hipGetLastError());
   if (rc != DFLASH_OK || n == 0) return rc;
   if (ranges > 1) {
     int32_t* merged = reinterpret_cast<int32_t*>(workspace + 2 * w.index_bytes);
     int32_t* merged_tokens = reinterpret_cast<int32_t*>(workspace + 3 * w.index_bytes);
-    hipLaunchKernelGGL(embedding_merge_kernel, dim3(static_cast<uint32_t>((n + 255) / 256)),
-                       dim3(256), 0, stream, ids, tokens, n, merged, merged_tokens);
+    hipLaunchKernelGGL(embedding_merge_kernel,
+                       dim3(static_cast<uint32_t>((n + kMergeThreads - 1) / kMergeThreads)),
+                       dim3(kMergeThreads), kMergeLds, stream, ids, tokens, n, merged,
+                       merged_tokens);
     rc = static_cast<int>(hipGetLastError());
     if (rc != DFLASH_OK) return rc;
     ids = merged;
@@ -432,7 +479,7 @@ int launch_bwd(const void* ids_in, const void* dout_in, void* dtable_in, int64_t
   T* dtable = static_cast<T*>(dtable_in);
   const bool wide = hidden % N == 0 && (address(dout) | address(dtable)) % 16 == 0;
   const int accesses = wide ? hidden / N : hidden;
-  const int log2 = lanes_log2_for(accesses, 5);
+  const int log2 = lanes_log2_for(accesses, 3, 5);
   const int64_t tiles = tiles_of(n);
   hipLaunchKernelGGL((wide ? &embedding_sum_kernel<T, N> : &embedding_sum_kernel<T, 1>),
                      dim3(static_cast<uint32_t>(((tiles << log2) + 255) / 256),
@@ -442,8 +489,8 @@ int launch_bwd(const void* ids_in, const void* dout_in, void* dtable_in, int64_t
   rc = static_cast<int>(hipGetLastError());
   if (rc != DFLASH_OK || tiles == 1) return rc;
   hipLaunchKernelGGL((embedding_join_kernel<T>),
-                     dim3(static_cast<uint32_t>(tiles), (hidden + 63) / 64), dim3(256), 0, stream,
-                     ids, n, rows, dtable, hidden, scale, partials);
+                     dim3(static_cast<uint32_t>(tiles), (hidden + 255) / 256), dim3(64 * kJoinWaves), 0,
+                     stream, ids, n, rows, dtable, hidden, scale, partials);
   return static_cast<int>(hipGetLastError());
 }
 

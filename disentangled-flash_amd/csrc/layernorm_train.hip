@@ -30,6 +30,8 @@ constexpr int kMaxHidden = 8192;
 // Workgroups of the backward pass: each adds up the weight gradients of its rows and writes
 // one fp32 partial row of each.
 constexpr int kMaxPartials = 512;
+// Workgroups of the forward pass.
+constexpr int kMaxForward = 1024;
 
 struct Forward {
   const void *x, *residual, *gamma, *beta;
@@ -51,15 +53,41 @@ struct Backward {
   Dropout drop;
 };
 
+// Sums over groups of LANES (16, 32 or 64) neighbouring lanes, in every lane of the group:
+// within 16 lanes by DPP operands of the additions (neighbour pairs, quads, halves, the whole),
+// across them through scalar registers; nothing passes through LDS, whose latency
+// a butterfly of shuffles takes once a step.
+template <int CTRL>
+__device__ inline float moved(float v) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL,
+                                                               0xF, 0xF, true));
+}
+
+__device__ inline float lane_value(float v, int lane) {
+  return __builtin_bit_cast(float,
+                            __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), lane));
+}
+
+template <int LANES>
+__device__ inline float group_sum(float v) {
+  v += moved<0xB1>(v);   // quad_perm 1, 0, 3, 2
+  v += moved<0x4E>(v);   // quad_perm 2, 3, 0, 1
+  v += moved<0x141>(v);  // row_half_mirror
+  v += moved<0x140>(v);  // row_mirror
+  if constexpr (LANES >= 32) {
+    const float low = lane_value(v, 0) + lane_value(v, 16);
+    const float high = lane_value(v, 32) + lane_value(v, 48);
+    // (LANES = 32: the half of a row that does not exist holds anything, and nobody takes it.)
+    v = LANES == 64 ? low + high : threadIdx.x % 64 < 32 ? low : high;
+  }
+  return v;
+}
+
 // Sum over the LANES lanes of a row.  LANES = 256 (a row a workgroup): every thread calls it.
 template <int LANES, int VALUES>
 __device__ inline void row_sum(float (&v)[VALUES], float (*lds)[VALUES]) {
-  constexpr int kSpan = LANES < 64 ? LANES : 64;
 #pragma unroll
-  for (int m = kSpan / 2; m >= 1; m >>= 1) {
-#pragma unroll
-    for (int i = 0; i < VALUES; ++i) v[i] += __shfl_xor(v[i], m);
-  }
+  for (int i = 0; i < VALUES; ++i) v[i] = group_sum<(LANES < 64 ? LANES : 64)>(v[i]);
   if constexpr (LANES > 64) {
     constexpr int kRowWaves = LANES / 64;
     __syncthreads();  // the values of the call before have been read
@@ -77,102 +105,126 @@ __device__ inline void row_sum(float (&v)[VALUES], float (*lds)[VALUES]) {
   }
 }
 
-// s = drop(x) + r of this lane's chunks (0 past the row's end); `dropped`: their mask.
+// This lane's chunks of the next row to work on: loaded while the row before is worked on, so
+// that the registers of their fp32 values and of the loads in flight are not the same ones.
 template <typename T, int LANES, int CH, bool WIDE>
-__device__ inline void load_sum(const T* x, const T* r, int64_t base, int hidden, int sub,
-                                const Dropout& drop, DropoutKey key,
-                                float (&s)[CH][Chunk<T>::N], uint32_t (&dropped)[CH]) {
-  constexpr int N = Chunk<T>::N;
-  float rv[CH][N];
-#pragma unroll
-  for (int k = 0; k < CH; ++k) {
-    const int col = (sub + LANES * k) * N;
-    const int live = hidden - col;
-    dropped[k] = 0;
-#pragma unroll
-    for (int e = 0; e < N; ++e) s[k][e] = rv[k][e] = 0.0f;
-    if (live > 0) {
-      load_floats<T, N, WIDE>(x + base + col, live, s[k]);
-      if (r) load_floats<T, N, WIDE>(r + base + col, live, rv[k]);
-    }
-  }
-  if (drop.active) {
-#pragma unroll
-    for (int k = 0; k < CH; ++k) {
-      const int col = (sub + LANES * k) * N;
-      if (col < hidden) dropped[k] = dropped_from<N, WIDE>(drop, key, base + col);
-#pragma unroll
-      for (int e = 0; e < N; ++e) s[k][e] = (dropped[k] >> e) & 1 ? 0.0f : s[k][e] * drop.scale;
-    }
-  }
-#pragma unroll
-  for (int k = 0; k < CH; ++k) {
-#pragma unroll
-    for (int e = 0; e < N; ++e) s[k][e] += rv[k][e];
-  }
-}
+struct RowInput {
+  static constexpr int N = Chunk<T>::N;
+  RowChunk<T, N, WIDE> x[CH], r[CH];
 
+  __device__ void load(const T* xs, const T* rs, int64_t base, int hidden, int sub) {
+#pragma unroll
+    for (int k = 0; k < CH; ++k) x[k].load(xs + base, (sub + LANES * k) * N, hidden);
+    if (rs) {
+#pragma unroll
+      for (int k = 0; k < CH; ++k) r[k].load(rs + base, (sub + LANES * k) * N, hidden);
+    }
+  }
+
+  // s = drop(x) + r (0 past the row's end); `dropped`: the masks of the chunks, drawn while
+  // the loads are in flight.
+  __device__ void sum(bool has_r, int64_t base, int hidden, int sub, const Dropout& drop,
+                      DropoutKey key, float (&s)[CH][N], uint32_t (&dropped)[CH]) const {
+    if (drop.active) {
+#pragma unroll
+      for (int k = 0; k < CH; ++k)
+        dropped[k] = dropped_from<N, WIDE>(drop, key, base + (sub + LANES * k) * N);
+#pragma unroll
+      for (int k = 0; k < CH; ++k) {
+        x[k].floats((sub + LANES * k) * N, hidden, s[k]);
+        apply_dropout(drop, dropped[k], s[k]);
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < CH; ++k) x[k].floats((sub + LANES * k) * N, hidden, s[k]);
+    }
+    if (has_r) {
+#pragma unroll
+      for (int k = 0; k < CH; ++k) {
+        float v[N];
+        r[k].floats((sub + LANES * k) * N, hidden, v);
+#pragma unroll
+        for (int e = 0; e < N; ++e) s[k][e] += v[e];
+      }
+    }
+  }
+};
+
+// A workgroup walks its rows, every gridDim-th group of kThreads / LANES rows.  (LANES = 256:
+// the row is the workgroup's, so every thread makes the same rounds.)
 template <typename T, typename W, int LANES, int CH, bool WIDE>
 __global__ __launch_bounds__(kThreads) void layernorm_train_fwd_kernel(Forward a) {
   constexpr int N = Chunk<T>::N;
+  constexpr int kGroups = kThreads / LANES;
   __shared__ float lds[LANES > 64 ? LANES / 64 : 1][1];
   const int sub = threadIdx.x % LANES;
-  const int64_t row =
-      static_cast<int64_t>(blockIdx.x) * (kThreads / LANES) + threadIdx.x / LANES;
+  int64_t row = static_cast<int64_t>(blockIdx.x) * kGroups + threadIdx.x / LANES;
   if (row >= a.rows) return;  // all lanes of a row together
+  const int64_t step = static_cast<int64_t>(gridDim.x) * kGroups;
   const int hidden = a.hidden;
-  const int64_t base = row * hidden;
-  const DropoutKey key = dropout_key(a.drop);
-  float s[CH][N];
-  uint32_t dropped[CH];
-  load_sum<T, LANES, CH, WIDE>(static_cast<const T*>(a.x), static_cast<const T*>(a.residual), base,
-                               hidden, sub, a.drop, key, s, dropped);
-  float sum[1] = {0.0f};
-#pragma unroll
-  for (int k = 0; k < CH; ++k) {
-#pragma unroll
-    for (int e = 0; e < N; ++e) sum[0] += s[k][e];
-  }
-  row_sum<LANES>(sum, lds);
-  // (A division, not a product with 1 / hidden: equal elements have a variance of exactly 0.)
   const float width = static_cast<float>(hidden);
-  const float mean = sum[0] / width;
-  float sq[1] = {0.0f};
+  const T* x = static_cast<const T*>(a.x);
+  const T* r = static_cast<const T*>(a.residual);
+  RowInput<T, LANES, CH, WIDE> in;
+  in.load(x, r, row * hidden, hidden, sub);
+  RowChunk<W, N, WIDE, false> gamma[CH], beta[CH];
 #pragma unroll
   for (int k = 0; k < CH; ++k) {
-    const int col = (sub + LANES * k) * N;
+    gamma[k].load(static_cast<const W*>(a.gamma), (sub + LANES * k) * N, hidden);
+    beta[k].load(static_cast<const W*>(a.beta), (sub + LANES * k) * N, hidden);
+  }
+  const DropoutKey key = dropout_key(a.drop);
+  for (;;) {
+    float s[CH][N];
+    uint32_t dropped[CH];
+    in.sum(r != nullptr, row * hidden, hidden, sub, a.drop, key, s, dropped);
+    const int64_t next = row + step;
+    if (next < a.rows) in.load(x, r, next * hidden, hidden, sub);
+    float sum[1] = {0.0f};
 #pragma unroll
-    for (int e = 0; e < N; ++e) {
-      s[k][e] -= mean;
-      if (WIDE ? col < hidden : col + e < hidden) sq[0] += s[k][e] * s[k][e];
+    for (int k = 0; k < CH; ++k) {
+#pragma unroll
+      for (int e = 0; e < N; ++e) sum[0] += s[k][e];
     }
-  }
-  row_sum<LANES>(sq, lds);
-  const float rstd = rsqrtf(sq[0] / width + a.eps);
-  if (sub == 0 && a.mean) {
-    a.mean[row] = mean;
-    a.rstd[row] = rstd;
-  }
-  const W* gamma = static_cast<const W*>(a.gamma);
-  const W* beta = static_cast<const W*>(a.beta);
+    row_sum<LANES>(sum, lds);
+    // (A division, not a product with 1 / hidden: equal elements have a variance of exactly 0.)
+    const float mean = sum[0] / width;
+    float sq[1] = {0.0f};
 #pragma unroll
-  for (int k = 0; k < CH; ++k) {
-    const int col = (sub + LANES * k) * N;
-    const int live = hidden - col;
-    if (live > 0) {
+    for (int k = 0; k < CH; ++k) {
+      const int col = (sub + LANES * k) * N;
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+        s[k][e] -= mean;
+        const float live = (WIDE ? col : col + e) < hidden ? s[k][e] : 0.0f;
+        sq[0] += live * live;
+      }
+    }
+    row_sum<LANES>(sq, lds);
+    const float rstd = rsqrtf(sq[0] / width + a.eps);
+    if (sub == 0 && a.mean) {
+      a.mean[row] = mean;
+      a.rstd[row] = rstd;
+    }
+#pragma unroll
+    for (int k = 0; k < CH; ++k) {
+      const int col = (sub + LANES * k) * N;
       float g[N], b[N];
-      load_floats<W, N, WIDE>(gamma + col, live, g);
-      load_floats<W, N, WIDE>(beta + col, live, b);
+      gamma[k].renew();
+      beta[k].renew();
+      gamma[k].floats(col, hidden, g);
+      beta[k].floats(col, hidden, b);
 #pragma unroll
       for (int e = 0; e < N; ++e) g[e] = s[k][e] * rstd * g[e] + b[e];
-      store_floats<T, N, WIDE>(static_cast<T*>(a.y) + base + col, live, g);
+      store_chunk<T, N, WIDE>(static_cast<T*>(a.y) + row * hidden, col, hidden, g);
     }
+    if (next >= a.rows) return;
+    row = next;
   }
 }
 
-// A workgroup walks its rows (every gridDim-th group of kThreads / LANES rows) with the sums
-// for dgamma and dbeta of its columns in registers; at the end the lanes that hold
-// the same columns are added in order and one partial row is written.
+// As above, with the sums for dgamma and dbeta of the lane's columns in registers; at the end
+// the lanes that hold the same columns are added in order and one partial row is written.
 template <typename T, typename W, int LANES, int CH, bool WIDE>
 __global__ __launch_bounds__(kThreads) void layernorm_train_bwd_kernel(Backward a) {
   constexpr int N = Chunk<T>::N;
@@ -182,68 +234,72 @@ __global__ __launch_bounds__(kThreads) void layernorm_train_bwd_kernel(Backward 
   const int sub = threadIdx.x % LANES;
   const int group = threadIdx.x / LANES;
   const int hidden = a.hidden;
-  const float inv_h = 1.0f / static_cast<float>(hidden);
-  const DropoutKey key = dropout_key(a.drop);
+  const float width = static_cast<float>(hidden);
+  const T* x = static_cast<const T*>(a.x);
+  const T* r = static_cast<const T*>(a.residual);
   const T* dy = static_cast<const T*>(a.dy);
-  float gamma[CH][N], dgamma[CH][N], dbeta[CH][N];
+  int64_t row = static_cast<int64_t>(blockIdx.x) * kGroups + group;
+  const int64_t step = static_cast<int64_t>(gridDim.x) * kGroups;
+  RowInput<T, LANES, CH, WIDE> in;
+  RowChunk<T, N, WIDE> dys[CH];
+  RowChunk<W, N, WIDE, false> gamma[CH];
+  float mean = 0.0f, rstd = 0.0f;
+  auto load = [&](int64_t at) {
+#pragma unroll
+    for (int k = 0; k < CH; ++k) dys[k].load(dy + at * hidden, (sub + LANES * k) * N, hidden);
+    in.load(x, r, at * hidden, hidden, sub);
+    mean = a.mean[at];
+    rstd = a.rstd[at];
+  };
+  if (row < a.rows) load(row);
+  const DropoutKey key = dropout_key(a.drop);
+  float dgamma[CH][N], dbeta[CH][N];
 #pragma unroll
   for (int k = 0; k < CH; ++k) {
-    const int col = (sub + LANES * k) * N;
+    gamma[k].load(static_cast<const W*>(a.gamma), (sub + LANES * k) * N, hidden);
 #pragma unroll
-    for (int e = 0; e < N; ++e) gamma[k][e] = dgamma[k][e] = dbeta[k][e] = 0.0f;
-    if (col < hidden)
-      load_floats<W, N, WIDE>(static_cast<const W*>(a.gamma) + col, hidden - col, gamma[k]);
+    for (int e = 0; e < N; ++e) dgamma[k][e] = dbeta[k][e] = 0.0f;
   }
-  // (LANES = 256: the row is the workgroup's, so every thread makes the same rounds.)
-  for (int64_t row = static_cast<int64_t>(blockIdx.x) * kGroups + group; row < a.rows;
-       row += static_cast<int64_t>(gridDim.x) * kGroups) {
+  while (row < a.rows) {
     const int64_t base = row * hidden;
     float g[CH][N], xh[CH][N];
     uint32_t dropped[CH];
+    in.sum(r != nullptr, base, hidden, sub, a.drop, key, xh, dropped);
 #pragma unroll
-    for (int k = 0; k < CH; ++k) {
-      const int col = (sub + LANES * k) * N;
-#pragma unroll
-      for (int e = 0; e < N; ++e) g[k][e] = 0.0f;
-      if (col < hidden) load_floats<T, N, WIDE>(dy + base + col, hidden - col, g[k]);
-    }
-    const float mean = a.mean[row], rstd = a.rstd[row];
-    load_sum<T, LANES, CH, WIDE>(static_cast<const T*>(a.x), static_cast<const T*>(a.residual),
-                                 base, hidden, sub, a.drop, key, xh, dropped);
+    for (int k = 0; k < CH; ++k) dys[k].floats((sub + LANES * k) * N, hidden, g[k]);
+    const float row_mean = mean, row_rstd = rstd;
+    row += step;
+    if (row < a.rows) load(row);
     float sums[2] = {0.0f, 0.0f};
 #pragma unroll
     for (int k = 0; k < CH; ++k) {
+      float w[N];
+      gamma[k].renew();
+      gamma[k].floats((sub + LANES * k) * N, hidden, w);
       // (Past the row's end g is 0, so xh adds nothing there.)
 #pragma unroll
       for (int e = 0; e < N; ++e) {
-        xh[k][e] = (xh[k][e] - mean) * rstd;
+        xh[k][e] = (xh[k][e] - row_mean) * row_rstd;
         dbeta[k][e] += g[k][e];
         dgamma[k][e] += g[k][e] * xh[k][e];
-        g[k][e] *= gamma[k][e];
+        g[k][e] *= w[e];
         sums[0] += g[k][e];
         sums[1] += g[k][e] * xh[k][e];
       }
     }
     if (!a.dx && !a.dresidual) continue;
     row_sum<LANES>(sums, lds);
-    const float g_mean = sums[0] * inv_h, gx_mean = sums[1] * inv_h;
+    const float g_mean = sums[0] / width, gx_mean = sums[1] / width;
 #pragma unroll
     for (int k = 0; k < CH; ++k) {
       const int col = (sub + LANES * k) * N;
-      const int live = hidden - col;
-      if (live > 0) {
 #pragma unroll
-        for (int e = 0; e < N; ++e) g[k][e] = rstd * (g[k][e] - g_mean - xh[k][e] * gx_mean);
-        if (a.dresidual)
-          store_floats<T, N, WIDE>(static_cast<T*>(a.dresidual) + base + col, live, g[k]);
-        if (a.dx) {
-          if (a.drop.active) {
-#pragma unroll
-            for (int e = 0; e < N; ++e)
-              g[k][e] = (dropped[k] >> e) & 1 ? 0.0f : g[k][e] * a.drop.scale;
-          }
-          store_floats<T, N, WIDE>(static_cast<T*>(a.dx) + base + col, live, g[k]);
-        }
+      for (int e = 0; e < N; ++e) g[k][e] = row_rstd * (g[k][e] - g_mean - xh[k][e] * gx_mean);
+      if (a.dresidual)
+        store_chunk<T, N, WIDE>(static_cast<T*>(a.dresidual) + base, col, hidden, g[k]);
+      if (a.dx) {
+        if (a.drop.active) apply_dropout(a.drop, dropped[k], g[k]);
+        store_chunk<T, N, WIDE>(static_cast<T*>(a.dx) + base, col, hidden, g[k]);
       }
     }
   }
@@ -278,16 +334,18 @@ __global__ __launch_bounds__(kThreads) void layernorm_train_bwd_kernel(Backward 
   }
 }
 
-// dgamma and dbeta: the partial rows added in order, 16 columns a workgroup, 16 threads a
-// column each adding a contiguous range of the rows.
+// dgamma and dbeta: the partial rows added in order, 16 columns a workgroup, kSlices threads a
+// column, each adding a contiguous range of the rows (8 of 512: one round of loads).
+constexpr int kSlices = 64;
+
 template <typename W>
-__global__ __launch_bounds__(kThreads) void layernorm_weight_grad_kernel(
+__global__ __launch_bounds__(16 * kSlices) void layernorm_weight_grad_kernel(
     const float* __restrict__ partials, int count, int hidden, W* __restrict__ dgamma,
     W* __restrict__ dbeta) {
-  __shared__ float lds[16][17];
+  __shared__ float lds[kSlices][17];
   const int lane = threadIdx.x % 16, slice = threadIdx.x / 16;
   const int col = blockIdx.x * 16 + lane;
-  const int per = (count + 15) / 16;
+  const int per = (count + kSlices - 1) / kSlices;
   const int begin = slice * per;
   const int end = begin + per < count ? begin + per : count;
   float v = 0.0f;
@@ -298,8 +356,7 @@ __global__ __launch_bounds__(kThreads) void layernorm_weight_grad_kernel(
   lds[slice][lane] = v;
   __syncthreads();
   if (slice == 0 && col < 2 * hidden) {
-#pragma unroll
-    for (int i = 1; i < 16; ++i) v += lds[i][lane];
+    for (int i = 1; i < kSlices; ++i) v += lds[i][lane];
     if (col < hidden)
       dgamma[col] = static_cast<W>(v);
     else
@@ -321,7 +378,7 @@ int with_layout(int hidden, bool wide, Go go) {
   DFLASH_LAYOUT(32, 1)
   DFLASH_LAYOUT(32, 2)
   DFLASH_LAYOUT(32, 3)
-  DFLASH_LAYOUT(32, 4)
+  DFLASH_LAYOUT(64, 2)
   DFLASH_LAYOUT(64, 3)
   DFLASH_LAYOUT(64, 4)
   DFLASH_LAYOUT(256, 2)
@@ -339,9 +396,9 @@ int launch_forward(const Forward& a, bool wide, hipStream_t stream) {
     constexpr int kLanes = decltype(lanes)::value, kCh = decltype(ch)::value;
     constexpr int kRows = kThreads / kLanes;
     const int64_t blocks = (a.rows + kRows - 1) / kRows;
-    if (blocks > kMaxBlocks256) return static_cast<int>(DFLASH_ERR_TOO_LARGE);
+    const int count = static_cast<int>(blocks < kMaxForward ? blocks : kMaxForward);
     hipLaunchKernelGGL((layernorm_train_fwd_kernel<T, W, kLanes, kCh, decltype(is_wide)::value>),
-                       dim3(static_cast<uint32_t>(blocks)), dim3(kThreads), 0, stream, a);
+                       dim3(count), dim3(kThreads), 0, stream, a);
     return static_cast<int>(hipGetLastError());
   });
 }
@@ -365,7 +422,7 @@ int launch_backward(const Backward& a, bool wide, hipStream_t stream) {
   }
   if (!a.dgamma) return DFLASH_OK;
   hipLaunchKernelGGL((layernorm_weight_grad_kernel<W>), dim3((2 * a.hidden + 15) / 16),
-                     dim3(kThreads), 0, stream, a.partials, count, a.hidden,
+                     dim3(16 * kSlices), 0, stream, a.partials, count, a.hidden,
                      static_cast<W*>(a.dgamma), static_cast<W*>(a.dbeta));
   return static_cast<int>(hipGetLastError());
 }
