@@ -182,11 +182,26 @@ __device__ void sort_range(const I* __restrict__ ids, int64_t first, int count, 
   }
 }
 
+// Zeros for bytes [begin, end) of dtable, both multiples of 16 but for the table's end (elements
+// are 2 or 4 bytes), by workgroups `block` of `blocks`.
+struct Fill {
+  u32x4_t* table;
+  int64_t begin, end;
+};
+
+template <int THREADS>
+__device__ inline void fill_zeros(const Fill& f, int block, int blocks) {
+  const int64_t at = static_cast<int64_t>(block) * THREADS + threadIdx.x;
+  const int64_t chunks = f.end / 16;
+  for (int64_t i = f.begin / 16 + at; i < chunks; i += static_cast<int64_t>(blocks) * THREADS)
+    f.table[i] = u32x4_t{0, 0, 0, 0};
+  if (at < (f.end - chunks * 16) / 2) reinterpret_cast<uint16_t*>(f.table + chunks)[at] = 0;
+}
+
 template <typename I>
 __global__ __launch_bounds__(kSortThreads) void embedding_sort_kernel(
     const I* __restrict__ ids, int64_t n, int rows, int64_t padding, int bits, int ranges,
-    int32_t* __restrict__ sorted_ids, int32_t* __restrict__ sorted_tokens,
-    u32x4_t* __restrict__ table, int64_t table_bytes) {
+    int32_t* __restrict__ sorted_ids, int32_t* __restrict__ sorted_tokens, Fill fill) {
   __shared__ SortLds lds;
   if (static_cast<int>(blockIdx.x) < ranges) {
     const int64_t first = static_cast<int64_t>(blockIdx.x) * kSortTokens;
@@ -194,14 +209,7 @@ __global__ __launch_bounds__(kSortThreads) void embedding_sort_kernel(
     sort_range(ids, first, count, rows, padding, bits, sorted_ids, sorted_tokens, lds);
     return;
   }
-  const int64_t chunks = table_bytes / 16;
-  const int64_t step = static_cast<int64_t>(gridDim.x - ranges) * kSortThreads;
-  const int64_t at = static_cast<int64_t>(blockIdx.x - ranges) * kSortThreads + threadIdx.x;
-  for (int64_t i = at; i < chunks; i += step)
-    __builtin_nontemporal_store(u32x4_t{0, 0, 0, 0}, table + i);
-  // The last bytes of a table that is not whole chunks (elements are 2 or 4 bytes).
-  const int64_t rest = (table_bytes - chunks * 16) / 2;
-  if (at < rest) reinterpret_cast<uint16_t*>(table + chunks)[at] = 0;
+  fill_zeros<kSortThreads>(fill, blockIdx.x - ranges, gridDim.x - ranges);
 }
 
 // ---- merge -------------------------------------------------------------------
@@ -211,13 +219,19 @@ __global__ __launch_bounds__(kSortThreads) void embedding_sort_kernel(
 // LDS kMergeRanges at a time, where each search takes 11 steps and the searches of one
 // token are independent; from L2 the steps alone would take their latency 11 times over.
 constexpr int kMergeRanges = 8;
-constexpr int kMergeThreads = 512;
-constexpr int kMergeLds = kMergeRanges * kSortTokens * 4;
+constexpr int kMergeThreads = 256;
 
 __global__ __launch_bounds__(kMergeThreads) void embedding_merge_kernel(
     const int32_t* __restrict__ ids, const int32_t* __restrict__ tokens, int64_t n,
-    int32_t* __restrict__ merged_ids, int32_t* __restrict__ merged_tokens) {
-  extern __shared__ int32_t lds[];
+    int32_t* __restrict__ merged_ids, int32_t* __restrict__ merged_tokens, int blocks, Fill fill) {
+  typedef int32_t Four __attribute__((ext_vector_type(4)));
+  constexpr int kHeld = kMergeRanges * kSortTokens;
+  __shared__ Four lds4[kHeld / 4];
+  int32_t* lds = reinterpret_cast<int32_t*>(lds4);
+  if (static_cast<int>(blockIdx.x) >= blocks) {
+    fill_zeros<kMergeThreads>(fill, blockIdx.x - blocks, gridDim.x - blocks);
+    return;
+  }
   const int64_t i = static_cast<int64_t>(blockIdx.x) * kMergeThreads + threadIdx.x;
   const int32_t id = i < n ? ids[i] : 0;
   const int64_t own = i / kSortTokens;
@@ -225,13 +239,17 @@ __global__ __launch_bounds__(kMergeThreads) void embedding_merge_kernel(
   const int64_t ranges = (n + kSortTokens - 1) / kSortTokens;
   for (int64_t r0 = 0; r0 < ranges; r0 += kMergeRanges) {
     const int64_t first = r0 * kSortTokens;
-    const int64_t held = n - first < kMergeRanges * kSortTokens ? n - first
-                                                               : kMergeRanges * kSortTokens;
+    const int held = n - first < kHeld ? static_cast<int>(n - first) : kHeld;
     __syncthreads();  // the ranges before have been searched
-    for (int j = threadIdx.x * 4; j < kMergeRanges * kSortTokens; j += kMergeThreads * 4) {
+#pragma unroll
+    for (int k = 0; k < kHeld / 4 / kMergeThreads; ++k) {
+      const int j = (k * kMergeThreads + threadIdx.x) * 4;
+      // (The array is padded to 256 bytes: whole accesses; past the end above all ids.)
+      Four v = j < held ? *reinterpret_cast<const Four*>(ids + first + j) : Four{};
 #pragma unroll
       for (int e = 0; e < 4; ++e)
-        lds[j + e] = j + e < held ? ids[first + j + e] : INT32_MAX;  // past the end: above all
+        if (j + e >= held) v[e] = INT32_MAX;
+      lds4[j / 4] = v;
     }
     __syncthreads();
     int before[kMergeRanges];
@@ -363,17 +381,14 @@ __global__ __launch_bounds__(64 * kJoinWaves) void embedding_join_kernel(
   const int32_t id = ids[end - 1];
   if (id >= rows || ids[end] != id) return;
   if (ids[begin] == id && begin > 0 && ids[begin - 1] == id) return;  // began earlier
-  // Tiles whose first token is of the id: [tile + 1, low).
-  int64_t low = tile + 2, high = (n + kTile - 1) / kTile;
-  while (low < high) {
-    const int64_t middle = (low + high) / 2;
-    if (ids[middle * kTile] == id)
-      low = middle + 1;
-    else
-      high = middle;
+  // Tiles whose first token is of the id, [tile + 1, tile + count): every thread looks at one.
+  const int64_t tiles = (n + kTile - 1) / kTile;
+  int64_t count = 1;  // partial rows, this tile's among them
+  for (int found = 64 * kJoinWaves; found == 64 * kJoinWaves; count += found) {
+    const int64_t other = tile + count + threadIdx.x;
+    found = __syncthreads_count(other < tiles && ids[other * kTile] == id);
   }
   const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
-  const int64_t count = low - tile;  // partial rows, this tile's among them
   const int64_t per = (count + kJoinWaves - 1) / kJoinWaves;
   const int64_t from = wave * per;
   const int64_t to = from + per < count ? from + per : count;
@@ -423,9 +438,15 @@ int launch_fwd(const void* ids, const void* table, void* out, int64_t n, int row
   return static_cast<int>(hipGetLastError());
 }
 
-constexpr int kFillBlocks = 2048;  // workgroups that write zeros
+constexpr int kFillBlocks = 512;  // workgroups that write zeros
 constexpr int64_t kMaxTokens = int64_t{1} << 26;
 constexpr int kMaxHidden = 1 << 20;
+
+// Workgroups that write `bytes` of zeros: 64 bytes a thread, kFillBlocks at most, one at least.
+int fill_blocks(int64_t bytes, int threads) {
+  const int64_t blocks = (bytes + 64 * threads - 1) / (64 * threads);
+  return blocks < 1 ? 1 : blocks > kFillBlocks ? kFillBlocks : static_cast<int>(blocks);
+}
 
 int64_t tiles_of(int64_t n) { return (n + kTile - 1) / kTile; }
 int64_t ranges_of(int64_t n) { return (n + kSortTokens - 1) / kSortTokens; }
@@ -454,21 +475,25 @@ int launch_bwd(const void* ids_in, const void* dout_in, void* dtable_in, int64_t
   int bits = 1;
   while (bits < 32 && (int64_t{1} << bits) - 1 < rows) ++bits;
   const int64_t table_bytes = static_cast<int64_t>(rows) * hidden * sizeof(T);
-  // Zeros: 64 bytes a thread at least, kFillBlocks workgroups at most.
-  const int64_t fill = (table_bytes / 16 + 4 * kSortThreads - 1) / (4 * kSortThreads);
-  const int fill_blocks = fill < 1 ? 1 : fill > kFillBlocks ? kFillBlocks : static_cast<int>(fill);
-  hipLaunchKernelGGL((embedding_sort_kernel<I>), dim3(ranges + fill_blocks), dim3(kSortThreads), 0,
+  // The zeros go with the sort, and a part of them with the merge if there is one, so that
+  // neither has the card to itself.
+  const int64_t first_part = ranges > 1 ? table_bytes / 5 * 3 / 16 * 16 : table_bytes;
+  const Fill fill{static_cast<u32x4_t*>(dtable_in), 0, first_part};
+  hipLaunchKernelGGL((embedding_sort_kernel<I>),
+                     dim3(ranges + fill_blocks(first_part, kSortThreads)), dim3(kSortThreads), 0,
                      stream, static_cast<const I*>(ids_in), n, rows, padding, bits, ranges, ids,
-                     tokens, static_cast<u32x4_t*>(dtable_in), table_bytes);
+                     tokens, fill);
   int rc = static_cast<int>(hipGetLastError());
   if (rc != DFLASH_OK || n == 0) return rc;
   if (ranges > 1) {
     int32_t* merged = reinterpret_cast<int32_t*>(workspace + 2 * w.index_bytes);
     int32_t* merged_tokens = reinterpret_cast<int32_t*>(workspace + 3 * w.index_bytes);
+    const Fill rest{static_cast<u32x4_t*>(dtable_in), first_part, table_bytes};
+    const int blocks = static_cast<int>((n + kMergeThreads - 1) / kMergeThreads);
     hipLaunchKernelGGL(embedding_merge_kernel,
-                       dim3(static_cast<uint32_t>((n + kMergeThreads - 1) / kMergeThreads)),
-                       dim3(kMergeThreads), kMergeLds, stream, ids, tokens, n, merged,
-                       merged_tokens);
+                       dim3(blocks + fill_blocks(table_bytes - first_part, kMergeThreads)),
+                       dim3(kMergeThreads), 0, stream, ids, tokens, n, merged, merged_tokens,
+                       blocks, rest);
     rc = static_cast<int>(hipGetLastError());
     if (rc != DFLASH_OK) return rc;
     ids = merged;

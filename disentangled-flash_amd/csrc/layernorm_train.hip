@@ -19,17 +19,19 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include "device_common.h"
 #include "dflash.h"
 #include "training.h"
 
 namespace dflash {
 namespace {
 
-constexpr int kThreads = 256;
 constexpr int kMaxHidden = 8192;
 // Workgroups of the backward pass: each adds up the weight gradients of its rows and writes
 // one fp32 partial row of each.
 constexpr int kMaxPartials = 512;
+// Up to this many rows one workgroup takes them all, and there are no partial rows to add.
+constexpr int kAloneRows = 32;
 // Workgroups of the forward pass.
 constexpr int kMaxForward = 1024;
 
@@ -90,12 +92,13 @@ __device__ inline void row_sum(float (&v)[VALUES], float (*lds)[VALUES]) {
   for (int i = 0; i < VALUES; ++i) v[i] = group_sum<(LANES < 64 ? LANES : 64)>(v[i]);
   if constexpr (LANES > 64) {
     constexpr int kRowWaves = LANES / 64;
-    __syncthreads();  // the values of the call before have been read
+    // (Barriers that order LDS only: the next row's loads stay in flight.)
+    lds_barrier();  // the values of the call before have been read
     if (threadIdx.x % 64 == 0) {
 #pragma unroll
       for (int i = 0; i < VALUES; ++i) lds[threadIdx.x / 64][i] = v[i];
     }
-    __syncthreads();
+    lds_barrier();
 #pragma unroll
     for (int i = 0; i < VALUES; ++i) {
       v[i] = lds[0][i];
@@ -107,10 +110,12 @@ __device__ inline void row_sum(float (&v)[VALUES], float (*lds)[VALUES]) {
 
 // This lane's chunks of the next row to work on: loaded while the row before is worked on, so
 // that the registers of their fp32 values and of the loads in flight are not the same ones.
-template <typename T, int LANES, int CH, bool WIDE>
+// LAST: nobody reads them after the kernel (the forward pass's rows are read again by the
+// backward pass).
+template <typename T, int LANES, int CH, bool WIDE, bool LAST>
 struct RowInput {
   static constexpr int N = Chunk<T>::N;
-  RowChunk<T, N, WIDE> x[CH], r[CH];
+  RowChunk<T, N, WIDE, LAST> x[CH], r[CH];
 
   __device__ void load(const T* xs, const T* rs, int64_t base, int hidden, int sub) {
 #pragma unroll
@@ -165,7 +170,7 @@ __global__ __launch_bounds__(kThreads) void layernorm_train_fwd_kernel(Forward a
   const float width = static_cast<float>(hidden);
   const T* x = static_cast<const T*>(a.x);
   const T* r = static_cast<const T*>(a.residual);
-  RowInput<T, LANES, CH, WIDE> in;
+  RowInput<T, LANES, CH, WIDE, false> in;
   in.load(x, r, row * hidden, hidden, sub);
   RowChunk<W, N, WIDE, false> gamma[CH], beta[CH];
 #pragma unroll
@@ -240,8 +245,8 @@ __global__ __launch_bounds__(kThreads) void layernorm_train_bwd_kernel(Backward 
   const T* dy = static_cast<const T*>(a.dy);
   int64_t row = static_cast<int64_t>(blockIdx.x) * kGroups + group;
   const int64_t step = static_cast<int64_t>(gridDim.x) * kGroups;
-  RowInput<T, LANES, CH, WIDE> in;
-  RowChunk<T, N, WIDE> dys[CH];
+  RowInput<T, LANES, CH, WIDE, true> in;
+  RowChunk<T, N, WIDE, true> dys[CH];
   RowChunk<W, N, WIDE, false> gamma[CH];
   float mean = 0.0f, rstd = 0.0f;
   auto load = [&](int64_t at) {
@@ -251,7 +256,11 @@ __global__ __launch_bounds__(kThreads) void layernorm_train_bwd_kernel(Backward 
     mean = a.mean[at];
     rstd = a.rstd[at];
   };
-  if (row < a.rows) load(row);
+  // Narrow rows are loaded one ahead (1024 fp16, no dropout, 16384 rows: 27.5 -> 24.2 us); where
+  // their registers cost wavefronts, not (1536 fp32: 98.7 ahead, 89.6 not; 1536 bf16 52.9,
+  // 52.0; 768 bf16 30.2, 29.7).
+  constexpr bool kAhead = WIDE && LANES <= 64 && CH <= 2;
+  if (kAhead && row < a.rows) load(row);
   const DropoutKey key = dropout_key(a.drop);
   float dgamma[CH][N], dbeta[CH][N];
 #pragma unroll
@@ -261,6 +270,7 @@ __global__ __launch_bounds__(kThreads) void layernorm_train_bwd_kernel(Backward 
     for (int e = 0; e < N; ++e) dgamma[k][e] = dbeta[k][e] = 0.0f;
   }
   while (row < a.rows) {
+    if (!kAhead) load(row);
     const int64_t base = row * hidden;
     float g[CH][N], xh[CH][N];
     uint32_t dropped[CH];
@@ -269,7 +279,7 @@ __global__ __launch_bounds__(kThreads) void layernorm_train_bwd_kernel(Backward 
     for (int k = 0; k < CH; ++k) dys[k].floats((sub + LANES * k) * N, hidden, g[k]);
     const float row_mean = mean, row_rstd = rstd;
     row += step;
-    if (row < a.rows) load(row);
+    if (kAhead && row < a.rows) load(row);
     float sums[2] = {0.0f, 0.0f};
 #pragma unroll
     for (int k = 0; k < CH; ++k) {
@@ -304,7 +314,14 @@ __global__ __launch_bounds__(kThreads) void layernorm_train_bwd_kernel(Backward 
     }
   }
   if (!a.dgamma) return;
+  // A workgroup alone has the whole sums.
   float* out = a.partials + static_cast<int64_t>(blockIdx.x) * 2 * hidden;
+  auto put = [&](int which, int col, float v) {
+    if (gridDim.x > 1)
+      out[which * hidden + col] = v;
+    else
+      static_cast<W*>(which == 0 ? a.dgamma : a.dbeta)[col] = static_cast<W>(v);
+  };
 #pragma unroll
   for (int which = 0; which < 2; ++which) {
     float(&acc)[CH][N] = which == 0 ? dgamma : dbeta;
@@ -320,7 +337,7 @@ __global__ __launch_bounds__(kThreads) void layernorm_train_bwd_kernel(Backward 
         float v = part[0][col];
 #pragma unroll
         for (int i = 1; i < kGroups; ++i) v += part[i][col];
-        out[which * hidden + col] = v;
+        put(which, col, v);
       }
     } else {
 #pragma unroll
@@ -328,7 +345,7 @@ __global__ __launch_bounds__(kThreads) void layernorm_train_bwd_kernel(Backward 
         const int col = (sub + LANES * k) * N;
 #pragma unroll
         for (int e = 0; e < N; ++e)
-          if (col + e < hidden) out[which * hidden + col + e] = acc[k][e];
+          if (col + e < hidden) put(which, col + e, acc[k][e]);
       }
     }
   }
@@ -403,7 +420,9 @@ int launch_forward(const Forward& a, bool wide, hipStream_t stream) {
   });
 }
 
-int64_t partial_rows(int64_t rows) { return rows < kMaxPartials ? rows : kMaxPartials; }
+int64_t partial_rows(int64_t rows) {
+  return rows <= kAloneRows ? 0 : rows < kMaxPartials ? rows : kMaxPartials;
+}
 
 template <typename T, typename W>
 int launch_backward(const Backward& a, bool wide, hipStream_t stream) {
@@ -414,13 +433,14 @@ int launch_backward(const Backward& a, bool wide, hipStream_t stream) {
       constexpr int kRows = kThreads / kLanes;
       const int64_t blocks = (a.rows + kRows - 1) / kRows;
       count = static_cast<int>(blocks < kMaxPartials ? blocks : kMaxPartials);
+      if (a.rows <= kAloneRows) count = 1;
       hipLaunchKernelGGL((layernorm_train_bwd_kernel<T, W, kLanes, kCh, decltype(is_wide)::value>),
                          dim3(count), dim3(kThreads), 0, stream, a);
       return static_cast<int>(hipGetLastError());
     });
     if (rc != DFLASH_OK) return rc;
   }
-  if (!a.dgamma) return DFLASH_OK;
+  if (!a.dgamma || count == 1) return DFLASH_OK;
   hipLaunchKernelGGL((layernorm_weight_grad_kernel<W>), dim3((2 * a.hidden + 15) / 16),
                      dim3(16 * kSlices), 0, stream, a.partials, count, a.hidden,
                      static_cast<W*>(a.dgamma), static_cast<W*>(a.dbeta));
@@ -504,7 +524,7 @@ extern "C" int dflash_dropout_layernorm_bwd(
     if (rows_or % sizeof(T) != 0 || weights_or % sizeof(W) != 0 ||
         (address(mean) | address(rstd) | address(workspace)) % 4 != 0 || address(rng) % 8 != 0)
       return static_cast<int>(DFLASH_ERR_ALIGN);
-    if (dgamma && rows > 0) {
+    if (dgamma && partial_rows(rows) > 0) {
       if (!workspace) return static_cast<int>(DFLASH_ERR_NULL);
       if (workspace_bytes < dflash_dropout_layernorm_bwd_workspace_bytes(rows, hidden))
         return static_cast<int>(DFLASH_ERR_WORKSPACE);

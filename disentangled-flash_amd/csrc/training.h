@@ -121,7 +121,7 @@ inline bool make_dropout(double p, const int64_t* rng, uint32_t site, Dropout& d
 // 16-byte boundaries.  Otherwise element loads.  Either way every load is made, past the row's
 // end from a place inside it (a branch would wait for each load by itself);
 // floats() puts the zeros there.  STREAM: read once (past the L2's other lines).
-template <typename T, int N, bool WIDE, bool STREAM = true>
+template <typename T, int N, bool WIDE, bool STREAM = false>
 struct RowChunk {
   static constexpr int kPieces = N / Chunk<T>::N;  // 2: fp32 weights beside 16-bit rows
   typename Chunk<T>::type v[kPieces];
