@@ -1,8 +1,10 @@
-"""Build ``libdflash.so`` for gfx950 with hipcc (no torch extension machinery).
+"""Build ``libdflash.so`` for gfx950 with hipcc, and ``libdflash_torch.so`` beside it.
 
 Every ``*.hip`` file in this directory is compiled to an object in parallel,
 then linked into ``disentangled_flash/libdflash.so`` next to the Python package
-so the in-tree library travels with the source tree.
+so the in-tree library travels with the source tree.  ``torch_ops.cpp``, host code against
+the installed torch's headers (the training operators' autograd nodes), becomes a library of its
+own: ``libdflash.so`` knows nothing of torch.
 
     python disentangled-flash_amd/csrc/build.py [--jobs N] [--verbose]
 """
@@ -23,6 +25,7 @@ PACKAGE_ROOT = CSRC.parent
 REPO_ROOT = PACKAGE_ROOT.parent
 INCLUDE = REPO_ROOT / "include"
 OUTPUT = PACKAGE_ROOT / "disentangled_flash" / "libdflash.so"
+TORCH_OUTPUT = OUTPUT.with_name("libdflash_torch.so")
 ARCH = "gfx950"
 
 # -packed-fp32-ops: keep hipcc from emitting packed fp32 VALU instructions.
@@ -61,8 +64,31 @@ def _run(command: list[str], verbose: bool) -> None:
 
 
 def build(jobs: int | None = None, verbose: bool = False, output: Path = OUTPUT) -> Path:
-    _build_library(sorted(CSRC.glob("*.hip")), output, jobs, verbose)
+    with ThreadPoolExecutor(max_workers=1) as pool:
+        torch_ops = pool.submit(_build_torch_ops, output.with_name(TORCH_OUTPUT.name), verbose)
+        _build_library(sorted(CSRC.glob("*.hip")), output, jobs, verbose)
+        torch_ops.result()
     return output
+
+
+def _build_torch_ops(output: Path, verbose: bool) -> None:
+    import torch
+
+    root = Path(torch.__file__).resolve().parent
+    compiler = shutil.which("g++") or "g++"
+    rocm = Path(hipcc()).resolve().parent.parent
+    with tempfile.TemporaryDirectory(prefix="dflash_build_") as tmp:
+        staged = Path(tmp) / output.name
+        _run([compiler, "-std=c++17", "-O2", "-fPIC", "-fvisibility=hidden", "-shared",
+              "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
+              f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", f"-I{INCLUDE}",
+              "-isystem", str(root / "include"),
+              "-isystem", str(root / "include" / "torch" / "csrc" / "api" / "include"),
+              "-isystem", str(rocm / "include"), str(CSRC / "torch_ops.cpp"), "-o", str(staged),
+              f"-L{root / 'lib'}", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_hip", "-ldl"],
+             verbose)
+        output.parent.mkdir(parents=True, exist_ok=True)
+        shutil.move(str(staged), str(output))
 
 
 def _build_library(sources: list[Path], output: Path, jobs: int | None, verbose: bool) -> None:

@@ -20,6 +20,7 @@ from pathlib import Path
 import torch  # noqa: F401  (load torch's HIP runtime first)
 
 LIBRARY_NAME = "libdflash.so"
+TORCH_LIBRARY_NAME = "libdflash_torch.so"
 ABI_VERSION = 8
 
 ERR_WORKSPACE = -7  # DFLASH_ERR_WORKSPACE
@@ -55,6 +56,7 @@ ENCODER_LAYER_FORMAT = struct.Struct("@15P3f6i0P")
 
 _handle: ctypes.CDLL | None = None
 _load_error: str | None = None
+_torch_ops_loaded = False
 
 
 def library_path() -> Path:
@@ -210,6 +212,27 @@ def load() -> ctypes.CDLL:
         raise RuntimeError(f"{path} has ABI version {version}, expected {ABI_VERSION}")
     _handle = lib
     return lib
+
+
+def load_torch_ops() -> None:
+    """Load ``libdflash_torch.so`` (the training operators' autograd nodes) once and bind it to
+    the library of :func:`load`; raise ``RuntimeError`` if either is unusable."""
+
+    global _torch_ops_loaded
+    if _torch_ops_loaded:
+        return
+    load()
+    path = library_path().with_name(TORCH_LIBRARY_NAME)
+    if not path.exists():
+        raise RuntimeError(
+            f"{path} is missing: build the HIP library first "
+            "(python __graft_entry__.py, or python disentangled-flash_amd/csrc/build.py)")
+    try:
+        torch.ops.load_library(str(path))
+    except OSError as error:
+        raise RuntimeError(f"cannot load {path}: {error}") from error
+    torch.ops.disentangled_flash.bind_library(str(library_path()))
+    _torch_ops_loaded = True
 
 
 def is_available() -> bool:

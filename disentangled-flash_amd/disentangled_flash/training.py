@@ -21,184 +21,82 @@ its index in the flattened tensor, ``rng`` and ``site`` alone, whatever the dtyp
 rounded to a multiple of 2^-16 (to 0 and 1 only where it is 0 or 1), and kept elements are
 divided by the rounded probability of being kept.  A dropped element is 0 whatever it held.
 
-Work is launched on torch's current stream of the inputs' device.  Second derivatives are not
-implemented (they raise).  Inputs that are not contiguous are copied first.
+Work is launched on torch's current stream of the inputs' device.  Second derivatives raise,
+but for dropout's.  Inputs that are not contiguous are copied first.
 """
 
 from __future__ import annotations
 
-import contextlib
 from typing import Any
 
 import torch
 from torch import nn
-from torch.autograd.function import once_differentiable
-from torch.nn import functional as F
 
 from . import _lib
 
 MAX_HIDDEN = 8192  # widest row of layer_norm
 
 
-def _device_of(tensor: torch.Tensor):
-    """Makes ``tensor``'s device the current one (the library launches on the current device)."""
+class _Ops:
+    """The torch operators (``csrc/torch_ops.cpp``), loaded at the first call."""
 
-    if tensor.device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(tensor.device)
-
-
-def _pointer(tensor: torch.Tensor | None) -> int | None:
-    return None if tensor is None else tensor.data_ptr()
-
-
-# ---- ops: one library call each ----------------------------------------------------
+    def __getattr__(self, name: str) -> Any:
+        _lib.load_torch_ops()
+        _register_fakes()
+        namespace = torch.ops.disentangled_flash
+        for op in ("dropout", "dropout_layernorm", "embedding_lookup"):
+            setattr(self, op, getattr(namespace, op).default)
+        return self.__dict__[name]
 
 
-@_lib.hip_op("disentangled_flash::dropout")
-def dropout_op(x: torch.Tensor, rng: torch.Tensor, p: float, site: int) -> torch.Tensor:
-    """``x`` with the elements of ``(rng, site)`` dropped; ``x`` contiguous."""
-
-    lib = _lib.load()
-    out = torch.empty_like(x)
-    with _device_of(x):
-        code = lib.dflash_dropout(x.data_ptr(), out.data_ptr(), x.numel(), p, rng.data_ptr(), site,
-                                  _lib.DTYPE_CODES[x.dtype], _lib.current_stream_handle(x.device))
-    _lib.check(code, "dflash_dropout")
-    return out
+_ops = _Ops()
 
 
-@dropout_op.register_fake
-def _dropout_fake(x, rng, p, site):
-    return torch.empty_like(x)
+def _register_fakes() -> None:
+    """Shapes for tracing (torch.compile, export, FakeTensorMode)."""
 
+    fake = torch.library.register_fake
 
-@_lib.hip_op("disentangled_flash::dropout_layernorm")
-def dropout_layernorm_op(
-    x: torch.Tensor, residual: torch.Tensor | None, weight: torch.Tensor, bias: torch.Tensor,
-    rng: torch.Tensor | None, eps: float, p: float, site: int, statistics: bool
-) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
-    """``(y, mean, rstd)``; the statistics are empty unless asked for."""
+    @fake("disentangled_flash::dropout")
+    def _(x, rng, p, site):
+        return torch.empty_like(x)
 
-    lib = _lib.load()
-    hidden = x.shape[-1]
-    rows = x.numel() // hidden
-    y = torch.empty_like(x)
-    kept = torch.empty((2, rows if statistics else 0), device=x.device, dtype=torch.float32)
-    mean, rstd = kept[0], kept[1]
-    with _device_of(x):
-        code = lib.dflash_dropout_layernorm_fwd(
-            x.data_ptr(), _pointer(residual), weight.data_ptr(), bias.data_ptr(), y.data_ptr(),
-            mean.data_ptr() if statistics else None, rstd.data_ptr() if statistics else None,
-            rows, hidden, eps, p, _pointer(rng), site, _lib.DTYPE_CODES[x.dtype],
-            _lib.DTYPE_CODES[weight.dtype], _lib.current_stream_handle(x.device))
-    _lib.check(code, "dflash_dropout_layernorm_fwd")
-    return y, mean, rstd
+    @fake("disentangled_flash::dropout_layernorm")
+    def _(x, residual, weight, bias, rng, eps, p, site):
+        return torch.empty_like(x)
 
+    @fake("disentangled_flash::dropout_layernorm_train")
+    def _(x, residual, weight, bias, rng, eps, p, site):
+        return (torch.empty_like(x),
+                x.new_empty((2, x.numel() // x.shape[-1]), dtype=torch.float32))
 
-@dropout_layernorm_op.register_fake
-def _dropout_layernorm_fake(x, residual, weight, bias, rng, eps, p, site, statistics):
-    rows = x.numel() // x.shape[-1] if statistics else 0
-    mean, rstd = (x.new_empty(rows, dtype=torch.float32) for _ in range(2))
-    return torch.empty_like(x), mean, rstd
+    @fake("disentangled_flash::dropout_layernorm_backward")
+    def _(dy, x, residual, weight, statistics, rng, p, site, want_x, want_residual, want_weights):
+        hidden = x.shape[-1] if want_weights else 0
+        return (torch.empty_like(x) if want_x else x.new_empty(0),
+                torch.empty_like(x) if want_residual else x.new_empty(0),
+                weight.new_empty(hidden), weight.new_empty(hidden))
 
+    @fake("disentangled_flash::embedding_lookup")
+    def _(ids, table, scale, padding):
+        return table.new_empty(ids.shape + (table.shape[1],))
 
-@_lib.hip_op("disentangled_flash::dropout_layernorm_backward")
-def dropout_layernorm_backward_op(
-    dy: torch.Tensor, x: torch.Tensor, residual: torch.Tensor | None, weight: torch.Tensor,
-    mean: torch.Tensor, rstd: torch.Tensor, rng: torch.Tensor | None, p: float, site: int,
-    want_x: bool, want_residual: bool, want_weights: bool
-) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
-    """``(dx, dresidual, dweight, dbias)``; those not wanted are empty."""
-
-    lib = _lib.load()
-    hidden = x.shape[-1]
-    rows = x.numel() // hidden
-    dx = torch.empty_like(x) if want_x else x.new_empty(0)
-    dresidual = torch.empty_like(x) if want_residual else x.new_empty(0)
-    dweight = weight.new_empty(hidden if want_weights else 0)
-    dbias = weight.new_empty(hidden if want_weights else 0)
-    size = lib.dflash_dropout_layernorm_bwd_workspace_bytes(rows, hidden) if want_weights else 0
-    workspace = torch.empty(size, device=x.device, dtype=torch.uint8)
-    with _device_of(x):
-        code = lib.dflash_dropout_layernorm_bwd(
-            dy.data_ptr(), x.data_ptr(), _pointer(residual), weight.data_ptr(), mean.data_ptr(),
-            rstd.data_ptr(), dx.data_ptr() if want_x else None,
-            dresidual.data_ptr() if want_residual else None,
-            dweight.data_ptr() if want_weights else None,
-            dbias.data_ptr() if want_weights else None, rows, hidden, p, _pointer(rng), site,
-            _lib.DTYPE_CODES[x.dtype], _lib.DTYPE_CODES[weight.dtype], workspace.data_ptr(), size,
-            _lib.current_stream_handle(x.device))
-    _lib.check(code, "dflash_dropout_layernorm_bwd")
-    return dx, dresidual, dweight, dbias
-
-
-@dropout_layernorm_backward_op.register_fake
-def _dropout_layernorm_backward_fake(dy, x, residual, weight, mean, rstd, rng, p, site, want_x,
-                                     want_residual, want_weights):
-    hidden = x.shape[-1] if want_weights else 0
-    return (torch.empty_like(x) if want_x else x.new_empty(0),
-            torch.empty_like(x) if want_residual else x.new_empty(0),
-            weight.new_empty(hidden), weight.new_empty(hidden))
-
-
-@_lib.hip_op("disentangled_flash::embedding_lookup")
-def embedding_op(input_ids: torch.Tensor, weight: torch.Tensor, scale: float) -> torch.Tensor:
-    """``scale * weight[input_ids]``; both contiguous."""
-
-    lib = _lib.load()
-    rows, hidden = weight.shape
-    out = weight.new_empty(*input_ids.shape, hidden)
-    with _device_of(weight):
-        code = lib.dflash_embedding_fwd(
-            input_ids.data_ptr(), weight.data_ptr(), out.data_ptr(), input_ids.numel(), rows,
-            hidden, scale, input_ids.element_size(), _lib.DTYPE_CODES[weight.dtype],
-            _lib.current_stream_handle(weight.device))
-    _lib.check(code, "dflash_embedding_fwd")
-    return out
-
-
-@embedding_op.register_fake
-def _embedding_fake(input_ids, weight, scale):
-    return weight.new_empty(*input_ids.shape, weight.shape[1])
-
-
-@_lib.hip_op("disentangled_flash::embedding_gradient")
-def embedding_gradient_op(dy: torch.Tensor, input_ids: torch.Tensor, rows: int, scale: float,
-                          padding_idx: int) -> torch.Tensor:
-    """The table's dense gradient ``[rows, H]``; ``padding_idx`` -1: none."""
-
-    lib = _lib.load()
-    hidden = dy.shape[-1]
-    tokens = input_ids.numel()
-    out = dy.new_empty(rows, hidden)
-    size = lib.dflash_embedding_bwd_workspace_bytes(tokens, hidden)
-    workspace = torch.empty(size, device=dy.device, dtype=torch.uint8)
-    with _device_of(dy):
-        code = lib.dflash_embedding_bwd(
-            input_ids.data_ptr(), dy.data_ptr(), out.data_ptr(), tokens, rows, hidden, scale,
-            padding_idx, input_ids.element_size(), _lib.DTYPE_CODES[dy.dtype],
-            workspace.data_ptr(), size, _lib.current_stream_handle(dy.device))
-    _lib.check(code, "dflash_embedding_bwd")
-    return out
-
-
-@embedding_gradient_op.register_fake
-def _embedding_gradient_fake(dy, input_ids, rows, scale, padding_idx):
-    return dy.new_empty(rows, dy.shape[-1])
+    @fake("disentangled_flash::embedding_gradient")
+    def _(dy, ids, rows, scale, padding):
+        return dy.new_empty((rows, dy.shape[-1]))
 
 
 # ---- operators -----------------------------------------------------------------------
 
 
 def _check_floating(name: str, tensor: torch.Tensor) -> None:
-    if tensor.device.type != "cuda":
+    if not tensor.is_cuda:
         raise RuntimeError(f"{name} must be on a GPU, is on {tensor.device}")
     if tensor.dtype not in _lib.DTYPE_CODES:
         raise TypeError(f"{name} dtype {tensor.dtype} is not fp16, bf16 or fp32")
 
 
-def _check_dropout(p: float, rng: torch.Tensor | None, site: int, device: torch.device) -> None:
+def _check_dropout(p: float, rng: torch.Tensor | None, site: int, like: torch.Tensor) -> None:
     if not 0.0 <= p <= 1.0:  # (NaN too)
         raise ValueError(f"dropout probability must be in [0, 1], got {p}")
     if not 0 <= site < 1 << 32:
@@ -210,22 +108,8 @@ def _check_dropout(p: float, rng: torch.Tensor | None, site: int, device: torch.
     if rng.dtype != torch.int64 or rng.shape != (2,) or not rng.is_contiguous():
         raise ValueError(f"rng must be a contiguous int64 tensor [seed, step], got {rng.dtype} "
                          f"{tuple(rng.shape)}")
-    if rng.device != device:
-        raise ValueError(f"rng is on {rng.device}, the input on {device}")
-
-
-class _Dropout(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, rng, p, site):
-        ctx.save_for_backward(rng)
-        ctx.p, ctx.site = p, site
-        return dropout_op(x, rng, p, site)
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dy):
-        (rng,) = ctx.saved_tensors
-        return dropout_op(dy.contiguous(), rng, ctx.p, ctx.site), None, None, None
+    if rng.get_device() != like.get_device():
+        raise ValueError(f"rng is on {rng.device}, the input on {like.device}")
 
 
 def dropout(x: torch.Tensor, p: float, rng: torch.Tensor, site: int = 0) -> torch.Tensor:
@@ -237,36 +121,10 @@ def dropout(x: torch.Tensor, p: float, rng: torch.Tensor, site: int = 0) -> torc
 
     p, site = float(p), int(site)
     _check_floating("x", x)
-    _check_dropout(p, rng, site, x.device)
+    _check_dropout(p, rng, site, x)
     if p == 0.0:
         return x
-    x = x.contiguous()
-    if torch.is_grad_enabled() and x.requires_grad:
-        return _Dropout.apply(x, rng, p, site)
-    return dropout_op(x, rng, p, site)
-
-
-class _LayerNorm(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weight, bias, residual, rng, eps, p, site):
-        y, mean, rstd = dropout_layernorm_op(x, residual, weight, bias, rng, eps, p, site, True)
-        ctx.save_for_backward(x, residual, weight, mean, rstd, rng)
-        ctx.p, ctx.site = p, site
-        return y
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dy):
-        x, residual, weight, mean, rstd, rng = ctx.saved_tensors
-        want_x, want_weight, want_bias, want_residual = ctx.needs_input_grad[:4]
-        # Without dropout the gradients of x and of the residual are the same tensor.
-        shared = ctx.p == 0.0 and want_residual
-        dx, dresidual, dweight, dbias = dropout_layernorm_backward_op(
-            dy.contiguous(), x, residual, weight, mean, rstd, rng, ctx.p, ctx.site,
-            want_x or shared, want_residual and not shared, want_weight or want_bias)
-        return (dx if want_x else None, dweight if want_weight else None,
-                dbias if want_bias else None,
-                (dx if shared else dresidual) if want_residual else None, None, None, None, None)
+    return _ops.dropout(x.contiguous(), rng, p, site)
 
 
 def layer_norm(
@@ -289,44 +147,28 @@ def layer_norm(
 
     p, site, eps = float(p), int(site), float(eps)
     _check_floating("x", x)
-    if x.dim() == 0 or not 1 <= x.shape[-1] <= MAX_HIDDEN:
-        raise ValueError(f"x must be [..., H] with H in [1, {MAX_HIDDEN}], got {tuple(x.shape)}")
+    shape, dtype, device = x.shape, x.dtype, x.get_device()
+    if not shape or not 1 <= shape[-1] <= MAX_HIDDEN:
+        raise ValueError(f"x must be [..., H] with H in [1, {MAX_HIDDEN}], got {tuple(shape)}")
+    width, kind = shape[-1:], weight.dtype
     for name, tensor in (("weight", weight), ("bias", bias)):
-        if tensor.shape != x.shape[-1:]:
-            raise ValueError(f"{name} must be [H={x.shape[-1]}], got {tuple(tensor.shape)}")
-        if tensor.dtype not in (x.dtype, torch.float32) or tensor.dtype != weight.dtype:
+        if tensor.shape != width:
+            raise ValueError(f"{name} must be [H={shape[-1]}], got {tuple(tensor.shape)}")
+        if tensor.dtype != kind or (kind != dtype and kind != torch.float32):
             raise TypeError(f"{name} dtype {tensor.dtype}: weight and bias must both have the "
-                            f"dtype of x ({x.dtype}) or both be fp32")
-        if tensor.device != x.device:
+                            f"dtype of x ({dtype}) or both be fp32")
+        if tensor.get_device() != device:
             raise ValueError(f"{name} is on {tensor.device}, x on {x.device}")
-    if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype
-                                 or residual.device != x.device):
-        raise ValueError(f"residual must match x: {tuple(x.shape)} {x.dtype} on {x.device}, got "
-                         f"{tuple(residual.shape)} {residual.dtype} on {residual.device}")
-    _check_dropout(p, rng, site, x.device)
+    if residual is not None:
+        if residual.shape != shape or residual.dtype != dtype or residual.get_device() != device:
+            raise ValueError(f"residual must match x: {tuple(shape)} {dtype} on {x.device}, got "
+                             f"{tuple(residual.shape)} {residual.dtype} on {residual.device}")
+        residual = residual.contiguous()
+    _check_dropout(p, rng, site, x)
     if p == 0.0:
         rng = None
-    x, weight, bias = x.contiguous(), weight.contiguous(), bias.contiguous()
-    residual = None if residual is None else residual.contiguous()
-    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or bias.requires_grad
-                                    or (residual is not None and residual.requires_grad)):
-        return _LayerNorm.apply(x, weight, bias, residual, rng, eps, p, site)
-    return dropout_layernorm_op(x, residual, weight, bias, rng, eps, p, site, False)[0]
-
-
-class _Embedding(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, input_ids, weight, scale, padding_idx):
-        ctx.save_for_backward(input_ids)
-        ctx.rows, ctx.scale, ctx.padding_idx = weight.shape[0], scale, padding_idx
-        return embedding_op(input_ids, weight, scale)
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dy):
-        (input_ids,) = ctx.saved_tensors
-        return None, embedding_gradient_op(dy.contiguous(), input_ids, ctx.rows, ctx.scale,
-                                           ctx.padding_idx), None, None
+    return _ops.dropout_layernorm(x.contiguous(), residual, weight.contiguous(),
+                                  bias.contiguous(), rng, eps, p, site)
 
 
 def embedding(
@@ -350,7 +192,7 @@ def embedding(
         raise ValueError("weight must be contiguous")
     if input_ids.dtype not in (torch.int32, torch.int64):
         raise TypeError(f"input_ids dtype {input_ids.dtype} is not int32 or int64")
-    if input_ids.device != weight.device:
+    if input_ids.get_device() != weight.get_device():
         raise ValueError(f"input_ids are on {input_ids.device}, weight on {weight.device}")
     rows = weight.shape[0]
     padding = -1
@@ -358,10 +200,7 @@ def embedding(
         if not -rows <= padding_idx < rows:
             raise ValueError(f"padding_idx {padding_idx} is outside the table of {rows} rows")
         padding = int(padding_idx) % rows
-    input_ids = input_ids.contiguous()
-    if torch.is_grad_enabled() and weight.requires_grad:
-        return _Embedding.apply(input_ids, weight, scale, padding)
-    return embedding_op(input_ids, weight, scale)
+    return _ops.embedding_lookup(input_ids.contiguous(), weight, scale, padding)
 
 
 # ---- modules ---------------------------------------------------------------------------
@@ -404,7 +243,7 @@ class Dropout(nn.Module):
 
     def __init__(self, p: float, state: DropoutState, site: int) -> None:
         super().__init__()
-        _check_dropout(0.0 if p == 0 else p, state.counter, site, state.counter.device)
+        _check_dropout(p, state.counter, site, state.counter)
         self.p = p
         self.site = site
         self.__dict__["state"] = state  # the model's, registered there once

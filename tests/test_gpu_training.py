@@ -611,11 +611,16 @@ def test_second_derivatives_raise():
 
     x = torch.randn(4, 64, device="cuda", requires_grad=True)
     w, b = torch.ones(64, device="cuda"), torch.zeros(64, device="cuda")
-    for y in (layer_norm(x, w, b, 1e-5), dropout(x, 0.5, _rng()),
-              embedding(torch.arange(4, device="cuda"), x)):
+    for y in (layer_norm(x, w, b, 1e-5), embedding(torch.arange(4, device="cuda"), x)):
         (grad,) = torch.autograd.grad(y.square().sum(), x, create_graph=True)
         with pytest.raises(RuntimeError, match="differentiate"):
             grad.sum().backward()
+    # Dropout is linear: d/dx of (drop'(2 drop(x))) drops the same elements twice.
+    y = dropout(x, 0.5, _rng(), SITE)
+    (grad,) = torch.autograd.grad(y.square().sum(), x, create_graph=True)
+    (second,) = torch.autograd.grad(grad.sum(), x)
+    mult = ref.factor((4, 64), 0.5, _rng(), SITE)
+    assert torch.equal(second.double(), 2 * mult * mult)
 
 
 def test_changing_rng_before_the_backward_pass_raises():

@@ -208,14 +208,14 @@ def test_c_layernorm_refusals(lib):
     for over in ({"x": A + 1}, {"r": A + 1}, {"y": A + 1}, {"g": A + 1}, {"mean": A + 2},
                  {"rng": A + 4}, {"g": A + 2, "wdtype": 2}):
         assert fwd(**over) == ALIGN, over
-    assert fwd(rows=1 << 40) == LARGE
-
-    size = lib.dflash_dropout_layernorm_bwd_workspace_bytes(4, 64)
-    assert size == 4 * 2 * 64 * 4
+    size = lib.dflash_dropout_layernorm_bwd_workspace_bytes(40, 64)
+    assert size == 40 * 2 * 64 * 4
+    assert lib.dflash_dropout_layernorm_bwd_workspace_bytes(32, 64) == 0  # one workgroup's rows
+    assert lib.dflash_dropout_layernorm_bwd_workspace_bytes(1 << 40, 64) == 512 * 2 * 64 * 4
     assert lib.dflash_dropout_layernorm_bwd_workspace_bytes(-1, 64) == 0
     assert lib.dflash_dropout_layernorm_bwd_workspace_bytes(4, 9000) == 0
 
-    def bwd(dy=A, x=A, r=A, g=A, mean=A, rstd=A, dx=A, dr=A, dg=A, db=A, rows=4, hidden=64, p=0.1,
+    def bwd(dy=A, x=A, r=A, g=A, mean=A, rstd=A, dx=A, dr=A, dg=A, db=A, rows=40, hidden=64, p=0.1,
             rng=A, dtype=1, wdtype=1, ws=A, size=size):
         return lib.dflash_dropout_layernorm_bwd(dy, x, r, g, mean, rstd, dx, dr, dg, db, rows,
                                                 hidden, p, rng, 0, dtype, wdtype, ws, size, None)
