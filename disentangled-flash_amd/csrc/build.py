@@ -85,7 +85,8 @@ def _build_torch_ops(output: Path, verbose: bool) -> None:
               "-isystem", str(root / "include"),
               "-isystem", str(root / "include" / "torch" / "csrc" / "api" / "include"),
               "-isystem", str(rocm / "include"), str(CSRC / "torch_ops.cpp"), "-o", str(staged),
-              f"-L{root / 'lib'}", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_hip", "-ldl"],
+              f"-L{root / 'lib'}", "-ltorch", "-ltorch_cpu", "-ltorch_hip", "-lc10",
+              "-lc10_hip", "-ldl"],
              verbose)
         output.parent.mkdir(parents=True, exist_ok=True)
         shutil.move(str(staged), str(output))

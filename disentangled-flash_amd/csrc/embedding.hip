@@ -5,19 +5,23 @@
 //
 // The gradient sorts the tokens by id (stably), so that the rows of one id lie together and
 // their fp32 sum is taken in an order that depends on the ids alone: no floating-point
-// atomics, the same bits on every call.  Its kernels:
+// atomics, the same bits on every call.  Up to kFewTokens one launch does all of it (few).
+// Otherwise:
 //
-//   sort   one workgroup per kSortTokens tokens, a radix sort in LDS.  The other workgroups of
-//          the launch write the zeros of dtable, which for a vocabulary is most of the bytes.
-//   merge  (more than one sorted range) each token's place by binary searches in the others.
+//   rank   (up to kRankTokens) each token's place by comparing its id with all others;
+//   sort, merge  (more) ranges sorted in LDS, then each token's place by binary searches;
+//          the first of these launches also writes the zeros of dtable, which for a
+//          vocabulary is most of the bytes;
 //   sum    kTile sorted tokens per group of lanes; an id whose tokens all lie in the tile is
-//          written, one that crosses a tile's edge leaves an fp32 partial row.
+//          written, one that crosses a tile's edge leaves an fp32 partial row;
 //   join   the partial rows of ids that cross edges, added in order.
 //
 // Ids outside [0, rows): the lookup returns NaN for them, the gradient leaves them out.
 
 #include <hip/hip_runtime.h>
 #include <stdint.h>
+
+#include <type_traits>
 
 #include "device_common.h"
 #include "dflash.h"
@@ -54,6 +58,97 @@ __global__ __launch_bounds__(256) void embedding_fwd_kernel(
   }
 }
 
+// An id as the sort's key: ids that take no gradient become `rows`, past every other.
+template <typename I>
+__device__ inline int32_t key_of(I value, int rows, int64_t padding) {
+  const int64_t id = static_cast<int64_t>(value);
+  return id >= 0 && id < rows && id != padding ? static_cast<int32_t>(id) : rows;
+}
+
+// Zeros for bytes [begin, end) of dtable, both multiples of 16 but for the table's end (elements
+// are 2 or 4 bytes), by workgroups `block` of `blocks`.
+struct Fill {
+  u32x4_t* table;
+  int64_t begin, end;
+};
+
+template <int THREADS>
+__device__ inline void fill_zeros(const Fill& f, int block, int blocks) {
+  const int64_t at = static_cast<int64_t>(block) * THREADS + threadIdx.x;
+  const int64_t chunks = f.end / 16;
+  for (int64_t i = f.begin / 16 + at; i < chunks; i += static_cast<int64_t>(blocks) * THREADS)
+    f.table[i] = u32x4_t{0, 0, 0, 0};
+  if (at < (f.end - chunks * 16) / 2) reinterpret_cast<uint16_t*>(f.table + chunks)[at] = 0;
+}
+
+// ---- rank --------------------------------------------------------------------
+
+// A token's place is the number of ids below its own and of equal ids before it: every token is
+// compared with every id, two instructions a pair, ids four at a time from LDS.  A
+// workgroup takes 64 >> parts_log2 tokens; its 1024 threads share out the ids, and the
+// counts of a token are added.  Fewer tokens a workgroup where that fills more CUs.
+constexpr int kRankTokens = 8192;
+constexpr int kRankThreads = 1024;
+
+template <typename I>
+__global__ __launch_bounds__(kRankThreads) void embedding_rank_kernel(
+    const I* __restrict__ ids, int n, int rows, int64_t padding, int blocks, int parts_log2,
+    int32_t* __restrict__ sorted_ids, int32_t* __restrict__ sorted_tokens, Fill fill) {
+  typedef int32_t Four __attribute__((ext_vector_type(4)));
+  extern __shared__ Four keys[];  // n of them, whole groups of four; then the counts
+  if (static_cast<int>(blockIdx.x) >= blocks) {
+    fill_zeros<kRankThreads>(fill, blockIdx.x - blocks, gridDim.x - blocks);
+    return;
+  }
+  const int quads = (n + 3) / 4;
+  int32_t* flat = reinterpret_cast<int32_t*>(keys);
+  int32_t* counts = flat + quads * 4;
+  // (Every load is made, past the end of the last id, so that all are in flight together.)
+  I given[kRankTokens / kRankThreads];
+#pragma unroll
+  for (int k = 0; k < kRankTokens / kRankThreads; ++k)
+    given[k] = ids[min(k * kRankThreads + static_cast<int>(threadIdx.x), n - 1)];
+#pragma unroll
+  for (int k = 0; k < kRankTokens / kRankThreads; ++k) {
+    const int j = k * kRankThreads + threadIdx.x;
+    if (j < quads * 4)
+      flat[j] = j < n ? key_of(given[k], rows, padding) : INT32_MAX;  // above every key
+  }
+  __syncthreads();
+  // Neighbouring lanes hold the parts of one token.
+  const int tokens = 64 >> parts_log2;
+  const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+  const int token = blockIdx.x * tokens + (lane >> parts_log2);
+  const int part = wave << parts_log2 | (lane & ((1 << parts_log2) - 1));
+  const int parts = (kRankThreads / 64) << parts_log2;
+  const int32_t key = flat[min(token, n - 1)];
+  const int own = token / 4;  // equal ids count in the groups of four before this one
+  int count = 0;
+#pragma unroll 4
+  for (int j = part; j < quads; j += parts) {
+    const Four k = keys[j];
+    const int32_t limit = key + (j < own);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) count += k[e] < limit;
+  }
+  counts[threadIdx.x] = count;
+  __syncthreads();
+  if (static_cast<int>(threadIdx.x) < tokens) {
+    const int mine = blockIdx.x * tokens + threadIdx.x;
+    if (mine < n) {
+      int place = 0;
+      for (int w = 0; w < kRankThreads / 64; ++w) {
+        for (int i = 0; i < 1 << parts_log2; ++i)
+          place += counts[w * 64 + (threadIdx.x << parts_log2 | i)];
+      }
+      const int32_t id = flat[mine];
+      for (int j = mine / 4 * 4; j < mine; ++j) place += flat[j] == id;  // in its own group
+      sorted_ids[place] = id;
+      sorted_tokens[place] = mine;
+    }
+  }
+}
+
 // ---- sort --------------------------------------------------------------------
 
 constexpr int kSortTokens = 2048;    // per workgroup; a place in the range is 16 bits
@@ -76,7 +171,7 @@ __device__ inline void wave_order() {
   __builtin_amdgcn_wave_barrier();
 }
 
-// Stable radix sort of one range.  Ids that take no gradient become `rows`, past every other.
+// Stable radix sort of one range.
 // Each wavefront owns a contiguous part of the range and ranks 64 keys a round: the lanes of
 // equal digits are found with one ballot a bit, the digit's count so far is the
 // wavefront's counter.  A scan over (digit, wavefront) gives the places.
@@ -90,15 +185,14 @@ __device__ void sort_range(const I* __restrict__ ids, int64_t first, int count, 
   const uint32_t last = bits < 32 ? (1u << bits) - 1 : ~0u;  // at least `rows`
 
   uint32_t key[kSortRounds], place[kSortRounds], rank[kSortRounds];
+  I given[kSortRounds];  // (past the end the last id: every load in flight)
+#pragma unroll
+  for (int j = 0; j < kSortRounds; ++j) given[j] = ids[first + min(mine + 64 * j, count - 1)];
 #pragma unroll
   for (int j = 0; j < kSortRounds; ++j) {
-    key[j] = last;  // past the end: stays behind every token, by its value and its place
     place[j] = mine + 64 * j;
-    if (j < rounds && mine + 64 * j < count) {
-      const int64_t id = static_cast<int64_t>(ids[first + mine + 64 * j]);
-      key[j] = id >= 0 && id < rows && id != padding ? static_cast<uint32_t>(id)
-                                                     : static_cast<uint32_t>(rows);
-    }
+    // Past the end: behind every token, by its value and its place.
+    key[j] = mine + 64 * j < count ? static_cast<uint32_t>(key_of(given[j], rows, padding)) : last;
   }
   const int passes = (bits + kDigitBits - 1) / kDigitBits;
   const int digit_bits = (bits + passes - 1) / passes;
@@ -182,22 +276,6 @@ __device__ void sort_range(const I* __restrict__ ids, int64_t first, int count, 
   }
 }
 
-// Zeros for bytes [begin, end) of dtable, both multiples of 16 but for the table's end (elements
-// are 2 or 4 bytes), by workgroups `block` of `blocks`.
-struct Fill {
-  u32x4_t* table;
-  int64_t begin, end;
-};
-
-template <int THREADS>
-__device__ inline void fill_zeros(const Fill& f, int block, int blocks) {
-  const int64_t at = static_cast<int64_t>(block) * THREADS + threadIdx.x;
-  const int64_t chunks = f.end / 16;
-  for (int64_t i = f.begin / 16 + at; i < chunks; i += static_cast<int64_t>(blocks) * THREADS)
-    f.table[i] = u32x4_t{0, 0, 0, 0};
-  if (at < (f.end - chunks * 16) / 2) reinterpret_cast<uint16_t*>(f.table + chunks)[at] = 0;
-}
-
 template <typename I>
 __global__ __launch_bounds__(kSortThreads) void embedding_sort_kernel(
     const I* __restrict__ ids, int64_t n, int rows, int64_t padding, int bits, int ranges,
@@ -233,7 +311,8 @@ __global__ __launch_bounds__(kMergeThreads) void embedding_merge_kernel(
     return;
   }
   const int64_t i = static_cast<int64_t>(blockIdx.x) * kMergeThreads + threadIdx.x;
-  const int32_t id = i < n ? ids[i] : 0;
+  const int64_t at = i < n ? i : n - 1;
+  const int32_t id = ids[at], token = tokens[at];
   const int64_t own = i / kSortTokens;
   int64_t place = i - own * kSortTokens;
   const int64_t ranges = (n + kSortTokens - 1) / kSortTokens;
@@ -241,11 +320,17 @@ __global__ __launch_bounds__(kMergeThreads) void embedding_merge_kernel(
     const int64_t first = r0 * kSortTokens;
     const int held = n - first < kHeld ? static_cast<int>(n - first) : kHeld;
     __syncthreads();  // the ranges before have been searched
+    // (The array is padded to 256 bytes: whole accesses, past the end the last one again.)
+    Four given[kHeld / 4 / kMergeThreads];
 #pragma unroll
     for (int k = 0; k < kHeld / 4 / kMergeThreads; ++k) {
       const int j = (k * kMergeThreads + threadIdx.x) * 4;
-      // (The array is padded to 256 bytes: whole accesses; past the end above all ids.)
-      Four v = j < held ? *reinterpret_cast<const Four*>(ids + first + j) : Four{};
+      given[k] = *reinterpret_cast<const Four*>(ids + first + min(j, (held - 1) / 4 * 4));
+    }
+#pragma unroll
+    for (int k = 0; k < kHeld / 4 / kMergeThreads; ++k) {
+      const int j = (k * kMergeThreads + threadIdx.x) * 4;
+      Four v = given[k];  // past the end: above all ids
 #pragma unroll
       for (int e = 0; e < 4; ++e)
         if (j + e >= held) v[e] = INT32_MAX;
@@ -272,7 +357,7 @@ __global__ __launch_bounds__(kMergeThreads) void embedding_merge_kernel(
   }
   if (i < n) {
     merged_ids[place] = id;
-    merged_tokens[place] = tokens[i];
+    merged_tokens[place] = token;
   }
 }
 
@@ -282,13 +367,32 @@ constexpr int kTile = 32;      // sorted tokens of a group of lanes
 constexpr int kAhead = 16;     // rows of dout in flight
 constexpr int kMinLanes = 8;   // of a group, so that its workgroup's tokens fit LDS
 
+// The loads into `v` are all issued before the first is used: the compiler would otherwise move
+// each down to where its row is added, and wait for it there.
+template <typename A, int N>
+__device__ inline void in_flight(A (&v)[N]) {
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    if constexpr (sizeof(A) > 4) {
+      asm volatile("" : "+v"(v[j]));
+    } else {  // a single element
+      using Bits = std::conditional_t<sizeof(A) == 4, uint32_t, uint16_t>;
+      uint32_t word = __builtin_bit_cast(Bits, v[j]);
+      asm volatile("" : "+v"(word));
+      v[j] = __builtin_bit_cast(A, static_cast<Bits>(word));
+    }
+  }
+}
+
 template <int V>
 __device__ inline void store_partial(float* p, const float (&v)[V]) {
 #pragma unroll
   for (int e = 0; e < V; ++e) p[e] = v[e];
 }
 
-// A group of `lanes` lanes sums one tile over lanes * V columns (blockIdx.y: which).
+// A group of `lanes` lanes sums one tile over lanes * V columns, slice `blockIdx.x % slices` of
+// them: the workgroups that share rows of dout are neighbours, so that a row's pieces are
+// fetched together.
 // partials[tile][0]: what the tile holds of an id that began in an earlier tile;
 // partials[tile][1]: of an id that begins here and goes on in the next tile.
 // Bound by the latency of rows gathered from HBM: the tile's ids and tokens come through LDS
@@ -297,14 +401,16 @@ template <typename T, int V>
 __global__ __launch_bounds__(256) void embedding_sum_kernel(
     const int32_t* __restrict__ ids, const int32_t* __restrict__ tokens, int64_t n, int rows,
     const T* __restrict__ dout, T* __restrict__ dtable, int hidden, float scale,
-    float* __restrict__ partials, int lanes_log2) {
+    float* __restrict__ partials, int lanes_log2, int slices) {
   typedef T Access __attribute__((ext_vector_type(V)));
   constexpr int kMost = 256 / kMinLanes * kTile;
   __shared__ int32_t lds_ids[kMost + 2];  // with the neighbours on both sides, -1 past the ends
   __shared__ int32_t lds_tokens[kMost];
   const int lanes = 1 << lanes_log2;
   const int tiles = 256 >> lanes_log2;
-  const int64_t start = static_cast<int64_t>(blockIdx.x) * tiles * kTile;
+  const int64_t block = blockIdx.x / slices;
+  const int slice = static_cast<int>(blockIdx.x - block * slices);
+  const int64_t start = block * tiles * kTile;
   for (int i = threadIdx.x; i < tiles * kTile + 2; i += 256) {
     const int64_t at = start + i - 1;
     lds_ids[i] = at >= 0 && at < n ? ids[at] : -1;
@@ -312,9 +418,9 @@ __global__ __launch_bounds__(256) void embedding_sum_kernel(
   }
   __syncthreads();
   const int group = threadIdx.x >> lanes_log2;
-  const int64_t tile = static_cast<int64_t>(blockIdx.x) * tiles + group;
+  const int64_t tile = block * tiles + group;
   const int64_t begin = tile * kTile;
-  const int col = (static_cast<int>(blockIdx.y) * lanes + (threadIdx.x & (lanes - 1))) * V;
+  const int col = (slice * lanes + static_cast<int>(threadIdx.x & (lanes - 1))) * V;
   if (begin >= n || col >= hidden) return;
   const int count = n - begin < kTile ? static_cast<int>(n - begin) : kTile;
   const int32_t* id = lds_ids + 1 + group * kTile;
@@ -326,43 +432,43 @@ __global__ __launch_bounds__(256) void embedding_sum_kernel(
   for (int e = 0; e < V; ++e) acc[e] = 0.0f;
   int32_t current = id[0];
   bool first = id[-1] == current;  // the sum in acc belongs to partials[tile][0]
+  auto put = [&](bool goes_on) {
+    if (first || goes_on) {
+      store_partial(first ? partial : partial + hidden, acc);
+    } else {
+#pragma unroll
+      for (int e = 0; e < V; ++e) acc[e] *= scale;
+      store_floats<T, V>(dtable + static_cast<int64_t>(current) * hidden + col, acc);
+    }
+  };
   for (int i0 = 0; i0 < count; i0 += kAhead) {
     Access row[kAhead];
+    int32_t next[kAhead];
 #pragma unroll
-    for (int j = 0; j < kAhead; ++j)  // (past the tile's end its last row again)
-      row[j] = *reinterpret_cast<const Access*>(
-          dout + static_cast<int64_t>(token[min(i0 + j, count - 1)]) * hidden + col);
+    for (int j = 0; j < kAhead; ++j) {  // (past the tile's end its last row again)
+      const int at = min(i0 + j, count - 1);
+      next[j] = id[at];
+      row[j] =
+          *reinterpret_cast<const Access*>(dout + static_cast<int64_t>(token[at]) * hidden + col);
+    }
+    in_flight(row);
+    // (No exit from this loop: it has to unroll for its rows to stay in registers.  The tokens
+    // without a gradient come last; what is added up for them is never written.)
 #pragma unroll
     for (int j = 0; j < kAhead; ++j) {
-      if (i0 + j >= count) break;
-      const int32_t next = id[i0 + j];
-      if (next != current) {
-        if (first) {
-          store_partial(partial, acc);
-        } else {
-#pragma unroll
-          for (int e = 0; e < V; ++e) acc[e] *= scale;
-          store_floats<T, V>(dtable + static_cast<int64_t>(current) * hidden + col, acc);
-        }
+      if (next[j] != current) {
+        put(false);
 #pragma unroll
         for (int e = 0; e < V; ++e) acc[e] = 0.0f;
-        current = next;
+        current = next[j];
         first = false;
       }
-      if (current >= rows) return;  // the ids without a gradient come last
+      const bool live = i0 + j < count;
 #pragma unroll
-      for (int e = 0; e < V; ++e) acc[e] += static_cast<float>(row[j][e]);
+      for (int e = 0; e < V; ++e) acc[e] += live ? static_cast<float>(row[j][e]) : 0.0f;
     }
   }
-  if (first) {
-    store_partial(partial, acc);
-  } else if (id[count] == current) {
-    store_partial(partial + hidden, acc);
-  } else {
-#pragma unroll
-    for (int e = 0; e < V; ++e) acc[e] *= scale;
-    store_floats<T, V>(dtable + static_cast<int64_t>(current) * hidden + col, acc);
-  }
+  if (current < rows) put(id[count] == current);
 }
 
 // One workgroup per tile and 256 columns.  If an id begins in the tile and goes on, its partial
@@ -378,31 +484,45 @@ __global__ __launch_bounds__(64 * kJoinWaves) void embedding_join_kernel(
   const int64_t begin = tile * kTile;
   const int64_t end = begin + kTile;
   if (end >= n) return;  // (the last tile goes nowhere)
-  const int32_t id = ids[end - 1];
-  if (id >= rows || ids[end] != id) return;
-  if (ids[begin] == id && begin > 0 && ids[begin - 1] == id) return;  // began earlier
-  // Tiles whose first token is of the id, [tile + 1, tile + count): every thread looks at one.
+  // One round of loads for all that is decided on; the first token of the tile after next and of
+  // those behind it, a thread each, for the count below.
+  constexpr int kThreadsJoin = 64 * kJoinWaves;
   const int64_t tiles = (n + kTile - 1) / kTile;
-  int64_t count = 1;  // partial rows, this tile's among them
-  for (int found = 64 * kJoinWaves; found == 64 * kJoinWaves; count += found) {
-    const int64_t other = tile + count + threadIdx.x;
-    found = __syncthreads_count(other < tiles && ids[other * kTile] == id);
+  const int32_t id = ids[end - 1], next = ids[end], head = ids[begin];
+  const int32_t ahead = begin > 0 ? ids[begin - 1] : -1;
+  int64_t other = tile + 2 + threadIdx.x;
+  int32_t theirs = other < tiles ? ids[other * kTile] : -1;
+  if (id >= rows || next != id || (head == id && ahead == id)) return;  // ends, or began earlier
+  // Tiles whose first token is of the id: [tile + 1, tile + count).
+  int64_t count = 2;  // partial rows, this tile's among them
+  for (;;) {
+    const int found = __syncthreads_count(theirs == id);
+    count += found;
+    if (found < kThreadsJoin) break;
+    other += kThreadsJoin;
+    theirs = other < tiles ? ids[other * kTile] : -1;
   }
   const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
   const int64_t per = (count + kJoinWaves - 1) / kJoinWaves;
   const int64_t from = wave * per;
   const int64_t to = from + per < count ? from + per : count;
-#pragma unroll
-  for (int c = 0; c < 4; ++c) {
-    const int col = blockIdx.y * 256 + c * 64 + lane;
-    float v = 0.0f;
-    if (col < hidden) {
+  const int mine = blockIdx.y * 256 + lane * 4;
+  const bool whole = hidden % 4 == 0;  // then four columns are one access
+  f32x4_t v{};
+  if (mine < hidden) {
 #pragma unroll 8
-      for (int64_t i = from; i < to; ++i)
-        v += partials[((tile + i) * 2 + (i == 0)) * hidden + col];
+    for (int64_t i = from; i < to; ++i) {
+      const float* row = partials + ((tile + i) * 2 + (i == 0)) * hidden;
+      if (whole) {
+        v += *reinterpret_cast<const f32x4_t*>(row + mine);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] += row[min(mine + e, hidden - 1)];
+      }
     }
-    lds[wave][c * 64 + lane] = v;
   }
+#pragma unroll
+  for (int e = 0; e < 4; ++e) lds[wave][lane * 4 + e] = v[e];
   __syncthreads();
   const int col = blockIdx.y * 256 + threadIdx.x;
   if (threadIdx.x < 256 && col < hidden) {
@@ -410,6 +530,114 @@ __global__ __launch_bounds__(64 * kJoinWaves) void embedding_join_kernel(
 #pragma unroll
     for (int w = 1; w < kJoinWaves; ++w) v += lds[w][threadIdx.x];
     dtable[static_cast<int64_t>(id) * hidden + col] = static_cast<T>(v * scale);
+  }
+}
+
+// ---- few tokens ----------------------------------------------------------------
+
+// One launch for up to kFewTokens tokens: a workgroup owns rows of the table, zeroes them, picks
+// the tokens of its rows out of all (in order), sorts them and adds up theirs.
+constexpr int kFewTokens = 256;
+
+// The rows are dealt out `unit` at a time (ids next to each other are often frequent together):
+// one where rows are whole 16-byte chunks, else as many as together always are.
+template <typename T, typename I, int V>
+__global__ __launch_bounds__(256) void embedding_few_kernel(
+    const I* __restrict__ ids, int n, int rows, int64_t padding, int unit,
+    const T* __restrict__ dout, T* __restrict__ dtable, int hidden, float scale, int lanes_log2) {
+  typedef T Access __attribute__((ext_vector_type(V)));
+  constexpr int kAheadFew = 16;
+  __shared__ int32_t found[2][kFewTokens], sorted[2][kFewTokens];  // id, token
+  __shared__ int32_t run[kFewTokens];  // tokens of an id, at its first one; 0 at the others
+  __shared__ int32_t wave_counts[4];
+  const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+  const int blocks = gridDim.x;
+  const int32_t key = static_cast<int>(threadIdx.x) < n
+                          ? key_of(ids[threadIdx.x], rows, padding) : rows;
+  const bool mine = key < rows && key / unit % blocks == static_cast<int>(blockIdx.x);
+  const uint64_t mask = __ballot(mine);
+  if (lane == 0) wave_counts[wave] = __popcll(mask);
+
+  const int64_t per_unit = static_cast<int64_t>(unit) * hidden / Chunk<T>::N;  // chunks
+  const int64_t elements = static_cast<int64_t>(rows) * hidden;
+  const int64_t chunks = elements / Chunk<T>::N;
+  const int units = (rows + unit - 1) / unit;
+  u32x4_t* table = reinterpret_cast<u32x4_t*>(dtable);
+  if (per_unit < 256) {
+    // Several units at a time, each by the lanes that hold one.
+    const int at_once = 256 / static_cast<int>(per_unit);
+    const int which = threadIdx.x / static_cast<int>(per_unit);
+    const int64_t chunk = threadIdx.x % static_cast<int>(per_unit);
+    for (int64_t u = blockIdx.x + static_cast<int64_t>(which) * blocks;
+         which < at_once && u < units; u += static_cast<int64_t>(at_once) * blocks) {
+      if (u * per_unit + chunk < chunks) table[u * per_unit + chunk] = u32x4_t{0, 0, 0, 0};
+    }
+  } else {
+    for (int64_t u = blockIdx.x; u < units; u += blocks) {
+      for (int64_t i = threadIdx.x; i < per_unit; i += 256)
+        if (u * per_unit + i < chunks) table[u * per_unit + i] = u32x4_t{0, 0, 0, 0};
+    }
+  }
+  // The elements behind the last whole chunk are the last unit's.
+  if ((units - 1) % blocks == static_cast<int>(blockIdx.x) &&
+      chunks * Chunk<T>::N + threadIdx.x < elements)
+    dtable[chunks * Chunk<T>::N + threadIdx.x] = T(0);
+  __syncthreads();  // the counts, and the zeros before the sums
+  int count = 0, at = __popcll(mask & ((1ull << lane) - 1));
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    if (w < wave) at += wave_counts[w];
+    count += wave_counts[w];
+  }
+  if (count == 0) return;
+  if (mine) {
+    found[0][at] = key;
+    found[1][at] = threadIdx.x;
+  }
+  __syncthreads();
+  if (static_cast<int>(threadIdx.x) < count) {
+    const int32_t row = found[0][threadIdx.x];
+    int below = 0, equal = 0, before = 0;
+#pragma unroll 8
+    for (int i = 0; i < count; ++i) {
+      const int32_t other = found[0][i];
+      below += other < row;
+      equal += other == row;
+      before += other == row && i < static_cast<int>(threadIdx.x);
+    }
+    sorted[0][below + before] = row;
+    sorted[1][below + before] = found[1][threadIdx.x];
+    run[below + before] = before == 0 ? equal : 0;
+  }
+  __syncthreads();
+  // A group of lanes takes one id (at its first token) and a slice of the columns at a time.
+  const int lanes = 1 << lanes_log2, groups = 256 >> lanes_log2;
+  const int slices = (hidden / V + lanes - 1) >> lanes_log2;
+  for (int task = threadIdx.x >> lanes_log2; task < count * slices; task += groups) {
+    const int start = task / slices;
+    const int col = ((task - start * slices) * lanes + (threadIdx.x & (lanes - 1))) * V;
+    const int32_t row = sorted[0][start];
+    const int end = start + run[start];
+    if (col >= hidden || end == start) continue;
+    float acc[V];
+#pragma unroll
+    for (int e = 0; e < V; ++e) acc[e] = 0.0f;
+    for (int i = start; i < end; i += kAheadFew) {
+      Access v[kAheadFew];
+#pragma unroll
+      for (int j = 0; j < kAheadFew; ++j)
+        v[j] = *reinterpret_cast<const Access*>(
+            dout + static_cast<int64_t>(sorted[1][min(i + j, end - 1)]) * hidden + col);
+      in_flight(v);
+#pragma unroll
+      for (int j = 0; j < kAheadFew; ++j) {
+#pragma unroll
+        for (int e = 0; e < V; ++e) acc[e] += i + j < end ? static_cast<float>(v[j][e]) : 0.0f;
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < V; ++e) acc[e] *= scale;
+    store_floats<T, V>(dtable + static_cast<int64_t>(row) * hidden + col, acc);
   }
 }
 
@@ -438,6 +666,7 @@ int launch_fwd(const void* ids, const void* table, void* out, int64_t n, int row
   return static_cast<int>(hipGetLastError());
 }
 
+constexpr int kFewBlocks = 1024;   // workgroups of one launch for few tokens
 constexpr int kFillBlocks = 512;  // workgroups that write zeros
 constexpr int64_t kMaxTokens = int64_t{1} << 26;
 constexpr int kMaxHidden = 1 << 20;
@@ -457,10 +686,11 @@ struct Workspace {
 };
 
 Workspace workspace_of(int64_t n, int hidden) {
-  Workspace w;
+  Workspace w{0, 0, 0};
+  if (n <= kFewTokens) return w;
   w.index_bytes = aligned(n * 4);
-  w.partial_bytes = tiles_of(n) > 1 ? aligned(tiles_of(n) * 2 * hidden * 4) : 0;
-  w.total = (ranges_of(n) > 1 ? 4 : 2) * w.index_bytes + w.partial_bytes;
+  w.partial_bytes = aligned(tiles_of(n) * 2 * hidden * 4);
+  w.total = (n > kRankTokens ? 4 : 2) * w.index_bytes + w.partial_bytes;
   return w;
 }
 
@@ -475,17 +705,48 @@ int launch_bwd(const void* ids_in, const void* dout_in, void* dtable_in, int64_t
   int bits = 1;
   while (bits < 32 && (int64_t{1} << bits) - 1 < rows) ++bits;
   const int64_t table_bytes = static_cast<int64_t>(rows) * hidden * sizeof(T);
-  // The zeros go with the sort, and a part of them with the merge if there is one, so that
-  // neither has the card to itself.
-  const int64_t first_part = ranges > 1 ? table_bytes / 5 * 3 / 16 * 16 : table_bytes;
+  constexpr int N = Chunk<T>::N;
+  const I* ids_as_given = static_cast<const I*>(ids_in);
+  const T* dout = static_cast<const T*>(dout_in);
+  T* dtable = static_cast<T*>(dtable_in);
+  const bool wide = hidden % N == 0 && address(dout) % 16 == 0;
+  const int accesses = wide ? hidden / N : hidden;
+  const int log2 = lanes_log2_for(accesses, 3, 5);
+  // (Before anything is launched.)
+  if (tiles_of(n) * hidden > kMaxBlocks256 * 8) return DFLASH_ERR_TOO_LARGE;
+  if (n <= kFewTokens) {
+    const int unit = hidden % N == 0 ? 1 : N;
+    const int units = (rows + unit - 1) / unit;
+    hipLaunchKernelGGL((wide ? &embedding_few_kernel<T, I, N> : &embedding_few_kernel<T, I, 1>),
+                       dim3(units < kFewBlocks ? units : kFewBlocks), dim3(256), 0, stream,
+                       ids_as_given, static_cast<int>(n), rows, padding, unit, dout, dtable,
+                       hidden, scale, log2);
+    return static_cast<int>(hipGetLastError());
+  }
+  // The zeros go with the first launch, and a part of them with the merge if there is one, so
+  // that neither has the card to itself.
+  const bool by_rank = n <= kRankTokens;
+  const int64_t first_part = by_rank ? table_bytes : table_bytes / 5 * 3 / 16 * 16;
   const Fill fill{static_cast<u32x4_t*>(dtable_in), 0, first_part};
-  hipLaunchKernelGGL((embedding_sort_kernel<I>),
-                     dim3(ranges + fill_blocks(first_part, kSortThreads)), dim3(kSortThreads), 0,
-                     stream, static_cast<const I*>(ids_in), n, rows, padding, bits, ranges, ids,
-                     tokens, fill);
-  int rc = static_cast<int>(hipGetLastError());
-  if (rc != DFLASH_OK || n == 0) return rc;
-  if (ranges > 1) {
+  int rc;
+  if (by_rank) {
+    // 256 workgroups or more, of 8 to 64 tokens.
+    int parts_log2 = 0;
+    while (parts_log2 < 3 && n <= (256 * 64) >> (parts_log2 + 1)) ++parts_log2;
+    const int blocks = static_cast<int>((n + (64 >> parts_log2) - 1) >> (6 - parts_log2));
+    const int lds = static_cast<int>((n + 3) / 4 * 16) + kRankThreads * 4;
+    hipLaunchKernelGGL((embedding_rank_kernel<I>),
+                       dim3(blocks + fill_blocks(first_part, kRankThreads)), dim3(kRankThreads),
+                       lds, stream, ids_as_given, static_cast<int>(n), rows, padding, blocks,
+                       parts_log2, ids, tokens, fill);
+    rc = static_cast<int>(hipGetLastError());
+    if (rc != DFLASH_OK) return rc;
+  } else {
+    hipLaunchKernelGGL((embedding_sort_kernel<I>),
+                       dim3(ranges + fill_blocks(first_part, kSortThreads)), dim3(kSortThreads), 0,
+                       stream, ids_as_given, n, rows, padding, bits, ranges, ids, tokens, fill);
+    rc = static_cast<int>(hipGetLastError());
+    if (rc != DFLASH_OK) return rc;
     int32_t* merged = reinterpret_cast<int32_t*>(workspace + 2 * w.index_bytes);
     int32_t* merged_tokens = reinterpret_cast<int32_t*>(workspace + 3 * w.index_bytes);
     const Fill rest{static_cast<u32x4_t*>(dtable_in), first_part, table_bytes};
@@ -499,20 +760,14 @@ int launch_bwd(const void* ids_in, const void* dout_in, void* dtable_in, int64_t
     ids = merged;
     tokens = merged_tokens;
   }
-  constexpr int N = Chunk<T>::N;
-  const T* dout = static_cast<const T*>(dout_in);
-  T* dtable = static_cast<T*>(dtable_in);
-  const bool wide = hidden % N == 0 && (address(dout) | address(dtable)) % 16 == 0;
-  const int accesses = wide ? hidden / N : hidden;
-  const int log2 = lanes_log2_for(accesses, 3, 5);
   const int64_t tiles = tiles_of(n);
+  const int slices = (accesses + (1 << log2) - 1) >> log2;
+  const int64_t sum_blocks = ((tiles << log2) + 255) / 256 * slices;
   hipLaunchKernelGGL((wide ? &embedding_sum_kernel<T, N> : &embedding_sum_kernel<T, 1>),
-                     dim3(static_cast<uint32_t>(((tiles << log2) + 255) / 256),
-                          (accesses + (1 << log2) - 1) >> log2),
-                     dim3(256), 0, stream, ids, tokens, n, rows, dout, dtable, hidden, scale,
-                     partials, log2);
+                     dim3(static_cast<uint32_t>(sum_blocks)), dim3(256), 0, stream, ids, tokens, n,
+                     rows, dout, dtable, hidden, scale, partials, log2, slices);
   rc = static_cast<int>(hipGetLastError());
-  if (rc != DFLASH_OK || tiles == 1) return rc;
+  if (rc != DFLASH_OK) return rc;
   hipLaunchKernelGGL((embedding_join_kernel<T>),
                      dim3(static_cast<uint32_t>(tiles), (hidden + 255) / 256), dim3(64 * kJoinWaves), 0,
                      stream, ids, n, rows, dtable, hidden, scale, partials);
@@ -573,7 +828,7 @@ extern "C" int dflash_embedding_bwd(const void* ids, const void* dout, void* dta
   return with_types(dtype, id_bytes, [&](auto t, auto i) {
     using T = decltype(t);
     using I = decltype(i);
-    if (!dtable || (n > 0 && (!ids || !dout || !workspace)))
+    if (!dtable || (n > 0 && (!ids || !dout)) || (workspace_of(n, hidden).total && !workspace))
       return static_cast<int>(DFLASH_ERR_NULL);
     if (address(ids) % sizeof(I) != 0 || address(dout) % sizeof(T) != 0 ||
         address(dtable) % 16 != 0 || address(workspace) % 16 != 0)

@@ -11,8 +11,7 @@
 
 #include <ATen/core/Tensor.h>
 #include <ATen/core/dispatch/Dispatcher.h>
-#include <ATen/ops/empty.h>
-#include <ATen/ops/empty_like.h>
+#include <ATen/hip/EmptyTensor.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <dlfcn.h>
@@ -86,6 +85,12 @@ struct On {
       : guard(t.device()), stream(c10::hip::getCurrentHIPStream(t.get_device()).stream()) {}
 };
 
+// Uninitialised memory, past the dispatcher (five of them in a backward pass).
+Tensor fresh(at::IntArrayRef sizes, at::ScalarType type, const Tensor& like) {
+  return at::detail::empty_cuda(sizes, type, like.device(), std::nullopt);
+}
+Tensor fresh_like(const Tensor& t) { return fresh(t.sizes(), t.scalar_type(), t); }
+
 void* data(const Tensor& t) { return t.data_ptr(); }
 void* data(const MaybeTensor& t) { return t ? t->data_ptr() : nullptr; }
 const int64_t* words(const MaybeTensor& rng) {
@@ -95,7 +100,7 @@ const int64_t* words(const MaybeTensor& rng) {
 // ---- the calls (inputs contiguous, checked by the caller) --------------------------
 
 Tensor dropout(const Tensor& x, const Tensor& rng, double p, int64_t site) {
-  Tensor out = at::empty_like(x);
+  Tensor out = fresh_like(x);
   On on(x);
   check(lib.dropout(data(x), data(out), x.numel(), p, words(rng), site, code_of(x), on.stream),
         "dflash_dropout");
@@ -105,7 +110,7 @@ Tensor dropout(const Tensor& x, const Tensor& rng, double p, int64_t site) {
 Tensor layernorm(const Tensor& x, const MaybeTensor& residual, const Tensor& weight,
                  const Tensor& bias, const MaybeTensor& rng, double eps, double p, int64_t site,
                  float* statistics) {
-  Tensor y = at::empty_like(x);
+  Tensor y = fresh_like(x);
   const int64_t hidden = x.size(-1), rows = x.numel() / hidden;
   On on(x);
   check(lib.layernorm_fwd(data(x), data(residual), data(weight), data(bias), data(y), statistics,
@@ -126,7 +131,7 @@ std::tuple<Tensor, Tensor> dropout_layernorm_train(const Tensor& x, const MaybeT
                                                    const Tensor& weight, const Tensor& bias,
                                                    const MaybeTensor& rng, double eps, double p,
                                                    int64_t site) {
-  Tensor statistics = at::empty({2, x.numel() / x.size(-1)}, x.options().dtype(at::kFloat));
+  Tensor statistics = fresh({2, x.numel() / x.size(-1)}, at::kFloat, x);
   Tensor y = layernorm(x, residual, weight, bias, rng, eps, p, site,
                        static_cast<float*>(data(statistics)));
   return {y, statistics};
@@ -139,13 +144,13 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> dropout_layernorm_backward(
     bool want_residual, bool want_weights) {
   const int64_t hidden = x.size(-1), rows = x.numel() / hidden;
   auto made = [](bool wanted, const Tensor& like) {
-    return wanted ? at::empty_like(like) : at::empty({0}, like.options());
+    return wanted ? fresh_like(like) : fresh({0}, like.scalar_type(), like);
   };
   Tensor dx = made(want_x, x), dresidual = made(want_residual, x);
   Tensor dweight = made(want_weights, weight), dbias = made(want_weights, weight);
   const size_t bytes = want_weights ? lib.layernorm_bwd_workspace_bytes(rows, hidden) : 0;
   Tensor workspace;
-  if (bytes) workspace = at::empty({static_cast<int64_t>(bytes)}, x.options().dtype(at::kByte));
+  if (bytes) workspace = fresh({static_cast<int64_t>(bytes)}, at::kByte, x);
   const float* mean = static_cast<const float*>(data(statistics));
   On on(x);
   check(lib.layernorm_bwd(data(dy), data(x), data(residual), data(weight), mean, mean + rows,
@@ -162,7 +167,7 @@ Tensor embedding_lookup(const Tensor& ids, const Tensor& table, double scale,
                         int64_t /*padding*/) {
   auto shape = ids.sizes().vec();
   shape.push_back(table.size(1));
-  Tensor out = at::empty(shape, table.options());
+  Tensor out = fresh(shape, table.scalar_type(), table);
   On on(table);
   check(lib.embedding_fwd(data(ids), data(table), data(out), ids.numel(), table.size(0),
                           table.size(1), scale, ids.element_size(), code_of(table), on.stream),
@@ -173,10 +178,10 @@ Tensor embedding_lookup(const Tensor& ids, const Tensor& table, double scale,
 Tensor embedding_gradient(const Tensor& dy, const Tensor& ids, c10::SymInt table_rows,
                           double scale, int64_t padding) {
   const int64_t hidden = dy.size(-1), rows = table_rows.expect_int();
-  Tensor out = at::empty({rows, hidden}, dy.options());
+  Tensor out = fresh({rows, hidden}, dy.scalar_type(), dy);
   const size_t bytes = lib.embedding_bwd_workspace_bytes(ids.numel(), hidden);
   Tensor workspace;
-  if (bytes) workspace = at::empty({static_cast<int64_t>(bytes)}, dy.options().dtype(at::kByte));
+  if (bytes) workspace = fresh({static_cast<int64_t>(bytes)}, at::kByte, dy);
   On on(dy);
   check(lib.embedding_bwd(data(ids), data(dy), data(out), ids.numel(), rows, hidden, scale, padding,
                           ids.element_size(), code_of(dy), bytes ? data(workspace) : nullptr,

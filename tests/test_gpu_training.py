@@ -368,7 +368,7 @@ def _ids(kind, n, rows, seed=0):
     return torch.randint(0, rows, (n,), device="cuda", generator=gen)
 
 
-@pytest.mark.parametrize("n", [1, 2, 31, 32, 33, 64, 65, 1000, 1024, 1025, 4097])
+@pytest.mark.parametrize("n", [1, 2, 31, 32, 33, 64, 65, 255, 256, 257, 300, 1000, 1025, 4097])
 @pytest.mark.parametrize("kind", ["uniform", "one", "distinct", "frequent"])
 def test_embedding_tokens(dtype, n, kind):
     _check_embedding(_ids(kind, n, 513), 513, 96, dtype, seed=n)
@@ -379,19 +379,22 @@ def test_embedding_tables(rows):
     """Tables of one id up to three digits of the sort."""
 
     for padding in (None, 0, rows - 1):
-        _check_embedding(_ids("frequent", 700, rows), rows, 64, torch.bfloat16, 1.5, padding)
+        for n in (150, 700, 9000):
+            _check_embedding(_ids("frequent", n, rows), rows, 64, torch.bfloat16, 1.5, padding)
+    _check_embedding(_ids("frequent", 100, rows), rows, 13, torch.bfloat16)
 
 
 @pytest.mark.parametrize("hidden", [1, 2, 7, 8, 12, 64, 100, 250, 256, 264, 513, 768, 1024, 1537])
 def test_embedding_widths(dtype, hidden):
     _check_embedding(_ids("frequent", 211, 50).view(1, 211), 50, hidden, dtype, 27.7)
+    _check_embedding(_ids("frequent", 811, 50), 50, hidden, dtype, 27.7)
 
 
-@pytest.mark.parametrize("n", [16383, 16384, 16385, 40000])
+@pytest.mark.parametrize("n", [8191, 8192, 8193, 10240, 16385, 40000])
 @pytest.mark.parametrize("kind", ["uniform", "one", "frequent"])
 @pytest.mark.parametrize("rows", [2, 1500])
 def test_embedding_many_tokens(n, kind, rows):
-    """One sorted range, and several that are merged."""
+    """Either side of the forms for few, some and many tokens; ranges that are merged."""
 
     _check_embedding(_ids(kind, n, rows, n), rows, 72, torch.float16)
     _check_embedding(_ids(kind, n, rows, n), rows, 5, torch.float32, 2.0, 0)

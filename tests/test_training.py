@@ -247,10 +247,10 @@ def test_c_embedding_refusals(lib):
     for over in ({"ids": A + 4}, {"table": A + 1}, {"out": A + 1}):
         assert fwd(**over) == ALIGN, over
 
-    size = lib.dflash_embedding_bwd_workspace_bytes(40, 64)
+    size = lib.dflash_embedding_bwd_workspace_bytes(400, 64)
     assert size > 0 and lib.dflash_embedding_bwd_workspace_bytes(-1, 64) == 0
 
-    def bwd(ids=A, dout=A, dtable=A, n=40, rows=10, hidden=64, bytes_=8, dtype=1, ws=A, size=size):
+    def bwd(ids=A, dout=A, dtable=A, n=400, rows=10, hidden=64, bytes_=8, dtype=1, ws=A, size=size):
         return lib.dflash_embedding_bwd(ids, dout, dtable, n, rows, hidden, 1.0, -1, bytes_, dtype,
                                         ws, size, None)
 
