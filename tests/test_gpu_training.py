@@ -7,6 +7,7 @@ derived there; masks are compared as they are.
 from __future__ import annotations
 
 import copy
+import functools
 
 import pytest
 import torch
@@ -609,6 +610,45 @@ def test_calls_on_other_streams():
             assert torch.equal(a, c)
 
 
+def test_compiled_step_is_the_eager_one():
+    """Traced as one graph (fake implementations, the ops' autograd), run eagerly: equal bits."""
+
+    from disentangled_flash import training
+
+    leaves = _tail_leaves()
+    ids = _ids("frequent", 120, 300).view(4, 30)
+    state = training.DropoutState(6, "cuda")
+    rng = state.rng
+
+    def tail(table, ids, w, b, rng):
+        e = training.embedding(ids, table, 3.0, 0)
+        h = training.dropout(e, 0.2, rng, 1)
+        return training.layer_norm(h, w, b, 1e-6, residual=e, p=0.1, rng=rng, site=2)
+
+    want = _tail_step(leaves[0], ids, leaves[1], leaves[2], state)
+    y = torch.compile(tail, backend="aot_eager", fullgraph=True)(leaves[0], ids, leaves[1],
+                                                                 leaves[2], rng)
+    grads = torch.autograd.grad(y, leaves, 2 * y.detach())
+    for got, expected in zip((y.detach(), *grads), want):
+        assert torch.equal(got, expected)
+
+
+def test_residual_may_be_the_input():
+    """layer_norm(x, residual=x): both gradients reach the one leaf."""
+
+    from disentangled_flash.training import layer_norm
+
+    for p in (0.0, 0.3):
+        x, _, w, b, dy = _norm_case(13, 20, 192, torch.float32, torch.float32, False)
+        leaf = x.clone().requires_grad_()
+        layer_norm(leaf, w, b, 1e-5, residual=leaf, p=p, rng=_rng(), site=SITE).backward(dy)
+        mult = ref.factor((20, 192), p, _rng(), SITE)
+        want = ref.layer_norm(x, w, b, 1e-5, x, mult, dy)
+        value = want["dx"][0] + want["dresidual"][0]
+        bound = want["dx"][1] + want["dresidual"][1] + ref.rounding(value, torch.float32)
+        ref.check(leaf.grad, (value, bound), "both")
+
+
 def test_second_derivatives_raise():
     from disentangled_flash.training import dropout, embedding, layer_norm
 
@@ -733,6 +773,37 @@ def test_model_with_dropout_steps():
         run(leaf, r).square().sum().backward()
         grads.append(leaf.grad)
     assert torch.equal(grads[0], grads[1])
+
+
+def test_checkpointed_layers_recompute_their_own_forward():
+    """Two forwards before one backward pass over both, with and without checkpointed layers:
+    the same gradients.  (Other masks would change them by their own size.)"""
+
+    from torch.utils.checkpoint import checkpoint
+
+    from disentangled_flash import enable_deberta_training
+
+    grads = []
+    for checkpointed in (False, True):
+        model = enable_deberta_training(_backbone(0.2).cuda().train(), seed=8)
+        if checkpointed:
+            for layer in model.encoder.layer:
+                block = layer.output
+                block.forward = functools.partial(checkpoint, block.forward, use_reentrant=False)
+        ids, mask, types = _batch()
+        first = _loss(model, (ids, mask, types))
+        second = _loss(model, (ids.flip(0), mask.flip(0), types))
+        (first + second).backward()
+        third = _loss(model, (ids, mask, types))
+        third.backward()
+        grads.append({n: p.grad for n, p in model.named_parameters() if p.grad is not None})
+    assert grads[0].keys() == grads[1].keys()
+    for name in grads[0]:
+        # torch adds the gradients of the attention's gathers with atomics: the same terms in
+        # another order, through two layers and three forwards; 100 half steps of the largest.
+        size = grads[0][name].abs().max().item()
+        difference = (grads[1][name] - grads[0][name]).abs().max().item()
+        assert difference <= 100 * ref.U * size, (name, difference, size)
 
 
 def test_output_block_under_autocast():
