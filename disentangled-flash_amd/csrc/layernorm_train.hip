@@ -13,8 +13,17 @@
 // bytes a row.
 //
 // Layout: LANES lanes hold a row, CH chunks of 16 bytes a lane, so a row is read once and
-// stays in registers between its statistics and its output.  Rows that are not whole
-// chunks on 16-byte boundaries take the same kernels with element accesses.
+// stays in registers between its statistics and its output.  Rows that are not whole chunks
+// take the same accesses, on the 16-byte boundaries of the flattened tensor: a row then begins
+// `shift` elements inside its first chunk.  A group of lanes only meets rows of one shift (they
+// are a multiple of a chunk's elements apart), so its weights and the sums for their gradients
+// stay with the lanes; only a row's first and last chunk are written by elements.
+//
+// Bound by bytes: 16384 x 768 bf16 with residual and dropout 16.0 us forward (75 MB, 4.7 TB/s)
+// and 29.7 backward (129 MB with the partial rows, 4.3 TB/s, of which 4 us are the second
+// launch); 16384 x 1536 fp32 55 (5.5 TB/s) and 89 us (5.7).  A copy of as many bytes runs at
+// 4.8 to 5.4 TB/s.  16384 x 769 bf16: 22.4 and 39.4 us; 3059 x 1001: 10.5 and 18.1 (by
+// element accesses 17.0 and 28.0).
 
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -30,11 +39,13 @@ namespace {
 
 constexpr int kMaxHidden = 8192;
 // Workgroups of the backward pass: each adds up the weight gradients of its rows and writes
-// one fp32 partial row of each.
+// one fp32 partial row of each.  (16384 x 768 bf16: 256 35.8 us, 512 32.9, 768 34.1, 1024 36.0.)
 constexpr int kMaxPartials = 512;
-// Up to this many rows one workgroup takes them all, and there are no partial rows to add.
+// Up to this many rows one workgroup takes them all, and there are no partial rows to add: 17
+// rows of 768 take 9.8 us alone, 5.4 + 2.7 and the gap between them in two launches, of
+// which the host is spared one.
 constexpr int kAloneRows = 32;
-// Workgroups of the forward pass.
+// Workgroups of the forward pass.  (16384 x 768 bf16: 1024 15.9 us, 2048 16.6; 1536 fp32 55, 58.)
 constexpr int kMaxForward = 1024;
 
 struct Forward {
@@ -114,42 +125,44 @@ __device__ inline void row_sum(float (&v)[VALUES], float (*lds)[VALUES]) {
 // that the registers of their fp32 values and of the loads in flight are not the same ones.
 // LAST: nobody reads them after the kernel (the forward pass's rows are read again by the
 // backward pass).
-template <typename T, int LANES, int CH, bool WIDE, bool LAST>
+template <typename T, int LANES, int CH, bool WHOLE, bool LAST>
 struct RowInput {
   static constexpr int N = Chunk<T>::N;
-  RowChunk<T, N, WIDE, LAST> x[CH], r[CH];
+  RowChunk<T, WHOLE, LAST> x[CH], r[CH];
 
-  __device__ void load(const T* xs, const T* rs, int64_t base, int hidden, int sub) {
+  __device__ void load(const T* xs, const T* rs, int64_t base, int col, int first_col, int hidden,
+                       int64_t total) {
 #pragma unroll
-    for (int k = 0; k < CH; ++k) x[k].load(xs + base, (sub + LANES * k) * N, hidden);
+    for (int k = 0; k < CH; ++k) x[k].load(xs, base, col + LANES * N * k, first_col, hidden, total);
     if (rs) {
 #pragma unroll
-      for (int k = 0; k < CH; ++k) r[k].load(rs + base, (sub + LANES * k) * N, hidden);
+      for (int k = 0; k < CH; ++k)
+        r[k].load(rs, base, col + LANES * N * k, first_col, hidden, total);
     }
   }
 
-  // s = drop(x) + r (0 past the row's end); `dropped`: the masks of the chunks, drawn while
-  // the loads are in flight.
-  __device__ void sum(bool has_r, int64_t base, int hidden, int sub, const Dropout& drop,
+  // s = drop(x) + r (0 outside the row); `dropped`: the masks of the chunks, drawn while the
+  // loads are in flight.
+  __device__ void sum(bool has_r, int64_t base, int col, int hidden, const Dropout& drop,
                       DropoutKey key, float (&s)[CH][N], uint32_t (&dropped)[CH]) const {
     if (drop.active) {
 #pragma unroll
       for (int k = 0; k < CH; ++k)
-        dropped[k] = dropped_from<N, WIDE>(drop, key, base + (sub + LANES * k) * N);
+        dropped[k] = dropped_from<N>(drop, key, base + col + LANES * N * k);
 #pragma unroll
       for (int k = 0; k < CH; ++k) {
-        x[k].floats((sub + LANES * k) * N, hidden, s[k]);
+        x[k].floats(col + LANES * N * k, hidden, s[k]);
         apply_dropout(drop, dropped[k], s[k]);
       }
     } else {
 #pragma unroll
-      for (int k = 0; k < CH; ++k) x[k].floats((sub + LANES * k) * N, hidden, s[k]);
+      for (int k = 0; k < CH; ++k) x[k].floats(col + LANES * N * k, hidden, s[k]);
     }
     if (has_r) {
 #pragma unroll
       for (int k = 0; k < CH; ++k) {
         float v[N];
-        r[k].floats((sub + LANES * k) * N, hidden, v);
+        r[k].floats(col + LANES * N * k, hidden, v);
 #pragma unroll
         for (int e = 0; e < N; ++e) s[k][e] += v[e];
       }
@@ -158,8 +171,9 @@ struct RowInput {
 };
 
 // A workgroup walks its rows, every gridDim-th group of kThreads / LANES rows.  (LANES = 256:
-// the row is the workgroup's, so every thread makes the same rounds.)
-template <typename T, typename W, int LANES, int CH, bool WIDE>
+// the row is the workgroup's, so every thread makes the same rounds.)  Without WHOLE the step is
+// a multiple of N or there is no second round (the launch sees to it).
+template <typename T, typename W, int LANES, int CH, bool WHOLE>
 __global__ __launch_bounds__(kThreads) void layernorm_train_fwd_kernel(Forward a) {
   constexpr int N = Chunk<T>::N;
   constexpr int kGroups = kThreads / LANES;
@@ -172,21 +186,24 @@ __global__ __launch_bounds__(kThreads) void layernorm_train_fwd_kernel(Forward a
   const float width = static_cast<float>(hidden);
   const T* x = static_cast<const T*>(a.x);
   const T* r = static_cast<const T*>(a.residual);
-  RowInput<T, LANES, CH, WIDE, false> in;
-  in.load(x, r, row * hidden, hidden, sub);
-  RowChunk<W, N, WIDE, false> gamma[CH], beta[CH];
+  const int64_t total = a.rows * hidden;
+  const int first_col = WHOLE ? 0 : -static_cast<int>(row * hidden % N);
+  const int lane_col = sub * N + first_col;  // + LANES * N a chunk
+  RowInput<T, LANES, CH, WHOLE, false> in;
+  in.load(x, r, row * hidden, lane_col, first_col, hidden, total);
+  WeightChunk<W, N, WHOLE> gamma[CH], beta[CH];
 #pragma unroll
   for (int k = 0; k < CH; ++k) {
-    gamma[k].load(static_cast<const W*>(a.gamma), (sub + LANES * k) * N, hidden);
-    beta[k].load(static_cast<const W*>(a.beta), (sub + LANES * k) * N, hidden);
+    gamma[k].load(static_cast<const W*>(a.gamma), lane_col + LANES * N * k, hidden);
+    beta[k].load(static_cast<const W*>(a.beta), lane_col + LANES * N * k, hidden);
   }
   const DropoutKey key = dropout_key(a.drop);
   for (;;) {
     float s[CH][N];
     uint32_t dropped[CH];
-    in.sum(r != nullptr, row * hidden, hidden, sub, a.drop, key, s, dropped);
+    in.sum(r != nullptr, row * hidden, lane_col, hidden, a.drop, key, s, dropped);
     const int64_t next = row + step;
-    if (next < a.rows) in.load(x, r, next * hidden, hidden, sub);
+    if (next < a.rows) in.load(x, r, next * hidden, lane_col, first_col, hidden, total);
     float sum[1] = {0.0f};
 #pragma unroll
     for (int k = 0; k < CH; ++k) {
@@ -199,12 +216,12 @@ __global__ __launch_bounds__(kThreads) void layernorm_train_fwd_kernel(Forward a
     float sq[1] = {0.0f};
 #pragma unroll
     for (int k = 0; k < CH; ++k) {
-      const int col = (sub + LANES * k) * N;
+      const int col = lane_col + LANES * N * k;
 #pragma unroll
       for (int e = 0; e < N; ++e) {
         s[k][e] -= mean;
-        const float live = (WIDE ? col : col + e) < hidden ? s[k][e] : 0.0f;
-        sq[0] += live * live;
+        const bool live = WHOLE ? col < hidden : col + e >= 0 && col + e < hidden;
+        sq[0] += live ? s[k][e] * s[k][e] : 0.0f;
       }
     }
     row_sum<LANES>(sq, lds);
@@ -215,15 +232,15 @@ __global__ __launch_bounds__(kThreads) void layernorm_train_fwd_kernel(Forward a
     }
 #pragma unroll
     for (int k = 0; k < CH; ++k) {
-      const int col = (sub + LANES * k) * N;
       float g[N], b[N];
       gamma[k].renew();
       beta[k].renew();
-      gamma[k].floats(col, hidden, g);
-      beta[k].floats(col, hidden, b);
+      gamma[k].floats(g);
+      beta[k].floats(b);
 #pragma unroll
       for (int e = 0; e < N; ++e) g[e] = s[k][e] * rstd * g[e] + b[e];
-      store_chunk<T, N, WIDE>(static_cast<T*>(a.y) + row * hidden, col, hidden, g);
+      store_chunk<T, WHOLE>(static_cast<T*>(a.y), row * hidden, lane_col + LANES * N * k, hidden,
+                            g);
     }
     if (next >= a.rows) return;
     row = next;
@@ -232,7 +249,7 @@ __global__ __launch_bounds__(kThreads) void layernorm_train_fwd_kernel(Forward a
 
 // As above, with the sums for dgamma and dbeta of the lane's columns in registers; at the end
 // the lanes that hold the same columns are added in order and one partial row is written.
-template <typename T, typename W, int LANES, int CH, bool WIDE>
+template <typename T, typename W, int LANES, int CH, bool WHOLE>
 __global__ __launch_bounds__(kThreads) void layernorm_train_bwd_kernel(Backward a) {
   constexpr int N = Chunk<T>::N;
   constexpr int kGroups = kThreads / LANES;
@@ -247,27 +264,31 @@ __global__ __launch_bounds__(kThreads) void layernorm_train_bwd_kernel(Backward 
   const T* dy = static_cast<const T*>(a.dy);
   int64_t row = static_cast<int64_t>(blockIdx.x) * kGroups + group;
   const int64_t step = static_cast<int64_t>(gridDim.x) * kGroups;
-  RowInput<T, LANES, CH, WIDE, true> in;
-  RowChunk<T, N, WIDE, true> dys[CH];
-  RowChunk<W, N, WIDE, false> gamma[CH];
+  const int64_t total = a.rows * hidden;
+  const int first_col = WHOLE ? 0 : -static_cast<int>(row * hidden % N);
+  const int lane_col = sub * N + first_col;  // + LANES * N a chunk
+  RowInput<T, LANES, CH, WHOLE, true> in;
+  RowChunk<T, WHOLE, true> dys[CH];
+  WeightChunk<W, N, WHOLE> gamma[CH];
   float mean = 0.0f, rstd = 0.0f;
   auto load = [&](int64_t at) {
 #pragma unroll
-    for (int k = 0; k < CH; ++k) dys[k].load(dy + at * hidden, (sub + LANES * k) * N, hidden);
-    in.load(x, r, at * hidden, hidden, sub);
+    for (int k = 0; k < CH; ++k)
+      dys[k].load(dy, at * hidden, lane_col + LANES * N * k, first_col, hidden, total);
+    in.load(x, r, at * hidden, lane_col, first_col, hidden, total);
     mean = a.mean[at];
     rstd = a.rstd[at];
   };
   // Narrow rows are loaded one ahead (1024 fp16, no dropout, 16384 rows: 27.5 -> 24.2 us); where
   // their registers cost wavefronts, not (1536 fp32: 98.7 ahead, 89.6 not; 1536 bf16 52.9,
   // 52.0; 768 bf16 30.2, 29.7).
-  constexpr bool kAhead = WIDE && LANES <= 64 && CH <= 2;
+  constexpr bool kAhead = WHOLE && LANES <= 64 && CH <= 2;
   if (kAhead && row < a.rows) load(row);
   const DropoutKey key = dropout_key(a.drop);
   float dgamma[CH][N], dbeta[CH][N];
 #pragma unroll
   for (int k = 0; k < CH; ++k) {
-    gamma[k].load(static_cast<const W*>(a.gamma), (sub + LANES * k) * N, hidden);
+    gamma[k].load(static_cast<const W*>(a.gamma), lane_col + LANES * N * k, hidden);
 #pragma unroll
     for (int e = 0; e < N; ++e) dgamma[k][e] = dbeta[k][e] = 0.0f;
   }
@@ -276,9 +297,9 @@ __global__ __launch_bounds__(kThreads) void layernorm_train_bwd_kernel(Backward 
     const int64_t base = row * hidden;
     float g[CH][N], xh[CH][N];
     uint32_t dropped[CH];
-    in.sum(r != nullptr, base, hidden, sub, a.drop, key, xh, dropped);
+    in.sum(r != nullptr, base, lane_col, hidden, a.drop, key, xh, dropped);
 #pragma unroll
-    for (int k = 0; k < CH; ++k) dys[k].floats((sub + LANES * k) * N, hidden, g[k]);
+    for (int k = 0; k < CH; ++k) dys[k].floats(lane_col + LANES * N * k, hidden, g[k]);
     const float row_mean = mean, row_rstd = rstd;
     row += step;
     if (kAhead && row < a.rows) load(row);
@@ -287,8 +308,8 @@ __global__ __launch_bounds__(kThreads) void layernorm_train_bwd_kernel(Backward 
     for (int k = 0; k < CH; ++k) {
       float w[N];
       gamma[k].renew();
-      gamma[k].floats((sub + LANES * k) * N, hidden, w);
-      // (Past the row's end g is 0, so xh adds nothing there.)
+      gamma[k].floats(w);
+      // (Outside the row g is 0, so xh adds nothing there.)
 #pragma unroll
       for (int e = 0; e < N; ++e) {
         xh[k][e] = (xh[k][e] - row_mean) * row_rstd;
@@ -304,14 +325,14 @@ __global__ __launch_bounds__(kThreads) void layernorm_train_bwd_kernel(Backward 
     const float g_mean = sums[0] / width, gx_mean = sums[1] / width;
 #pragma unroll
     for (int k = 0; k < CH; ++k) {
-      const int col = (sub + LANES * k) * N;
+      const int col = lane_col + LANES * N * k;
 #pragma unroll
       for (int e = 0; e < N; ++e) g[k][e] = row_rstd * (g[k][e] - g_mean - xh[k][e] * gx_mean);
       if (a.dresidual)
-        store_chunk<T, N, WIDE>(static_cast<T*>(a.dresidual) + base, col, hidden, g[k]);
+        store_chunk<T, WHOLE>(static_cast<T*>(a.dresidual), base, col, hidden, g[k]);
       if (a.dx) {
         if (a.drop.active) apply_dropout(a.drop, dropped[k], g[k]);
-        store_chunk<T, N, WIDE>(static_cast<T*>(a.dx) + base, col, hidden, g[k]);
+        store_chunk<T, WHOLE>(static_cast<T*>(a.dx), base, col, hidden, g[k]);
       }
     }
   }
@@ -332,7 +353,10 @@ __global__ __launch_bounds__(kThreads) void layernorm_train_bwd_kernel(Backward 
 #pragma unroll
       for (int k = 0; k < CH; ++k) {
 #pragma unroll
-        for (int e = 0; e < N; ++e) part[group][(sub + LANES * k) * N + e] = acc[k][e];
+        for (int e = 0; e < N; ++e) {
+          const int col = lane_col + LANES * N * k + e;
+          if (WHOLE || (col >= 0 && col < hidden)) part[group][col] = acc[k][e];
+        }
       }
       __syncthreads();
       for (int col = threadIdx.x; col < hidden; col += kThreads) {
@@ -344,10 +368,10 @@ __global__ __launch_bounds__(kThreads) void layernorm_train_bwd_kernel(Backward 
     } else {
 #pragma unroll
       for (int k = 0; k < CH; ++k) {
-        const int col = (sub + LANES * k) * N;
+        const int col = lane_col + LANES * N * k;
 #pragma unroll
         for (int e = 0; e < N; ++e)
-          if (col + e < hidden) put(which, col + e, acc[k][e]);
+          if (col + e >= 0 && col + e < hidden) put(which, col + e, acc[k][e]);
       }
     }
   }
@@ -383,16 +407,21 @@ __global__ __launch_bounds__(16 * kSlices) void layernorm_weight_grad_kernel(
   }
 }
 
-// Calls go(LANES, CH, WIDE) with the smallest layout that holds a row of `hidden` elements.
+// Calls go(LANES, CH, WHOLE) with the smallest layout that holds a row of `hidden` elements: few
+// chunks a lane, for their registers (1024 16-bit: 32 lanes of 4 chunks 32.5 us backward, 64 of
+// 2 24.2), but 32 lanes of 3 before 64 of 2 half empty (768: 33.0, 34.8), and a row in
+// one wavefront where three chunks a lane hold it (1536: 55.4, a workgroup a row 76.3).
 template <typename T, typename Go>
-int with_layout(int hidden, bool wide, Go go) {
-  const int chunks = (hidden + Chunk<T>::N - 1) / Chunk<T>::N;
-#define DFLASH_LAYOUT(L, C)                                                            \
-  if (chunks <= L * C)                                                                 \
-    return wide ? go(std::integral_constant<int, L>(), std::integral_constant<int, C>(), \
-                     std::true_type())                                                 \
-                : go(std::integral_constant<int, L>(), std::integral_constant<int, C>(), \
-                     std::false_type());
+int with_layout(int hidden, bool whole, Go go) {
+  constexpr int N = Chunk<T>::N;
+  // A row that begins inside a chunk may touch one more.
+  const int chunks = whole ? hidden / N : (hidden + 2 * (N - 1)) / N;
+#define DFLASH_LAYOUT(L, C)                                                              \
+  if (chunks <= L * C)                                                                   \
+    return whole ? go(std::integral_constant<int, L>(), std::integral_constant<int, C>(), \
+                      std::true_type())                                                  \
+                 : go(std::integral_constant<int, L>(), std::integral_constant<int, C>(), \
+                      std::false_type());
   DFLASH_LAYOUT(16, 1)
   DFLASH_LAYOUT(32, 1)
   DFLASH_LAYOUT(32, 2)
@@ -402,41 +431,49 @@ int with_layout(int hidden, bool wide, Go go) {
   DFLASH_LAYOUT(64, 4)
   DFLASH_LAYOUT(256, 2)
   DFLASH_LAYOUT(256, 4)
-  if constexpr (Chunk<T>::N == 4) {
+  if constexpr (N == 4) {
     DFLASH_LAYOUT(256, 8)
+    DFLASH_LAYOUT(256, 9)  // 8191 elements that begin inside a chunk
+  } else {
+    DFLASH_LAYOUT(256, 5)
   }
 #undef DFLASH_LAYOUT
   return DFLASH_ERR_SHAPE;
 }
 
 template <typename T, typename W>
-int launch_forward(const Forward& a, bool wide, hipStream_t stream) {
-  return with_layout<T>(a.hidden, wide, [&](auto lanes, auto ch, auto is_wide) {
+int launch_forward(const Forward& a, bool whole, hipStream_t stream) {
+  return with_layout<T>(a.hidden, whole, [&](auto lanes, auto ch, auto is_whole) {
     constexpr int kLanes = decltype(lanes)::value, kCh = decltype(ch)::value;
     constexpr int kRows = kThreads / kLanes;
     const int64_t blocks = (a.rows + kRows - 1) / kRows;
     const int count = static_cast<int>(blocks < kMaxForward ? blocks : kMaxForward);
-    hipLaunchKernelGGL((layernorm_train_fwd_kernel<T, W, kLanes, kCh, decltype(is_wide)::value>),
+    hipLaunchKernelGGL((layernorm_train_fwd_kernel<T, W, kLanes, kCh, decltype(is_whole)::value>),
                        dim3(count), dim3(kThreads), 0, stream, a);
     return static_cast<int>(hipGetLastError());
   });
 }
 
-int64_t partial_rows(int64_t rows) {
-  return rows <= kAloneRows ? 0 : rows < kMaxPartials ? rows : kMaxPartials;
+// (Rows that are not whole chunks have their second round only a multiple of 8 rows on, which
+// kMaxForward and kMaxPartials workgroups are apart and one workgroup is not.)
+static_assert(kMaxForward % 8 == 0 && kMaxPartials % 8 == 0, "a multiple of a chunk's elements");
+bool alone(int64_t rows, int hidden) { return rows <= kAloneRows && hidden % 8 == 0; }
+
+int64_t partial_rows(int64_t rows, int hidden) {
+  return alone(rows, hidden) ? 0 : rows < kMaxPartials ? rows : kMaxPartials;
 }
 
 template <typename T, typename W>
-int launch_backward(const Backward& a, bool wide, hipStream_t stream) {
+int launch_backward(const Backward& a, bool whole, hipStream_t stream) {
   int count = 0;
   if (a.rows > 0) {
-    const int rc = with_layout<T>(a.hidden, wide, [&](auto lanes, auto ch, auto is_wide) {
+    const int rc = with_layout<T>(a.hidden, whole, [&](auto lanes, auto ch, auto is_whole) {
       constexpr int kLanes = decltype(lanes)::value, kCh = decltype(ch)::value;
       constexpr int kRows = kThreads / kLanes;
       const int64_t blocks = (a.rows + kRows - 1) / kRows;
       count = static_cast<int>(blocks < kMaxPartials ? blocks : kMaxPartials);
-      if (a.rows <= kAloneRows) count = 1;
-      hipLaunchKernelGGL((layernorm_train_bwd_kernel<T, W, kLanes, kCh, decltype(is_wide)::value>),
+      if (alone(a.rows, a.hidden)) count = 1;
+      hipLaunchKernelGGL((layernorm_train_bwd_kernel<T, W, kLanes, kCh, decltype(is_whole)::value>),
                          dim3(count), dim3(kThreads), 0, stream, a);
       return static_cast<int>(hipGetLastError());
     });
@@ -493,17 +530,17 @@ extern "C" int dflash_dropout_layernorm_fwd(const void* x, const void* residual,
       return static_cast<int>(DFLASH_ERR_NULL);
     const uintptr_t rows_or = address(x) | address(residual) | address(y);
     const uintptr_t weights_or = address(gamma) | address(beta);
-    if (rows_or % sizeof(T) != 0 || weights_or % sizeof(W) != 0 ||
+    if (rows_or % 16 != 0 || weights_or % sizeof(W) != 0 ||
         (address(mean) | address(rstd)) % 4 != 0 || address(rng) % 8 != 0)
       return static_cast<int>(DFLASH_ERR_ALIGN);
-    const bool wide = hidden % Chunk<T>::N == 0 && (rows_or | weights_or) % 16 == 0;
-    return launch_forward<T, W>(a, wide, static_cast<hipStream_t>(stream));
+    const bool whole = hidden % Chunk<T>::N == 0 && weights_or % 16 == 0;
+    return launch_forward<T, W>(a, whole, static_cast<hipStream_t>(stream));
   });
 }
 
 extern "C" size_t dflash_dropout_layernorm_bwd_workspace_bytes(int64_t rows, int hidden) {
   if (!shape_taken(rows, hidden)) return 0;
-  return static_cast<size_t>(partial_rows(rows)) * 2 * hidden * sizeof(float);
+  return static_cast<size_t>(partial_rows(rows, hidden)) * 2 * hidden * sizeof(float);
 }
 
 extern "C" int dflash_dropout_layernorm_bwd(
@@ -523,16 +560,16 @@ extern "C" int dflash_dropout_layernorm_bwd(
     const uintptr_t rows_or = address(dy) | address(x) | address(residual) | address(dx) |
                               address(dresidual);
     const uintptr_t weights_or = address(gamma) | address(dgamma) | address(dbeta);
-    if (rows_or % sizeof(T) != 0 || weights_or % sizeof(W) != 0 ||
+    if (rows_or % 16 != 0 || weights_or % sizeof(W) != 0 ||
         (address(mean) | address(rstd) | address(workspace)) % 4 != 0 || address(rng) % 8 != 0)
       return static_cast<int>(DFLASH_ERR_ALIGN);
-    if (dgamma && partial_rows(rows) > 0) {
+    if (dgamma && partial_rows(rows, hidden) > 0) {
       if (!workspace) return static_cast<int>(DFLASH_ERR_NULL);
       if (workspace_bytes < dflash_dropout_layernorm_bwd_workspace_bytes(rows, hidden))
         return static_cast<int>(DFLASH_ERR_WORKSPACE);
     }
     if (!dx && !dresidual && !dgamma) return static_cast<int>(DFLASH_OK);
-    const bool wide = hidden % Chunk<T>::N == 0 && rows_or % 16 == 0 && address(gamma) % 16 == 0;
-    return launch_backward<T, W>(a, wide, static_cast<hipStream_t>(stream));
+    const bool whole = hidden % Chunk<T>::N == 0 && address(gamma) % 16 == 0;
+    return launch_backward<T, W>(a, whole, static_cast<hipStream_t>(stream));
   });
 }

@@ -91,6 +91,11 @@ Tensor fresh(at::IntArrayRef sizes, at::ScalarType type, const Tensor& like) {
 }
 Tensor fresh_like(const Tensor& t) { return fresh(t.sizes(), t.scalar_type(), t); }
 
+// The LayerNorm's rows start on 16-byte boundaries.
+bool is_aligned(const Tensor& t) { return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0; }
+Tensor aligned(const Tensor& t) { return is_aligned(t) ? t : t.clone(); }
+MaybeTensor aligned(const MaybeTensor& t) { return t && !is_aligned(*t) ? t->clone() : t; }
+
 void* data(const Tensor& t) { return t.data_ptr(); }
 void* data(const MaybeTensor& t) { return t ? t->data_ptr() : nullptr; }
 const int64_t* words(const MaybeTensor& rng) {
@@ -107,9 +112,11 @@ Tensor dropout(const Tensor& x, const Tensor& rng, double p, int64_t site) {
   return out;
 }
 
-Tensor layernorm(const Tensor& x, const MaybeTensor& residual, const Tensor& weight,
+Tensor layernorm(const Tensor& given, const MaybeTensor& given_residual, const Tensor& weight,
                  const Tensor& bias, const MaybeTensor& rng, double eps, double p, int64_t site,
                  float* statistics) {
+  const Tensor x = aligned(given);
+  const MaybeTensor residual = aligned(given_residual);
   Tensor y = fresh_like(x);
   const int64_t hidden = x.size(-1), rows = x.numel() / hidden;
   On on(x);
@@ -139,9 +146,11 @@ std::tuple<Tensor, Tensor> dropout_layernorm_train(const Tensor& x, const MaybeT
 
 // (dx, dresidual, dweight, dbias); those not wanted are empty.
 std::tuple<Tensor, Tensor, Tensor, Tensor> dropout_layernorm_backward(
-    const Tensor& dy, const Tensor& x, const MaybeTensor& residual, const Tensor& weight,
-    const Tensor& statistics, const MaybeTensor& rng, double p, int64_t site, bool want_x,
-    bool want_residual, bool want_weights) {
+    const Tensor& given_dy, const Tensor& given, const MaybeTensor& given_residual,
+    const Tensor& weight, const Tensor& statistics, const MaybeTensor& rng, double p, int64_t site,
+    bool want_x, bool want_residual, bool want_weights) {
+  const Tensor dy = aligned(given_dy), x = aligned(given);
+  const MaybeTensor residual = aligned(given_residual);
   const int64_t hidden = x.size(-1), rows = x.numel() / hidden;
   auto made = [](bool wanted, const Tensor& like) {
     return wanted ? fresh_like(like) : fresh({0}, like.scalar_type(), like);

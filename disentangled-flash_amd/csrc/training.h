@@ -83,17 +83,12 @@ __device__ inline uint32_t dropped_of_block(const Dropout& d, DropoutKey key, in
   return bits;
 }
 
-// Bit e: element `first + e` of the flattened tensor is dropped, for e < N.  WHOLE: first is a
-// multiple of N, so that the N elements lie in one block.
-template <int N, bool WHOLE>
+// Bit e: element `first + e` of the flattened tensor is dropped, for e < N; `first` is a multiple
+// of N, so that the N elements lie in one block.
+template <int N>
 __device__ inline uint32_t dropped_from(const Dropout& d, DropoutKey key, int64_t first) {
-  const int at = static_cast<int>(first & 7);
-  uint32_t bits = dropped_of_block(d, key, first >> 3);
-  if constexpr (!WHOLE) {
-    if (at + N > 8) bits |= dropped_of_block(d, key, (first >> 3) + 1) << 8;
-  }
-  if constexpr (!WHOLE || N < 8) bits >>= at;
-  return bits;
+  const uint32_t bits = dropped_of_block(d, key, first >> 3);
+  return N < 8 ? bits >> (first & 7) : bits;
 }
 
 template <int N>
@@ -117,74 +112,98 @@ inline bool make_dropout(double p, const int64_t* rng, uint32_t site, Dropout& d
   return true;
 }
 
-// The chunk at column `col` of a row of `width` elements.  WIDE: rows are whole chunks from
-// 16-byte boundaries.  Otherwise element loads.  Either way every load is made, past the row's
-// end from a place inside it (a branch would wait for each load by itself);
-// floats() puts the zeros there.  STREAM: read once (past the L2's other lines).
-template <typename T, int N, bool WIDE, bool STREAM = false>
+// A chunk of a tensor of rows, in registers.  Chunks lie on 16-byte boundaries of the flattened
+// tensor.  WHOLE: rows are whole chunks.  Otherwise a row begins and ends inside a chunk; the
+// column `col` of a chunk's first element may then be negative, and elements outside
+// [0, width) belong to the neighbouring rows.
+// Every load is made (for a chunk past the row's end of its first chunk): a branch would wait
+// for each load by itself.  STREAM: read once (past the L2's other lines).
+template <typename T, bool WHOLE, bool STREAM>
 struct RowChunk {
-  static constexpr int kPieces = N / Chunk<T>::N;  // 2: fp32 weights beside 16-bit rows
-  typename Chunk<T>::type v[kPieces];
+  static constexpr int N = Chunk<T>::N;
+  using Vector = typename Chunk<T>::type;
+  Vector v;
 
-  __device__ void load(const T* row, int col, int width) {
-    constexpr int C = Chunk<T>::N;
-    if constexpr (WIDE) {
-      const T* from = row + (col < width ? col : 0);
-#pragma unroll
-      for (int c = 0; c < kPieces; ++c) {
-        const auto* p = reinterpret_cast<const typename Chunk<T>::type*>(from + c * C);
-        if constexpr (STREAM)
-          v[c] = __builtin_nontemporal_load(p);
-        else
-          v[c] = *p;
-      }
+  // `base`: the row's first element, `first_col`: the column of its first chunk; `total`: the
+  // tensor's elements, whose last chunk may be a part of one.
+  __device__ void load(const T* tensor, int64_t base, int col, int first_col, int width,
+                       int64_t total) {
+    const int64_t at = base + (col < width ? col : first_col);
+    if (WHOLE || at + N <= total) {
+      const auto* p = reinterpret_cast<const Vector*>(tensor + at);
+      if constexpr (STREAM)
+        v = __builtin_nontemporal_load(p);
+      else
+        v = *p;
     } else {
 #pragma unroll
-      for (int c = 0; c < kPieces; ++c) {
+      for (int e = 0; e < N; ++e) v[e] = tensor[at + e < total ? at + e : total - 1];
+    }
+  }
+
+  __device__ void floats(int col, int width, float (&out)[N]) const {
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      const bool live = WHOLE ? col < width : col + e >= 0 && col + e < width;
+      out[e] = live ? static_cast<float>(v[e]) : 0.0f;
+    }
+  }
+};
+
+// The weights of a chunk's columns (fp32 beside 16-bit rows: two accesses).
+template <typename W, int N, bool WHOLE>
+struct WeightChunk {
+  static constexpr int C = Chunk<W>::N, kPieces = N / C;
+  typename Chunk<W>::type v[kPieces];
+
+  __device__ void load(const W* weights, int col, int width) {
+#pragma unroll
+    for (int c = 0; c < kPieces; ++c) {
+      if constexpr (WHOLE) {
+        v[c] = *reinterpret_cast<const typename Chunk<W>::type*>(
+            weights + (col < width ? col : 0) + c * C);
+      } else {
 #pragma unroll
         for (int e = 0; e < C; ++e) {
           const int at = col + c * C + e;
-          v[c][e] = row[at < width ? at : width - 1];
+          v[c][e] = weights[at < 0 ? 0 : at < width ? at : width - 1];
         }
       }
     }
   }
 
-  // Makes the compiler take the chunk as new here: what is computed from a chunk that is the
-  // same for every row (its fp32 values) is not kept in registers across the rows' loop.
+  // Makes the compiler take the weights as new here: their fp32 values, the same for every
+  // row, are not kept in registers across the rows' loop.
   __device__ void renew() {
 #pragma unroll
     for (int c = 0; c < kPieces; ++c) asm volatile("" : "+v"(v[c]));
   }
 
-  __device__ void floats(int col, int width, float (&out)[N]) const {
-    constexpr int C = Chunk<T>::N;
+  __device__ void floats(float (&out)[N]) const {
 #pragma unroll
     for (int c = 0; c < kPieces; ++c) {
 #pragma unroll
-      for (int e = 0; e < C; ++e) {
-        const bool live = (WIDE ? col : col + c * C + e) < width;
-        out[c * C + e] = live ? static_cast<float>(v[c][e]) : 0.0f;
-      }
+      for (int e = 0; e < C; ++e) out[c * C + e] = static_cast<float>(v[c][e]);
     }
   }
 };
 
 // Outputs are written once: non-temporal, 10 % of a pass over rows (LayerNorm forward of
 // 16384 x 768 bf16 17.9 -> 15.9 us, backward 32.8 -> 30.6; of 4096 rows 6.0 -> 5.5, 14.4 -> 12.5).
-template <typename T, int N, bool WIDE>
-__device__ inline void store_chunk(T* row, int col, int width, const float (&in)[N]) {
-  if constexpr (WIDE) {
-    static_assert(N == Chunk<T>::N, "one chunk");
+template <typename T, bool WHOLE>
+__device__ inline void store_chunk(T* tensor, int64_t base, int col, int width,
+                                   const float (&in)[Chunk<T>::N]) {
+  constexpr int N = Chunk<T>::N;
+  if (WHOLE ? col < width : col >= 0 && col + N <= width) {
     typename Chunk<T>::type v;
 #pragma unroll
     for (int e = 0; e < N; ++e) v[e] = static_cast<T>(in[e]);
-    if (col < width)
-      __builtin_nontemporal_store(v, reinterpret_cast<typename Chunk<T>::type*>(row + col));
-  } else {
+    __builtin_nontemporal_store(v,
+                                reinterpret_cast<typename Chunk<T>::type*>(tensor + base + col));
+  } else if constexpr (!WHOLE) {
 #pragma unroll
     for (int e = 0; e < N; ++e)
-      if (col + e < width) row[col + e] = static_cast<T>(in[e]);
+      if (col + e >= 0 && col + e < width) tensor[base + col + e] = static_cast<T>(in[e]);
   }
 }
 

@@ -26,11 +26,13 @@ to a thread of its own: under ``torch.autograd.set_multithreading_enabled(False)
 gradients of a norm tail took 28 us of host time instead of 61.
 
 Work is launched on torch's current stream of the inputs' device.  Second derivatives raise,
-but for dropout's.  Inputs that are not contiguous are copied first.
+but for dropout's.  Inputs that are not contiguous are copied first, and in :func:`layer_norm`
+those that do not start on a 16-byte boundary.
 """
 
 from __future__ import annotations
 
+import threading
 from collections.abc import Mapping
 from typing import Any
 
@@ -45,13 +47,22 @@ MAX_HIDDEN = 8192  # widest row of layer_norm
 class _Ops:
     """The torch operators (``csrc/torch_ops.cpp``), loaded at the first call."""
 
+    names = ("dropout", "dropout_layernorm", "embedding_lookup")
+
     def __getattr__(self, name: str) -> Any:
-        _lib.load_torch_ops()
-        _register_fakes()
-        namespace = torch.ops.disentangled_flash
-        for op in ("dropout", "dropout_layernorm", "embedding_lookup"):
-            setattr(self, op, getattr(namespace, op).default)
+        if name not in self.names:
+            raise AttributeError(name)
+        with _loading:
+            if name not in self.__dict__:
+                _lib.load_torch_ops()
+                _register_fakes()
+                namespace = torch.ops.disentangled_flash
+                for op in self.names:
+                    setattr(self, op, getattr(namespace, op).default)
         return self.__dict__[name]
+
+
+_loading = threading.Lock()
 
 
 _ops = _Ops()

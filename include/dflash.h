@@ -349,8 +349,9 @@ DFLASH_API int dflash_encoder_layer_fwd(const dflash_encoder_layer* layer, const
  *   rng  : device int64 [2] = seed, step (the step's low 32 bits are used); read by the kernels;
  *          may be NULL when p is 0
  *   site : numbers the places of a model that drop elements
- * Pointers need the alignment of their element type only; rows of whole 16-byte chunks on
- * 16-byte boundaries are faster.  Outputs must not overlap inputs.  The workspaces' contents
+ * Pointers need the alignment of their element type, where not said otherwise; tensors on
+ * 16-byte boundaries with rows of whole 16-byte chunks are faster.  Outputs must not overlap
+ * inputs.  The workspaces' contents
  * need not outlive the kernels; calls that share one must not overlap.
  */
 
@@ -361,7 +362,8 @@ DFLASH_API int dflash_dropout(const void* x, void* y, int64_t n, double p, const
 /*
  * y = LayerNorm(drop(x) + residual), the tail of DebertaV2SelfOutput / DebertaV2Output in
  * training (/root/reference/src/disentangled_flash/_reference.py:101-112, 474-485).
- *   x, residual, y : [rows, hidden], dtype `dtype`; residual may be NULL; hidden 1 to 8192
+ *   x, residual, y : [rows, hidden], dtype `dtype`, 16-byte aligned; residual may be NULL;
+ *                    hidden 1 to 8192
  *   gamma, beta    : [hidden], `weight_dtype`: `dtype` or fp32
  *   mean, rstd     : fp32 [rows], kept for the backward pass; both may be NULL
  * All in fp32, y rounded once (dflash_add_layernorm_fwd rounds the sum too).
@@ -374,7 +376,8 @@ DFLASH_API int dflash_dropout_layernorm_fwd(const void* x, const void* residual,
 
 /*
  * Its backward pass, from the same x, residual, p, rng and site.
- *   dx, dresidual  : [rows, hidden], `dtype`; each may be NULL (with p = 0 they are equal)
+ *   dx, dresidual  : [rows, hidden], `dtype`; each may be NULL (with p = 0 they are equal);
+ *                    all tensors of rows 16-byte aligned
  *   dgamma, dbeta  : [hidden], `weight_dtype`; both may be NULL, then no workspace is needed
  *   workspace      : dflash_dropout_layernorm_bwd_workspace_bytes(rows, hidden) bytes
  * The sums over rows are taken in an order that depends on rows and hidden alone.

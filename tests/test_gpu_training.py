@@ -172,6 +172,13 @@ def test_layer_norm_rows(dtype, rows, hidden, residual):
     _check_norm(*_norm_case(rows, rows, hidden, dtype, dtype, residual), 1e-5, p)
 
 
+@pytest.mark.parametrize("rows,hidden", [(1100, 2051), (9000, 33), (1030, 4103)])
+def test_layer_norm_many_odd_rows(dtype, rows, hidden):
+    """More rows than the launch has groups of lanes: each meets several of one shift."""
+
+    _check_norm(*_norm_case(rows, rows, hidden, dtype, dtype, True), 1e-5, 0.1)
+
+
 @pytest.mark.parametrize("hidden", [64, 200, 769, 1024])
 @pytest.mark.parametrize("kind", [torch.float16, torch.bfloat16])
 @pytest.mark.parametrize("p", [0.0, 0.6, 1.0])

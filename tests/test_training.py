@@ -206,11 +206,12 @@ def test_c_layernorm_refusals(lib):
                  {"rstd": None}, {"rng": None}):
         assert fwd(**over) == NULL, over
     for over in ({"x": A + 1}, {"r": A + 1}, {"y": A + 1}, {"g": A + 1}, {"mean": A + 2},
-                 {"rng": A + 4}, {"g": A + 2, "wdtype": 2}):
+                 {"rng": A + 4}, {"g": A + 2, "wdtype": 2}, {"x": A + 8}, {"r": A + 4}):
         assert fwd(**over) == ALIGN, over
     size = lib.dflash_dropout_layernorm_bwd_workspace_bytes(40, 64)
     assert size == 40 * 2 * 64 * 4
     assert lib.dflash_dropout_layernorm_bwd_workspace_bytes(32, 64) == 0  # one workgroup's rows
+    assert lib.dflash_dropout_layernorm_bwd_workspace_bytes(32, 63) == 32 * 2 * 63 * 4
     assert lib.dflash_dropout_layernorm_bwd_workspace_bytes(1 << 40, 64) == 512 * 2 * 64 * 4
     assert lib.dflash_dropout_layernorm_bwd_workspace_bytes(-1, 64) == 0
     assert lib.dflash_dropout_layernorm_bwd_workspace_bytes(4, 9000) == 0
