@@ -102,9 +102,31 @@ const int64_t* words(const MaybeTensor& rng) {
   return rng ? static_cast<const int64_t*>(rng->data_ptr()) : nullptr;
 }
 
-// ---- the calls (inputs contiguous, checked by the caller) --------------------------
+// What the C calls take on trust.  training.py refuses more, and says more; but the operators can
+// be called past it, from a traced graph or by their names.
+void expect(bool good, const char* name) {
+  TORCH_CHECK_VALUE(good, name, " does not fit the call: shape, dtype, device or strides");
+}
+bool fits(const Tensor& t, const Tensor& x) { return t.device() == x.device() && t.is_contiguous(); }
+bool same_form(const Tensor& t, const Tensor& x) {
+  return fits(t, x) && t.sizes() == x.sizes() && t.scalar_type() == x.scalar_type();
+}
+bool vector_of(const Tensor& t, int64_t n, const Tensor& x) {
+  return fits(t, x) && t.dim() == 1 && t.size(0) == n;
+}
+void expect_dropout(const MaybeTensor& rng, int64_t site, const Tensor& x) {
+  expect(!rng || (vector_of(*rng, 2, x) && rng->scalar_type() == at::kLong), "rng");
+  expect(site >= 0 && site <= UINT32_MAX, "site");
+}
+void expect_rows(const Tensor& x) {
+  expect(x.is_contiguous() && x.dim() >= 1 && x.size(-1) >= 1 && x.size(-1) <= INT32_MAX, "x");
+}
+
+// ---- the calls ----------------------------------------------------------------------
 
 Tensor dropout(const Tensor& x, const Tensor& rng, double p, int64_t site) {
+  expect(x.is_contiguous(), "x");
+  expect_dropout(rng, site, x);
   Tensor out = fresh_like(x);
   On on(x);
   check(lib.dropout(data(x), data(out), x.numel(), p, words(rng), site, code_of(x), on.stream),
@@ -115,6 +137,11 @@ Tensor dropout(const Tensor& x, const Tensor& rng, double p, int64_t site) {
 Tensor layernorm(const Tensor& given, const MaybeTensor& given_residual, const Tensor& weight,
                  const Tensor& bias, const MaybeTensor& rng, double eps, double p, int64_t site,
                  float* statistics) {
+  expect_rows(given);
+  expect(!given_residual || same_form(*given_residual, given), "residual");
+  expect(vector_of(weight, given.size(-1), given), "weight");
+  expect(same_form(bias, weight), "bias");
+  expect_dropout(rng, site, given);
   const Tensor x = aligned(given);
   const MaybeTensor residual = aligned(given_residual);
   Tensor y = fresh_like(x);
@@ -138,6 +165,7 @@ std::tuple<Tensor, Tensor> dropout_layernorm_train(const Tensor& x, const MaybeT
                                                    const Tensor& weight, const Tensor& bias,
                                                    const MaybeTensor& rng, double eps, double p,
                                                    int64_t site) {
+  expect_rows(x);
   Tensor statistics = fresh({2, x.numel() / x.size(-1)}, at::kFloat, x);
   Tensor y = layernorm(x, residual, weight, bias, rng, eps, p, site,
                        static_cast<float*>(data(statistics)));
@@ -149,6 +177,14 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> dropout_layernorm_backward(
     const Tensor& given_dy, const Tensor& given, const MaybeTensor& given_residual,
     const Tensor& weight, const Tensor& statistics, const MaybeTensor& rng, double p, int64_t site,
     bool want_x, bool want_residual, bool want_weights) {
+  expect_rows(given);
+  expect(same_form(given_dy, given), "dy");
+  expect(!given_residual || same_form(*given_residual, given), "residual");
+  expect(vector_of(weight, given.size(-1), given), "weight");
+  expect(fits(statistics, given) && statistics.scalar_type() == at::kFloat &&
+             statistics.numel() == given.numel() / given.size(-1) * 2,
+         "statistics");
+  expect_dropout(rng, site, given);
   const Tensor dy = aligned(given_dy), x = aligned(given);
   const MaybeTensor residual = aligned(given_residual);
   const int64_t hidden = x.size(-1), rows = x.numel() / hidden;
@@ -172,8 +208,17 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> dropout_layernorm_backward(
   return {dx, dresidual, dweight, dbias};
 }
 
+void expect_ids(const Tensor& ids, const Tensor& like) {
+  expect(fits(ids, like) && (ids.scalar_type() == at::kInt || ids.scalar_type() == at::kLong),
+         "ids");
+}
+
 Tensor embedding_lookup(const Tensor& ids, const Tensor& table, double scale,
                         int64_t /*padding*/) {
+  expect(table.dim() == 2 && table.is_contiguous() && table.size(0) < INT32_MAX &&
+             table.size(1) <= INT32_MAX,
+         "table");
+  expect_ids(ids, table);
   auto shape = ids.sizes().vec();
   shape.push_back(table.size(1));
   Tensor out = fresh(shape, table.scalar_type(), table);
@@ -186,7 +231,11 @@ Tensor embedding_lookup(const Tensor& ids, const Tensor& table, double scale,
 
 Tensor embedding_gradient(const Tensor& dy, const Tensor& ids, c10::SymInt table_rows,
                           double scale, int64_t padding) {
+  expect(dy.is_contiguous() && dy.dim() >= 1, "dy");
+  expect_ids(ids, dy);
   const int64_t hidden = dy.size(-1), rows = table_rows.expect_int();
+  expect(dy.numel() == ids.numel() * hidden, "dy");
+  expect(rows >= 1 && rows < INT32_MAX && hidden <= INT32_MAX, "the table");
   Tensor out = fresh({rows, hidden}, dy.scalar_type(), dy);
   const size_t bytes = lib.embedding_bwd_workspace_bytes(ids.numel(), hidden);
   Tensor workspace;

@@ -351,8 +351,8 @@ DFLASH_API int dflash_encoder_layer_fwd(const dflash_encoder_layer* layer, const
  *   site : numbers the places of a model that drop elements
  * Pointers need the alignment of their element type, where not said otherwise; tensors on
  * 16-byte boundaries with rows of whole 16-byte chunks are faster.  Outputs must not overlap
- * inputs.  The workspaces' contents
- * need not outlive the kernels; calls that share one must not overlap.
+ * inputs.  The workspaces' contents need not outlive the kernels; calls that share one must not
+ * overlap.
  */
 
 /* y = drop(x) over n elements; also the backward pass (dx = drop(dy)). */
@@ -361,7 +361,7 @@ DFLASH_API int dflash_dropout(const void* x, void* y, int64_t n, double p, const
 
 /*
  * y = LayerNorm(drop(x) + residual), the tail of DebertaV2SelfOutput / DebertaV2Output in
- * training (/root/reference/src/disentangled_flash/_reference.py:101-112, 474-485).
+ * training (reference _reference.py:101-112, 474-485).
  *   x, residual, y : [rows, hidden], dtype `dtype`, 16-byte aligned; residual may be NULL;
  *                    hidden 1 to 8192
  *   gamma, beta    : [hidden], `weight_dtype`: `dtype` or fp32
@@ -380,7 +380,8 @@ DFLASH_API int dflash_dropout_layernorm_fwd(const void* x, const void* residual,
  *                    all tensors of rows 16-byte aligned
  *   dgamma, dbeta  : [hidden], `weight_dtype`; both may be NULL, then no workspace is needed
  *   workspace      : dflash_dropout_layernorm_bwd_workspace_bytes(rows, hidden) bytes
- * The sums over rows are taken in an order that depends on rows and hidden alone.
+ * The sums over rows are taken in an order that depends on the shape, the dtypes and gamma's
+ * alignment alone.
  */
 DFLASH_API size_t dflash_dropout_layernorm_bwd_workspace_bytes(int64_t rows, int hidden);
 DFLASH_API int dflash_dropout_layernorm_bwd(

@@ -165,6 +165,18 @@ def test_embedding_refusals():
                 embedding(*args)
 
 
+def test_missing_torch_library_is_named(monkeypatch, tmp_path, lib):
+    from disentangled_flash import _lib
+
+    monkeypatch.setattr(_lib, "_torch_ops_loaded", False)
+    monkeypatch.setattr(_lib, "library_path", lambda: tmp_path / _lib.LIBRARY_NAME)
+    with pytest.raises(RuntimeError, match="libdflash_torch.so is missing: build"):
+        _lib.load_torch_ops()
+    (tmp_path / _lib.TORCH_LIBRARY_NAME).write_bytes(b"not a library")
+    with pytest.raises(RuntimeError, match="cannot load"):
+        _lib.load_torch_ops()
+
+
 @pytest.fixture(scope="module")
 def lib():
     from disentangled_flash import _lib
