@@ -9,7 +9,8 @@
 // Otherwise:
 //
 //   rank   (up to kRankTokens) each token's place by comparing its id with all others;
-//   sort, merge  (more) ranges sorted in LDS, then each token's place by binary searches;
+//   sort, merge  (more) ranges sorted in LDS, then each token's place by binary searches, runs of
+//          16384 tokens first and then several runs to one;
 //          the first of these launches also writes the zeros of dtable, which for a
 //          vocabulary is most of the bytes;
 //   sum    kTile sorted tokens per group of lanes; an id whose tokens all lie in the tile is
@@ -27,6 +28,7 @@
 #include <stdint.h>
 
 #include <type_traits>
+#include <utility>
 
 #include "device_common.h"
 #include "dflash.h"
@@ -299,19 +301,20 @@ __global__ __launch_bounds__(kSortThreads) void embedding_sort_kernel(
 
 // ---- merge -------------------------------------------------------------------
 
-// A token's place among all: its place in its own range, and in every other range the
-// number of ids before it (equal ids of earlier ranges come first).  The ranges pass through
-// LDS kMergeRanges at a time, where each search takes 11 steps and the searches of one
+// kMergeRanges ranges become one sorted run.  A token's place in it: its place in its own range,
+// and in every other range the number of ids before it (equal ids of earlier ranges come
+// first).  The run's ranges lie in LDS, where each search takes 11 steps and the searches of one
 // token are independent; from L2 the steps alone would take their latency 11 times over.
 constexpr int kMergeRanges = 8;
 constexpr int kMergeThreads = 256;
+constexpr int kRunTokens = kMergeRanges * kSortTokens;
 
 __global__ __launch_bounds__(kMergeThreads) void embedding_merge_kernel(
     const int32_t* __restrict__ ids, const int32_t* __restrict__ tokens, int64_t n,
     int32_t* __restrict__ merged_ids, int32_t* __restrict__ merged_tokens, int blocks, Fill fill) {
   typedef int32_t Four __attribute__((ext_vector_type(4)));
-  constexpr int kHeld = kMergeRanges * kSortTokens;
-  __shared__ Four lds4[kHeld / 4];
+  constexpr int kLoads = kRunTokens / 4 / kMergeThreads;
+  __shared__ Four lds4[kRunTokens / 4];
   int32_t* lds = reinterpret_cast<int32_t*>(lds4);
   if (static_cast<int>(blockIdx.x) >= blocks) {
     fill_zeros<kMergeThreads>(fill, blockIdx.x - blocks, gridDim.x - blocks);
@@ -320,52 +323,86 @@ __global__ __launch_bounds__(kMergeThreads) void embedding_merge_kernel(
   const int64_t i = static_cast<int64_t>(blockIdx.x) * kMergeThreads + threadIdx.x;
   const int64_t at = i < n ? i : n - 1;
   const int32_t id = ids[at], token = tokens[at];
-  const int64_t own = i / kSortTokens;
-  int64_t place = i - own * kSortTokens;
-  const int64_t ranges = (n + kSortTokens - 1) / kSortTokens;
-  for (int64_t r0 = 0; r0 < ranges; r0 += kMergeRanges) {
-    const int64_t first = r0 * kSortTokens;
-    const int held = n - first < kHeld ? static_cast<int>(n - first) : kHeld;
-    __syncthreads();  // the ranges before have been searched
-    // (The array is padded to 256 bytes: whole accesses, past the end the last one again.)
-    Four given[kHeld / 4 / kMergeThreads];
+  // (A workgroup's tokens are of one range.)
+  const int64_t first = i / kRunTokens * kRunTokens;
+  const int own = static_cast<int>((i - first) / kSortTokens);
+  const int held = n - first < kRunTokens ? static_cast<int>(n - first) : kRunTokens;
+  // (The array is padded to 256 bytes: whole accesses, past the end the last one again.)
+  Four given[kLoads];
 #pragma unroll
-    for (int k = 0; k < kHeld / 4 / kMergeThreads; ++k) {
-      const int j = (k * kMergeThreads + threadIdx.x) * 4;
-      given[k] = *reinterpret_cast<const Four*>(ids + first + min(j, (held - 1) / 4 * 4));
-    }
+  for (int k = 0; k < kLoads; ++k) {
+    const int j = (k * kMergeThreads + threadIdx.x) * 4;
+    given[k] = *reinterpret_cast<const Four*>(ids + first + min(j, (held - 1) / 4 * 4));
+  }
 #pragma unroll
-    for (int k = 0; k < kHeld / 4 / kMergeThreads; ++k) {
-      const int j = (k * kMergeThreads + threadIdx.x) * 4;
-      Four v = given[k];  // past the end: above all ids
+  for (int k = 0; k < kLoads; ++k) {
+    const int j = (k * kMergeThreads + threadIdx.x) * 4;
+    Four v = given[k];  // past the end: above all ids
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (j + e >= held) v[e] = INT32_MAX;
-      lds4[j / 4] = v;
-    }
-    __syncthreads();
-    int before[kMergeRanges];
+    for (int e = 0; e < 4; ++e)
+      if (j + e >= held) v[e] = INT32_MAX;
+    lds4[j / 4] = v;
+  }
+  __syncthreads();
+  int before[kMergeRanges];
 #pragma unroll
-    for (int r = 0; r < kMergeRanges; ++r) before[r] = 0;
-    for (int step = kSortTokens / 2; step >= 1; step /= 2) {
-#pragma unroll
-      for (int r = 0; r < kMergeRanges; ++r) {
-        const int32_t other = lds[r * kSortTokens + before[r] + step - 1];
-        before[r] += other < id || (other == id && r0 + r < own) ? step : 0;
-      }
-    }
+  for (int r = 0; r < kMergeRanges; ++r) before[r] = 0;
+  for (int step = kSortTokens / 2; step >= 1; step /= 2) {
 #pragma unroll
     for (int r = 0; r < kMergeRanges; ++r) {
-      // (The steps add up to kSortTokens - 1: the last id is still to be compared.)
-      const int32_t other = lds[r * kSortTokens + before[r]];
-      before[r] += other < id || (other == id && r0 + r < own) ? 1 : 0;
-      if (r0 + r != own) place += before[r];
+      const int32_t other = lds[r * kSortTokens + before[r] + step - 1];
+      before[r] += other < id || (other == id && r < own) ? step : 0;
     }
+  }
+  int64_t place = i - own * kSortTokens;
+#pragma unroll
+  for (int r = 0; r < kMergeRanges; ++r) {
+    // (The steps add up to kSortTokens - 1: the last id is still to be compared.)
+    const int32_t other = lds[r * kSortTokens + before[r]];
+    before[r] += other < id || (other == id && r < own) ? 1 : 0;
+    if (r != own) place += before[r];
   }
   if (i < n) {
     merged_ids[place] = id;
     merged_tokens[place] = token;
   }
+}
+
+// kFan sorted runs of `length` tokens (a power of two; the last may be shorter) become one, the
+// same way but from L2: neighbouring tokens search in the same places.  (Whole gradients into
+// 128100 x 768 bf16, by 4 runs at a time, 8 and 16: 20000 tokens 52, 54, 57 us; 65536 89, 90, 94;
+// 1048576 898, 914, 965.  Every range searched for every token, quadratic: 51, 96 and 4921.)
+constexpr int kFan = 4;
+
+__global__ __launch_bounds__(kMergeThreads) void embedding_merge_runs_kernel(
+    const int32_t* __restrict__ ids, const int32_t* __restrict__ tokens, int n, int length,
+    int32_t* __restrict__ merged_ids, int32_t* __restrict__ merged_tokens) {
+  const int i = blockIdx.x * kMergeThreads + threadIdx.x;  // (at most kMaxTokens)
+  if (i >= n) return;
+  const int32_t id = ids[i], token = tokens[i];
+  const int start = i / length / kFan * kFan * length;
+  const int own = (i - start) / length;
+  int before[kFan];
+#pragma unroll
+  for (int r = 0; r < kFan; ++r) before[r] = 0;
+  // A token behind the end is above all ids.
+  auto precedes = [&](int r, int at) {
+    const int32_t other = ids[at < n ? at : n - 1];
+    return at < n && (other < id || (other == id && r < own));
+  };
+  for (int step = length / 2; step >= 1; step /= 2) {
+#pragma unroll
+    for (int r = 0; r < kFan; ++r)
+      before[r] += precedes(r, start + r * length + before[r] + step - 1) ? step : 0;
+  }
+  int place = i - own * length;
+#pragma unroll
+  for (int r = 0; r < kFan; ++r) {
+    before[r] += precedes(r, start + r * length + before[r]) ? 1 : 0;
+    if (r != own) place += before[r];
+  }
+  merged_ids[place] = id;
+  merged_tokens[place] = token;
 }
 
 // ---- sum and join --------------------------------------------------------------
@@ -572,7 +609,7 @@ __global__ __launch_bounds__(256) void embedding_few_kernel(
   const int64_t per_unit = static_cast<int64_t>(unit) * hidden / Chunk<T>::N;  // chunks
   const int64_t elements = static_cast<int64_t>(rows) * hidden;
   const int64_t chunks = elements / Chunk<T>::N;
-  const int units = (rows + unit - 1) / unit;
+  const int units = (rows - 1) / unit + 1;
   u32x4_t* table = reinterpret_cast<u32x4_t*>(dtable);
   if (per_unit < 256) {
     // Several units at a time, each by the lanes that hold one.
@@ -727,7 +764,7 @@ int launch_bwd(const void* ids_in, const void* dout_in, void* dtable_in, int64_t
   if (sum_blocks > kMaxBlocks256) return DFLASH_ERR_TOO_LARGE;  // (before anything is launched)
   if (n <= kFewTokens) {
     const int unit = hidden % N == 0 ? 1 : N;
-    const int units = (rows + unit - 1) / unit;
+    const int units = (rows - 1) / unit + 1;
     hipLaunchKernelGGL((wide ? &embedding_few_kernel<T, I, N> : &embedding_few_kernel<T, I, 1>),
                        dim3(units < kFewBlocks ? units : kFewBlocks), dim3(256), 0, stream,
                        ids_as_given, static_cast<int>(n), rows, padding, unit, dout, dtable,
@@ -771,8 +808,17 @@ int launch_bwd(const void* ids_in, const void* dout_in, void* dtable_in, int64_t
                        blocks, rest);
     rc = static_cast<int>(hipGetLastError());
     if (rc != DFLASH_OK) return rc;
-    ids = merged;
-    tokens = merged_tokens;
+    std::swap(ids, merged);
+    std::swap(tokens, merged_tokens);
+    for (int64_t length = kRunTokens; length < n; length *= kFan) {
+      hipLaunchKernelGGL(embedding_merge_runs_kernel, dim3(blocks), dim3(kMergeThreads), 0, stream,
+                         ids, tokens, static_cast<int>(n), static_cast<int>(length), merged,
+                         merged_tokens);
+      rc = static_cast<int>(hipGetLastError());
+      if (rc != DFLASH_OK) return rc;
+      std::swap(ids, merged);
+      std::swap(tokens, merged_tokens);
+    }
   }
   hipLaunchKernelGGL((wide ? &embedding_sum_kernel<T, N> : &embedding_sum_kernel<T, 1>),
                      dim3(static_cast<uint32_t>(sum_blocks)), dim3(256), 0, stream, ids, tokens, n,

@@ -408,6 +408,82 @@ def test_embedding_many_tokens(n, kind, rows):
     _check_embedding(_ids(kind, n, rows, n), rows, 5, torch.float32, 2.0, 0)
 
 
+@pytest.mark.parametrize("n", [16384, 65536, 65537, 131073, 300000])
+@pytest.mark.parametrize("kind", ["uniform", "one", "frequent"])
+def test_embedding_runs_that_are_merged(n, kind):
+    """More tokens than one run holds: one, two and three launches that join runs."""
+
+    _check_embedding(_ids(kind, n, 70001, n), 70001, 16, torch.bfloat16, 1.0, 3)
+
+
+@pytest.mark.parametrize("n", [9, 300, 9000])
+def test_embedding_most_rows(n):
+    """The largest table that is taken, and its last rows."""
+
+    from disentangled_flash.training import embedding
+
+    rows = (1 << 31) - 2
+    table = torch.zeros(rows, 1, device="cuda", dtype=torch.float16, requires_grad=True)
+    ids = rows - 1 - torch.arange(n, device="cuda") % 7
+    dy = torch.ones(n, 1, device="cuda", dtype=torch.float16)
+    (grad,) = torch.autograd.grad(embedding(ids, table), table, dy)
+    counts = torch.bincount(rows - 1 - ids, minlength=7).flip(0).half()
+    assert torch.equal(grad[-7:, 0], counts)
+    assert int(torch.count_nonzero(grad[:-7])) == 0
+    del table, grad
+    torch.cuda.empty_cache()
+
+
+def test_operators_called_by_name_refuse_what_does_not_fit():
+    """Past the Python checks: nothing is launched."""
+
+    from disentangled_flash import training
+
+    x, w = torch.zeros(4, 8, device="cuda"), torch.zeros(8, device="cuda")
+    rng, ids = _rng(), torch.zeros(4, device="cuda", dtype=torch.int64)
+    training.layer_norm(x, w, w, 1e-5)  # (loads the operators)
+    ops = torch.ops.disentangled_flash
+    stats = torch.zeros(2, 4, device="cuda")
+    sparse, wide = torch.zeros(4, 16, device="cuda")[:, ::2], torch.zeros(4, 9, device="cuda")
+    for call in (
+        lambda: ops.dropout(sparse, rng, 0.1, 0),
+        lambda: ops.dropout(x, rng.cpu(), 0.1, 0),
+        lambda: ops.dropout(x, rng.int(), 0.1, 0),
+        lambda: ops.dropout(x, rng, 0.1, -1),
+        lambda: ops.dropout(x, rng, 0.1, 1 << 32),
+        lambda: ops.dropout_layernorm(sparse, None, w, w, None, 1e-5, 0.0, 0),
+        lambda: ops.dropout_layernorm(x[:, :0], None, w[:0], w[:0], None, 1e-5, 0.0, 0),
+        lambda: ops.dropout_layernorm(x[0, 0], None, w, w, None, 1e-5, 0.0, 0),
+        lambda: ops.dropout_layernorm(x, wide, w, w, None, 1e-5, 0.0, 0),
+        lambda: ops.dropout_layernorm(x, x.half(), w, w, None, 1e-5, 0.0, 0),
+        lambda: ops.dropout_layernorm(x, None, w[:7], w[:7], None, 1e-5, 0.0, 0),
+        lambda: ops.dropout_layernorm(x, None, w, w.half(), None, 1e-5, 0.0, 0),
+        lambda: ops.dropout_layernorm(x, None, w.cpu(), w.cpu(), None, 1e-5, 0.0, 0),
+        lambda: ops.dropout_layernorm_train(x[0, 0], None, w, w, None, 1e-5, 0.0, 0),
+        lambda: ops.dropout_layernorm_backward(wide, x, None, w, stats, None, 0.0, 0, *[True] * 3),
+        lambda: ops.dropout_layernorm_backward(x, x, None, w, stats[:1], None, 0.0, 0,
+                                               *[True] * 3),
+        lambda: ops.embedding_lookup(ids.short(), x, 1.0, -1),
+        lambda: ops.embedding_lookup(ids.cpu(), x, 1.0, -1),
+        lambda: ops.embedding_lookup(ids, sparse, 1.0, -1),
+        lambda: ops.embedding_lookup(ids, w, 1.0, -1),
+        lambda: ops.embedding_gradient(wide[:3], ids, 5, 1.0, -1),
+        lambda: ops.embedding_gradient(x, ids, 0, 1.0, -1),
+        lambda: ops.embedding_gradient(x, ids, 1 << 31, 1.0, -1),
+    ):
+        with pytest.raises(ValueError, match="does not fit"):
+            call()
+    for call in (  # refused by the library
+        lambda: ops.dropout(x, rng, 1.5, 0),
+        lambda: ops.dropout_layernorm(x, None, w, w, None, 1e-5, 0.1, 0),  # no rng
+        lambda: ops.dropout_layernorm(x, None, w.half(), w.half(), None, 1e-5, 0.0, 0),
+        lambda: ops.dropout_layernorm(torch.zeros(1, 8200, device="cuda"), None,
+                                      *[torch.zeros(8200, device="cuda")] * 2, None, 1e-5, 0.0, 0),
+    ):
+        with pytest.raises(RuntimeError, match="failed with code"):
+            call()
+
+
 def test_embedding_ids_of_other_kinds(dtype):
     from disentangled_flash.training import embedding
 

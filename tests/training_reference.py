@@ -4,9 +4,10 @@ Tests only.  The generator is written with numpy's 64-bit words; the operators a
 gradients are the formulas in float64 on whatever device the inputs are on.
 
 Bounds.  u = 2^-24 is fp32's half step.  A sum of terms t_i taken in chains of at most k
-additions is off by at most k u sum|t_i|.  A row of layer_norm is summed in chains of at most 32
-elements a lane and 8 halvings, so k = 40; with the roundings of s itself (two products and
-a sum), 48 covers mean and sum of squares.  Results are rounded once more to their dtype:
+additions is off by at most k u sum|t_i|.  A row of layer_norm is summed in chains of at most 40
+elements a lane (8191 of 16 bits: 256 lanes of 5 chunks), 6 steps across a wavefront and 3 across
+four of them, so k = 49; with the division by the width and the roundings of s itself (two
+products and a sum) the mean is off by 53 u.  Results are rounded once more to their dtype:
 ``finfo(dtype).eps / 2`` of the value, or half the smallest subnormal.
 """
 
@@ -87,9 +88,10 @@ def layer_norm(x, weight, bias, eps, residual=None, mult=None, dy=None):
     rstd = (var + eps).rsqrt()
     xh = (s - mean) * rstd
     ratio = size * rstd
-    # xh: s and the mean are off by 51 u size; the variance by 48 u of itself and by 2 x 51 u
-    # size / sigma, half of which reaches rstd, and rsqrt by 2 u; products 2 u.
-    e_xh = U * (51 * ratio * (1 + xh.abs()) + 32 * xh.abs())
+    # xh: s and the mean are off by 53 u size; the variance by 51 u of itself (49 additions, the
+    # square and the division) and by 2 x 53 u size / sigma, half of which reaches rstd, and
+    # rsqrt by 2 u; products 2 u: 25.5 + 4 < 32.
+    e_xh = U * (53 * ratio * (1 + xh.abs()) + 32 * xh.abs())
     y = xh * w + b
     out = {"y": (y, w.abs() * e_xh + 2 * U * ((xh * w).abs() + b.abs()) + rounding(y, dtype))}
     if dy is None:
@@ -101,15 +103,15 @@ def layer_norm(x, weight, bias, eps, residual=None, mult=None, dy=None):
     ds = rstd * inner
     size_g = g.abs() + g.abs().mean(-1, keepdim=True) \
         + xh.abs() * (g * xh).abs().mean(-1, keepdim=True)
-    e_rstd = U * (32 + 51 * ratio)
+    e_rstd = U * (32 + 53 * ratio)
     e_ds = rstd * (e_rstd * size_g + 52 * U * size_g + m2.abs() * e_xh
                    + xh.abs() * (g.abs() * e_xh).mean(-1, keepdim=True))
     out["dresidual"] = (ds, e_ds + rounding(ds, dtype))
     dx = torch.where(c == 0, torch.zeros_like(ds), ds * c)
     out["dx"] = (dx, e_ds * c + 2 * U * dx.abs() + rounding(dx, dtype))
-    # Rows: a lane adds rows / 512 of them at most (one at least), then 16 groups, then
-    # 512 partial rows in 16 slices.
-    chain = (x.shape[0] / 512 + 1 + 16 + 32 + 16 + 2) * U
+    # Rows: a lane adds rows / 512 of them at most (one at least), then 16 groups, then 512
+    # partial rows in 64 slices of 8; two roundings of the products.
+    chain = (x.shape[0] / 512 + 1 + 16 + 8 + 64 + 2) * U
     dw = (d * xh).sum(0)
     out["dweight"] = (dw, (d.abs() * e_xh).sum(0) + chain * (d * xh).abs().sum(0)
                       + rounding(dw, wtype))
@@ -131,8 +133,10 @@ def embedding_gradient(ids, dy, rows, scale, padding=None):
     value.index_add_(0, ids, d)
     size.index_add_(0, ids, d.abs())
     value, size = value * scale, size * abs(scale)
-    # 32 rows of a tile, a quarter of the tiles of one id, four quarters, the scale's product.
-    chain = 32 + ids.numel() / 128 + 1 + 4 + 2
+    # Up to 256 tokens one after the other; else the 32 rows of a tile, an eighth of the tiles of
+    # one id, the eight parts.  Then the scale's product.
+    n = ids.numel()
+    chain = (n if n <= 256 else 32 + n / 256 + 1 + 8) + 2
     return value, chain * U * size + rounding(value, dy.dtype)
 
 
