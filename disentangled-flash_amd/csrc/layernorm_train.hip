@@ -22,7 +22,7 @@
 // Bound by bytes: 16384 x 768 bf16 with residual and dropout 16.0 us forward (75 MB, 4.7 TB/s)
 // and 29.7 backward (129 MB with the partial rows, 4.3 TB/s, of which 4 us are the second
 // launch); 16384 x 1536 fp32 55 (5.5 TB/s) and 89 us (5.7).  A copy of as many bytes runs at
-// 4.8 to 5.4 TB/s.  16384 x 769 bf16: 22.4 and 39.4 us; 3059 x 1001: 10.5 and 18.1 (by
+// 4.8 to 5.4 TB/s.  16384 x 769 bf16: 20.1 and 39.4 us; 3059 x 1001: 7.7 and 18.0 (by
 // element accesses 17.0 and 28.0).
 
 #include <hip/hip_runtime.h>
@@ -170,6 +170,40 @@ struct RowInput {
   }
 };
 
+// gamma and beta in LDS, weight i of each at [8 + i], for 16-bit rows that begin inside a chunk:
+// each thread loads a chunk of both, and stores it when the rows' loads are on their way.
+template <typename W>
+struct WeightStage {
+  using Vector = typename Chunk<W>::type;
+  static constexpr int C = Chunk<W>::N;
+  Vector gamma, beta;
+  int at;
+  bool whole;
+
+  __device__ void load(const W* gammas, const W* betas, int hidden) {
+    const uintptr_t both = reinterpret_cast<uintptr_t>(gammas) | reinterpret_cast<uintptr_t>(betas);
+    at = threadIdx.x * C;
+    whole = both % 16 == 0 && at + C <= hidden;
+    if (whole) {
+      gamma = *reinterpret_cast<const Vector*>(gammas + at);
+      beta = *reinterpret_cast<const Vector*>(betas + at);
+    }
+  }
+
+  __device__ void store(const W* gammas, const W* betas, int hidden, W* lds_gamma, W* lds_beta) {
+    if (whole) {
+      *reinterpret_cast<Vector*>(lds_gamma + 8 + at) = gamma;
+      *reinterpret_cast<Vector*>(lds_beta + 8 + at) = beta;
+    } else {
+      for (int e = at; e < at + C && e < hidden; ++e) {
+        lds_gamma[8 + e] = gammas[e];
+        lds_beta[8 + e] = betas[e];
+      }
+    }
+    lds_barrier();
+  }
+};
+
 // A workgroup walks its rows, every gridDim-th group of kThreads / LANES rows.  (LANES = 256:
 // the row is the workgroup's, so every thread makes the same rounds.)  Without WHOLE the step is
 // a multiple of N or there is no second round (the launch sees to it).
@@ -180,22 +214,44 @@ __global__ __launch_bounds__(kThreads) void layernorm_train_fwd_kernel(Forward a
   __shared__ float lds[LANES > 64 ? LANES / 64 : 1][1];
   const int sub = threadIdx.x % LANES;
   int64_t row = static_cast<int64_t>(blockIdx.x) * kGroups + threadIdx.x / LANES;
-  if (row >= a.rows) return;  // all lanes of a row together
+  // 16-bit weights that lie askew of the row's chunks pass through LDS: 3059 x 1001 bf16, where a
+  // group has one row, 7.7 us instead of 10.5 with 32 element loads a lane; 16384 x 769 20.1, 23.0.
+  // (The backward pass has gamma alone and more rows a group: 0.5 us of 18 are its weights'.  Rows
+  // wider than a wavefront holds are a workgroup's, which has no other group to share them with.)
+  constexpr bool kStaged = !WHOLE && LANES <= 64 && sizeof(W) == 2;
+  __shared__ alignas(16) W staged[2][kStaged ? (LANES * CH + 2) * 8 : 8];
+  static_assert(!kStaged || LANES * CH * N <= kThreads * Chunk<W>::N, "a chunk a thread");
+  WeightStage<W> stage;
+  if constexpr (kStaged)
+    stage.load(static_cast<const W*>(a.gamma), static_cast<const W*>(a.beta), a.hidden);
+  else if (row >= a.rows)
+    return;  // all lanes of a row together
   const int64_t step = static_cast<int64_t>(gridDim.x) * kGroups;
   const int hidden = a.hidden;
   const float width = static_cast<float>(hidden);
   const T* x = static_cast<const T*>(a.x);
   const T* r = static_cast<const T*>(a.residual);
   const int64_t total = a.rows * hidden;
-  const int first_col = WHOLE ? 0 : -static_cast<int>(row * hidden % N);
+  const int64_t first_row = row < a.rows ? row : a.rows - 1;
+  const int first_col = WHOLE ? 0 : -static_cast<int>(first_row * hidden % N);
   const int lane_col = sub * N + first_col;  // + LANES * N a chunk
   RowInput<T, LANES, CH, WHOLE, false> in;
-  in.load(x, r, row * hidden, lane_col, first_col, hidden, total);
+  in.load(x, r, first_row * hidden, lane_col, first_col, hidden, total);
+  if constexpr (kStaged) {
+    stage.store(static_cast<const W*>(a.gamma), static_cast<const W*>(a.beta), hidden, staged[0],
+                staged[1]);
+    if (row >= a.rows) return;
+  }
   WeightChunk<W, N, WHOLE> gamma[CH], beta[CH];
 #pragma unroll
   for (int k = 0; k < CH; ++k) {
-    gamma[k].load(static_cast<const W*>(a.gamma), lane_col + LANES * N * k, hidden);
-    beta[k].load(static_cast<const W*>(a.beta), lane_col + LANES * N * k, hidden);
+    if constexpr (kStaged) {
+      gamma[k].load_staged(staged[0], lane_col + LANES * N * k);
+      beta[k].load_staged(staged[1], lane_col + LANES * N * k);
+    } else {
+      gamma[k].load(static_cast<const W*>(a.gamma), lane_col + LANES * N * k, hidden);
+      beta[k].load(static_cast<const W*>(a.beta), lane_col + LANES * N * k, hidden);
+    }
   }
   const DropoutKey key = dropout_key(a.drop);
   for (;;) {

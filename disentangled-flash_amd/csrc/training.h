@@ -172,6 +172,28 @@ struct WeightChunk {
     }
   }
 
+  // The same of 16-bit weights staged in LDS, weight i at staged[8 + i] and two whole chunks
+  // after the last that is asked for: two aligned accesses, shifted together.
+  __device__ void load_staged(const W* staged, int col) {
+    static_assert(sizeof(W) == 2 && kPieces == 1, "16-bit weights of 16-bit rows");
+    typedef uint32_t Four __attribute__((ext_vector_type(4)));
+    const uint32_t at = col + 8;  // (col is above -8)
+    const Four* p = reinterpret_cast<const Four*>(staged) + at / 8;
+    const Four low = p[0], high = p[1];
+    const uint32_t a[8] = {low[0], low[1], low[2], low[3], high[0], high[1], high[2], high[3]};
+    uint32_t b[6], c[5];
+    Four d;
+    // (Values: a choice between elements of an array would put it into memory.)
+    auto select = [](uint32_t bit, uint32_t one, uint32_t zero) { return bit ? one : zero; };
+#pragma unroll
+    for (int i = 0; i < 6; ++i) b[i] = select(at & 4, a[i + 2], a[i]);
+#pragma unroll
+    for (int i = 0; i < 5; ++i) c[i] = select(at & 2, b[i + 1], b[i]);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) d[i] = __builtin_amdgcn_alignbit(c[i + 1], c[i], (at & 1) * 16);
+    v[0] = __builtin_bit_cast(typename Chunk<W>::type, d);
+  }
+
   // Makes the compiler take the weights as new here: their fp32 values, the same for every
   // row, are not kept in registers across the rows' loop.
   __device__ void renew() {
