@@ -889,6 +889,32 @@ def test_checkpointed_layers_recompute_their_own_forward():
         assert difference <= 100 * ref.U * size, (name, difference, size)
 
 
+def test_compiled_model_draws_the_masks_of_its_step():
+    """A compiled backbone steps and drops as the eager one; the counter is not baked in."""
+
+    from disentangled_flash import enable_deberta_training
+
+    batch, grads = _batch(), []
+    for compiled in (False, True):
+        model = enable_deberta_training(_backbone(0.2).cuda().train(), seed=8)
+        call = torch.compile(model, backend="aot_eager") if compiled else model
+        steps = []
+        for _ in range(3):
+            model.zero_grad()
+            _loss(call, batch).backward()
+            steps.append({n: p.grad for n, p in model.named_parameters() if p.grad is not None})
+        assert model.dropout_state.counter.tolist() == [8, 3]
+        grads.append(steps)
+    for eager, compiled in zip(*grads):
+        assert eager.keys() == compiled.keys()
+        for name in eager:
+            # torch's own operators may be decomposed otherwise: 1000 half steps of the largest,
+            # where other masks would change a gradient by its own size.
+            size = eager[name].abs().max().item()
+            difference = (compiled[name] - eager[name]).abs().max().item()
+            assert difference <= 1000 * ref.U * size, (name, difference, size)
+
+
 def test_output_block_under_autocast():
     from disentangled_flash import enable_deberta_training
 
