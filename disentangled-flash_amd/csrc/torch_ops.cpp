@@ -284,6 +284,15 @@ const auto& gradient_op() {
   return op;
 }
 
+// Forward-mode derivatives are not implemented; below autograd a tangent would be lost unseen.
+void no_tangent(const Tensor& t, const char* name) {
+  TORCH_CHECK_NOT_IMPLEMENTED(!t.defined() || !t._fw_grad(/*level=*/0).defined(), name,
+                              ": forward-mode derivatives are not implemented");
+}
+void no_tangent(const MaybeTensor& t, const char* name) {
+  if (t) no_tangent(*t, name);
+}
+
 // Gradients whose own gradient is not implemented: differentiating them raises.
 variable_list only_once(variable_list grads, const char* name) {
   if (!at::GradMode::is_enabled()) return grads;
@@ -341,6 +350,7 @@ struct LayerNormNode : Function<LayerNormNode> {
     const int64_t wanted = ctx->saved_data["wanted"].toInt();
     const bool want_x = wanted & 1, want_residual = wanted & 2, want_weight = wanted & 4,
                want_bias = wanted & 8;
+    no_tangent(grads[0], "layer_norm");
     // Without dropout the gradients of x and of the residual are the same tensor.
     const bool shared = p == 0.0 && want_residual;
     Tensor dx, dresidual, dweight, dbias;
@@ -372,6 +382,7 @@ struct EmbeddingNode : Function<EmbeddingNode> {
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const Tensor ids = ctx->get_saved_variables()[0];
+    no_tangent(grads[0], "embedding");
     Tensor grad;
     {
       at::AutoDispatchBelowADInplaceOrView below;
@@ -386,6 +397,7 @@ struct EmbeddingNode : Function<EmbeddingNode> {
 bool records(const Tensor& t) { return t.requires_grad() && at::GradMode::is_enabled(); }
 
 Tensor dropout_autograd(const Tensor& x, const Tensor& rng, double p, int64_t site) {
+  no_tangent(x, "dropout");
   if (records(x)) return DropoutNode::apply(x, rng, p, site);
   at::AutoDispatchBelowADInplaceOrView below;
   return dropout_op().call(x, rng, p, site);
@@ -394,6 +406,8 @@ Tensor dropout_autograd(const Tensor& x, const Tensor& rng, double p, int64_t si
 Tensor dropout_layernorm_autograd(const Tensor& x, const MaybeTensor& residual,
                                   const Tensor& weight, const Tensor& bias, const MaybeTensor& rng,
                                   double eps, double p, int64_t site) {
+  for (const Tensor* t : {&x, &weight, &bias}) no_tangent(*t, "layer_norm");
+  no_tangent(residual, "layer_norm");
   if (records(x) || records(weight) || records(bias) || (residual && records(*residual)))
     return LayerNormNode::apply(x, residual, weight, bias, rng, eps, p, site);
   at::AutoDispatchBelowADInplaceOrView below;
@@ -402,6 +416,7 @@ Tensor dropout_layernorm_autograd(const Tensor& x, const MaybeTensor& residual,
 
 Tensor embedding_lookup_autograd(const Tensor& ids, const Tensor& table, double scale,
                                  int64_t padding) {
+  no_tangent(table, "embedding");
   if (records(table)) return EmbeddingNode::apply(ids, table, scale, padding);
   at::AutoDispatchBelowADInplaceOrView below;
   return lookup_op().call(ids, table, scale, padding);

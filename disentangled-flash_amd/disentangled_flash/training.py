@@ -26,7 +26,7 @@ to a thread of its own: under ``torch.autograd.set_multithreading_enabled(False)
 gradients of a norm tail took 28 us of host time instead of 61.
 
 Work is launched on torch's current stream of the inputs' device.  Second derivatives raise,
-but for dropout's.  Inputs that are not contiguous are copied first, and in :func:`layer_norm`
+but for dropout's, and forward-mode derivatives do.  Inputs that are not contiguous are copied first, and in :func:`layer_norm`
 those that do not start on a 16-byte boundary.
 """
 
