@@ -20,6 +20,7 @@ replay; ``site`` numbers the places of a model that drop elements.  An element i
 its index in the flattened tensor, ``rng`` and ``site`` alone, whatever the dtype.  ``p`` is
 rounded to a multiple of 2^-16 (to 0 and 1 only where it is 0 or 1), and kept elements are
 divided by the rounded probability of being kept.  A dropped element is 0 whatever it held.
+Under ``torch.func.vmap`` each sample needs an ``rng`` of its own.
 
 Small steps are bound by the host, and most of that is torch's hand-over of the backward pass
 to a thread of its own: under ``torch.autograd.set_multithreading_enabled(False)`` the
@@ -112,6 +113,19 @@ def _check_floating(name: str, tensor: torch.Tensor) -> None:
         raise TypeError(f"{name} dtype {tensor.dtype} is not fp16, bf16 or fp32")
 
 
+_is_batched = torch._C._functorch.is_batchedtensor
+
+
+def _vmap_levels(tensor: torch.Tensor) -> set[int]:
+    """The vmaps, by their levels, over which ``tensor`` holds a value for each sample."""
+
+    levels = set()
+    while _is_batched(tensor):
+        levels.add(torch._C._functorch.maybe_get_level(tensor))
+        tensor = torch._C._functorch.get_unwrapped(tensor)
+    return levels
+
+
 def _check_dropout(p: float, rng: torch.Tensor | None, site: int, like: torch.Tensor) -> None:
     if not 0.0 <= p <= 1.0:  # (NaN too)
         raise ValueError(f"dropout probability must be in [0, 1], got {p}")
@@ -126,6 +140,9 @@ def _check_dropout(p: float, rng: torch.Tensor | None, site: int, like: torch.Te
                          f"{tuple(rng.shape)}")
     if rng.get_device() != like.get_device():
         raise ValueError(f"rng is on {rng.device}, the input on {like.device}")
+    if _is_batched(like) and not _vmap_levels(like) <= _vmap_levels(rng):
+        raise ValueError("under vmap every sample would drop the same elements: map over rng too, "
+                         "[seed, step] of each sample")
 
 
 def dropout(x: torch.Tensor, p: float, rng: torch.Tensor, site: int = 0) -> torch.Tensor:
@@ -183,6 +200,8 @@ def layer_norm(
     _check_dropout(p, rng, site, x)
     if p == 0.0:
         rng = None
+    elif residual is not None and _is_batched(residual):
+        _check_dropout(p, rng, site, residual)
     return _ops.dropout_layernorm(x.contiguous(), residual, weight.contiguous(),
                                   bias.contiguous(), rng, eps, p, site)
 

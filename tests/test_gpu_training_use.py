@@ -43,3 +43,25 @@ def test_tangents_of_a_gradient_are_refused(which):
         dy = forward_ad.make_dual(torch.ones_like(y), torch.ones_like(y))
         with pytest.raises(NotImplementedError, match="forward-mode"):
             torch.autograd.grad(y, x, dy)
+
+
+def test_vmap_with_an_rng_for_every_sample():
+    """The samples' values are those of calls by themselves."""
+
+    from disentangled_flash import training
+
+    x = torch.randn(4, 6, 72, device="cuda")
+    w, b = torch.rand(2, 72, device="cuda")
+    rngs = torch.stack([_rng() + i for i in range(4)])
+
+    def tail(t, r):
+        return training.layer_norm(training.dropout(t, 0.3, r, 1), w, b, 1e-5, t, 0.5, r, SITE)
+
+    got = torch.func.vmap(tail)(x, rngs)
+    for i in range(4):
+        assert torch.equal(got[i], tail(x[i], rngs[i]))
+    assert not torch.equal(torch.func.vmap(tail)(x[:1].expand(2, 6, 72), rngs[:2])[0],
+                           tail(x[0], rngs[1]))
+    table = torch.randn(9, 72, device="cuda")
+    ids = torch.arange(8, device="cuda").view(4, 2)
+    assert torch.equal(torch.func.vmap(lambda i: training.embedding(i, table))(ids), table[ids])

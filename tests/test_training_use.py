@@ -62,3 +62,37 @@ def test_tangents_through_functions_are_refused():
                          (lambda t: training.embedding(ids, t), table)):
             with pytest.raises(NotImplementedError, match="forward-mode"):
                 torch.func.jvp(call, (at,), (torch.ones_like(at),))
+
+
+def test_one_mask_for_every_sample_is_refused():
+    """Under vmap: the samples' masks come from their own rng, or the call raises."""
+
+    from disentangled_flash import training
+
+    vmap = torch.func.vmap
+    with FakeTensorMode():
+        x = torch.empty(4, 3, 16, device="cuda")
+        w = torch.empty(16, device="cuda")
+        rng = torch.empty(2, dtype=torch.int64, device="cuda")
+        rngs = torch.empty(4, 2, dtype=torch.int64, device="cuda")
+
+        def drop(t, r):
+            return training.dropout(t, 0.5, r)
+
+        def tail(t, residual, r, p=0.5):
+            return training.layer_norm(t, w, w, 1e-5, residual, p, r)
+
+        for call in (
+            lambda: vmap(drop, (0, None))(x, rng),
+            lambda: vmap(tail, (0, 0, None))(x, x, rng),
+            lambda: vmap(tail, (0, None, None))(x, x[0], rng),
+            lambda: vmap(tail, (None, 0, None))(x[0], x, rng),
+            lambda: vmap(vmap(drop, (0, None)), (0, 0))(x, rngs),  # the inner samples share one
+            lambda: vmap(vmap(drop, (0, 0)), (0, None))(x, rngs[:3]),  # the outer ones
+        ):
+            with pytest.raises(ValueError, match="vmap"):
+                call()
+        assert vmap(drop)(x, rngs).shape == x.shape
+        assert vmap(tail)(x, x, rngs).shape == x.shape
+        assert vmap(lambda t: tail(t, None, None, 0.0))(x).shape == x.shape
+        assert vmap(lambda t: training.dropout(t, 0.0, rng))(x).shape == x.shape
