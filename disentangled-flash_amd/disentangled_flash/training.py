@@ -53,20 +53,23 @@ class _Ops:
     def __getattr__(self, name: str) -> Any:
         if name not in self.names:
             raise AttributeError(name)
-        with _loading:
-            if name not in self.__dict__:
-                _lib.load_torch_ops()
-                _register_fakes()
-                namespace = torch.ops.disentangled_flash
-                for op in self.names:
-                    setattr(self, op, getattr(namespace, op).default)
-        return self.__dict__[name]
-
-
-_loading = threading.Lock()
+        _load()
+        return getattr(torch.ops.disentangled_flash, name).default
 
 
 _ops = _Ops()
+_loading = threading.Lock()
+
+
+@torch.compiler.assume_constant_result  # (a first use may be traced: this runs, and is not)
+def _load() -> bool:
+    with _loading:
+        if _Ops.names[0] not in _ops.__dict__:
+            _lib.load_torch_ops()
+            _register_fakes()
+            for op in reversed(_Ops.names):
+                setattr(_ops, op, getattr(torch.ops.disentangled_flash, op).default)
+    return True
 
 
 def _register_fakes() -> None:

@@ -4,6 +4,9 @@ tensors, or are recorded."""
 
 from __future__ import annotations
 
+import subprocess
+import sys
+
 import pytest
 import torch
 from torch._subclasses.fake_tensor import FakeTensorMode
@@ -96,3 +99,39 @@ def test_one_mask_for_every_sample_is_refused():
         assert vmap(tail)(x, x, rngs).shape == x.shape
         assert vmap(lambda t: tail(t, None, None, 0.0))(x).shape == x.shape
         assert vmap(lambda t: training.dropout(t, 0.0, rng))(x).shape == x.shape
+
+
+_FIRST_USE = """
+import sys
+import torch
+sys.path.insert(0, {package!r})
+from disentangled_flash import training
+
+training._check_floating = lambda name, tensor: None  # (CPU tensors: nothing is run)
+graphs = []
+
+def backend(graph, inputs):
+    graphs.append(graph)
+    return lambda *args: (torch.zeros(3, 16),)
+
+x, w, rng = torch.zeros(3, 16), torch.zeros(16), torch.zeros(2, dtype=torch.int64)
+table, ids = torch.zeros(9, 16), torch.zeros(3, dtype=torch.int64)
+call = {call}
+torch.compile(call, backend=backend, fullgraph=True)()
+names = [str(node.target) for graph in graphs for node in graph.graph.nodes]
+assert any("disentangled_flash." in name for name in names), names
+"""
+
+
+@pytest.mark.parametrize("call", ["lambda: training.dropout(x, 0.5, rng)",
+                                  "lambda: training.layer_norm(x, w, w, 1e-5, x, 0.5, rng)",
+                                  "lambda: training.embedding(ids, table)"])
+def test_first_use_may_be_traced(call):
+    """A process whose first call of an operator is inside torch.compile, as one graph."""
+
+    from disentangled_flash import _lib
+
+    program = _FIRST_USE.format(package=str(_lib.library_path().parents[1]), call=call)
+    done = subprocess.run([sys.executable, "-c", program], capture_output=True, text=True,
+                          timeout=300)
+    assert done.returncode == 0, done.stderr[-2000:]
