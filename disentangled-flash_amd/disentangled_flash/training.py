@@ -250,6 +250,7 @@ class DropoutState(nn.Module):
     :meth:`advance` starts the next step.  It adds to the buffer in place (so a captured step
     goes on at every replay) and takes a copy as this step's ``rng``: a forward whose backward
     pass is still to come keeps its own.  The buffer is not saved with the model.
+    :meth:`begin` leaves it to the first place that asks for ``rng``.
 
     :meth:`keep_for` ties a step to a forward's outputs: when their backward pass begins, the
     step's ``rng`` is the current one again, so that layers recomputed in it (checkpointing)
@@ -263,15 +264,22 @@ class DropoutState(nn.Module):
         self.register_buffer("counter", torch.tensor([int(seed), 0], dtype=torch.int64,
                                                      device=device), persistent=False)
         self._rng: torch.Tensor | None = None
+        self._begun = False
 
     @property
     def rng(self) -> torch.Tensor:
+        if self._begun:
+            self.advance()
         if self._rng is None or self._rng.device != self.counter.device:
             self._rng = self.counter.clone()
         return self._rng
 
+    def begin(self) -> None:
+        self._begun = True
+
     @torch.no_grad()
     def advance(self) -> None:
+        self._begun = False
         self.counter[1:].add_(1)
         self._rng = self.counter.clone()
 
@@ -280,6 +288,7 @@ class DropoutState(nn.Module):
 
         def restore(_: torch.Tensor) -> None:
             self._rng = rng
+            self._begun = False
 
         pending = [outputs]
         while pending:
@@ -293,7 +302,7 @@ class DropoutState(nn.Module):
                 pending.extend(item)
 
 
-class Dropout(nn.Module):
+class Dropout(nn.Dropout):
     """``nn.Dropout`` on :func:`dropout`: the identity in eval mode.
 
     Called again before the next :meth:`DropoutState.advance` it drops the same elements, which
@@ -301,15 +310,16 @@ class Dropout(nn.Module):
     """
 
     def __init__(self, p: float, state: DropoutState, site: int) -> None:
-        super().__init__()
         _check_dropout(p, state.counter, site, state.counter)
-        self.p = p
+        super().__init__(p)
         self.site = site
         self.__dict__["state"] = state  # the model's, registered there once
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         if not self.training or self.p == 0:
             return x
+        if self.inplace:
+            return super().forward(x)
         return dropout(x, self.p, self.state.rng, self.site)
 
     def extra_repr(self) -> str:
@@ -409,11 +419,14 @@ def _training_form(module: nn.Module, state: DropoutState, sites: Any) -> nn.Mod
 def _advance_state(model: nn.Module, args: Any) -> None:
     if model.training:
         model.dropout_state.advance()
+    elif not model.dropout_state._begun:  # parts of it may be in training mode
+        model.dropout_state.begin()
 
 
 def _keep_state(model: nn.Module, args: Any, outputs: Any) -> None:
-    if model.training:
-        model.dropout_state.keep_for(outputs)
+    state = model.dropout_state
+    if model.training or not state._begun:
+        state.keep_for(outputs)
 
 
 def enable_deberta_training(model: nn.Module, *, seed: int = 0) -> nn.Module:
@@ -428,7 +441,9 @@ def enable_deberta_training(model: nn.Module, *, seed: int = 0) -> nn.Module:
 
     Every training forward of the backbone starts with ``model.dropout_state.advance()``, and
     its backward pass has the same step again, so checkpointed layers recompute what they
-    computed.  Recomputing the whole backbone would draw new masks.
+    computed.  Recomputing the whole backbone would draw new masks.  A forward of a backbone in
+    eval mode advances where a dropout in training mode first drops (Monte Carlo dropout, a few
+    layers in training).
     """
 
     from .deberta import DebertaV2InferenceEncoder

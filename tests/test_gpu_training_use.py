@@ -3,6 +3,8 @@ layouts and ids."""
 
 from __future__ import annotations
 
+import copy
+
 import pytest
 import torch
 from torch.autograd import forward_ad
@@ -65,3 +67,62 @@ def test_vmap_with_an_rng_for_every_sample():
     table = torch.randn(9, 72, device="cuda")
     ids = torch.arange(8, device="cuda").view(4, 2)
     assert torch.equal(torch.func.vmap(lambda i: training.embedding(i, table))(ids), table[ids])
+
+
+# ---- a model -------------------------------------------------------------------------
+
+
+def _backbone(p):
+    from transformers import DebertaV2Config, DebertaV2Model
+
+    torch.manual_seed(5)
+    return DebertaV2Model(DebertaV2Config(
+        vocab_size=100, hidden_size=64, num_hidden_layers=2, num_attention_heads=2,
+        intermediate_size=128, hidden_act="gelu", type_vocab_size=2, max_position_embeddings=64,
+        relative_attention=True, position_buckets=16, pos_att_type=["p2c", "c2p"],
+        norm_rel_ebd="layer_norm", share_att_key=True, conv_kernel_size=3, conv_act="gelu",
+        position_biased_input=True, hidden_dropout_prob=p, attention_probs_dropout_prob=p)).cuda()
+
+
+def _batch():
+    gen = torch.Generator().manual_seed(2)
+    return torch.randint(1, 100, (3, 24), generator=gen).cuda()
+
+
+def _grads(model):
+    return {n: p.grad.clone() for n, p in model.named_parameters() if p.grad is not None}
+
+
+def _same_gradients(got, want):
+    """torch adds the gradients of the attention's gathers with atomics, and a compiled graph may
+    decompose its operators otherwise: 1000 half steps of the largest, where other masks would
+    change a gradient by its own size."""
+
+    assert got.keys() == want.keys()
+    for name in want:
+        size = want[name].abs().max().item()
+        assert (got[name] - want[name]).abs().max().item() <= 1000 * ref.U * size, name
+
+
+@pytest.mark.parametrize("compiled", [False, True])
+def test_layers_in_training_in_a_backbone_in_eval_mode(compiled):
+    """Each forward draws new masks, and its gradients are those of its masks."""
+
+    from disentangled_flash import enable_deberta_training
+
+    ids = _batch()
+    model = enable_deberta_training(_backbone(0.3), seed=4).eval()
+    twin = copy.deepcopy(model)
+    for m in (model, twin):
+        m.encoder.layer[1].train()
+    call = torch.compile(model, backend="aot_eager") if compiled else model
+    seen = []
+    for step in range(1, 4):
+        out = call(ids).last_hidden_state
+        out.square().sum().backward()
+        seen.append(out.detach())
+        assert model.dropout_state.counter.tolist() == [4, step]
+        twin.dropout_state.counter[1] = step - 1
+        twin(ids).last_hidden_state.square().sum().backward()
+        _same_gradients(_grads(model), _grads(twin))
+    assert not torch.equal(seen[0], seen[1]) and not torch.equal(seen[1], seen[2])

@@ -4,13 +4,16 @@ tensors, or are recorded."""
 
 from __future__ import annotations
 
+import functools
 import subprocess
 import sys
 
 import pytest
 import torch
+from torch import nn
 from torch._subclasses.fake_tensor import FakeTensorMode
 from torch.autograd import forward_ad
+from torch.utils.checkpoint import checkpoint
 
 
 @pytest.fixture(autouse=True)
@@ -135,3 +138,105 @@ def test_first_use_may_be_traced(call):
     done = subprocess.run([sys.executable, "-c", program], capture_output=True, text=True,
                           timeout=300)
     assert done.returncode == 0, done.stderr[-2000:]
+
+
+def _backbone(**over):
+    from transformers import DebertaV2Config, DebertaV2Model
+
+    fields = dict(vocab_size=100, hidden_size=64, num_hidden_layers=2, num_attention_heads=2,
+                  intermediate_size=128, hidden_act="gelu", type_vocab_size=2,
+                  max_position_embeddings=64, relative_attention=True, position_buckets=16,
+                  pos_att_type=["p2c", "c2p"], norm_rel_ebd="layer_norm", share_att_key=True)
+    fields.update(over)
+    torch.manual_seed(5)
+    return DebertaV2Model(DebertaV2Config(**fields))
+
+
+@pytest.fixture
+def drops(monkeypatch):
+    """The (site, seed, step) of every element-wise dropout, which returns its input."""
+
+    from disentangled_flash import training
+
+    seen = []
+
+    def dropout(x, p, rng, site=0):
+        seen.append((site, *rng.tolist()))
+        return x
+
+    monkeypatch.setattr(training, "dropout", dropout)
+    return seen
+
+
+def _forward(model):
+    return model(torch.arange(20).reshape(2, 10)).last_hidden_state
+
+
+def _steps(drops):
+    """The steps met since the last call, and forgets them."""
+
+    steps = {step for _, _, step in drops}
+    drops.clear()
+    return steps
+
+
+@pytest.mark.parametrize("found_by", ["class name", "type", "layer"])
+def test_dropout_of_a_backbone_in_eval_mode_draws_new_masks(drops, found_by):
+    """Monte Carlo dropout, and a layer in training in a backbone that is not."""
+
+    from disentangled_flash import enable_deberta_training
+
+    model = enable_deberta_training(_backbone(), seed=3).eval()
+    with torch.no_grad():
+        _forward(model)
+    assert not drops and model.dropout_state.counter.tolist() == [3, 0]
+    if found_by == "layer":
+        model.encoder.layer[1].train()
+    else:
+        for module in model.modules():
+            if isinstance(module, nn.Dropout) if found_by == "type" \
+                    else type(module).__name__.startswith("Dropout"):
+                module.train()
+    with torch.no_grad():
+        for step in (1, 2, 3):
+            _forward(model)
+            assert _steps(drops) == {step}
+    model.eval()
+    with torch.no_grad():
+        _forward(model)
+    assert not drops
+    model.train()
+    _forward(model)
+    assert _steps(drops) == {4}
+
+
+def test_backward_pass_after_a_forward_in_eval_mode(drops):
+    """A forward in eval mode between a forward and its backward pass, whose checkpointed layer
+    recomputes what it computed; a head that drops behind a backbone in eval mode draws new masks."""
+
+    from disentangled_flash import enable_deberta_training, training
+
+    model = enable_deberta_training(_backbone(), seed=3).train()
+    for layer in model.encoder.layer:
+        layer.forward = functools.partial(checkpoint, layer.forward, use_reentrant=False)
+    out = _forward(model)
+    with torch.no_grad():
+        _forward(model.eval())
+    model.train()
+    assert _steps(drops) == {1}
+    out.sum().backward()
+    assert _steps(drops) == {1}
+    head = training.Dropout(0.5, model.dropout_state, 1000)
+    model.eval()
+    for step in (2, 3):
+        head(_forward(model)).sum().backward()
+        assert _steps(drops) == {step}
+
+
+def test_dropout_made_in_place_is_torchs(drops):
+    from disentangled_flash import training
+
+    drop = training.Dropout(1.0, training.DropoutState(0), 0)
+    drop.inplace = True
+    x = torch.ones(4)
+    assert drop(x) is x and not x.any() and not drops
