@@ -33,7 +33,9 @@ those that do not start on a 16-byte boundary.
 
 from __future__ import annotations
 
+import itertools
 import threading
+from collections import OrderedDict
 from collections.abc import Mapping
 from typing import Any
 
@@ -244,13 +246,97 @@ def embedding(
 # ---- modules ---------------------------------------------------------------------------
 
 
+# Where torch's generator stood when a state drew a step: (the state's token, device, seed,
+# offset) -> that step's rng.  torch.utils.checkpoint puts the generator back for its
+# recomputations, so one of a whole backbone finds the step of its forward here.
+_drawn: OrderedDict[tuple[int, ...], torch.Tensor] = OrderedDict()
+_DRAWN_KEPT = 1 << 14  # forwards whose backward pass is still to come; 512 bytes each on the GPU
+_tokens = itertools.count()
+
+
+def _generator(counter: torch.Tensor) -> Any:
+    """torch's generator of the counter's GPU, where its position can be read."""
+
+    if not _lib.runs_directly(counter) or torch.cuda.is_current_stream_capturing():
+        return None
+    return torch.cuda.default_generators[counter.get_device()]
+
+
+def _leave_position(counter: torch.Tensor) -> None:
+    """Moves torch's generator on, as a dropout of its own would: positions are met once."""
+
+    generator = _generator(counter)
+    if generator is not None:
+        generator.set_offset(generator.get_offset() + 4)
+
+
+def _position(counter: torch.Tensor, token: int) -> tuple[int, ...] | None:
+    generator = _generator(counter)
+    if generator is None:
+        return None
+    return (token, counter.get_device(), generator.initial_seed(), generator.get_offset())
+
+
+def _in_backward_pass() -> bool:
+    return torch._C._current_graph_task_id() != -1
+
+
+_UNKNOWN_STEP = (
+    "a forward that draws dropout masks ran inside a backward pass, and none began where torch's "
+    "generator stands: its masks would not be those of the forward that it recomputes "
+    "(torch.utils.checkpoint puts the generator back with preserve_rng_state=True and the input "
+    "ids as positional arguments, outside graph capture)")
+
+
+def _remember(place: tuple[int, ...] | None, rng: torch.Tensor) -> None:
+    if place is not None:
+        _drawn[place] = rng
+        _drawn.move_to_end(place)
+        if len(_drawn) > _DRAWN_KEPT:
+            _drawn.popitem(last=False)
+
+
+@torch.library.custom_op("disentangled_flash::next_step", mutates_args=())
+def _next_step(counter: torch.Tensor, token: int) -> tuple[torch.Tensor, torch.Tensor]:
+    """:meth:`DropoutState.advance` for a traced graph: the counter's new value, and rng."""
+
+    place = _position(counter, token)
+    _leave_position(counter)
+    if _in_backward_pass():
+        if place not in _drawn:
+            raise RuntimeError(_UNKNOWN_STEP)
+        return counter.clone(), _drawn[place].clone()
+    advanced = counter.clone()
+    advanced[1:].add_(1)
+    _remember(place, advanced.clone())
+    return advanced, advanced.clone()
+
+
+@_next_step.register_fake
+def _(counter, token):
+    return torch.empty_like(counter), torch.empty_like(counter)
+
+
+class _Phase:
+    """Where a state stands (apart from it: an nn.Module's attributes are slow to set)."""
+
+    begun = False  # the next place that asks for rng advances
+    inside = False  # a forward in eval mode runs
+    unknown = False  # the forward that is recomputed was not found
+
+
 class DropoutState(nn.Module):
     """Seed and step of a model's dropout: one buffer that its :class:`Dropout` modules share.
 
     :meth:`advance` starts the next step.  It adds to the buffer in place (so a captured step
     goes on at every replay) and takes a copy as this step's ``rng``: a forward whose backward
     pass is still to come keeps its own.  The buffer is not saved with the model.
-    :meth:`begin` leaves it to the first place that asks for ``rng``.
+    Between :meth:`begin` and :meth:`end` the first place that asks for ``rng`` advances.
+
+    In a backward pass ``advance`` belongs to a recomputation (``torch.utils.checkpoint`` around
+    the backbone): ``rng`` is that of the forward which drew where torch's generator of the GPU
+    stands again.  Where there is none (the generator was not put back) asking for it raises.
+    Advancing moves that generator on, as ``nn.Dropout`` does.
 
     :meth:`keep_for` ties a step to a forward's outputs: when their backward pass begins, the
     step's ``rng`` is the current one again, so that layers recomputed in it (checkpointing)
@@ -264,31 +350,66 @@ class DropoutState(nn.Module):
         self.register_buffer("counter", torch.tensor([int(seed), 0], dtype=torch.int64,
                                                      device=device), persistent=False)
         self._rng: torch.Tensor | None = None
-        self._begun = False
+        self._phase = _Phase()
+        self._token = next(_tokens)
+
+    def __setstate__(self, state: dict[str, Any]) -> None:
+        super().__setstate__(state)
+        self._token = next(_tokens)  # (a copy draws steps of its own)
 
     @property
     def rng(self) -> torch.Tensor:
-        if self._begun:
-            self.advance()
+        if self._phase.begun:
+            # (The place that asks may lie in a checkpointed layer, whose recomputation does not
+            # come here: inside a forward torch's generator stays where it is until the end.)
+            self._advance(moves=not self._phase.inside)
+        if self._phase.unknown:
+            raise RuntimeError(_UNKNOWN_STEP)
         if self._rng is None or self._rng.device != self.counter.device:
             self._rng = self.counter.clone()
         return self._rng
 
     def begin(self) -> None:
-        self._begun = True
+        self._phase.begun = self._phase.inside = True
+
+    def end(self) -> bool:
+        """Whether rng was asked for since :meth:`begin`."""
+
+        self._phase.inside = False
+        if not self._phase.begun:
+            _leave_position(self.counter)
+        return not self._phase.begun
+
+    def advance(self) -> None:
+        self._advance(moves=True)
 
     @torch.no_grad()
-    def advance(self) -> None:
-        self._begun = False
+    def _advance(self, moves: bool) -> None:
+        phase = self._phase
+        phase.begun = phase.unknown = False
+        if torch.compiler.is_compiling():
+            advanced, self._rng = _next_step(self.counter, self._token)
+            self.counter.copy_(advanced)
+            return
+        place = _position(self.counter, self._token)
+        if moves:
+            _leave_position(self.counter)
+        if _in_backward_pass():
+            self._rng = _drawn.get(place)
+            phase.unknown = self._rng is None  # (an error where masks are drawn)
+            return
         self.counter[1:].add_(1)
         self._rng = self.counter.clone()
+        _remember(place, self._rng)
 
     def keep_for(self, outputs: Any) -> None:
+        if self._phase.unknown:
+            return
         rng = self.rng
 
         def restore(_: torch.Tensor) -> None:
             self._rng = rng
-            self._begun = False
+            self._phase.begun = self._phase.unknown = False
 
         pending = [outputs]
         while pending:
@@ -419,13 +540,13 @@ def _training_form(module: nn.Module, state: DropoutState, sites: Any) -> nn.Mod
 def _advance_state(model: nn.Module, args: Any) -> None:
     if model.training:
         model.dropout_state.advance()
-    elif not model.dropout_state._begun:  # parts of it may be in training mode
+    else:  # parts of it may be in training mode
         model.dropout_state.begin()
 
 
 def _keep_state(model: nn.Module, args: Any, outputs: Any) -> None:
     state = model.dropout_state
-    if model.training or not state._begun:
+    if model.training or state.end():
         state.keep_for(outputs)
 
 
@@ -440,9 +561,8 @@ def enable_deberta_training(model: nn.Module, *, seed: int = 0) -> nn.Module:
     without weights) stay as they are.
 
     Every training forward of the backbone starts with ``model.dropout_state.advance()``, and
-    its backward pass has the same step again, so checkpointed layers recompute what they
-    computed.  Recomputing the whole backbone would draw new masks.  A forward of a backbone in
-    eval mode advances where a dropout in training mode first drops (Monte Carlo dropout, a few
+    its backward pass has the same step again, so what is checkpointed (a layer, or the whole
+    backbone) recomputes what it computed.  A forward of a backbone in eval mode advances where a dropout in training mode first drops (Monte Carlo dropout, a few
     layers in training).
     """
 

@@ -4,10 +4,13 @@ layouts and ids."""
 from __future__ import annotations
 
 import copy
+import functools
 
 import pytest
 import torch
+from torch import nn
 from torch.autograd import forward_ad
+from torch.utils.checkpoint import checkpoint
 
 import training_reference as ref  # noqa: E402 (tests/ is on the path)
 
@@ -126,3 +129,63 @@ def test_layers_in_training_in_a_backbone_in_eval_mode(compiled):
         twin(ids).last_hidden_state.square().sum().backward()
         _same_gradients(_grads(model), _grads(twin))
     assert not torch.equal(seen[0], seen[1]) and not torch.equal(seen[1], seen[2])
+
+
+def _gradients(model, ids, call, forwards=2):
+    """Two forwards before the backward pass over both, and one by itself."""
+
+    model.zero_grad()
+    outs = [call(ids.roll(i, 0)) for i in range(forwards)]
+    sum((out * (i + 1)).square().sum() for i, out in enumerate(outs)).backward()
+    call(ids).square().sum().backward()
+    return _grads(model)
+
+
+@pytest.mark.parametrize("how", ["plain", "reentrant", "with its head", "nested", "compiled",
+                                 "eval mode"])
+def test_checkpointed_backbone_has_the_gradients_of_its_masks(how):
+    """The same gradients as without torch.utils.checkpoint; an nn.Dropout of the program in the
+    region keeps its masks too.  (Other masks would change a gradient by its own size.)"""
+
+    from disentangled_flash import enable_deberta_training
+
+    ids = _batch()
+    grads = []
+    for checkpointed in (False, True):
+        model = enable_deberta_training(_backbone(0.3), seed=8).train()
+        if how == "eval mode":
+            model.eval().encoder.layer[1].train()
+        own = nn.Dropout(0.5)
+        head = nn.Linear(64, 64, device="cuda")
+        leaf = torch.ones(1, device="cuda", requires_grad=True)
+        call = torch.compile(model, backend="aot_eager") if how == "compiled" else model
+        if how == "nested" and checkpointed:
+            for layer in model.encoder.layer:
+                layer.forward = functools.partial(checkpoint, layer.forward, use_reentrant=False)
+
+        def region(ids, leaf):
+            out = own(call(ids).last_hidden_state) * leaf
+            return head(out) if how == "with its head" else out
+
+        def step(ids):
+            if checkpointed:
+                return checkpoint(region, ids, leaf, use_reentrant=how == "reentrant")
+            return region(ids, leaf)
+
+        torch.manual_seed(9)
+        grads.append(_gradients(model, ids, step))
+        assert model.dropout_state.counter.tolist() == [8, 3]
+    _same_gradients(grads[1], grads[0])
+
+
+def test_checkpointed_backbone_without_its_generator_raises():
+    from disentangled_flash import enable_deberta_training
+
+    ids = _batch()
+    model = enable_deberta_training(_backbone(0.3), seed=8).train()
+    for out in (checkpoint(model, ids, use_reentrant=False, preserve_rng_state=False),
+                checkpoint(model, input_ids=ids, use_reentrant=False)):
+        with pytest.raises(RuntimeError, match="generator"):
+            out.last_hidden_state.sum().backward()
+    model(ids).last_hidden_state.sum().backward()
+    assert model.dropout_state.counter.tolist() == [8, 3]

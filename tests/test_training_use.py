@@ -4,6 +4,8 @@ tensors, or are recorded."""
 
 from __future__ import annotations
 
+import contextlib
+import copy
 import functools
 import subprocess
 import sys
@@ -240,3 +242,118 @@ def test_dropout_made_in_place_is_torchs(drops):
     drop.inplace = True
     x = torch.ones(4)
     assert drop(x) is x and not x.any() and not drops
+
+
+class _Generator:
+    """torch's generator of a GPU, as far as the state reads it."""
+
+    offset = 0
+
+    def initial_seed(self):
+        return 1234
+
+    def get_offset(self):
+        return self.offset
+
+    def set_offset(self, offset):
+        self.offset = offset
+
+    @contextlib.contextmanager
+    def back_at(self, offset):
+        self.offset, now = offset, self.offset
+        yield
+        self.offset = now
+
+
+@pytest.fixture
+def generator(monkeypatch):
+    from disentangled_flash import training
+
+    made = _Generator()
+    monkeypatch.setattr(training, "_generator", lambda counter: made)
+    return made
+
+
+def _checkpointed(model, generator, use_reentrant):
+    """torch.utils.checkpoint around the backbone, which puts ``generator`` back."""
+
+    start = generator.offset
+    weight = torch.ones(1, requires_grad=True)  # (what a reentrant one has to differentiate)
+
+    def call(weight):
+        with generator.back_at(start) if torch._C._current_graph_task_id() != -1 \
+                else contextlib.nullcontext():
+            return _forward(model) * weight
+
+    return checkpoint(call, weight, use_reentrant=use_reentrant)
+
+
+@pytest.mark.parametrize("use_reentrant", [False, True])
+@pytest.mark.parametrize("mode", ["train", "eval"])
+def test_checkpointed_backbone_recomputes_its_own_masks(drops, generator, use_reentrant, mode):
+    """Two forwards before their backward passes, in either order."""
+
+    from disentangled_flash import enable_deberta_training
+
+    model = enable_deberta_training(_backbone(), seed=3).train()
+    if mode == "eval":
+        model.eval().encoder.layer[1].train()
+    for order in ((0, 1), (1, 0)):
+        steps, outs = [], []
+        for _ in range(2):
+            outs.append(_checkpointed(model, generator, use_reentrant))
+            steps.append(_steps(drops))
+            assert len(steps[-1]) == 1
+        assert steps[0] != steps[1]
+        counter = model.dropout_state.counter.tolist()
+        for i in order:
+            outs[i].sum().backward()
+            assert _steps(drops) == steps[i]
+        assert model.dropout_state.counter.tolist() == counter
+    _forward(model)
+    assert _steps(drops) == {counter[1] + 1}
+
+
+def test_recomputation_without_its_generator_raises(drops, generator):
+    from disentangled_flash import enable_deberta_training
+
+    model = enable_deberta_training(_backbone(), seed=3).train()
+    out = checkpoint(lambda: _forward(model), use_reentrant=False)
+    with pytest.raises(RuntimeError, match="generator"):
+        out.sum().backward()
+    drops.clear()
+    _forward(model).sum().backward()  # the state goes on
+    assert _steps(drops) == {2}
+    # Where nothing is dropped nothing is wrong.
+    model = enable_deberta_training(
+        _backbone(hidden_dropout_prob=0.0, attention_probs_dropout_prob=0.0)).train()
+    checkpoint(lambda: _forward(model), use_reentrant=False).sum().backward()
+    assert not drops
+
+
+def test_copies_of_a_model_have_steps_of_their_own(drops, generator):
+    from disentangled_flash import enable_deberta_training
+
+    model = enable_deberta_training(_backbone(), seed=3).train()
+    twin = copy.deepcopy(model)
+    twin.dropout_state.counter[1] = 10
+    start = generator.offset
+    first = _checkpointed(model, generator, False)
+    generator.offset = start  # (the same position)
+    second = _checkpointed(twin, generator, False)
+    assert _steps(drops) == {1, 11}
+    first.sum().backward()
+    assert _steps(drops) == {1}
+    second.sum().backward()
+    assert _steps(drops) == {11}
+
+
+def test_steps_remembered_are_bounded(drops, generator, monkeypatch):
+    from disentangled_flash import training
+
+    monkeypatch.setattr(training, "_DRAWN_KEPT", 3)
+    training._drawn.clear()
+    state = training.DropoutState(1)
+    for _ in range(5):
+        state.advance()
+    assert [rng.tolist() for rng in training._drawn.values()] == [[1, 3], [1, 4], [1, 5]]
