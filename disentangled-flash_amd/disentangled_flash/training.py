@@ -41,6 +41,7 @@ from typing import Any
 
 import torch
 from torch import nn
+from torch.nn.modules import module as torch_module
 
 from . import _lib
 
@@ -447,11 +448,15 @@ class Dropout(nn.Dropout):
         return f"p={self.p}, site={self.site}"
 
 
+def _on_gpu(x: torch.Tensor) -> bool:
+    return x.device.type == "cuda"
+
+
 class LayerNorm(nn.LayerNorm):
     """``nn.LayerNorm`` over the last dimension on :func:`layer_norm`; torch's on the CPU."""
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
-        if x.device.type != "cuda":
+        if not _on_gpu(x):
             return super().forward(x)
         return layer_norm(x, self.weight, self.bias, self.eps)
 
@@ -460,14 +465,18 @@ class Embedding(nn.Embedding):
     """``nn.Embedding`` on :func:`embedding`; torch's on the CPU."""
 
     def forward(self, input_ids: torch.Tensor) -> torch.Tensor:
-        if input_ids.device.type != "cuda":
+        if not _on_gpu(input_ids):
             return super().forward(input_ids)
         return embedding(input_ids, self.weight, padding_idx=self.padding_idx)
 
 
 class OutputBlock(nn.Module):
     """``LayerNorm(dropout(dense(x)) + input)`` with the sub-modules of a Hugging Face
-    ``DebertaV2SelfOutput`` / ``DebertaV2Output`` under their names."""
+    ``DebertaV2SelfOutput`` / ``DebertaV2Output`` under their names.
+
+    Dropout, sum and norm are one call while ``LayerNorm`` and ``dropout`` are what they were:
+    where one is replaced or has hooks, they are called themselves.
+    """
 
     def __init__(self, dense: nn.Module, norm: nn.LayerNorm, drop: Dropout) -> None:
         super().__init__()
@@ -478,7 +487,8 @@ class OutputBlock(nn.Module):
     def forward(self, hidden_states: torch.Tensor, input_tensor: torch.Tensor) -> torch.Tensor:
         x = self.dense(hidden_states)
         norm, drop = self.LayerNorm, self.dropout
-        if x.device.type != "cuda":
+        if not (_on_gpu(x) and _norm_fits(norm) and _dropout_fits(drop)) \
+                or _hooks_on_all_modules():
             return norm(drop(x) + input_tensor)
         if x.dtype != input_tensor.dtype:  # (under autocast: as the sum would promote them)
             dtype = torch.promote_types(x.dtype, input_tensor.dtype)
@@ -497,10 +507,22 @@ def _has_hooks(module: nn.Module) -> bool:
                 or module._backward_pre_hooks or "forward" in module.__dict__)
 
 
+def _hooks_on_all_modules() -> bool:
+    return bool(torch_module._global_forward_hooks or torch_module._global_forward_pre_hooks
+                or torch_module._global_backward_hooks or torch_module._global_backward_pre_hooks)
+
+
 def _norm_fits(module: Any) -> bool:
-    return (isinstance(module, nn.LayerNorm) and module.weight is not None
+    """Whether calling ``module`` is :func:`layer_norm` of its weights and nothing else."""
+
+    return ((type(module) is nn.LayerNorm or type(module) is LayerNorm)
+            and module.weight is not None
             and module.bias is not None and len(module.normalized_shape) == 1
             and module.normalized_shape[0] <= MAX_HIDDEN and not _has_hooks(module))
+
+
+def _dropout_fits(module: Any) -> bool:
+    return type(module) is Dropout and not module.inplace and not _has_hooks(module)
 
 
 def _adopt(made: nn.Module, module: nn.Module) -> nn.Module:

@@ -189,3 +189,30 @@ def test_checkpointed_backbone_without_its_generator_raises():
             out.last_hidden_state.sum().backward()
     model(ids).last_hidden_state.sum().backward()
     assert model.dropout_state.counter.tolist() == [8, 3]
+
+
+def test_output_block_whose_children_change():
+    """Hooks put on later run, and what replaced a child is called.  (Between two norms in fp32:
+    1e-5 is 42 half steps of values up to 4.)"""
+
+    from disentangled_flash import enable_deberta_training
+
+    block = enable_deberta_training(_backbone(0.0)).encoder.layer[0].output
+    x, r = torch.randn(5, 128, device="cuda"), torch.randn(5, 64, device="cuda")
+    want = block(x, r)
+    seen = []
+    handles = [child.register_forward_hook(lambda m, i, o: seen.append(type(m).__name__))
+               for child in (block.LayerNorm, block.dropout)]
+    torch.testing.assert_close(block(x, r), want, atol=1e-5, rtol=1e-5)
+    assert seen == ["Dropout", "LayerNorm"]
+    for handle in handles:
+        handle.remove()
+    assert torch.equal(block(x, r), want) and len(seen) == 2
+    plain = block.LayerNorm
+    block.LayerNorm = nn.RMSNorm(64, device="cuda")
+    assert torch.equal(block(x, r), block.LayerNorm(block.dense(x) + r))
+    block.LayerNorm = plain
+    for drop in (nn.Identity(), nn.Dropout(1.0)):
+        block.dropout = drop
+        torch.testing.assert_close(block(x, r), plain(drop(block.dense(x)) + r), atol=1e-5,
+                                   rtol=1e-5)

@@ -357,3 +357,90 @@ def test_steps_remembered_are_bounded(drops, generator, monkeypatch):
     for _ in range(5):
         state.advance()
     assert [rng.tolist() for rng in training._drawn.values()] == [[1, 3], [1, 4], [1, 5]]
+
+
+# ---- output blocks whose children change ---------------------------------------------
+
+
+@pytest.fixture
+def block(monkeypatch):
+    """An output block that takes CPU tensors for a GPU's, and records what it computes itself."""
+
+    from disentangled_flash import enable_deberta_training, training
+
+    made = enable_deberta_training(_backbone()).encoder.layer[0].output.train()
+    assert type(made) is training.OutputBlock
+    made.calls = calls = []
+
+    def layer_norm(x, weight, bias, eps, residual=None, p=0.0, rng=None, site=0):
+        calls.append("layer_norm")
+        return nn.functional.layer_norm(x + residual, (64,), weight, bias, eps)
+
+    monkeypatch.setattr(training, "layer_norm", layer_norm)
+    monkeypatch.setattr(training, "dropout", lambda x, p, rng, site=0: calls.append("dropout") or x)
+    monkeypatch.setattr(training, "_on_gpu", lambda x: True)
+    return made
+
+
+def _call(block):
+    block.calls.clear()
+    return block(torch.ones(2, 128), torch.linspace(-1, 1, 128).view(2, 64))
+
+
+def test_output_block_is_one_call(block):
+    want = _call(block)
+    assert block.calls == ["layer_norm"]
+    assert torch.equal(_call(block.eval()), want) and block.calls == ["layer_norm"]
+
+
+@pytest.mark.parametrize("child", ["LayerNorm", "dropout"])
+@pytest.mark.parametrize("kind", ["forward", "forward_pre", "full_backward", "full_backward_pre"])
+def test_hooks_put_on_later_run(block, child, kind):
+    seen = []
+    module = getattr(block, child)
+    handle = getattr(module, f"register_{kind}_hook")(lambda *a: seen.append(child) and None)
+    _call(block).sum().backward()
+    assert seen == [child] and block.calls == ["dropout"]
+    handle.remove()
+    _call(block)
+    assert seen == [child] and block.calls == ["layer_norm"]
+
+
+@pytest.mark.parametrize("kind", ["forward", "forward_pre", "full_backward", "full_backward_pre"])
+def test_hooks_of_all_modules_run(block, kind):
+    seen = []
+    register = getattr(torch.nn.modules.module, f"register_module_{kind}_hook")
+    handle = register(lambda module, *a: seen.append(type(module).__name__) and None)
+    try:
+        _call(block).sum().backward()
+    finally:
+        handle.remove()
+    assert "LayerNorm" in seen and "Dropout" in seen
+
+
+def test_forward_set_on_a_child_is_called(block):
+    block.LayerNorm.forward = lambda x: x * 0 + 5
+    assert bool((_call(block) == 5).all())
+
+
+def test_replaced_children_are_called(block):
+    class Scaled(nn.LayerNorm):
+        def forward(self, x):
+            return 3 * super().forward(x)
+
+    want = _call(block)
+    plain = block.LayerNorm
+    block.LayerNorm = Scaled(64, plain.eps)
+    assert torch.equal(_call(block), 3 * want)
+    block.LayerNorm = nn.RMSNorm(64)
+    assert not torch.equal(_call(block), want) and block.calls == ["dropout"]
+    block.LayerNorm = nn.LayerNorm(64, elementwise_affine=False)
+    _call(block)
+    block.LayerNorm = nn.Identity()
+    _call(block)
+    block.LayerNorm = plain
+    for drop in (nn.Dropout(0.0), nn.Identity()):
+        block.dropout = drop
+        assert torch.equal(_call(block), want) and block.calls == []
+    block.dropout = nn.Dropout(1.0)
+    assert torch.equal(_call(block)[0], _call(block)[0]) and block.calls == []
