@@ -500,6 +500,13 @@ class OutputBlock(nn.Module):
 
 
 _OUTPUT_BLOCKS = ("DebertaV2SelfOutput", "DebertaV2Output")
+_OUTPUT_BLOCKS_FROM = "transformers.models.deberta_v2.modeling_deberta_v2"
+
+
+def _is_output_block(module: nn.Module) -> bool:
+    kind = type(module)
+    return (kind.__name__ in _OUTPUT_BLOCKS and kind.__module__ == _OUTPUT_BLOCKS_FROM
+            and kind.forward.__module__ == _OUTPUT_BLOCKS_FROM)
 
 
 def _has_hooks(module: nn.Module) -> bool:
@@ -547,7 +554,7 @@ def _training_form(module: nn.Module, state: DropoutState, sites: Any) -> nn.Mod
         made = Embedding(module.num_embeddings, module.embedding_dim, module.padding_idx,
                          device="meta")
         return _adopt(made, module)
-    if type(module).__name__ in _OUTPUT_BLOCKS:
+    if _is_output_block(module):
         children = dict(module.named_children())
         drop = children.get("dropout")
         if set(children) == {"dense", "LayerNorm", "dropout"} and type(drop) is nn.Dropout \

@@ -444,3 +444,49 @@ def test_replaced_children_are_called(block):
         assert torch.equal(_call(block), want) and block.calls == []
     block.dropout = nn.Dropout(1.0)
     assert torch.equal(_call(block)[0], _call(block)[0]) and block.calls == []
+
+
+# ---- which modules are replaced ------------------------------------------------------
+
+
+def test_blocks_are_recognised_by_more_than_their_name():
+    """A class of the same name elsewhere, and a subclass of the norm, keep their own forward."""
+
+    from transformers.models.deberta_v2 import modeling_deberta_v2 as hf
+
+    from disentangled_flash import enable_deberta_training, training
+
+    class DebertaV2Output(nn.Module):
+        def __init__(self, block):
+            super().__init__()
+            self.dense, self.LayerNorm, self.dropout = block.dense, block.LayerNorm, block.dropout
+
+        def forward(self, hidden_states, input_tensor):
+            return self.dropout(self.LayerNorm(self.dense(hidden_states))) + input_tensor
+
+    class Scaled(nn.LayerNorm):
+        def forward(self, x):
+            return 3 * super().forward(x)
+
+    model = _backbone().eval()
+    first, second = model.encoder.layer
+    first.output = DebertaV2Output(first.output)
+    second.output.LayerNorm = Scaled(64)
+    want = _forward(model)
+    enable_deberta_training(model)
+    assert type(first.output) is DebertaV2Output and type(second.output) is hf.DebertaV2Output
+    assert type(first.output.dropout) is training.Dropout  # (its children are replaced)
+    assert type(second.output.LayerNorm) is Scaled
+    assert type(first.attention.output) is training.OutputBlock
+    assert torch.equal(_forward(model), want)
+
+
+def test_a_patched_block_class_keeps_its_forward(monkeypatch):
+    from transformers.models.deberta_v2 import modeling_deberta_v2 as hf
+
+    from disentangled_flash import enable_deberta_training, training
+
+    monkeypatch.setattr(hf.DebertaV2Output, "forward", lambda self, h, x: self.dense(h) + x)
+    model = enable_deberta_training(_backbone())
+    assert type(model.encoder.layer[0].output) is hf.DebertaV2Output
+    assert type(model.encoder.layer[0].attention.output) is training.OutputBlock
