@@ -425,7 +425,7 @@ class DropoutState(nn.Module):
 
 
 class Dropout(nn.Dropout):
-    """``nn.Dropout`` on :func:`dropout`: the identity in eval mode.
+    """``nn.Dropout`` on :func:`dropout`: the identity in eval mode, torch's for float64.
 
     Called again before the next :meth:`DropoutState.advance` it drops the same elements, which
     is what recomputing a checkpointed layer needs.
@@ -440,7 +440,7 @@ class Dropout(nn.Dropout):
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         if not self.training or self.p == 0:
             return x
-        if self.inplace:
+        if self.inplace or (_on_gpu(x) and x.dtype not in _lib.DTYPE_CODES):
             return super().forward(x)
         return dropout(x, self.p, self.state.rng, self.site)
 
@@ -452,20 +452,40 @@ def _on_gpu(x: torch.Tensor) -> bool:
     return x.device.type == "cuda"
 
 
+def _single(*tensors: torch.Tensor) -> tuple[torch.Tensor, ...]:
+    """As ``torch.autocast`` gives them to torch's own LayerNorm: 16 bits become fp32."""
+
+    return tuple(t.float() if t.dtype in (torch.float16, torch.bfloat16) else t for t in tensors)
+
+
+def _types_fit(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor) -> bool:
+    """Whether :func:`layer_norm` takes these types."""
+
+    kind = weight.dtype
+    return (x.dtype in _lib.DTYPE_CODES and kind == bias.dtype
+            and (kind == x.dtype or kind == torch.float32))
+
+
 class LayerNorm(nn.LayerNorm):
-    """``nn.LayerNorm`` over the last dimension on :func:`layer_norm`; torch's on the CPU."""
+    """``nn.LayerNorm`` over the last dimension on :func:`layer_norm`; torch's on the CPU and for
+    types that the operator lacks.  Under ``torch.autocast`` in fp32, as torch's."""
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         if not _on_gpu(x):
             return super().forward(x)
-        return layer_norm(x, self.weight, self.bias, self.eps)
+        rows, weight, bias = x, self.weight, self.bias
+        if torch.is_autocast_enabled("cuda"):
+            rows, weight, bias = _single(rows, weight, bias)
+        if not _types_fit(rows, weight, bias):
+            return super().forward(x)
+        return layer_norm(rows, weight, bias, self.eps)
 
 
 class Embedding(nn.Embedding):
-    """``nn.Embedding`` on :func:`embedding`; torch's on the CPU."""
+    """``nn.Embedding`` on :func:`embedding`; torch's on the CPU and for float64."""
 
     def forward(self, input_ids: torch.Tensor) -> torch.Tensor:
-        if not _on_gpu(input_ids):
+        if not _on_gpu(input_ids) or self.weight.dtype not in _lib.DTYPE_CODES:
             return super().forward(input_ids)
         return embedding(input_ids, self.weight, padding_idx=self.padding_idx)
 
@@ -490,11 +510,16 @@ class OutputBlock(nn.Module):
         if not (_on_gpu(x) and _norm_fits(norm) and _dropout_fits(drop)) \
                 or _hooks_on_all_modules():
             return norm(drop(x) + input_tensor)
-        if x.dtype != input_tensor.dtype:  # (under autocast: as the sum would promote them)
-            dtype = torch.promote_types(x.dtype, input_tensor.dtype)
-            x, input_tensor = x.to(dtype), input_tensor.to(dtype)
+        rows, residual, weight, bias = x, input_tensor, norm.weight, norm.bias
+        if torch.is_autocast_enabled("cuda"):  # (the norm's part of it; 16-bit sums are not rounded)
+            rows, residual, weight, bias = _single(rows, residual, weight, bias)
+        if rows.dtype != residual.dtype:  # as their sum promotes them
+            dtype = torch.promote_types(rows.dtype, residual.dtype)
+            rows, residual = rows.to(dtype), residual.to(dtype)
+        if not _types_fit(rows, weight, bias):
+            return norm(drop(x) + input_tensor)
         dropping = drop.training and drop.p > 0
-        return layer_norm(x, norm.weight, norm.bias, norm.eps, residual=input_tensor,
+        return layer_norm(rows, weight, bias, norm.eps, residual=residual,
                           p=drop.p if dropping else 0.0, rng=drop.state.rng if dropping else None,
                           site=drop.site)
 

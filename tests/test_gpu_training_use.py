@@ -75,7 +75,7 @@ def test_vmap_with_an_rng_for_every_sample():
 # ---- a model -------------------------------------------------------------------------
 
 
-def _backbone(p):
+def _backbone(p, **over):
     from transformers import DebertaV2Config, DebertaV2Model
 
     torch.manual_seed(5)
@@ -84,7 +84,8 @@ def _backbone(p):
         intermediate_size=128, hidden_act="gelu", type_vocab_size=2, max_position_embeddings=64,
         relative_attention=True, position_buckets=16, pos_att_type=["p2c", "c2p"],
         norm_rel_ebd="layer_norm", share_att_key=True, conv_kernel_size=3, conv_act="gelu",
-        position_biased_input=True, hidden_dropout_prob=p, attention_probs_dropout_prob=p)).cuda()
+        position_biased_input=True, hidden_dropout_prob=p, attention_probs_dropout_prob=p,
+        **over)).cuda()
 
 
 def _batch():
@@ -216,3 +217,122 @@ def test_output_block_whose_children_change():
         block.dropout = drop
         torch.testing.assert_close(block(x, r), plain(drop(block.dense(x)) + r), atol=1e-5,
                                    rtol=1e-5)
+
+
+# ---- types ---------------------------------------------------------------------------
+
+KINDS = [torch.float16, torch.bfloat16, torch.float32, torch.float64]
+
+
+def _either(call):
+    """The result, or None where torch refuses the types."""
+
+    try:
+        return call()
+    except RuntimeError as error:
+        assert "type" in str(error) or "Half" in str(error), error
+        return None
+
+
+def _close(got, want, half_steps):
+    """Within so many half steps of the coarsest type on the way, bf16, at values up to 8."""
+
+    assert got.dtype == want.dtype
+    assert (got.double() - want.double()).abs().max().item() <= half_steps * 8 * 2.0 ** -8
+
+
+@pytest.mark.parametrize("autocast", [False, True])
+@pytest.mark.parametrize("weights", KINDS, ids=str)
+@pytest.mark.parametrize("kind", KINDS, ids=str)
+def test_norm_takes_the_types_that_torchs_takes(kind, weights, autocast):
+    """The result and the gradients have the types that nn.LayerNorm's have, and their values.
+    (16-bit rows beside fp32 weights, which it refuses outside autocast, are taken.)"""
+
+    from disentangled_flash import training
+
+    norm = nn.LayerNorm(64, device="cuda", dtype=weights)
+    ours = training.LayerNorm(64, device="cuda", dtype=weights)
+    results = []
+    for module in (norm, ours):
+        x = torch.randn(9, 64, device="cuda", generator=_gen(1)).to(kind).requires_grad_()
+        with torch.autocast("cuda", dtype=torch.bfloat16, enabled=autocast):
+            y = _either(lambda: module(x))
+        if y is not None:
+            y.backward(torch.randn(9, 64, device="cuda", generator=_gen(2)).to(y.dtype))
+            results.append((y, x.grad, module.weight.grad, module.bias.grad))
+        else:
+            results.append(None)
+    if results[0] is None:
+        assert results[1] is None or weights == torch.float32
+        return
+    for want, got in zip(*results):
+        _close(got, want, 2 if torch.float64 not in (kind, weights) else 0.01)
+
+
+@pytest.mark.parametrize("autocast", [False, True])
+@pytest.mark.parametrize("weights", KINDS, ids=str)
+@pytest.mark.parametrize("residual", KINDS, ids=str)
+def test_output_block_takes_the_types_that_torchs_takes(weights, residual, autocast):
+    from disentangled_flash import enable_deberta_training
+
+    plain = _backbone(0.0).to(weights).train()
+    ours = enable_deberta_training(copy.deepcopy(plain))
+    results = []
+    for model in (plain, ours):
+        block = model.encoder.layer[0].output
+        x = torch.randn(9, 128, device="cuda", generator=_gen(1)).to(weights)
+        r = torch.randn(9, 64, device="cuda", generator=_gen(2)).to(residual).requires_grad_()
+        with torch.autocast("cuda", dtype=torch.bfloat16, enabled=autocast):
+            y = _either(lambda: block(x, r))
+        if y is not None:
+            y.backward(torch.randn(9, 64, device="cuda", generator=_gen(3)).to(y.dtype))
+            results.append((y, r.grad, block.LayerNorm.weight.grad, block.LayerNorm.bias.grad,
+                            block.dense.bias.grad))
+        else:
+            results.append(None)
+    if results[0] is None:
+        assert results[1] is None
+        return
+    for want, got in zip(*results):
+        # (A 16-bit product, sum and norm on the way; gradients of weights add 9 rows.)
+        _close(got, want, 8)
+
+
+@pytest.mark.parametrize("projected", [False, True])
+def test_model_under_autocast(projected):
+    """Hidden states keep the types that the unchanged model's have, fp32 between the blocks, and
+    the values are as close to the fp32 model's as the unchanged model's are."""
+
+    from disentangled_flash import enable_deberta_training
+
+    ids = _batch()
+    plain = _backbone(0.0, embedding_size=32) if projected else _backbone(0.0)
+    plain.train()
+    ours = enable_deberta_training(copy.deepcopy(plain))
+    exact = plain(ids, output_hidden_states=True).hidden_states
+    with torch.autocast("cuda", dtype=torch.bfloat16):
+        want = plain(ids, output_hidden_states=True).hidden_states
+        got = ours(ids, output_hidden_states=True).hidden_states
+    got[-1].sum().backward()
+    for e, w, g in zip(exact, want, got):
+        assert g.dtype == w.dtype
+        # A chain of two layers: three times the unchanged model's distance, at least 2 half steps.
+        size = e.abs().max().item()
+        assert (g - e).abs().max().item() <= 3 * (w - e).abs().max().item() + size * 2.0 ** -7
+
+
+def test_model_in_double_precision():
+    """Types that the operators lack stay torch's, dropout too."""
+
+    from disentangled_flash import enable_deberta_training
+
+    ids = _batch()
+    plain = _backbone(0.0).double().train()
+    ours = enable_deberta_training(copy.deepcopy(plain))
+    want, got = (m(ids).last_hidden_state for m in (plain, ours))
+    torch.testing.assert_close(got, want, rtol=1e-12, atol=1e-12)
+    got.sum().backward()
+    dropping = enable_deberta_training(_backbone(0.2).double().train())
+    first, second = (dropping(ids).last_hidden_state for _ in range(2))
+    assert first.dtype == torch.float64 and not torch.equal(first, second)
+    first.sum().backward()
