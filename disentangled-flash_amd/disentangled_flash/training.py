@@ -466,12 +466,19 @@ def _types_fit(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor) -> boo
             and (kind == x.dtype or kind == torch.float32))
 
 
+def _norm_is_affine(norm: nn.LayerNorm) -> bool:
+    """Over the last dimension, with weight and bias, and as wide as :func:`layer_norm` takes."""
+
+    return (norm.weight is not None and norm.bias is not None and len(norm.normalized_shape) == 1
+            and norm.normalized_shape[0] <= MAX_HIDDEN)
+
+
 class LayerNorm(nn.LayerNorm):
-    """``nn.LayerNorm`` over the last dimension on :func:`layer_norm`; torch's on the CPU and for
-    types that the operator lacks.  Under ``torch.autocast`` in fp32, as torch's."""
+    """``nn.LayerNorm`` on :func:`layer_norm`; torch's on the CPU and for types and settings that
+    the operator lacks.  Under ``torch.autocast`` in fp32, as torch's."""
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
-        if not _on_gpu(x):
+        if not _on_gpu(x) or not _norm_is_affine(self):
             return super().forward(x)
         rows, weight, bias = x, self.weight, self.bias
         if torch.is_autocast_enabled("cuda"):
@@ -481,13 +488,22 @@ class LayerNorm(nn.LayerNorm):
         return layer_norm(rows, weight, bias, self.eps)
 
 
+def _settings_fit(module: nn.Embedding) -> bool:
+    """Whether :func:`embedding` and its dense gradient are what the module asks for."""
+
+    return module.max_norm is None and not module.sparse and not module.scale_grad_by_freq
+
+
 class Embedding(nn.Embedding):
-    """``nn.Embedding`` on :func:`embedding`; torch's on the CPU and for float64."""
+    """``nn.Embedding`` on :func:`embedding`; torch's on the CPU and for types, settings and
+    strides that the operator lacks."""
 
     def forward(self, input_ids: torch.Tensor) -> torch.Tensor:
-        if not _on_gpu(input_ids) or self.weight.dtype not in _lib.DTYPE_CODES:
+        weight = self.weight
+        if not _on_gpu(input_ids) or not _settings_fit(self) \
+                or weight.dtype not in _lib.DTYPE_CODES or not weight.is_contiguous():
             return super().forward(input_ids)
-        return embedding(input_ids, self.weight, padding_idx=self.padding_idx)
+        return embedding(input_ids, weight, padding_idx=self.padding_idx)
 
 
 class OutputBlock(nn.Module):
@@ -548,9 +564,7 @@ def _norm_fits(module: Any) -> bool:
     """Whether calling ``module`` is :func:`layer_norm` of its weights and nothing else."""
 
     return ((type(module) is nn.LayerNorm or type(module) is LayerNorm)
-            and module.weight is not None
-            and module.bias is not None and len(module.normalized_shape) == 1
-            and module.normalized_shape[0] <= MAX_HIDDEN and not _has_hooks(module))
+            and _norm_is_affine(module) and not _has_hooks(module))
 
 
 def _dropout_fits(module: Any) -> bool:
@@ -574,8 +588,7 @@ def _training_form(module: nn.Module, state: DropoutState, sites: Any) -> nn.Mod
     if type(module) is nn.LayerNorm and _norm_fits(module):
         made = LayerNorm(module.normalized_shape, module.eps, device="meta")
         return _adopt(made, module)
-    if type(module) is nn.Embedding and module.max_norm is None and not module.sparse \
-            and not module.scale_grad_by_freq:
+    if type(module) is nn.Embedding and _settings_fit(module):
         made = Embedding(module.num_embeddings, module.embedding_dim, module.padding_idx,
                          device="meta")
         return _adopt(made, module)

@@ -490,3 +490,51 @@ def test_a_patched_block_class_keeps_its_forward(monkeypatch):
     model = enable_deberta_training(_backbone())
     assert type(model.encoder.layer[0].output) is hf.DebertaV2Output
     assert type(model.encoder.layer[0].attention.output) is training.OutputBlock
+
+
+# ---- settings that the operators lack ------------------------------------------------
+
+
+def test_settings_changed_later_are_honoured(monkeypatch):
+    """torch's own module computes what the operator does not."""
+
+    from disentangled_flash import training
+
+    calls = []
+    monkeypatch.setattr(training, "_on_gpu", lambda x: True)
+    monkeypatch.setattr(training, "embedding",
+                        lambda ids, weight, padding_idx=None: calls.append("embedding") or
+                        nn.functional.embedding(ids, weight, padding_idx))
+    monkeypatch.setattr(training, "layer_norm",
+                        lambda x, w, b, eps: calls.append("layer_norm") or
+                        nn.functional.layer_norm(x, x.shape[-1:], w, b, eps))
+    ids = torch.tensor([1, 1, 2])
+    made = training.Embedding(5, 8)
+    made(ids)
+    assert calls == ["embedding"]
+    for name, value in (("max_norm", 0.5), ("sparse", True), ("scale_grad_by_freq", True)):
+        calls.clear()
+        made = training.Embedding(5, 8)
+        setattr(made, name, value)
+        out = made(ids)
+        out.sum().backward()
+        assert not calls
+        if name == "max_norm":
+            assert out.norm(dim=-1).max() <= 0.5 * (1 + 1e-5)
+        assert made.weight.grad.is_sparse == (name == "sparse")
+        if name == "scale_grad_by_freq":
+            assert torch.equal(made.weight.grad[1], torch.ones(8))
+    made = training.Embedding(5, 8)
+    made.weight = nn.Parameter(torch.randn(8, 5).t())
+    assert torch.equal(made(ids), made.weight[ids]) and not calls
+
+    x = torch.randn(2, 3, 8)
+    assert training.LayerNorm(8)(x).shape == x.shape and calls == ["layer_norm"]
+    calls.clear()
+    for norm, plain in ((training.LayerNorm(8, elementwise_affine=False),
+                         nn.LayerNorm(8, elementwise_affine=False)),
+                        (training.LayerNorm(8, bias=False), nn.LayerNorm(8, bias=False)),
+                        (training.LayerNorm((3, 8)), nn.LayerNorm((3, 8)))):
+        assert torch.equal(norm(x), plain(x)) and not calls
+    wide = training.MAX_HIDDEN + 1
+    assert training.LayerNorm(wide)(torch.ones(wide)).shape == (wide,) and not calls
