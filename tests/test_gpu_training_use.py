@@ -336,3 +336,89 @@ def test_model_in_double_precision():
     first, second = (dropping(ids).last_hidden_state for _ in range(2))
     assert first.dtype == torch.float64 and not torch.equal(first, second)
     first.sum().backward()
+
+
+# ---- ids and addresses ---------------------------------------------------------------
+
+BAD_IDS = {torch.int32: [-1, 30, 31, 2 ** 31 - 1, -2 ** 31, -30],
+           torch.int64: [-1, 30, 31, 2 ** 31 - 1, -2 ** 31, -30, 1 << 40, -(1 << 40), 2 ** 63 - 1,
+                         -2 ** 63, (1 << 32) + 4, -(1 << 32) + 4]}  # (low words inside the table)
+
+
+@pytest.mark.parametrize("kind", list(BAD_IDS), ids=str)
+@pytest.mark.parametrize("n", [200, 700, 9000, 40000])
+@pytest.mark.parametrize("dtype,hidden", [(torch.bfloat16, 64), (torch.float32, 33)], ids=str)
+def test_ids_outside_the_table_in_every_form(dtype, hidden, n, kind):
+    """One launch, ranks, one run and merged runs: such ids give NaN and add to nothing, whatever
+    their gradient rows hold, and neither do the padding's."""
+
+    from disentangled_flash.training import embedding
+
+    rows, gen = 30, _gen(n)
+    ids = torch.randint(0, rows, (n,), device="cuda", generator=gen)
+    outside = torch.rand(n, device="cuda", generator=gen) < 0.2
+    outside[[0, n - 1]] = True  # at both ends
+    bad = torch.tensor(BAD_IDS[kind], device="cuda")
+    ids = torch.where(outside, bad[torch.arange(n, device="cuda") % len(bad)], ids).to(kind)
+    table = _normal(gen, (rows, hidden), dtype).requires_grad_()
+    y = embedding(ids, table, 2.0, 4)
+    assert bool(torch.isnan(y[outside]).all())
+    assert torch.equal(y[~outside], 2 * table[ids[~outside].long()])
+    dy = _normal(gen, (n, hidden), dtype)
+    for worst in (None, float("nan"), float("inf")):
+        if worst is not None:
+            dy[outside | (ids == 4)] = worst
+        (grad,) = torch.autograd.grad(y, table, dy, retain_graph=True)
+        ref.check(grad, ref.embedding_gradient(ids[~outside], dy[~outside], rows, 2.0, 4), "table")
+        assert not grad[4].any()
+    (none,) = torch.autograd.grad(embedding(bad.to(kind).repeat(n)[:n], table), table, dy)
+    assert torch.equal(none, torch.zeros_like(none))
+
+
+def _off(t):
+    """The same values, contiguous, one element behind a 16-byte boundary."""
+
+    store = torch.empty(t.numel() + 1, device="cuda", dtype=t.dtype)
+    made = store[1:].view(t.shape).copy_(t)
+    assert made.is_contiguous() and made.data_ptr() % 16 == t.element_size()
+    return made
+
+
+@pytest.mark.parametrize("rows", [20, 96, 2100])
+@pytest.mark.parametrize("dtype", KINDS[:3], ids=str)
+@pytest.mark.parametrize("which", ["rows", "weights", "all"])
+def test_norm_gradients_off_the_boundaries(dtype, rows, which):
+    """x, residual and dy, or the weights, behind a 16-byte boundary, at a width of whole chunks."""
+
+    from disentangled_flash.training import layer_norm
+
+    gen = _gen(rows)
+    x, dy = (_normal(gen, (rows, 256), dtype) for _ in range(2))
+    r = _normal(gen, (rows, 256), dtype, 1.3, 0.25)
+    w, b = _normal(gen, (256,), dtype, 0.1, 1.0), _normal(gen, (256,), dtype, 0.1)
+    want = ref.layer_norm(x, w, b, 1e-5, r, ref.factor((rows, 256), 0.2, _rng(), SITE), dy)
+    if which != "weights":
+        x, r, dy = _off(x), _off(r), _off(dy)
+    if which != "rows":
+        w, b = _off(w), _off(b)
+    leaves = [t.requires_grad_() for t in (x, w, b, r)]
+    y = layer_norm(x, w, b, 1e-5, r, 0.2, _rng(), SITE)
+    ref.check(y.detach(), want["y"], "y")
+    grads = torch.autograd.grad(y, leaves, dy)
+    for name, grad in zip(("dx", "dweight", "dbias", "dresidual"), grads):
+        ref.check(grad, want[name], name)
+
+
+@pytest.mark.parametrize("n", [200, 700, 9000, 40000])
+@pytest.mark.parametrize("dtype", KINDS[:3], ids=str)
+def test_embedding_gradients_off_the_boundaries(dtype, n):
+    from disentangled_flash.training import embedding
+
+    gen = _gen(n)
+    table = _off(_normal(gen, (50, 64), dtype)).requires_grad_()
+    ids = torch.randint(0, 50, (n,), device="cuda", generator=gen)
+    dy = _off(_normal(gen, (n, 64), dtype))
+    y = embedding(ids, table, 0.5)
+    (grad,) = torch.autograd.grad(y, table, dy)
+    assert torch.equal(y, (table[ids].float() * 0.5).to(dtype))
+    ref.check(grad, ref.embedding_gradient(ids, dy, 50, 0.5), "table")
