@@ -251,7 +251,7 @@ def embedding(
 # offset) -> that step's rng.  torch.utils.checkpoint puts the generator back for its
 # recomputations, so one of a whole backbone finds the step of its forward here.
 _drawn: OrderedDict[tuple[int, ...], torch.Tensor] = OrderedDict()
-_DRAWN_KEPT = 1 << 14  # forwards whose backward pass is still to come; 512 bytes each on the GPU
+_DRAWN_KEPT = 1 << 12  # forwards whose backward pass is still to come; 512 bytes each on the GPU
 _tokens = itertools.count()
 
 
@@ -356,7 +356,7 @@ class DropoutState(nn.Module):
 
     def __setstate__(self, state: dict[str, Any]) -> None:
         super().__setstate__(state)
-        self._token = next(_tokens)  # (a copy draws steps of its own)
+        self._phase, self._token = _Phase(), next(_tokens)  # (a copy draws steps of its own)
 
     @property
     def rng(self) -> torch.Tensor:
