@@ -5,8 +5,8 @@
 // Forward and backward are the same kernel (dx is the same function of dy).  A dropped element
 // is 0 whatever it held (infinities and NaN too): it is selected, not multiplied by 0.
 // One 16-byte chunk a lane: n * sizeof(T) bytes read and written, and one generator block
-// for 8 elements, drawn while the chunk is loaded.  Bound by bytes: 25 M bf16 elements take 18 us
-// (5.5 TB/s), 4.7 M fp32 7.6 us (5.0 TB/s); 75 k fp16 2.6 us, most of it the launch.
+// for 8 elements, drawn while the chunk is loaded.  Bound by bytes: 25 M bf16 elements take
+// 19.5 us (5.2 TB/s), 4.7 M fp32 7.6 us (5.0 TB/s); 75 k fp16 2.5 us, most of it the launch.
 
 #include <hip/hip_runtime.h>
 #include <stdint.h>

@@ -18,9 +18,12 @@
 //   join   the partial rows of ids that cross edges, added in order.
 //
 // Bound by bytes where the table is large: 16384 tokens (frequencies ~ 1 / id) into 128100 x 768
-// bf16 take 52 us, of which the 197 MB of zeros alone would take 32 (6.1 TB/s); by latency
-// where it is small: 512 x 1024 fp32 35 us (sort 11.0, merge 8.1, sum 14.2 for 67 MB, join
-// 3.9), 4096 tokens into 5000 x 64 19 us.  The lookup of 16384 rows of 768 bf16 takes 7.4 us.
+// bf16 take 44 us of kernels (sort 15.8, merge 12.6, sum 11.9, join 4.0; 52 with the gaps between
+// the launches), of which the 197 MB of zeros alone would take 30 (6.6 TB/s); by latency where it
+// is small: 512 x 1024 fp32 37 us (sort 11.0, merge 8.1, sum 14.2 for 67 MB, join 3.9), 4096
+// tokens into 5000 x 64 19 us.  The lookup of 16384 rows of 768 bf16 takes 10.8 us.  (Device times
+// of single launches, traced; whole gradients, here and below, are timed by events around many in
+// a row, where a launch overlaps the end of the one before it: 35 us for the 512 x 1024.)
 //
 // Ids outside [0, rows): the lookup returns NaN for them, the gradient leaves them out.
 
@@ -772,7 +775,10 @@ int launch_bwd(const void* ids_in, const void* dout_in, void* dtable_in, int64_t
     return static_cast<int>(hipGetLastError());
   }
   // The zeros go with the first launch, and a part of them with the merge if there is one, so
-  // that neither has the card to itself.
+  // that neither has the card to itself.  (With 2/5, 3/5, 4/5 and all of them in the first: 16384
+  // tokens into 128100 x 768 bf16 54.5, 52.1, 54.8, 59.1 us, x 1536 96.9, 98.7, 98.0, 104.2,
+  // 30000 x 768 37.3, 37.2, 36.5, 35.5; 65536 into 128100 x 768 97.3, 97.3, 101.4, 103.4; 10000
+  // into 128100 x 1024 fp32 121.5, 120.0, 119.5, 126.4; 262144 tokens or 512 rows within 1 %.)
   const bool by_rank = n <= kRankTokens;
   const int64_t first_part = by_rank ? table_bytes : table_bytes / 5 * 3 / 16 * 16;
   const Fill fill{static_cast<u32x4_t*>(dtable_in), 0, first_part};

@@ -19,11 +19,12 @@
 // are a multiple of a chunk's elements apart), so its weights and the sums for their gradients
 // stay with the lanes; only a row's first and last chunk are written by elements.
 //
-// Bound by bytes: 16384 x 768 bf16 with residual and dropout 16.0 us forward (75 MB, 4.7 TB/s)
-// and 29.7 backward (129 MB with the partial rows, 4.3 TB/s, of which 4 us are the second
-// launch); 16384 x 1536 fp32 55 (5.5 TB/s) and 89 us (5.7).  A copy of as many bytes runs at
-// 4.8 to 5.4 TB/s.  16384 x 769 bf16: 20.1 and 39.4 us; 3059 x 1001: 7.7 and 18.0 (by
-// element accesses 17.0 and 28.0).
+// Bound by bytes: 16384 x 768 bf16 with residual and dropout 16.3 us forward (75 MB, 4.6 TB/s)
+// and 25.0 + 4.0 backward (129 MB with the partial rows, 5.2 TB/s, and the second launch); 16384 x
+// 1536 fp32 54.4 (5.6 TB/s) and 84.3 + 4.7 us (6.0).  A copy of as many bytes runs at 4.5 to
+// 5.4 TB/s.  (Device times of single launches, traced; those below are of many in a row, by
+// events: 15.9 and 29.7, 55 and 89.)  16384 x 769 bf16: 19.9 and 39.4 us; 3059 x 1001: 7.7 and
+// 18.0 (by element accesses 17.0 and 28.0).
 
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -39,7 +40,9 @@ namespace {
 
 constexpr int kMaxHidden = 8192;
 // Workgroups of the backward pass: each adds up the weight gradients of its rows and writes
-// one fp32 partial row of each.  (16384 x 768 bf16: 256 35.8 us, 512 32.9, 768 34.1, 1024 36.0.)
+// one fp32 partial row of each.  (Backward, bf16, by 256, 512 and 1024: 2048 x 768 11.0, 11.0,
+// 11.0 us; 4096 14.6, 13.3, 13.3; 8192 22.0, 19.8, 23.7; 65536 99.2, 93.4, 95.4; 3059 x 1000 14.5,
+// 13.1, 15.2; 16384 x 769 55.2, 39.4, 44.6; 16384 x 1024 fp16 30.9, 24.4, 28.9.)
 constexpr int kMaxPartials = 512;
 // Up to this many rows one workgroup takes them all, and there are no partial rows to add: 17
 // rows of 768 take 9.8 us alone, 5.4 + 2.7 and the gap between them in two launches, of
@@ -466,7 +469,12 @@ __global__ __launch_bounds__(16 * kSlices) void layernorm_weight_grad_kernel(
 // Calls go(LANES, CH, WHOLE) with the smallest layout that holds a row of `hidden` elements: few
 // chunks a lane, for their registers (1024 16-bit: 32 lanes of 4 chunks 32.5 us backward, 64 of
 // 2 24.2), but 32 lanes of 3 before 64 of 2 half empty (768: 33.0, 34.8), and a row in
-// one wavefront where three chunks a lane hold it (1536: 55.4, a workgroup a row 76.3).
+// one wavefront where three chunks a lane hold it (1536: 55.4, a workgroup a row 76.3).  Above 4
+// chunks a lane of one wavefront a row is a workgroup's (forward and backward, against 8 chunks a
+// lane: 8192 x 2560 bf16 30.9 and 61.8 us, 38.1 and 111.7; 4096 x 4096 20.1 and 49.3, 29.0 and
+// 76.7; 16384 x 1536 fp32 55.0 and 89.7, 55.6 and 96.8; 4096 x 2048 19.6 and 36.9, 22.1 and 42.4).
+// By the layouts that are a workgroup's alone: 2048 x 4096 fp32 20.6 and 42.0 us, 1024 x 8192 22.0
+// and 59.3, 2048 x 8192 bf16 21.0 and 76.8, 4096 x 2051 21.2 and 43.0.
 template <typename T, typename Go>
 int with_layout(int hidden, bool whole, Go go) {
   constexpr int N = Chunk<T>::N;
