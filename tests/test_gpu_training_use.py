@@ -422,3 +422,43 @@ def test_embedding_gradients_off_the_boundaries(dtype, n):
     (grad,) = torch.autograd.grad(y, table, dy)
     assert torch.equal(y, (table[ids].float() * 0.5).to(dtype))
     ref.check(grad, ref.embedding_gradient(ids, dy, 50, 0.5), "table")
+
+
+def test_captured_and_eager_steps_in_turn():
+    """Replays advance on the device; eager steps between them, of another state and of torch's own
+    dropout, move torch's generator, which the graph uses too."""
+
+    from disentangled_flash import training
+
+    state, other = training.DropoutState(5, "cuda"), training.DropoutState(6, "cuda")
+    x = torch.randn(64, 72, device="cuda")
+    leaf = x.clone().requires_grad_()
+    own = nn.Dropout(0.5)
+
+    def step(state):
+        state.advance()
+        y = training.dropout(leaf, 0.5, state.rng, 3)
+        return y.detach(), own(x), *torch.autograd.grad(y, leaf, x)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(state)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            outputs = step(state)
+    torch.cuda.current_stream().wait_stream(side)
+    state.counter[1] = 10
+    torchs = []
+    for i in range(4):
+        graph.replay()
+        y, drawn, dx = (t.clone() for t in outputs)
+        mult = ref.factor((64, 72), 0.5, torch.tensor([5, 11 + i], device="cuda"), 3).float()
+        assert torch.equal(y, x * mult) and torch.equal(dx, x * mult)
+        y, also, dx = step(other)
+        mult = ref.factor((64, 72), 0.5, torch.tensor([6, 1 + i], device="cuda"), 3).float()
+        assert torch.equal(y, x * mult) and torch.equal(dx, x * mult)
+        torch.cuda.synchronize()
+        torchs += [drawn, also]
+    for i in range(8):  # torch's masks differ from one another
+        assert all(not torch.equal(torchs[i], torchs[j]) for j in range(i))

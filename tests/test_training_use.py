@@ -7,6 +7,7 @@ from __future__ import annotations
 import contextlib
 import copy
 import functools
+import pickle
 import subprocess
 import sys
 
@@ -538,3 +539,14 @@ def test_settings_changed_later_are_honoured(monkeypatch):
         assert torch.equal(norm(x), plain(x)) and not calls
     wide = training.MAX_HIDDEN + 1
     assert training.LayerNorm(wide)(torch.ones(wide)).shape == (wide,) and not calls
+
+
+def test_state_is_pickled_with_its_step(drops, generator):
+    from disentangled_flash import training
+
+    state = training.DropoutState(7)
+    state.advance()
+    state.begin()
+    back = pickle.loads(pickle.dumps(state))
+    assert back.rng.tolist() == [7, 1] and back._token != state._token
+    assert state.rng.tolist() == [7, 2]  # (begun)
