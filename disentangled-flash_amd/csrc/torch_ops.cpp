@@ -41,6 +41,10 @@ struct Library {
   decltype(&dflash_embedding_fwd) embedding_fwd;
   decltype(&dflash_embedding_bwd) embedding_bwd;
   decltype(&dflash_embedding_bwd_workspace_bytes) embedding_bwd_workspace_bytes;
+  decltype(&dflash_attention_train_bits_bytes) attention_bits_bytes;
+  decltype(&dflash_attention_train_fwd) attention_fwd;
+  decltype(&dflash_attention_train_bwd) attention_bwd;
+  decltype(&dflash_attention_train_bwd_workspace_bytes) attention_bwd_workspace_bytes;
   decltype(&dflash_error_string) error_string;
 } lib;
 
@@ -61,6 +65,10 @@ void bind_library(std::string path) {
   find(handle, "dflash_embedding_fwd", lib.embedding_fwd);
   find(handle, "dflash_embedding_bwd", lib.embedding_bwd);
   find(handle, "dflash_embedding_bwd_workspace_bytes", lib.embedding_bwd_workspace_bytes);
+  find(handle, "dflash_attention_train_bits_bytes", lib.attention_bits_bytes);
+  find(handle, "dflash_attention_train_fwd", lib.attention_fwd);
+  find(handle, "dflash_attention_train_bwd", lib.attention_bwd);
+  find(handle, "dflash_attention_train_bwd_workspace_bytes", lib.attention_bwd_workspace_bytes);
   find(handle, "dflash_error_string", lib.error_string);
 }
 
@@ -248,6 +256,165 @@ Tensor embedding_gradient(const Tensor& dy, const Tensor& ids, c10::SymInt table
   return out;
 }
 
+// Rows of whole 16-byte accesses: the last dimension contiguous, the others' strides and the
+// start on 16-byte boundaries.
+bool has_rows(const Tensor& t) {
+  if (t.numel() == 0) return true;
+  int64_t every = 0;
+  for (int64_t n = 0; n + 1 < t.dim(); ++n) every |= t.size(n) > 1 ? t.stride(n) : 0;
+  return t.stride(-1) == 1 && every * t.element_size() % 16 == 0 && is_aligned(t);
+}
+Tensor with_rows(const Tensor& t) {
+  return has_rows(t) ? t : t.is_contiguous() ? t.clone() : t.contiguous();
+}
+MaybeTensor with_rows(const MaybeTensor& t) { return t ? MaybeTensor(with_rows(*t)) : t; }
+
+// The arguments of the C calls; the tensors must have rows and outlive it.
+dflash_attention_train attention_of(const Tensor& q, const Tensor& k, const Tensor& v,
+                                    const MaybeTensor& pk, const MaybeTensor& pq,
+                                    const Tensor& places, const MaybeTensor& mask, double scale,
+                                    double p) {
+  const int64_t length = q.dim() == 4 ? q.size(1) : 0, heads = q.dim() == 4 ? q.size(2) : 0;
+  expect(q.dim() == 4 && q.size(0) <= INT32_MAX && length <= INT32_MAX && heads <= INT32_MAX,
+         "query");
+  auto same = [&](const Tensor& t) {
+    return t.sizes() == q.sizes() && t.scalar_type() == q.scalar_type() &&
+           t.device() == q.device();
+  };
+  expect(same(k), "key");
+  expect(same(v), "value");
+  auto table = [&](const MaybeTensor& t) {
+    return !t || (t->dim() == 3 && t->size(0) == heads && t->size(2) == q.size(3) &&
+                  t->size(1) >= 1 && t->size(1) <= INT32_MAX &&
+                  t->scalar_type() == q.scalar_type() && t->device() == q.device());
+  };
+  expect(table(pk), "pos_key");
+  expect(table(pq) && (!pk || !pq || pk->size(1) == pq->size(1)), "pos_query");
+  expect(fits(places, q) && places.scalar_type() == at::kInt &&
+             (length == 0 || places.numel() == 2 * length - 1),
+         "delta_to_slot");
+  expect(!mask || (fits(*mask, q) && mask->element_size() == 1 && mask->dim() == 2 &&
+                   mask->size(0) == q.size(0) && mask->size(1) == length),
+         "mask");
+  for (const Tensor* t : {&q, &k, &v}) expect(has_rows(*t), "rows");
+  expect((!pk || has_rows(*pk)) && (!pq || has_rows(*pq)), "position rows");
+  // (A dimension of one element may have any stride.)
+  auto stride = [](const Tensor& t, int64_t n) { return t.size(n) > 1 ? t.stride(n) : 0; };
+  dflash_attention_train a{};
+  a.query = data(q);
+  a.key = data(k);
+  a.value = data(v);
+  const Tensor* tensors[] = {&q, &k, &v};
+  int64_t* strides[] = {a.query_strides, a.key_strides, a.value_strides};
+  for (int n = 0; n < 3; ++n) {
+    strides[n][0] = stride(*tensors[n], 0);
+    strides[n][1] = stride(*tensors[n], 2);
+    strides[n][2] = stride(*tensors[n], 1);
+  }
+  a.pos_key = data(pk);
+  a.pos_query = data(pq);
+  for (int n = 0; n < 2; ++n) {
+    if (pk) a.pos_key_strides[n] = stride(*pk, n);
+    if (pq) a.pos_query_strides[n] = stride(*pq, n);
+  }
+  a.delta_to_slot = static_cast<const int32_t*>(data(places));
+  a.mask = mask ? static_cast<const uint8_t*>(data(*mask)) : nullptr;
+  a.B = q.size(0);
+  a.H = heads;
+  a.L = length;
+  a.D = q.size(3);
+  a.S = pk ? pk->size(1) : pq ? pq->size(1) : 0;
+  a.dtype = code_of(q);
+  a.scale = scale;
+  a.p = p;
+  return a;
+}
+
+// (out, lse, bits); without `statistics` the last two are empty.
+std::tuple<Tensor, Tensor, Tensor> attention_forward(
+    const Tensor& given_q, const Tensor& given_k, const Tensor& given_v,
+    const MaybeTensor& given_pk, const MaybeTensor& given_pq, const Tensor& places,
+    const MaybeTensor& mask, const MaybeTensor& rng, double scale, double p, int64_t site,
+    bool statistics) {
+  const Tensor q = with_rows(given_q), k = with_rows(given_k), v = with_rows(given_v);
+  const MaybeTensor pk = with_rows(given_pk), pq = with_rows(given_pq);
+  const dflash_attention_train a = attention_of(q, k, v, pk, pq, places, mask, scale, p);
+  expect_dropout(rng, site, q);
+  expect(p == 0 || rng, "rng");
+  Tensor out = fresh(q.sizes(), q.scalar_type(), q);
+  const bool any = q.numel() > 0;
+  Tensor lse = fresh({statistics ? a.B : 0, a.H, a.L}, at::kFloat, q);
+  const size_t bytes = p > 0 && any ? lib.attention_bits_bytes(a.B, a.H, a.L) : 0;
+  Tensor bits = fresh({static_cast<int64_t>(bytes)}, at::kByte, q);
+  if (any) {
+    On on(q);
+    check(lib.attention_fwd(&a, words(rng), site, data(out),
+                            statistics ? static_cast<float*>(data(lse)) : nullptr,
+                            bytes ? data(bits) : nullptr, on.stream),
+          "dflash_attention_train_fwd");
+  }
+  return {out, lse, bits};
+}
+
+Tensor attention(const Tensor& q, const Tensor& k, const Tensor& v, const MaybeTensor& pk,
+                 const MaybeTensor& pq, const Tensor& places, const MaybeTensor& mask,
+                 const MaybeTensor& rng, double scale, double p, int64_t site) {
+  return std::get<0>(
+      attention_forward(q, k, v, pk, pq, places, mask, rng, scale, p, site, false));
+}
+
+std::tuple<Tensor, Tensor, Tensor> attention_train(
+    const Tensor& q, const Tensor& k, const Tensor& v, const MaybeTensor& pk,
+    const MaybeTensor& pq, const Tensor& places, const MaybeTensor& mask, const MaybeTensor& rng,
+    double scale, double p, int64_t site) {
+  return attention_forward(q, k, v, pk, pq, places, mask, rng, scale, p, site, true);
+}
+
+// (dquery, dkey, dvalue, dpos_key, dpos_query); the tables' [S, H, D], empty where not wanted.
+std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> attention_backward(
+    const Tensor& given_dout, const Tensor& out, const Tensor& lse, const Tensor& bits,
+    const Tensor& given_q, const Tensor& given_k, const Tensor& given_v,
+    const MaybeTensor& given_pk, const MaybeTensor& given_pq, const Tensor& places,
+    const MaybeTensor& mask, double scale, double p, bool want_pk, bool want_pq) {
+  const Tensor q = with_rows(given_q), k = with_rows(given_k), v = with_rows(given_v);
+  const MaybeTensor pk = with_rows(given_pk), pq = with_rows(given_pq);
+  const dflash_attention_train a = attention_of(q, k, v, pk, pq, places, mask, scale, p);
+  expect(given_dout.is_contiguous() && given_dout.sizes() == q.sizes() &&
+             given_dout.scalar_type() == q.scalar_type() && given_dout.device() == q.device(),
+         "dout");
+  expect(same_form(out, given_dout), "out");
+  const bool any = q.numel() > 0;
+  expect(fits(lse, q) && lse.scalar_type() == at::kFloat &&
+             lse.numel() == static_cast<int64_t>(a.B) * a.H * a.L,
+         "lse");
+  expect(fits(bits, q) && (p == 0 || !any ||
+                           bits.nbytes() == lib.attention_bits_bytes(a.B, a.H, a.L)),
+         "bits");
+  const Tensor dout = aligned(given_dout);
+  Tensor dq = fresh(q.sizes(), q.scalar_type(), q), dk = fresh(q.sizes(), q.scalar_type(), q),
+         dv = fresh(q.sizes(), q.scalar_type(), q);
+  auto made = [&](bool wanted) {
+    return wanted ? fresh({a.S, a.H, a.D}, q.scalar_type(), q) : fresh({0}, q.scalar_type(), q);
+  };
+  want_pk = want_pk && pk;
+  want_pq = want_pq && pq;
+  Tensor dpk = made(want_pk), dpq = made(want_pq);
+  if (!any) {
+    dpk.zero_();
+    dpq.zero_();
+    return {dq, dk, dv, dpk, dpq};
+  }
+  const size_t bytes = lib.attention_bwd_workspace_bytes(&a);
+  Tensor workspace = fresh({static_cast<int64_t>(bytes)}, at::kByte, q);
+  On on(q);
+  check(lib.attention_bwd(&a, data(out), static_cast<const float*>(data(lse)),
+                          p > 0 ? data(bits) : nullptr, data(dout), data(dq), data(dk), data(dv),
+                          want_pk ? data(dpk) : nullptr, want_pq ? data(dpq) : nullptr,
+                          data(workspace), bytes, on.stream),
+        "dflash_attention_train_bwd");
+  return {dq, dk, dv, dpk, dpq};
+}
+
 // ---- autograd ------------------------------------------------------------------------
 
 template <typename F>
@@ -281,6 +448,19 @@ const auto& lookup_op() {
 }
 const auto& gradient_op() {
   static const auto op = operator_of<decltype(embedding_gradient)>("embedding_gradient");
+  return op;
+}
+
+const auto& attention_op() {
+  static const auto op = operator_of<decltype(attention)>("attention");
+  return op;
+}
+const auto& attention_train_op() {
+  static const auto op = operator_of<decltype(attention_train)>("attention_train");
+  return op;
+}
+const auto& attention_backward_op() {
+  static const auto op = operator_of<decltype(attention_backward)>("attention_backward");
   return op;
 }
 
@@ -394,6 +574,45 @@ struct EmbeddingNode : Function<EmbeddingNode> {
   }
 };
 
+struct AttentionNode : Function<AttentionNode> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v,
+                        const MaybeTensor& pk, const MaybeTensor& pq, const Tensor& places,
+                        const MaybeTensor& mask, const MaybeTensor& rng, double scale, double p,
+                        int64_t site) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    auto [out, lse, bits] =
+        attention_train_op().call(q, k, v, pk, pq, places, mask, rng, scale, p, site);
+    ctx->save_for_backward({out, lse, bits, q, k, v, pk.value_or(Tensor()), pq.value_or(Tensor()),
+                            places, mask.value_or(Tensor())});
+    ctx->saved_data["scale"] = scale;
+    ctx->saved_data["p"] = p;
+    ctx->saved_data["wanted"] = static_cast<int64_t>(
+        q.requires_grad() | k.requires_grad() << 1 | v.requires_grad() << 2 |
+        (pk && pk->requires_grad()) << 3 | (pq && pq->requires_grad()) << 4);
+    return out;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const int64_t wanted = ctx->saved_data["wanted"].toInt();
+    no_tangent(grads[0], "attention");
+    Tensor all[5];
+    {
+      at::AutoDispatchBelowADInplaceOrView below;
+      std::tie(all[0], all[1], all[2], all[3], all[4]) = attention_backward_op().call(
+          grads[0].contiguous(), saved[0], saved[1], saved[2], saved[3], saved[4], saved[5],
+          maybe(saved[6]), maybe(saved[7]), saved[8], maybe(saved[9]),
+          ctx->saved_data["scale"].toDouble(), ctx->saved_data["p"].toDouble(), wanted & 8,
+          wanted & 16);
+      for (int n : {3, 4})
+        if (wanted >> n & 1) all[n] = all[n].transpose(0, 1);
+    }
+    variable_list out(11);
+    for (int n = 0; n < 5; ++n)
+      if (wanted >> n & 1) out[n] = all[n];
+    return only_once(std::move(out), "attention");
+  }
+};
+
 bool records(const Tensor& t) { return t.requires_grad() && at::GradMode::is_enabled(); }
 
 Tensor dropout_autograd(const Tensor& x, const Tensor& rng, double p, int64_t site) {
@@ -422,6 +641,18 @@ Tensor embedding_lookup_autograd(const Tensor& ids, const Tensor& table, double 
   return lookup_op().call(ids, table, scale, padding);
 }
 
+Tensor attention_autograd(const Tensor& q, const Tensor& k, const Tensor& v, const MaybeTensor& pk,
+                          const MaybeTensor& pq, const Tensor& places, const MaybeTensor& mask,
+                          const MaybeTensor& rng, double scale, double p, int64_t site) {
+  for (const Tensor* t : {&q, &k, &v}) no_tangent(*t, "attention");
+  no_tangent(pk, "attention");
+  no_tangent(pq, "attention");
+  if (records(q) || records(k) || records(v) || (pk && records(*pk)) || (pq && records(*pq)))
+    return AttentionNode::apply(q, k, v, pk, pq, places, mask, rng, scale, p, site);
+  at::AutoDispatchBelowADInplaceOrView below;
+  return attention_op().call(q, k, v, pk, pq, places, mask, rng, scale, p, site);
+}
+
 }  // namespace
 
 TORCH_LIBRARY_FRAGMENT(disentangled_flash, m) {
@@ -440,6 +671,18 @@ TORCH_LIBRARY_FRAGMENT(disentangled_flash, m) {
   m.def("embedding_lookup(Tensor ids, Tensor table, float scale, int padding) -> Tensor");
   m.def(
       "embedding_gradient(Tensor dy, Tensor ids, SymInt rows, float scale, int padding) -> Tensor");
+  m.def(
+      "attention(Tensor query, Tensor key, Tensor value, Tensor? pos_key, Tensor? pos_query, "
+      "Tensor delta_to_slot, Tensor? mask, Tensor? rng, float scale, float p, int site) -> Tensor");
+  m.def(
+      "attention_train(Tensor query, Tensor key, Tensor value, Tensor? pos_key, "
+      "Tensor? pos_query, Tensor delta_to_slot, Tensor? mask, Tensor? rng, float scale, float p, "
+      "int site) -> (Tensor, Tensor, Tensor)");
+  m.def(
+      "attention_backward(Tensor dout, Tensor out, Tensor lse, Tensor bits, Tensor query, "
+      "Tensor key, Tensor value, Tensor? pos_key, Tensor? pos_query, Tensor delta_to_slot, "
+      "Tensor? mask, float scale, float p, bool want_pos_key, bool want_pos_query) -> (Tensor, "
+      "Tensor, Tensor, Tensor, Tensor)");
 }
 
 TORCH_LIBRARY_IMPL(disentangled_flash, CUDA, m) {
@@ -449,10 +692,14 @@ TORCH_LIBRARY_IMPL(disentangled_flash, CUDA, m) {
   m.impl("dropout_layernorm_backward", &dropout_layernorm_backward);
   m.impl("embedding_lookup", &embedding_lookup);
   m.impl("embedding_gradient", &embedding_gradient);
+  m.impl("attention", &attention);
+  m.impl("attention_train", &attention_train);
+  m.impl("attention_backward", &attention_backward);
 }
 
 TORCH_LIBRARY_IMPL(disentangled_flash, Autograd, m) {
   m.impl("dropout", &dropout_autograd);
   m.impl("dropout_layernorm", &dropout_layernorm_autograd);
   m.impl("embedding_lookup", &embedding_lookup_autograd);
+  m.impl("attention", &attention_autograd);
 }

@@ -21,7 +21,7 @@ import torch  # noqa: F401  (load torch's HIP runtime first)
 
 LIBRARY_NAME = "libdflash.so"
 TORCH_LIBRARY_NAME = "libdflash_torch.so"
-ABI_VERSION = 8
+ABI_VERSION = 9
 
 ERR_WORKSPACE = -7  # DFLASH_ERR_WORKSPACE
 
@@ -51,7 +51,19 @@ class EncoderLayer(ctypes.Structure):
         (name, _c_int) for name in ("heads", "head_dim", "slots", "hidden", "inner", "dtype")]
 
 
-# The same fields for struct.pack (a Structure takes its fields one by one, 3 us).
+class AttentionTrain(ctypes.Structure):
+    """``dflash_attention_train``: the inputs and sizes of a training attention."""
+
+    _fields_ = [(name, _c_void_p) for name in ("query", "key", "value")] + [
+        (name, _c_int64 * 3) for name in ("query_strides", "key_strides", "value_strides")] + [
+        (name, _c_void_p) for name in ("pos_key", "pos_query")] + [
+        (name, _c_int64 * 2) for name in ("pos_key_strides", "pos_query_strides")] + [
+        (name, _c_void_p) for name in ("delta_to_slot", "mask")] + [
+        (name, _c_int) for name in ("B", "H", "L", "D", "S", "dtype")] + [
+        ("scale", _c_float), ("p", _c_double)]
+
+
+# EncoderLayer's fields for struct.pack (a Structure takes its fields one by one, 3 us).
 ENCODER_LAYER_FORMAT = struct.Struct("@15P3f6i0P")
 
 _handle: ctypes.CDLL | None = None
@@ -180,6 +192,22 @@ def _bind(lib: ctypes.CDLL) -> None:
         _c_void_p, _c_void_p, _c_void_p,                         # ids, dout, dtable
         _c_int64, _c_int, _c_int, _c_float, _c_int64,            # n, rows, hidden, scale, padding
         _c_int, _c_int,                                          # id bytes, dtype
+        _c_void_p, ctypes.c_size_t, _c_void_p,                   # workspace, bytes, stream
+    ]
+    lib.dflash_attention_train_bits_bytes.restype = ctypes.c_size_t
+    lib.dflash_attention_train_bits_bytes.argtypes = [_c_int, _c_int, _c_int]  # B, H, L
+    lib.dflash_attention_train_fwd.restype = _c_int
+    lib.dflash_attention_train_fwd.argtypes = [
+        ctypes.POINTER(AttentionTrain), _c_void_p, _c_uint32,    # attention, rng, site
+        _c_void_p, _c_void_p, _c_void_p, _c_void_p,              # out, lse, bits, stream
+    ]
+    lib.dflash_attention_train_bwd_workspace_bytes.restype = ctypes.c_size_t
+    lib.dflash_attention_train_bwd_workspace_bytes.argtypes = [ctypes.POINTER(AttentionTrain)]
+    lib.dflash_attention_train_bwd.restype = _c_int
+    lib.dflash_attention_train_bwd.argtypes = [
+        ctypes.POINTER(AttentionTrain), _c_void_p, _c_void_p,    # attention, out, lse
+        _c_void_p, _c_void_p,                                    # bits, dout
+        _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p,   # dq, dk, dv, dpos_key, dpos_query
         _c_void_p, ctypes.c_size_t, _c_void_p,                   # workspace, bytes, stream
     ]
     lib.dflash_error_string.restype = ctypes.c_char_p

@@ -46,12 +46,14 @@ from torch.nn.modules import module as torch_module
 from . import _lib
 
 MAX_HIDDEN = 8192  # widest row of layer_norm
+ATTENTION_WIDTHS = (32, 64, 128)  # head widths of attention
+MAX_LENGTH = 16384  # longest sequence of attention
 
 
 class _Ops:
     """The torch operators (``csrc/torch_ops.cpp``), loaded at the first call."""
 
-    names = ("dropout", "dropout_layernorm", "embedding_lookup")
+    names = ("dropout", "dropout_layernorm", "embedding_lookup", "attention")
 
     def __getattr__(self, name: str) -> Any:
         if name not in self.names:
@@ -107,6 +109,32 @@ def _register_fakes() -> None:
     @fake("disentangled_flash::embedding_gradient")
     def _(dy, ids, rows, scale, padding):
         return dy.new_empty((rows, dy.shape[-1]))
+
+    def contiguous(t):  # the outputs are, whatever the inputs' strides
+        return t.new_empty(t.shape)
+
+    @fake("disentangled_flash::attention")
+    def _(query, key, value, pos_key, pos_query, delta_to_slot, mask, rng, scale, p, site):
+        return contiguous(query)
+
+    @fake("disentangled_flash::attention_train")
+    def _(query, key, value, pos_key, pos_query, delta_to_slot, mask, rng, scale, p, site):
+        batch, length, heads, _ = query.shape
+        row = (length + 63) // 64 * 8
+        bits = batch * heads * length * row if p > 0 else 0
+        return (contiguous(query), query.new_empty((batch, heads, length), dtype=torch.float32),
+                query.new_empty(bits, dtype=torch.uint8))
+
+    @fake("disentangled_flash::attention_backward")
+    def _(dout, out, lse, bits, query, key, value, pos_key, pos_query, delta_to_slot, mask, scale,
+          p, want_pos_key, want_pos_query):
+        def table(t, wanted):
+            if t is None or not wanted:
+                return query.new_empty(0)
+            return t.new_empty((t.shape[1], t.shape[0], t.shape[2]))
+
+        return (contiguous(query), contiguous(key), contiguous(value),
+                table(pos_key, want_pos_key), table(pos_query, want_pos_query))
 
 
 # ---- operators -----------------------------------------------------------------------
@@ -242,6 +270,93 @@ def embedding(
             raise ValueError(f"padding_idx {padding_idx} is outside the table of {rows} rows")
         padding = int(padding_idx) % rows
     return _ops.embedding_lookup(input_ids.contiguous(), weight, scale, padding)
+
+
+def attention(
+    query: torch.Tensor,
+    key: torch.Tensor,
+    value: torch.Tensor,
+    pos_key: torch.Tensor | None,
+    pos_query: torch.Tensor | None,
+    delta_to_slot: torch.Tensor,
+    scale: float,
+    mask: torch.Tensor | None = None,
+    p: float = 0.0,
+    rng: torch.Tensor | None = None,
+    site: int = 0,
+) -> torch.Tensor:
+    """Disentangled attention with dropout on its probabilities, ``[B, L, H, d]``.
+
+    The score of query ``i`` and key ``j`` is ``scale * (q_i.k_j + q_i.pos_key[t] +
+    k_j.pos_query[t])`` with the learned row ``t = delta_to_slot[i - j + L - 1]`` of the relative
+    distance (``position.SharedPositionPlanCache.compact`` has that table, an int32 ``[2L - 1]``).
+    An entry outside the tables stands for a row of zeros.
+
+    ``query``, ``key`` and ``value`` are ``[B, L, H, d]`` with ``d`` 32, 64 or 128 and at most
+    16384 tokens, ``pos_key`` and ``pos_query`` ``[H, S, d]`` (``None``: no such term), all of one
+    dtype; views whose rows of ``d`` start on 16-byte boundaries (the projections' outputs
+    are) are read where they lie, others are copied.
+    ``mask`` is a bool or uint8 ``[B, L]``, nonzero for tokens that are kept.  A kept query has
+    the softmax over the kept keys, whatever the padded places hold; a padded query has ``1 / L``
+    for every key, as in Hugging Face's attention.  ``p``, ``rng`` and ``site`` as in
+    :func:`dropout`, on the probabilities ``[B, H, L, L]``.
+
+    Scores and softmax are fp32; the probabilities, and in the backward pass the gradients of
+    the scores, are rounded to the dtype where they are multiplied.  One bit for each probability is kept for the
+    backward pass, and no ``[L, L]`` tensor besides; the backward pass takes up to 2 GiB of
+    memory for such a tensor at a time.
+    """
+
+    p, site, scale = float(p), int(site), float(scale)
+    _check_floating("query", query)
+    shape, dtype, device = query.shape, query.dtype, query.get_device()
+    if len(shape) != 4 or shape[3] not in ATTENTION_WIDTHS or shape[2] < 1:
+        raise ValueError(f"query must be [B, L, H, d] with d in {ATTENTION_WIDTHS}, "
+                         f"got {tuple(shape)}")
+    if shape[1] > MAX_LENGTH:
+        raise ValueError(f"at most {MAX_LENGTH} tokens, got {shape[1]}")
+    for name, tensor in (("key", key), ("value", value)):
+        if tensor.shape != shape or tensor.dtype != dtype or tensor.get_device() != device:
+            raise ValueError(f"{name} must match query: {tuple(shape)} {dtype} on {query.device}, "
+                             f"got {tuple(tensor.shape)} {tensor.dtype} on {tensor.device}")
+    slots = None
+    for name, tensor in (("pos_key", pos_key), ("pos_query", pos_query)):
+        if tensor is None:
+            continue
+        if tensor.dim() != 3 or tensor.shape[0] != shape[2] or tensor.shape[2] != shape[3] \
+                or tensor.shape[1] < 1:
+            raise ValueError(f"{name} must be [H={shape[2]}, S, d={shape[3]}], got "
+                             f"{tuple(tensor.shape)}")
+        if tensor.dtype != dtype:
+            raise TypeError(f"{name} dtype {tensor.dtype} is not that of query ({dtype})")
+        if tensor.get_device() != device:
+            raise ValueError(f"{name} is on {tensor.device}, query on {query.device}")
+        if slots is not None and tensor.shape[1] != slots:
+            raise ValueError(f"pos_key has {slots} slots, pos_query {tensor.shape[1]}")
+        slots = tensor.shape[1]
+    if delta_to_slot.dtype != torch.int32 or delta_to_slot.dim() != 1:
+        raise TypeError("delta_to_slot must be a 1-D int32 tensor")
+    if shape[1] > 0 and delta_to_slot.shape[0] != 2 * shape[1] - 1:
+        raise ValueError(f"delta_to_slot has {delta_to_slot.shape[0]} entries, expected 2L-1 = "
+                         f"{2 * shape[1] - 1}")
+    if delta_to_slot.get_device() != device:
+        raise ValueError(f"delta_to_slot is on {delta_to_slot.device}, query on {query.device}")
+    if mask is not None:
+        if mask.shape != shape[:2] or mask.dtype not in (torch.bool, torch.uint8):
+            raise ValueError(f"mask must be bool or uint8 {tuple(shape[:2])}, got {mask.dtype} "
+                             f"{tuple(mask.shape)}")
+        if mask.get_device() != device:
+            raise ValueError(f"mask is on {mask.device}, query on {query.device}")
+        mask = mask.contiguous()
+    _check_dropout(p, rng, site, query)
+    if p == 0.0:
+        rng = None
+    else:
+        for tensor in (key, value, pos_key, pos_query, mask):
+            if tensor is not None and _is_batched(tensor):
+                _check_dropout(p, rng, site, tensor)
+    return _ops.attention(query, key, value, pos_key, pos_query, delta_to_slot.contiguous(), mask,
+                          rng, scale, p, site)
 
 
 # ---- modules ---------------------------------------------------------------------------
@@ -663,6 +778,7 @@ __all__ = [
     "Embedding",
     "LayerNorm",
     "OutputBlock",
+    "attention",
     "dropout",
     "embedding",
     "enable_deberta_training",

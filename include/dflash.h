@@ -25,7 +25,7 @@ extern "C" {
 
 #define DFLASH_API __attribute__((visibility("default")))
 
-#define DFLASH_ABI_VERSION 8
+#define DFLASH_ABI_VERSION 9
 
 #define DFLASH_DTYPE_FP16 0
 #define DFLASH_DTYPE_BF16 1
@@ -410,6 +410,59 @@ DFLASH_API int dflash_embedding_bwd(const void* ids, const void* dout, void* dta
                                     int rows, int hidden, float scale, int64_t padding,
                                     int id_bytes, int dtype, void* workspace,
                                     size_t workspace_bytes, void* stream);
+
+/*
+ * Disentangled attention in training: dropout on the probabilities, and gradients.  (The
+ * attention of DebertaV2SelfAttention, reference kernel.py:196-345, which is inference-only.)
+ *   s(i, j) = scale (Q_i.K_j + Q_i.pos_key[t] + K_j.pos_query[t]), t = delta_to_slot[i - j + L - 1]
+ * A kept query has the softmax over the kept keys, a padded one 1/L for each of the L keys.  The
+ * probability (b, h, i, j) is dropped as dflash_dropout drops that element of [B, H, L, L].
+ *   query, key, value  : [B, H, L, D] by their strides (batch, head, position, in elements),
+ *                        D (32, 64 or 128) elements contiguous
+ *   pos_key, pos_query : [H, S, D] by their strides (head, slot); NULL: no such term
+ *   delta_to_slot      : int32 [2L - 1]; an entry outside [0, S) stands for a row of zeros
+ *                        that takes no gradient
+ *   mask               : uint8 [B, L], nonzero: kept; NULL: all kept
+ * Tensors and strides are multiples of 16 bytes.  L is at most 16384, B H at most 2^20.
+ */
+typedef struct dflash_attention_train {
+  const void *query, *key, *value;
+  int64_t query_strides[3], key_strides[3], value_strides[3];
+  const void *pos_key, *pos_query;
+  int64_t pos_key_strides[2], pos_query_strides[2];
+  const int32_t* delta_to_slot;
+  const uint8_t* mask;
+  int B, H, L, D, S, dtype;
+  float scale;
+  double p;
+} dflash_attention_train;
+
+/*
+ *   out  : [B, L, H, D] contiguous
+ *   lse  : fp32 [B, H, L], kept for the backward pass; may be NULL
+ *   bits : dflash_attention_train_bits_bytes(B, H, L) bytes, 8-byte aligned: the dropped places,
+ *          one bit each, kept for the backward pass; may be NULL when p is 0
+ */
+DFLASH_API size_t dflash_attention_train_bits_bytes(int B, int H, int L);
+DFLASH_API int dflash_attention_train_fwd(const dflash_attention_train* attention,
+                                          const int64_t* rng, uint32_t site, void* out, float* lse,
+                                          void* bits, void* stream);
+
+/*
+ * Its backward pass, from the same inputs and what the forward pass wrote.
+ *   dout, dquery, dkey, dvalue : [B, L, H, D] contiguous
+ *   dpos_key, dpos_query       : [S, H, D] contiguous; either may be NULL
+ *   workspace                  : dflash_attention_train_bwd_workspace_bytes(attention) bytes,
+ *                                16-byte aligned (0: arguments the call refuses)
+ * Sums are taken in an order that depends on the shapes and the mask alone.
+ */
+DFLASH_API size_t dflash_attention_train_bwd_workspace_bytes(
+    const dflash_attention_train* attention);
+DFLASH_API int dflash_attention_train_bwd(const dflash_attention_train* attention, const void* out,
+                                          const float* lse, const void* bits, const void* dout,
+                                          void* dquery, void* dkey, void* dvalue, void* dpos_key,
+                                          void* dpos_query, void* workspace,
+                                          size_t workspace_bytes, void* stream);
 
 /* Text for a return code of any dflash_* entry point. */
 DFLASH_API const char* dflash_error_string(int code);
