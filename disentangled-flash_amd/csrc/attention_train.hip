@@ -136,6 +136,24 @@ __device__ inline typename Op<T>::frag pack(f32x4_t a, f32x4_t b) {
   return f;
 }
 
+// The same from global memory; `from`: byte offset of the eight.
+template <typename T>
+__device__ inline typename Op<T>::frag load_frag(__amdgpu_buffer_rsrc_t memory, uint32_t from) {
+  const u32x4_t lo = __builtin_amdgcn_raw_buffer_load_b128(memory, from, 0, 0);
+  if constexpr (sizeof(T) == 4) {
+    const u32x4_t hi = __builtin_amdgcn_raw_buffer_load_b128(memory, from + 16, 0, 0);
+    f32x8_t f;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      f[e] = __builtin_bit_cast(float, static_cast<uint32_t>(lo[e]));
+      f[4 + e] = __builtin_bit_cast(float, static_cast<uint32_t>(hi[e]));
+    }
+    return f;
+  } else {
+    return __builtin_bit_cast(typename Op<T>::frag, lo);
+  }
+}
+
 template <typename T>
 __device__ inline void store4(T* p, f32x4_t v) {
   Quad<T> q;
@@ -146,33 +164,125 @@ __device__ inline void store4(T* p, f32x4_t v) {
 
 // ---- tiles ----------------------------------------------------------------------------
 
-// ROWS rows of D elements into LDS; source(r) gives row r's address, or NULL for a row of 0.
-template <typename T, int D, int ROWS, int NT, typename Source>
-__device__ inline void load_rows(T* tile, const Source& source) {
-  constexpr int kChunks = D * static_cast<int>(sizeof(T)) / 16, kPer = 16 / static_cast<int>(sizeof(T));
-#pragma unroll
-  for (int at = 0; at < (ROWS * kChunks + NT - 1) / NT; ++at) {
-    const int n = at * NT + threadIdx.x;
-    if (ROWS * kChunks % NT != 0 && n >= ROWS * kChunks) break;
-    const int row = n / kChunks, chunk = n % kChunks;
-    const T* p = source(row);
-    u32x4_t v{};
-    if (p) v = *reinterpret_cast<const u32x4_t*>(p + chunk * kPer);
-    *reinterpret_cast<u32x4_t*>(tile + row * kLd<T, D> + chunk * kPer) = v;
-  }
+// Rows are read through buffer resources: an offset past the size gives zeros, so that rows
+// that are not to be read cost no branch, and all loads of a tile are in flight together
+// (behind a branch for each of them a tile took 11 us).
+constexpr uint32_t kNoRow = 0x80000000u;  // past every resource's size
+constexpr int kBufferFlags = 0x00020000;  // raw buffer, gfx9 family descriptor word 3
+
+__device__ inline __amdgpu_buffer_rsrc_t resource(const void* base, int64_t bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), static_cast<short>(0),
+                                           static_cast<int>(bytes), kBufferFlags);
 }
 
-// The position rows of deltas first .. first + ROWS - 1.
+// Tokens of one head: rows `stride` elements apart.
+template <typename T, int D>
+struct Tokens {
+  __amdgpu_buffer_rsrc_t memory;
+  uint32_t stride;  // bytes
+  __device__ Tokens(const void* base, const Strides& s, int b, int h, int L)
+      : memory(resource(static_cast<const T*>(base) + b * s.b + h * s.h,
+                        ((L - 1) * s.l + D) * static_cast<int64_t>(sizeof(T)))),
+        stride(static_cast<uint32_t>(s.l * sizeof(T))) {}
+};
+
+// ROWS rows of D elements on their way into LDS, in the registers of NT threads.
 template <typename T, int D, int ROWS, int NT>
-__device__ inline void load_window(T* tile, const T* table, int64_t row_stride, const int32_t* lut,
-                                   int first, int L, int S) {
-  load_rows<T, D, ROWS, NT>(tile, [&](int r) -> const T* {
-    const int at = first + r + L - 1;
-    if (at < 0 || at > 2 * L - 2) return nullptr;
-    const int slot = lut[at];
-    return slot >= 0 && slot < S ? table + slot * row_stride : nullptr;
-  });
-}
+struct Stage {
+  static constexpr int kChunks = D * static_cast<int>(sizeof(T)) / 16;
+  static constexpr int kPer = 16 / static_cast<int>(sizeof(T));
+  static constexpr int N = (ROWS * kChunks + NT - 1) / NT;
+  u32x4_t v[N];
+
+  __device__ static int row(int n) { return (n * NT + threadIdx.x) / kChunks; }
+  __device__ static int chunk(int n) { return (n * NT + threadIdx.x) % kChunks; }
+  __device__ static bool inside(int n) { return ROWS * kChunks % NT == 0 || row(n) < ROWS; }
+
+  // offset(n, row): the row's byte offset, or kNoRow.
+  template <typename Offset>
+  __device__ void load(__amdgpu_buffer_rsrc_t memory, const Offset& offset) {
+#pragma unroll
+    for (int n = 0; n < N; ++n)
+      v[n] = __builtin_amdgcn_raw_buffer_load_b128(memory, offset(n, row(n)) + 16 * chunk(n), 0, 0);
+  }
+  // Rows whose bit of `wanted` is 0 are zeros.
+  __device__ void load_tokens(const Tokens<T, D>& tokens, int first, uint64_t wanted) {
+    load(tokens.memory, [&](int, int r) {
+      return r < ROWS && (wanted >> (r & 63)) & 1 ? (first + r) * tokens.stride : kNoRow;
+    });
+  }
+  // Row r goes to row place(r) of the tile.
+  template <typename Place>
+  __device__ void store(T* tile, const Place& place) const {
+#pragma unroll
+    for (int n = 0; n < N; ++n)
+      if (inside(n))
+        *reinterpret_cast<u32x4_t*>(tile + place(row(n)) * kLd<T, D> + chunk(n) * kPer) = v[n];
+  }
+  __device__ void store(T* tile) const {
+    store(tile, [](int r) { return r; });
+  }
+};
+
+// A window: ROWS position rows of successive deltas in LDS.  A step moves it STEP deltas on; the
+// rows form a ring, so that only the new ones are read.  They are read through the table of slots
+// two steps ahead of their use: first the slots, then the rows, then LDS.
+template <typename T, int D, int ROWS, int STEP, int NT>
+struct Window {
+  static_assert(ROWS % 16 == 0 && STEP % 16 == 0 && STEP <= ROWS, "blocks of 16 rows");
+  using First = Stage<T, D, ROWS, NT>;
+  using Next = Stage<T, D, STEP, NT>;
+  __amdgpu_buffer_rsrc_t table, lut;
+  uint32_t stride;  // bytes
+  int L, S;
+  int ring;  // the first row's place
+  int slots[Next::N];
+  Next rows;
+
+  __device__ Window(const void* base, int64_t row_stride, const int32_t* lut_, int L_, int S_)
+      : table(resource(base, ((S_ - 1) * row_stride + D) * static_cast<int64_t>(sizeof(T)))),
+        lut(resource(lut_, (2 * static_cast<int64_t>(L_) - 1) * 4)),
+        stride(static_cast<uint32_t>(row_stride * sizeof(T))), L(L_), S(S_), ring(0) {}
+
+  __device__ int slot_of(int delta) const {
+    const int at = delta + L - 1;
+    const bool inside = at >= 0 && at <= 2 * L - 2;
+    const int slot = static_cast<int>(
+        __builtin_amdgcn_raw_buffer_load_b32(lut, inside ? 4 * at : kNoRow, 0, 0));
+    return inside ? slot : -1;
+  }
+  __device__ uint32_t offset_of(int slot) const {
+    return slot >= 0 && slot < S ? slot * stride : kNoRow;
+  }
+  // All rows, from the delta `first`.
+  __device__ void fill(T* tile, int first) {
+    int at[First::N];
+#pragma unroll
+    for (int n = 0; n < First::N; ++n) at[n] = slot_of(first + First::row(n));
+    First all;
+    all.load(table, [&](int n, int) { return offset_of(at[n]); });
+    all.store(tile);
+    ring = 0;
+  }
+  // The slots of the rows that come after those of the window from `first`.
+  __device__ void read_slots(int first) {
+#pragma unroll
+    for (int n = 0; n < Next::N; ++n) slots[n] = slot_of(first + ROWS + Next::row(n));
+  }
+  __device__ void read_rows() {
+    rows.load(table, [&](int n, int) { return offset_of(slots[n]); });
+  }
+  __device__ void advance(T* tile) {
+    rows.store(tile, [&](int r) { return r + ring < ROWS ? r + ring : r + ring - ROWS; });
+    ring += STEP;
+    if (ring >= ROWS) ring -= ROWS;
+  }
+  // Where row r of the window lies; 16 rows from a multiple of 16 lie together.
+  __device__ int place(int r) const {
+    const int at = r + ring;
+    return at < ROWS ? at : at - ROWS;
+  }
+};
 
 // Bit j % 64 of words[j / 64]: token j is kept (0 for j >= L).
 __device__ inline void read_mask(uint64_t* words, const uint8_t* mask, int b, int L) {
@@ -194,9 +304,17 @@ __device__ inline uint64_t tokens_from(int at, int L) {
   return n >= 64 ? ~uint64_t{0} : n <= 0 ? 0 : (uint64_t{1} << n) - 1;
 }
 
-template <typename T>
-__device__ inline const T* head(const void* base, const Strides& s, int b, int h) {
-  return static_cast<const T*>(base) + b * s.b + h * s.h;
+// Bits at .. at + 63 of the sequence's words, at a multiple of 16.
+__device__ inline uint64_t kept_from(const uint64_t* words, int at, int L) {
+  return at < L ? words[at >> 6] >> (at & 63) : 0;
+}
+
+// The first and last block of 64 tokens of [from, to) that holds a kept one; first > last: none.
+__device__ inline void kept_range(const uint64_t* words, int from, int to, int* first, int* last) {
+  while (from < to && words[from] == 0) ++from;
+  while (to > from && words[to - 1] == 0) --to;
+  *first = from;
+  *last = to - 1;
 }
 
 // ---- dropped places ---------------------------------------------------------------------
@@ -223,134 +341,164 @@ __global__ __launch_bounds__(256) void dropped_bits_kernel(uint8_t* bits, int64_
 
 // ---- forward ------------------------------------------------------------------------------
 
-// A workgroup of NW wavefronts takes 16 NW queries and walks the keys in tiles of 16 NW.  Scores
-// are computed transposed (a lane holds one query and four keys of a block), so that the
-// probabilities are the operand of O^T += V^T R^T as they are.
-template <typename T, int D, int NW>
+// A workgroup of NW wavefronts takes 16 NW queries and walks the keys in tiles of BK, the last
+// first (so that its windows move up).  Scores are computed transposed (a lane holds one query
+// and four keys of a block), so that the probabilities are the operand of O^T += V^T R^T as they are.
+template <typename T, int D, int NW, int BK>
 struct FwdLayout {
-  static constexpr int BT = 16 * NW, W = BT + 16, LDW = W + 4;
+  static constexpr int BQ = 16 * NW, W = BQ + BK, LDC = BK + 20, LDP = BQ + 20;
   static constexpr int LD = kLd<T, D>;
-  T k[BT * LD], v[BT * LD], pk[2 * BT * LD], pq[2 * BT * LD];
-  float c2p[BT * LDW], p2c[BT * LDW];
+  T k[BK * LD], v[BK * LD], pk[W * LD], pq[W * LD];
+  float c2p[BQ * LDC], p2c[BK * LDP];
   uint64_t kept[kWords];
 };
 
-template <typename T, int D, int NW>
+template <typename T, int D, int NW, int BK>
 __global__ __launch_bounds__(64 * NW) void attention_train_fwd_kernel(Params p) {
-  using Y = FwdLayout<T, D, NW>;
+  using Y = FwdLayout<T, D, NW, BK>;
   using F = typename Op<T>::frag;
-  constexpr int BT = Y::BT, LD = Y::LD, LDW = Y::LDW, NT = 64 * NW;
+  constexpr int BQ = Y::BQ, LD = Y::LD, LDC = Y::LDC, LDP = Y::LDP, NT = 64 * NW, KB = BK / 16;
   extern __shared__ __align__(16) unsigned char memory[];
   Y& s = *reinterpret_cast<Y*>(memory);
-  const int blocks = (p.L + BT - 1) / BT;
+  const int blocks = (p.L + BQ - 1) / BQ;
   const int at = xcd_logical_block(blockIdx.x, gridDim.x);
-  const int bh = at / blocks, i0 = at % blocks * BT;
+  const int bh = at / blocks, i0 = at % blocks * BQ;
   const int b = bh / p.H, h = bh % p.H;
   const bool uniform = blockIdx.y == 1;  // the block's padded queries, otherwise its kept ones
   const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, c = lane % 16, g = lane / 16;
   const int i = i0 + 16 * wave + c;
 
   read_mask(s.kept, p.mask, b, p.L);
-  constexpr uint64_t kBlock = BT == 64 ? ~uint64_t{0} : (uint64_t{1} << (BT % 64)) - 1;
-  const uint64_t rows = tokens_from(i0, p.L) & kBlock;
-  const uint64_t kept_rows = (s.kept[i0 / 64] >> (i0 % 64)) & kBlock;
-  if (uniform ? rows == kept_rows : kept_rows == 0) return;
+  const int words = (p.L + 63) / 64;
+  bool any = false;
+  for (int at2 = i0; at2 < i0 + BQ && at2 < p.L; at2 += 16) {
+    const uint64_t kept = kept_from(s.kept, at2, p.L), inside = tokens_from(at2, p.L);
+    any |= ((uniform ? inside & ~kept : kept) & 0xFFFF) != 0;
+  }
+  int first = 0, last = words - 1;
+  if (!uniform) kept_range(s.kept, 0, words, &first, &last);
+  if (!any) return;
 
-  const T* q = head<T>(p.q, p.sq, b, h);
-  const T* k = head<T>(p.k, p.sk, b, h);
-  const T* v = head<T>(p.v, p.sv, b, h);
-  const T* pk = p.pos_key ? static_cast<const T*>(p.pos_key) + h * p.pk_h : nullptr;
-  const T* pq = p.pos_query ? static_cast<const T*>(p.pos_query) + h * p.pq_h : nullptr;
-  const bool mine = (kept_rows >> (16 * wave + c)) & 1;
+  const Tokens<T, D> q(p.q, p.sq, b, h, p.L), k(p.k, p.sk, b, h, p.L), v(p.v, p.sv, b, h, p.L);
+  const bool has_pk = p.pos_key && !uniform, has_pq = p.pos_query && !uniform;
+  Window<T, D, Y::W, BK, NT> pk(static_cast<const T*>(p.pos_key) + h * p.pk_h, p.pk_s, p.lut, p.L,
+                                p.S);
+  Window<T, D, Y::W, BK, NT> pq(static_cast<const T*>(p.pos_query) + h * p.pq_h, p.pq_s, p.lut,
+                                p.L, p.S);
+  const bool mine = i < p.L && bit_of(s.kept, i);
 
   F qf[D / 32];
 #pragma unroll
   for (int ks = 0; ks < D / 32; ++ks) {
-    qf[ks] = F{};
-    if (mine) qf[ks] = *reinterpret_cast<const F*>(q + i * p.sq.l + 32 * ks + 8 * g);
+    const uint32_t from = mine ? i * q.stride + (32 * ks + 8 * g) * sizeof(T) : kNoRow;
+    qf[ks] = load_frag<T>(q.memory, from);
   }
 
   f32x4_t o[D / 16] = {};
   float top = -INFINITY, sum = 0;
-  const uint8_t* bits =
-      p.bits ? p.bits + (static_cast<int64_t>(bh) * p.L + (i < p.L ? i : p.L - 1)) * p.bit_row
-             : nullptr;
+  const __amdgpu_buffer_rsrc_t bits = resource(
+      p.bits ? p.bits + static_cast<int64_t>(bh) * p.L * p.bit_row : nullptr,
+      p.bits ? p.L * p.bit_row : 0);
 
-  for (int j0 = 0; j0 < p.L; j0 += BT) {
-    const uint64_t inside = tokens_from(j0, p.L) & kBlock;
-    const uint64_t kept = (s.kept[j0 / 64] >> (j0 % 64)) & kBlock;
-    const uint64_t taken = uniform ? inside : kept;
-    if (taken == 0) continue;
-    __syncthreads();
-    load_rows<T, D, BT, NT>(s.v, [&](int r) {
-      return (taken >> r) & 1 ? v + (j0 + r) * p.sv.l : nullptr;
-    });
-    if (!uniform) {
-      load_rows<T, D, BT, NT>(s.k, [&](int r) {
-        return (kept >> r) & 1 ? k + (j0 + r) * p.sk.l : nullptr;
-      });
-      if (pk) load_window<T, D, 2 * BT, NT>(s.pk, pk, p.pk_s, p.lut, i0 - j0 - BT, p.L, p.S);
-      if (pq) load_window<T, D, 2 * BT, NT>(s.pq, pq, p.pq_s, p.lut, i0 - j0 - BT, p.L, p.S);
-    }
-    uint64_t dropped = 0;
-    if (bits) {
-      dropped = *reinterpret_cast<const uint64_t*>(bits + j0 / 64 * 8);
-      dropped = (dropped >> (j0 % 64)) >> (4 * g);
-    }
-    __syncthreads();
+  auto taken_of = [&](int j0) {
+    constexpr uint64_t kBlock = BK == 64 ? ~uint64_t{0} : (uint64_t{1} << (BK % 64)) - 1;
+    return (uniform ? tokens_from(j0, p.L) : kept_from(s.kept, j0, p.L)) & kBlock;
+  };
+  Stage<T, D, BK, NT> next_k, next_v;
+  auto read_tile = [&](int j0) {
+    const uint64_t taken = taken_of(j0);
+    next_v.load_tokens(v, j0, taken);
+    if (!uniform) next_k.load_tokens(k, j0, taken);
+  };
 
-    f32x4_t x[NW] = {};  // x[kb][r]: key j0 + 16 kb + 4g + r
+  const int stop = first * 64;
+  int j0 = last * 64 + 64 - BK;
+  read_tile(j0);
+  if (has_pk) {
+    pk.fill(s.pk, i0 - j0 - BK);
+    pk.read_slots(i0 - j0 - BK);
+  }
+  if (has_pq) {
+    pq.fill(s.pq, i0 - j0 - BK);
+    pq.read_slots(i0 - j0 - BK);
+  }
+  for (bool begun = false;; j0 -= BK, begun = true) {
+    lds_barrier();
+    next_v.store(s.v);
+    if (!uniform) next_k.store(s.k);
+    if (begun && has_pk) pk.advance(s.pk);
+    if (begun && has_pq) pq.advance(s.pq);
+    lds_barrier();
+    const uint64_t taken = taken_of(j0);
+    const u32x2_t word = __builtin_amdgcn_raw_buffer_load_b64(
+        bits, i < p.L ? i * static_cast<uint32_t>(p.bit_row) + j0 / 64 * 8 : kNoRow, 0, 0);
+    if (j0 > stop) {
+      read_tile(j0 - BK);
+      if (has_pk) {
+        pk.read_rows();
+        pk.read_slots(i0 - j0);
+      }
+      if (has_pq) {
+        pq.read_rows();
+        pq.read_slots(i0 - j0);
+      }
+    }
+
+    f32x4_t x[KB] = {};  // x[kb][r]: key j0 + 16 kb + 4g + r
     if (!uniform) {
-      if (pq) {
-        // Keys of block `wave` against deltas from i0 - j0 - 16 wave - 16.
+      if (has_pq) {
+        // Keys of block kb against deltas from i0 - j0 - 16 kb - 16.
 #pragma unroll
-        for (int wb = 0; wb < NW + 1; ++wb) {
+        for (int n = 0; n < (KB * (NW + 1) + NW - 1) / NW; ++n) {
+          const int at2 = n * NW + wave, kb = at2 % KB, wb = at2 / KB;
+          if (at2 < KB * (NW + 1)) {
+            const T* from = s.pq + pq.place(BK - 16 - 16 * kb + 16 * wb) * LD;
+            f32x4_t acc{};
+#pragma unroll
+            for (int ks = 0; ks < D / 32; ++ks)
+              acc = Op<T>::run(read_row<T>(from + c * LD + 32 * ks, g),
+                               read_row<T>(s.k + (16 * kb + c) * LD + 32 * ks, g), acc);
+            *reinterpret_cast<f32x4_t*>(s.p2c + (16 * kb + c) * LDP + 16 * wb + 4 * g) = acc;
+          }
+        }
+      }
+      if (has_pk) {
+        // This wavefront's queries against deltas from i0 + 16 wave - j0 - BK.
+#pragma unroll
+        for (int wb = 0; wb < KB + 1; ++wb) {
+          const T* from = s.pk + pk.place(16 * wave + 16 * wb) * LD;
           f32x4_t acc{};
 #pragma unroll
           for (int ks = 0; ks < D / 32; ++ks)
-            acc = Op<T>::run(
-                read_row<T>(s.pq + (BT - 16 - 16 * wave + 16 * wb + c) * LD + 32 * ks, g),
-                read_row<T>(s.k + (16 * wave + c) * LD + 32 * ks, g), acc);
-          *reinterpret_cast<f32x4_t*>(s.p2c + (16 * wave + c) * LDW + 16 * wb + 4 * g) = acc;
-        }
-      }
-      if (pk) {
-        // This wavefront's queries against deltas from i0 + 16 wave - j0 - BT.
-#pragma unroll
-        for (int wb = 0; wb < NW + 1; ++wb) {
-          f32x4_t acc{};
-#pragma unroll
-          for (int ks = 0; ks < D / 32; ++ks)
-            acc = Op<T>::run(read_row<T>(s.pk + (16 * wave + 16 * wb + c) * LD + 32 * ks, g),
-                             qf[ks], acc);
-          *reinterpret_cast<f32x4_t*>(s.c2p + (16 * wave + c) * LDW + 16 * wb + 4 * g) = acc;
+            acc = Op<T>::run(read_row<T>(from + c * LD + 32 * ks, g), qf[ks], acc);
+          *reinterpret_cast<f32x4_t*>(s.c2p + (16 * wave + c) * LDC + 16 * wb + 4 * g) = acc;
         }
       }
 #pragma unroll
-      for (int kb = 0; kb < NW; ++kb)
+      for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
         for (int ks = 0; ks < D / 32; ++ks)
           x[kb] = Op<T>::run(read_row<T>(s.k + (16 * kb + c) * LD + 32 * ks, g), qf[ks], x[kb]);
-      __syncthreads();
-      if (pk) {
+      lds_barrier();
+      if (has_pk) {
 #pragma unroll
-        for (int kb = 0; kb < NW; ++kb)
+        for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
           for (int r = 0; r < 4; ++r)
-            x[kb][r] += s.c2p[(16 * wave + c) * LDW + BT + c - 16 * kb - 4 * g - r];
+            x[kb][r] += s.c2p[(16 * wave + c) * LDC + BK + c - 16 * kb - 4 * g - r];
       }
-      if (pq) {
+      if (has_pq) {
 #pragma unroll
-        for (int kb = 0; kb < NW; ++kb)
+        for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
           for (int r = 0; r < 4; ++r)
-            x[kb][r] += s.p2c[(16 * kb + 4 * g + r) * LDW + 16 * wave + 16 + c - 4 * g - r];
+            x[kb][r] += s.p2c[(16 * kb + 4 * g + r) * LDP + 16 * wave + 16 + c - 4 * g - r];
       }
     }
     const uint64_t lane_taken = taken >> (4 * g);
     float high = -INFINITY;
 #pragma unroll
-    for (int kb = 0; kb < NW; ++kb)
+    for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         x[kb][r] = (lane_taken >> (16 * kb + r)) & 1 ? x[kb][r] * p.scale_log2 : -INFINITY;
@@ -358,23 +506,26 @@ __global__ __launch_bounds__(64 * NW) void attention_train_fwd_kernel(Params p) 
       }
     high = fmaxf(high, __shfl_xor(high, 16));
     high = fmaxf(high, __shfl_xor(high, 32));
-    high = fmaxf(high, top);  // (finite: the tile holds a key that is taken)
-    const float shrink = __builtin_amdgcn_exp2f(top - high);
+    high = fmaxf(high, top);
+    const float base = high == -INFINITY ? 0.0f : high;  // (no key is taken so far)
+    const float shrink = __builtin_amdgcn_exp2f(top - base);
     top = high;
     sum *= shrink;
 #pragma unroll
     for (int db = 0; db < D / 16; ++db) o[db] *= shrink;
+    const uint64_t dropped =
+        ((static_cast<uint64_t>(word[1]) << 32 | word[0]) >> (j0 % 64)) >> (4 * g);
 #pragma unroll
-    for (int kb = 0; kb < NW; ++kb)
+    for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const float e = __builtin_amdgcn_exp2f(x[kb][r] - top);
+        const float e = __builtin_amdgcn_exp2f(x[kb][r] - base);
         sum += e;
         x[kb][r] = (dropped >> (16 * kb + r)) & 1 ? 0.0f : e;
       }
     // (Rounded to T here, as the operand of the product: off by half a step of each probability.)
 #pragma unroll
-    for (int ks = 0; ks < NW / 2; ++ks) {
+    for (int ks = 0; ks < KB / 2; ++ks) {
       const F r = pack<T>(x[2 * ks], x[2 * ks + 1]);
 #pragma unroll
       for (int db = 0; db < D / 16; ++db)
@@ -382,6 +533,7 @@ __global__ __launch_bounds__(64 * NW) void attention_train_fwd_kernel(Params p) 
             read_columns<T>(s.v + 16 * db, LD, 32 * ks + 4 * g, 32 * ks + 16 + 4 * g, c), r,
             o[db]);
     }
+    if (j0 <= stop) break;
   }
 
   sum += __shfl_xor(sum, 16);
@@ -432,12 +584,15 @@ struct KeyLayout {
   static constexpr int KF = (WK + 31) / 32 * 32, LDF = KF + 16 / static_cast<int>(sizeof(T));
   static constexpr int LD = kLd<T, D>;
   // (dK's product reads KF rows of pq from row BK - 16 - 16 wave.)
-  static constexpr int PQ = BK - 16 + KF;
-  T q[BQ * LD], dout[BQ * LD], pk[(BQ + BK) * LD], pq[PQ * LD];
-  float c2p[BQ * LDC], p2c[BK * LDP];
-  T skew[BK * LDF];
+  static constexpr int PK = BQ + BK, PQ = BK - 16 + KF;
+  static constexpr int kWide = BK < 64 ? 1 : BK / 64;  // words of dropped places a query
+  // A wavefront's scores of its keys by delta, and after them G by delta.
+  static constexpr int kScores = 16 * LDP * 4, kSkew = 16 * LDF * static_cast<int>(sizeof(T));
+  T q[BQ * LD], dout[BQ * LD], pk[PK * LD], pq[PQ * LD];
+  float c2p[BQ * LDC];
+  unsigned char own[NW * (kScores > kSkew ? kScores : kSkew)];
   float lse[BQ], delta[BQ];
-  uint64_t dropped[BQ];
+  uint64_t dropped[BQ * kWide];
   uint64_t kept[kWords];
 };
 
@@ -446,105 +601,158 @@ __global__ __launch_bounds__(64 * NW) void attention_train_key_kernel(Params p) 
   using Y = KeyLayout<T, D, NW, BQ>;
   using F = typename Op<T>::frag;
   constexpr int BK = Y::BK, LD = Y::LD, LDC = Y::LDC, LDP = Y::LDP, LDF = Y::LDF, NT = 64 * NW;
-  constexpr int QB = BQ / 16;
+  constexpr int QB = BQ / 16, kWide = Y::kWide;
+  constexpr uint64_t kBlock = BQ == 64 ? ~uint64_t{0} : (uint64_t{1} << (BQ % 64)) - 1;
   extern __shared__ __align__(16) unsigned char memory[];
   Y& s = *reinterpret_cast<Y*>(memory);
-  const int blocks = (p.L + 63) / 64 * (64 / BK);  // whole blocks of 64: all of G is written
+  const int words = (p.L + 63) / 64;
+  const int blocks = (words * 64 + BK - 1) / BK;
   const int at = xcd_logical_block(blockIdx.x, gridDim.x);
   const int pair = at / blocks, j0 = at % blocks * BK;
   const int b = p.b0 + pair / p.nh, h = p.h0 + pair % p.nh;
   const int64_t bh = static_cast<int64_t>(b) * p.H + h;
   const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, c = lane % 16, g = lane / 16;
   const int j = j0 + 16 * wave + c;
+  float* scores = reinterpret_cast<float*>(s.own + wave * (sizeof(s.own) / NW));
+  T* skew = reinterpret_cast<T*>(scores);
 
   read_mask(s.kept, p.mask, b, p.L);
-  for (int n = threadIdx.x; n < BK * LDF; n += NT) s.skew[n] = static_cast<T>(0.0f);
-  const bool any_key = s.kept[j0 / 64] != 0;
   const bool mine = j < p.L && bit_of(s.kept, j);
   const float even = 1.0f / static_cast<float>(p.L);
+  // The queries' blocks that are scored; none where no key of the block is kept.
+  int first = 0, last = -1, key_first, key_last;
+  kept_range(s.kept, j0 / 64, min((j0 + BK + 63) / 64, words), &key_first, &key_last);
+  if (key_first <= key_last) kept_range(s.kept, 0, words, &first, &last);
 
-  const T* q = head<T>(p.q, p.sq, b, h);
-  const T* k = head<T>(p.k, p.sk, b, h);
-  const T* v = head<T>(p.v, p.sv, b, h);
-  const T* pk = p.pos_key ? static_cast<const T*>(p.pos_key) + h * p.pk_h : nullptr;
-  const T* pq = p.pos_query ? static_cast<const T*>(p.pos_query) + h * p.pq_h : nullptr;
-  const T* dout = static_cast<const T*>(p.dout) + (static_cast<int64_t>(b) * p.L * p.H + h) * D;
+  const Tokens<T, D> q(p.q, p.sq, b, h, p.L), k(p.k, p.sk, b, h, p.L), v(p.v, p.sv, b, h, p.L);
   const int64_t row = static_cast<int64_t>(p.H) * D;
+  const Tokens<T, D> dout(p.dout, Strides{p.L * row, D, row}, b, h, p.L);
+  const bool has_pk = p.pos_key, has_pq = p.pos_query;
+  Window<T, D, Y::PK, BQ, NT> pk(static_cast<const T*>(p.pos_key) + h * p.pk_h, p.pk_s, p.lut, p.L,
+                                 p.S);
+  Window<T, D, Y::PQ, BQ, NT> pq(static_cast<const T*>(p.pos_query) + h * p.pq_h, p.pq_s, p.lut,
+                                 p.L, p.S);
   // Fragments of this pair: [16 keys][32 queries].
-  const int q32 = (p.L + 63) / 64 * 2;
+  const int q32 = 2 * words;
   T* out_g = static_cast<T*>(p.g) +
-             (static_cast<int64_t>(pair) * (2 * q32) + j0 / 16 + wave) * q32 * kFragment;
+             (static_cast<int64_t>(pair) * (2 * q32) + j0 / 16 + wave) * q32 * kFragment + lane * 8;
+  const bool writes = j0 + 16 * wave < 64 * words;
 
   F kf[D / 32], vf[D / 32];
 #pragma unroll
   for (int ks = 0; ks < D / 32; ++ks) {
-    kf[ks] = F{};
-    vf[ks] = F{};
-    if (mine) kf[ks] = *reinterpret_cast<const F*>(k + j * p.sk.l + 32 * ks + 8 * g);
-    if (j < p.L) vf[ks] = *reinterpret_cast<const F*>(v + j * p.sv.l + 32 * ks + 8 * g);
+    const uint32_t in_row = (32 * ks + 8 * g) * sizeof(T);
+    kf[ks] = load_frag<T>(k.memory, mine ? j * k.stride + in_row : kNoRow);
+    vf[ks] = load_frag<T>(v.memory, j < p.L ? j * v.stride + in_row : kNoRow);
   }
   f32x4_t dk[D / 16] = {}, dv[D / 16] = {};
 
-  for (int i0 = 0; i0 < (p.L + 63) / 64 * 64; i0 += BQ) {
-    constexpr uint64_t kBlock = BQ == 64 ? ~uint64_t{0} : (uint64_t{1} << (BQ % 64)) - 1;
-    const uint64_t inside = tokens_from(i0, p.L) & kBlock;
-    const uint64_t kept = (s.kept[i0 / 64] >> (i0 % 64)) & kBlock;
-    // (By whole words of 64 queries: the readers of G go by the same.)
-    const bool scored = any_key && s.kept[i0 / 64] != 0;
-    if (!scored && kept == inside) continue;  // no padded query either
-    __syncthreads();
-    load_rows<T, D, BQ, NT>(s.dout, [&](int r) {
-      return (inside >> r) & 1 ? dout + (i0 + r) * row : nullptr;
-    });
-    if (scored) {
-      load_rows<T, D, BQ, NT>(s.q, [&](int r) {
-        return (kept >> r) & 1 ? q + (i0 + r) * p.sq.l : nullptr;
-      });
-      if (pk) load_window<T, D, BQ + BK, NT>(s.pk, pk, p.pk_s, p.lut, i0 - j0 - BK, p.L, p.S);
-      if (pq) load_window<T, D, Y::PQ, NT>(s.pq, pq, p.pq_s, p.lut, i0 - j0 - BK, p.L, p.S);
+  Stage<T, D, BQ, NT> next_q, next_dout;
+  float next_lse = 0, next_delta = 0;
+  uint64_t next_dropped = 0;
+  static_assert(BQ * kWide <= NT, "one word of dropped places a thread");
+  const int64_t bit_words = p.bit_row / 8;
+  auto read_rest = [&](int i0) {
+    next_dout.load_tokens(dout, i0, tokens_from(i0, p.L));
+    const int r = threadIdx.x / kWide, word = j0 / 64 + threadIdx.x % kWide;
+    if (p.bits && r < BQ && i0 + r < p.L && word < words)
+      next_dropped = reinterpret_cast<const uint64_t*>(
+          p.bits)[(bh * p.L + i0 + r) * bit_words + word];
+  };
+  auto store_rest = [&]() {
+    next_dout.store(s.dout);
+    if (threadIdx.x < BQ * kWide) s.dropped[threadIdx.x] = next_dropped;
+  };
+  // Place 4g + r of query block qb in the generator's bits, bit c.
+  const uint16_t* dropped16 =
+      reinterpret_cast<const uint16_t*>(s.dropped) + j0 % 64 / 16 + wave + 4 * g * 4 * kWide;
+  auto factor_of = [&](int qb, int r) {
+    return (dropped16[(16 * qb + r) * 4 * kWide] >> c) & 1 ? 0.0f : p.keep_scale;
+  };
+  // dV += R^T dO of a tile, R as an operand.  (R is rounded to T: off by half a step of each.)
+  auto add_dv = [&](const f32x4_t (&x)[QB]) {
+#pragma unroll
+    for (int ks = 0; ks < QB / 2; ++ks) {
+      const F r = pack<T>(x[2 * ks], x[2 * ks + 1]);
+#pragma unroll
+      for (int db = 0; db < D / 16; ++db)
+        dv[db] = Op<T>::run(
+            read_columns<T>(s.dout + 16 * db, LD, 32 * ks + 4 * g, 32 * ks + 16 + 4 * g, c), r,
+            dv[db]);
     }
-    if (threadIdx.x < BQ) {
-      const int r = threadIdx.x, i = i0 + r < p.L ? i0 + r : p.L - 1;
-      if (scored) {
-        s.lse[r] = p.lse[bh * p.L + i];
-        s.delta[r] = p.delta[bh * p.L + i];
-      }
-      s.dropped[r] = 0;
-      if (p.bits)
-        s.dropped[r] = *reinterpret_cast<const uint64_t*>(
-                           p.bits + (bh * p.L + i) * p.bit_row + j0 / 64 * 8) >>
-                       (j0 % 64);
-    }
-    __syncthreads();
+  };
 
-    f32x4_t x[QB] = {}, y[QB] = {};  // [qb][r]: query i0 + 16 qb + 4g + r
-    if (scored) {
-      if (pk) {
+  if (first <= last) {
+    auto read_tile = [&](int i0) {
+      read_rest(i0);
+      next_q.load_tokens(q, i0, kept_from(s.kept, i0, p.L) & kBlock);
+      const int i = i0 + threadIdx.x;
+      if (threadIdx.x < BQ && i < p.L) {
+        next_lse = p.lse[bh * p.L + i];
+        next_delta = p.delta[bh * p.L + i];
+      }
+    };
+    const int stop = 64 * last + 64 - BQ;
+    int i0 = 64 * first;
+    read_tile(i0);
+    if (has_pk) {
+      pk.fill(s.pk, i0 - j0 - BK);
+      pk.read_slots(i0 - j0 - BK);
+    }
+    if (has_pq) {
+      pq.fill(s.pq, i0 - j0 - BK);
+      pq.read_slots(i0 - j0 - BK);
+    }
+    for (bool begun = false;; i0 += BQ, begun = true) {
+      lds_barrier();
+      store_rest();
+      next_q.store(s.q);
+      if (threadIdx.x < BQ) {
+        s.lse[threadIdx.x] = next_lse;
+        s.delta[threadIdx.x] = next_delta;
+      }
+      if (begun && has_pk) pk.advance(s.pk);
+      if (begun && has_pq) pq.advance(s.pq);
+      lds_barrier();
+      if (i0 < stop) {
+        read_tile(i0 + BQ);
+        if (has_pk) {
+          pk.read_rows();
+          pk.read_slots(i0 + BQ - j0 - BK);
+        }
+        if (has_pq) {
+          pq.read_rows();
+          pq.read_slots(i0 + BQ - j0 - BK);
+        }
+      }
+
+      f32x4_t x[QB] = {}, y[QB] = {};  // [qb][r]: query i0 + 16 qb + 4g + r
+      if (has_pk) {
         // Blocks of 16 queries against deltas from i0 + 16 qb - j0 - BK, shared by the wavefronts.
 #pragma unroll
         for (int n = 0; n < (QB * (NW + 1) + NW - 1) / NW; ++n) {
-          const int at2 = n * NW + wave, qb = at2 / (NW + 1), wb = at2 % (NW + 1);
+          const int at2 = n * NW + wave, qb = at2 % QB, wb = at2 / QB;
           if (at2 < QB * (NW + 1)) {
+            const T* from = s.pk + pk.place(16 * qb + 16 * wb) * LD;
             f32x4_t acc{};
 #pragma unroll
             for (int ks = 0; ks < D / 32; ++ks)
-              acc = Op<T>::run(read_row<T>(s.pk + (16 * qb + 16 * wb + c) * LD + 32 * ks, g),
+              acc = Op<T>::run(read_row<T>(from + c * LD + 32 * ks, g),
                                read_row<T>(s.q + (16 * qb + c) * LD + 32 * ks, g), acc);
             *reinterpret_cast<f32x4_t*>(s.c2p + (16 * qb + c) * LDC + 16 * wb + 4 * g) = acc;
           }
         }
       }
-      if (pq) {
+      if (has_pq) {
         // This wavefront's keys against deltas from i0 - j0 - 16 wave - 16.
 #pragma unroll
         for (int wb = 0; wb < QB + 1; ++wb) {
+          const T* from = s.pq + pq.place(BK - 16 - 16 * wave + 16 * wb) * LD;
           f32x4_t acc{};
 #pragma unroll
           for (int ks = 0; ks < D / 32; ++ks)
-            acc = Op<T>::run(
-                read_row<T>(s.pq + (BK - 16 - 16 * wave + 16 * wb + c) * LD + 32 * ks, g), kf[ks],
-                acc);
-          *reinterpret_cast<f32x4_t*>(s.p2c + (16 * wave + c) * LDP + 16 * wb + 4 * g) = acc;
+            acc = Op<T>::run(read_row<T>(from + c * LD + 32 * ks, g), kf[ks], acc);
+          *reinterpret_cast<f32x4_t*>(scores + c * LDP + 16 * wb + 4 * g) = acc;
         }
       }
 #pragma unroll
@@ -554,79 +762,104 @@ __global__ __launch_bounds__(64 * NW) void attention_train_key_kernel(Params p) 
           x[qb] = Op<T>::run(read_row<T>(s.q + (16 * qb + c) * LD + 32 * ks, g), kf[ks], x[qb]);
           y[qb] = Op<T>::run(read_row<T>(s.dout + (16 * qb + c) * LD + 32 * ks, g), vf[ks], y[qb]);
         }
-      __syncthreads();
-      if (pk) {
+      lds_barrier();
+      if (has_pk) {
 #pragma unroll
         for (int qb = 0; qb < QB; ++qb)
 #pragma unroll
           for (int r = 0; r < 4; ++r)
-            x[qb][r] +=
-                s.c2p[(16 * qb + 4 * g + r) * LDC + 4 * g + r - c - 16 * wave + BK];
+            x[qb][r] += s.c2p[(16 * qb + 4 * g + r) * LDC + 4 * g + r - c - 16 * wave + BK];
       }
-      if (pq) {
+      if (has_pq) {
 #pragma unroll
         for (int qb = 0; qb < QB; ++qb)
 #pragma unroll
           for (int r = 0; r < 4; ++r)
-            x[qb][r] += s.p2c[(16 * wave + c) * LDP + 16 * qb + 4 * g + r - c + 16];
+            x[qb][r] += scores[c * LDP + 16 * qb + 4 * g + r - c + 16];
       }
-    }
-    const uint64_t lane_kept = kept >> (4 * g), lane_inside = inside >> (4 * g);
+      const uint64_t kept = kept_from(s.kept, i0, p.L) >> (4 * g);
+      const uint64_t inside = tokens_from(i0, p.L) >> (4 * g);
 #pragma unroll
-    for (int qb = 0; qb < QB; ++qb)
+      for (int qb = 0; qb < QB; ++qb) {
+        const f32x4_t lse = *reinterpret_cast<const f32x4_t*>(s.lse + 16 * qb + 4 * g);
+        const f32x4_t delta = *reinterpret_cast<const f32x4_t*>(s.delta + 16 * qb + 4 * g);
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int at2 = 16 * qb + 4 * g + r;
-        const bool live = (lane_kept >> (16 * qb + r)) & 1;
-        const bool padded = ((lane_inside >> (16 * qb + r)) & 1) && !live && j < p.L;
-        const float m = (s.dropped[at2] >> (16 * wave + c)) & 1 ? 0.0f : p.keep_scale;
-        // (One token has one probability, 1, and no gradient.)
-        float prob = 0, grad = 0;
-        if (scored && live && mine) {
-          prob = __builtin_amdgcn_exp2f(x[qb][r] * p.scale_log2 - s.lse[at2]);
-          if (p.L > 1) grad = prob * (m == 0.0f ? -s.delta[at2] : y[qb][r] * m - s.delta[at2]);
+        for (int r = 0; r < 4; ++r) {
+          const bool live = (kept >> (16 * qb + r)) & 1;
+          const bool padded = ((inside >> (16 * qb + r)) & 1) && !live && j < p.L;
+          const float m = factor_of(qb, r);
+          const bool scored = live && mine;
+          const float prob =
+              scored ? __builtin_amdgcn_exp2f(x[qb][r] * p.scale_log2 - lse[r])
+                     : padded ? even : 0.0f;
+          // (One token has one probability, 1, and no gradient.)
+          y[qb][r] = scored && p.L > 1 ? prob * ((m == 0.0f ? 0.0f : y[qb][r] * m) - delta[r]) : 0.0f;
+          x[qb][r] = prob * m;
         }
-        if (padded) prob = even;
-        x[qb][r] = prob * m;
-        y[qb][r] = grad;
       }
-    // (R and G are rounded to T as operands: off by half a step of each.)
+      add_dv(x);
+      asm volatile("" ::: "memory");  // (`skew` takes the place of `scores`)
+      if (has_pq) {
+        // Places outside the band, which holds the 16 - c .. 15 - c + BQ of row c.
+        constexpr int kPer = 16 / static_cast<int>(sizeof(T));
+        constexpr int kLow = 16 / kPer, kChunks = kLow + (Y::KF - BQ) / kPer;
+        for (int n = lane; n < 16 * kChunks; n += 64) {
+          const int chunk = n % kChunks;
+          *reinterpret_cast<u32x4_t*>(skew + n / kChunks * LDF +
+                                      (chunk < kLow ? chunk * kPer : BQ + (chunk - kLow) * kPer)) =
+              u32x4_t{};
+        }
+        asm volatile("" ::: "memory");
+      }
+      // (G is rounded to T as an operand and as it is stored: off by half a step of each.)
 #pragma unroll
-    for (int ks = 0; ks < QB / 2; ++ks) {
-      const F r = pack<T>(x[2 * ks], x[2 * ks + 1]);
-#pragma unroll
-      for (int db = 0; db < D / 16; ++db)
-        dv[db] = Op<T>::run(
-            read_columns<T>(s.dout + 16 * db, LD, 32 * ks + 4 * g, 32 * ks + 16 + 4 * g, c), r,
-            dv[db]);
-      if (scored) {
+      for (int ks = 0; ks < QB / 2; ++ks) {
         const F dg = pack<T>(y[2 * ks], y[2 * ks + 1]);
-        *reinterpret_cast<F*>(out_g + static_cast<int64_t>(i0 / 32 + ks) * kFragment + lane * 8) =
-            dg;
+        if (writes)
+          *reinterpret_cast<F*>(out_g + static_cast<int64_t>(i0 / 32 + ks) * kFragment) = dg;
 #pragma unroll
         for (int db = 0; db < D / 16; ++db)
           dk[db] = Op<T>::run(
               read_columns<T>(s.q + 16 * db, LD, 32 * ks + 4 * g, 32 * ks + 16 + 4 * g, c), dg,
               dk[db]);
-        if (pq) {
+        if (has_pq) {
 #pragma unroll
           for (int e = 0; e < 8; ++e)
-            s.skew[(16 * wave + c) * LDF + 32 * ks + (e < 4 ? e : 12 + e) + 4 * g - c + 16] =
-                dg[e];
+            skew[c * LDF + 32 * ks + (e < 4 ? e : 12 + e) + 4 * g - c + 16] = dg[e];
         }
       }
-    }
-    if (scored && pq) {
-      __builtin_amdgcn_wave_barrier();
+      if (has_pq) {
+        asm volatile("" ::: "memory");
 #pragma unroll
-      for (int ks = 0; ks < Y::KF / 32; ++ks) {
-        const F sk = read_row<T>(s.skew + (16 * wave + c) * LDF + 32 * ks, g);
-        const int lo = BK - 16 - 16 * wave + 32 * ks + 8 * g;
+        for (int ks = 0; ks < Y::KF / 32; ++ks) {
+          const F sk = read_row<T>(skew + c * LDF + 32 * ks, g);
+          const int lo = pq.place(BK - 16 - 16 * wave + 32 * ks + 16 * (g / 2)) + 8 * (g % 2);
 #pragma unroll
-        for (int db = 0; db < D / 16; ++db)
-          dk[db] = Op<T>::run(read_columns<T>(s.pq + 16 * db, LD, lo, lo + 4, c), sk, dk[db]);
+          for (int db = 0; db < D / 16; ++db)
+            dk[db] = Op<T>::run(read_columns<T>(s.pq + 16 * db, LD, lo, lo + 4, c), sk, dk[db]);
+        }
       }
+      if (i0 >= stop) break;
     }
+  }
+
+  // Padded queries of the tiles that are not scored: 1 / L for every key.
+  for (int i0 = 0; i0 < p.L; i0 += BQ) {
+    if (i0 / 64 >= first && i0 / 64 <= last) continue;
+    const uint64_t padded =
+        tokens_from(i0, p.L) & ~kept_from(s.kept, i0, p.L) & kBlock;
+    if (padded == 0) continue;
+    read_rest(i0);
+    lds_barrier();
+    store_rest();
+    lds_barrier();
+    f32x4_t x[QB];
+#pragma unroll
+    for (int qb = 0; qb < QB; ++qb)
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        x[qb][r] = (padded >> (16 * qb + 4 * g + r)) & 1 && j < p.L ? even * factor_of(qb, r) : 0.0f;
+    add_dv(x);
   }
 
   if (j >= p.L) return;
@@ -643,7 +876,8 @@ __global__ __launch_bounds__(64 * NW) void attention_train_key_kernel(Params p) 
 template <typename T, int D>
 struct QueryLayout {
   static constexpr int LD = kLd<T, D>, LDG = kLd<T, 64>, LDE = kLd<T, 96>;
-  T k[64 * LD], pk[144 * LD];
+  static constexpr int W = 144;
+  T k[64 * LD], pk[W * LD];
   T g[64 * LDG];     // [key][query]
   T skew[64 * LDE];  // [query][delta]
   uint64_t kept[kWords];
@@ -668,53 +902,79 @@ __global__ __launch_bounds__(256) void attention_train_query_kernel(Params p) {
   read_mask(s.kept, p.mask, b, p.L);
   for (int n = threadIdx.x; n < 64 * LDE; n += 256) s.skew[n] = static_cast<T>(0.0f);
 
-  const T* k = head<T>(p.k, p.sk, b, h);
-  const T* pk = p.pos_key ? static_cast<const T*>(p.pos_key) + h * p.pk_h : nullptr;
+  int first, last;
+  kept_range(s.kept, 0, blocks, &first, &last);
+  const Tokens<T, D> k(p.k, p.sk, b, h, p.L);
+  const bool has_pk = p.pos_key;
+  Window<T, D, Y::W, 64, 256> pk(static_cast<const T*>(p.pos_key) + h * p.pk_h, p.pk_s, p.lut, p.L,
+                                 p.S);
   const int q32 = 2 * blocks;
-  const T* fragments = static_cast<const T*>(p.g) + static_cast<int64_t>(pair) * 2 * q32 * q32 * kFragment;
+  const T* fragments = static_cast<const T*>(p.g) +
+                       (static_cast<int64_t>(pair) * 2 * q32 + wave) * q32 * kFragment +
+                       static_cast<int64_t>(i0 / 32) * kFragment + lane * 8;
   f32x4_t dq[D / 16] = {};
-  for (int jb = 0; jb < blocks && s.kept[i0 / 64] != 0; ++jb) {
-    const uint64_t kept = s.kept[jb];
-    if (kept == 0) continue;
-    const int j0 = 64 * jb;
-    F f[2];
+  if (s.kept[i0 / 64] != 0) {
+    Stage<T, D, 64, 256> next_k;
+    F next_g[2];
+    auto read_tile = [&](int jb) {
+      const uint64_t kept = s.kept[jb];
+      next_k.load_tokens(k, 64 * jb, kept);
+      // (G of a block of keys without a kept one may not have been written.)
 #pragma unroll
-    for (int n = 0; n < 2; ++n)
-      f[n] = *reinterpret_cast<const F*>(
-          fragments + (static_cast<int64_t>(j0 / 16 + wave) * q32 + i0 / 32 + n) * kFragment +
-          lane * 8);
-    __syncthreads();
-    load_rows<T, D, 64, 256>(s.k, [&](int r) {
-      return (kept >> r) & 1 ? k + (j0 + r) * p.sk.l : nullptr;
-    });
-    if (pk) load_window<T, D, 144, 256>(s.pk, pk, p.pk_s, p.lut, i0 - j0 - 64, p.L, p.S);
-    const int key = 16 * wave + c;
-#pragma unroll
-    for (int n = 0; n < 2; ++n)
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const int query = 32 * n + query_of(g, e);
-        s.g[key * LDG + query] = f[n][e];
-        if (pk) s.skew[query * LDE + query % 16 - key + 64] = f[n][e];
+      for (int n = 0; n < 2; ++n) {
+        next_g[n] = F{};
+        if (kept)
+          next_g[n] = *reinterpret_cast<const F*>(
+              fragments + (static_cast<int64_t>(4 * jb) * q32 + n) * kFragment);
       }
-    __syncthreads();
-#pragma unroll
-    for (int ks = 0; ks < 2; ++ks) {
-      const int lo = 32 * ks + 8 * g;
-      const F dg = read_columns<T>(s.g + 16 * wave, LDG, lo, lo + 4, c);
-#pragma unroll
-      for (int db = 0; db < D / 16; ++db)
-        dq[db] = Op<T>::run(read_columns<T>(s.k + 16 * db, LD, lo, lo + 4, c), dg, dq[db]);
+    };
+    // The last keys first: the window moves up.
+    int jb = last;
+    read_tile(jb);
+    if (has_pk) {
+      pk.fill(s.pk, i0 - 64 * jb - 64);
+      pk.read_slots(i0 - 64 * jb - 64);
     }
-    if (pk) {
+    for (bool begun = false;; --jb, begun = true) {
+      lds_barrier();
+      next_k.store(s.k);
+      const int key = 16 * wave + c;
 #pragma unroll
-      for (int ks = 0; ks < 3; ++ks) {
-        const F sk = read_row<T>(s.skew + (16 * wave + c) * LDE + 32 * ks, g);
-        const int lo = 16 * wave + 32 * ks + 8 * g;
+      for (int n = 0; n < 2; ++n)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const int query = 32 * n + query_of(g, e);
+          s.g[key * LDG + query] = next_g[n][e];
+          if (has_pk) s.skew[query * LDE + query % 16 - key + 64] = next_g[n][e];
+        }
+      if (begun && has_pk) pk.advance(s.pk);
+      lds_barrier();
+      if (jb > first) {
+        read_tile(jb - 1);
+        if (has_pk) {
+          pk.read_rows();
+          pk.read_slots(i0 - 64 * jb);
+        }
+      }
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks) {
+        const int lo = 32 * ks + 8 * g;
+        const F dg = read_columns<T>(s.g + 16 * wave, LDG, lo, lo + 4, c);
 #pragma unroll
         for (int db = 0; db < D / 16; ++db)
-          dq[db] = Op<T>::run(read_columns<T>(s.pk + 16 * db, LD, lo, lo + 4, c), sk, dq[db]);
+          dq[db] = Op<T>::run(read_columns<T>(s.k + 16 * db, LD, lo, lo + 4, c), dg, dq[db]);
       }
+      if (has_pk) {
+#pragma unroll
+        for (int ks = 0; ks < 3; ++ks) {
+          const F sk = read_row<T>(s.skew + (16 * wave + c) * LDE + 32 * ks, g);
+          const int lo = pk.place(16 * wave + 32 * ks + 16 * (g / 2)) + 8 * (g % 2);
+#pragma unroll
+          for (int db = 0; db < D / 16; ++db)
+            dq[db] = Op<T>::run(read_columns<T>(s.pk + 16 * db, LD, lo, lo + 4, c), sk, dq[db]);
+        }
+      }
+      if (jb <= first) break;
     }
   }
   if (i >= p.L) return;
@@ -773,45 +1033,49 @@ __global__ __launch_bounds__(256) void attention_train_position_kernel(Params p,
   const bool pk = p.pos_key != nullptr, pq = p.pos_query != nullptr;
   f32x4_t dpk[2][D / 16] = {}, dpq[2][D / 16] = {};
   const int end = min((part + 1) * dg.tiles, dg.batch * along);
-  for (int u = part * dg.tiles; u < end; ++u) {
-    const int bb = u / along, qt = u % along + (m > 0 ? m : 0), kt = qt - m;
-    const int b = p.b0 + bb, pair = bb * p.nh + hh;
-    const int i0 = 64 * qt, j0 = 64 * kt;
-    // (Every wavefront reads the masks of both blocks.)
-    auto kept_of = [&](int at) {
-      return __ballot(at + lane < p.L &&
-                      (!p.mask || p.mask[static_cast<int64_t>(b) * p.L + at + lane]));
-    };
-    const uint64_t kept_q = kept_of(i0), kept_k = kept_of(j0);
-    if (kept_q == 0 || kept_k == 0) continue;
-    const T* fragments =
-        static_cast<const T*>(p.g) +
-        ((static_cast<int64_t>(pair) * 2 * q32 + j0 / 16 + wave) * q32 + i0 / 32) * kFragment;
-    F f[2];
+  Stage<T, D, 64, 256> next_q, next_k;
+  F next_g[2];
+  // Reads the tile `u` or the first after it that has kept queries and keys.
+  auto read_tile = [&](int u) {
+    for (; u < end; ++u) {
+      const int bb = u / along, qt = u % along + (m > 0 ? m : 0), kt = qt - m;
+      const int b = p.b0 + bb, i0 = 64 * qt, j0 = 64 * kt;
+      // (Every wavefront reads the masks of both blocks.)
+      auto kept_of = [&](int at) {
+        return __ballot(at + lane < p.L &&
+                        (!p.mask || p.mask[static_cast<int64_t>(b) * p.L + at + lane]));
+      };
+      const uint64_t kept_q = kept_of(i0), kept_k = kept_of(j0);
+      if (kept_q == 0 || kept_k == 0) continue;
+      const T* fragments =
+          static_cast<const T*>(p.g) +
+          ((static_cast<int64_t>(bb * p.nh + hh) * 2 * q32 + j0 / 16 + wave) * q32 + i0 / 32) *
+              kFragment +
+          lane * 8;
 #pragma unroll
-    for (int x = 0; x < 2; ++x)
-      f[x] = *reinterpret_cast<const F*>(fragments + x * kFragment + lane * 8);
-    __syncthreads();
-    const T* q = head<T>(p.q, p.sq, b, h);
-    const T* k = head<T>(p.k, p.sk, b, h);
-    if (pk)
-      load_rows<T, D, 64, 256>(s.q, [&](int r) {
-        return (kept_q >> r) & 1 ? q + (i0 + r) * p.sq.l : nullptr;
-      });
-    if (pq)
-      load_rows<T, D, 64, 256>(s.k, [&](int r) {
-        return (kept_k >> r) & 1 ? k + (j0 + r) * p.sk.l : nullptr;
-      });
+      for (int x = 0; x < 2; ++x)
+        next_g[x] = *reinterpret_cast<const F*>(fragments + x * kFragment);
+      if (pk) next_q.load_tokens(Tokens<T, D>(p.q, p.sq, b, h, p.L), i0, kept_q);
+      if (pq) next_k.load_tokens(Tokens<T, D>(p.k, p.sk, b, h, p.L), j0, kept_k);
+      break;
+    }
+    return u;
+  };
+  for (int u = read_tile(part * dg.tiles); u < end;) {
+    lds_barrier();
+    if (pk) next_q.store(s.q);
+    if (pq) next_k.store(s.k);
     const int key = 16 * wave + c;
 #pragma unroll
     for (int x = 0; x < 2; ++x)
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         const int query = 32 * x + query_of(g, e), place = 64 + query - key;
-        if (pk) s.by_query[place * LDX + query] = f[x][e];
-        if (pq) s.by_key[place * LDX + key] = f[x][e];
+        if (pk) s.by_query[place * LDX + query] = next_g[x][e];
+        if (pq) s.by_key[place * LDX + key] = next_g[x][e];
       }
-    __syncthreads();
+    lds_barrier();
+    u = read_tile(u + 1);
     // Blocks of 16 places `wave` and `wave` + 4; those that a step of 32 queries or keys does not
     // reach are left out.
 #pragma unroll
@@ -903,23 +1167,28 @@ __global__ __launch_bounds__(256) void attention_train_slot_kernel(
 
 // ---- host -------------------------------------------------------------------------------------
 
+// What fits 160 KB of LDS.
 template <typename T, int D>
-constexpr int kWaves16 = sizeof(T) == 4 && D == 128 ? 2 : 4;  // what fits 160 KB of LDS
-template <typename T, int D>
-constexpr int kQueries = sizeof(T) == 4 || D == 128 ? 32 : 64;
+struct Sizes {
+  static constexpr bool kWord = sizeof(T) == 4;
+  static constexpr int kFwdWaves = !kWord ? (D == 128 ? 4 : 8) : D == 32 ? 8 : D == 64 ? 4 : 2;
+  static constexpr int kFwdKeys = kWord && D == 128 ? 32 : 64;
+  static constexpr int kKeyWaves = !kWord || D == 32 ? 8 : D == 64 ? 4 : 2;
+  static constexpr int kKeyQueries = kWord || D == 128 ? 32 : 64;
+};
 
 int hip_code(hipError_t e) { return static_cast<int>(e); }
 
 template <typename T, int D>
 int launch_forward(const Params& p, hipStream_t stream) {
-  constexpr int NW = kWaves16<T, D>;
-  using Y = FwdLayout<T, D, NW>;
+  constexpr int NW = Sizes<T, D>::kFwdWaves, BK = Sizes<T, D>::kFwdKeys;
+  using Y = FwdLayout<T, D, NW, BK>;
   static_assert(sizeof(Y) <= 160 * 1024, "LDS");
-  const int64_t blocks = static_cast<int64_t>((p.L + Y::BT - 1) / Y::BT) * p.B * p.H;
+  const int64_t blocks = static_cast<int64_t>((p.L + Y::BQ - 1) / Y::BQ) * p.B * p.H;
   if (blocks > kMaxBlocks256) return DFLASH_ERR_TOO_LARGE;
-  hipError_t e = ensure_dynamic_lds<&attention_train_fwd_kernel<T, D, NW>>(sizeof(Y));
+  hipError_t e = ensure_dynamic_lds<&attention_train_fwd_kernel<T, D, NW, BK>>(sizeof(Y));
   if (e != hipSuccess) return hip_code(e);
-  hipLaunchKernelGGL((attention_train_fwd_kernel<T, D, NW>),
+  hipLaunchKernelGGL((attention_train_fwd_kernel<T, D, NW, BK>),
                      dim3(static_cast<uint32_t>(blocks), p.mask ? 2 : 1), dim3(64 * NW), sizeof(Y),
                      stream, p);
   return hip_code(hipGetLastError());
@@ -960,7 +1229,7 @@ Plan make_plan(int B, int H, int L, int S, int D, int esize) {
 template <typename T, int D>
 int launch_backward(Params p, const void* out, void* dpos_key, void* dpos_query, char* workspace,
                     hipStream_t stream) {
-  constexpr int NW = kWaves16<T, D>, BQ = kQueries<T, D>;
+  constexpr int NW = Sizes<T, D>::kKeyWaves, BQ = Sizes<T, D>::kKeyQueries;
   using YK = KeyLayout<T, D, NW, BQ>;
   using YQ = QueryLayout<T, D>;
   using YP = PositionLayout<T, D>;
@@ -991,7 +1260,7 @@ int launch_backward(Params p, const void* out, void* dpos_key, void* dpos_query,
       p.nh = p.H - h0 < plan.heads ? p.H - h0 : plan.heads;
       const int pairs = p.nb * p.nh;
       hipLaunchKernelGGL((attention_train_key_kernel<T, D, NW, BQ>),
-                         dim3(pairs * plan.blocks * (64 / YK::BK)), dim3(64 * NW), sizeof(YK),
+                         dim3(pairs * ((64 * plan.blocks + YK::BK - 1) / YK::BK)), dim3(64 * NW), sizeof(YK),
                          stream, p);
       hipLaunchKernelGGL((attention_train_query_kernel<T, D>), dim3(pairs * plan.blocks), dim3(256),
                          sizeof(YQ), stream, p);
@@ -1047,6 +1316,17 @@ int make_params(const dflash_attention_train* a, Params& p) {
   for (const void* t : tensors)
     if (off(t, 16)) return DFLASH_ERR_ALIGN;
   if (every * esize % 16 != 0 || off(a->delta_to_slot, 4)) return DFLASH_ERR_ALIGN;
+  // A head's rows are read through 31-bit byte offsets.
+  auto spans = [&](int64_t rows, int64_t stride) {
+    return stride < 0 || stride > INT32_MAX ||
+           ((rows - 1) * stride + a->D) * esize >= int64_t{1} << 31;
+  };
+  for (const int64_t* x : strides)
+    if (spans(a->L, x[2])) return DFLASH_ERR_TOO_LARGE;
+  if ((a->pos_key && spans(a->S, a->pos_key_strides[1])) ||
+      (a->pos_query && spans(a->S, a->pos_query_strides[1])) ||
+      spans(a->L, static_cast<int64_t>(a->H) * a->D))
+    return DFLASH_ERR_TOO_LARGE;
   p = Params{};
   p.q = a->query;
   p.k = a->key;
