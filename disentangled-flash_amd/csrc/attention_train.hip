@@ -23,9 +23,9 @@
 // G is kept in fragments: 16 keys x 32 queries are 512 elements in the order in which the
 // lanes of a wavefront hold them, so that they are written and read 16 bytes a lane.
 //
-// Padded rows.  Rows of K (and of V in the forward pass) at padded keys and rows of Q at padded
-// queries are taken as 0 in every product, so that whatever they hold, NaN too, reaches no
-// kept row; padded queries, whose probabilities are 1/L, have blocks of their own forward.
+// Padded rows.  Rows of K at padded keys and of Q at padded queries are taken as 0 in every product,
+// and so is what is not finite in V at padded keys, so that whatever they hold, NaN too,
+// reaches no kept row.
 
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -75,14 +75,29 @@ struct Params {
 
 // ---- operands -------------------------------------------------------------------------
 
+// One step is 32 deep, of eight elements a lane; a half step is 16 deep, of four.
 template <typename T>
 struct Op {
   using frag = typename Mma<T>::frag;
+  using half = Quad<T>;
   __device__ static f32x4_t run(frag a, frag b, f32x4_t c) { return Mma<T>::run(a, b, c); }
+  // (The 32-deep instruction beside zeros: the 16-deep one, on the accumulators of a 32-deep one
+  // two instructions before, left half of them without the older sum.)
+  __device__ static f32x4_t run_half(half a, half b, f32x4_t c) {
+    const half none{};
+    return run(__builtin_shufflevector(a, none, 0, 1, 2, 3, 4, 5, 6, 7),
+               __builtin_shufflevector(b, none, 0, 1, 2, 3, 4, 5, 6, 7), c);
+  }
 };
 template <>
 struct Op<float> {
   using frag = f32x8_t;
+  using half = Quad<float>;
+  __device__ static f32x4_t run_half(half a, half b, f32x4_t c) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[e], b[e], c, 0, 0, 0);
+    return c;
+  }
   __device__ static f32x4_t run(frag a, frag b, f32x4_t c) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[e], b[e], c, 0, 0, 0);
@@ -123,6 +138,28 @@ __device__ inline typename Op<T>::frag read_columns(const T* p, int ld, int lo, 
     return __builtin_bit_cast(typename Op<T>::frag, u32x4_t{x[0], x[1], y[0], y[1]});
   }
 }
+
+// Lane (c, g): column c of the 16 at `p` of rows `lo` + 0..3.
+template <typename T>
+__device__ inline typename Op<T>::half read_columns_half(const T* p, int ld, int lo, int c) {
+  if constexpr (sizeof(T) == 4) {
+    Quad<float> f;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) f[e] = p[(lo + e) * ld + c];
+    return f;
+  } else {
+    const T* a = p + (lo + (c >> 2)) * ld + 4 * (c & 3);
+    return __builtin_bit_cast(typename Op<T>::half,
+                              __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4_t*)a));
+  }
+}
+
+// Scores by delta, scaled, in LDS.  Beside 16-bit inputs they are fp16: off by at most half a step, 2^-12
+// of their size, which moves a probability by 2^-12 |score| of itself where its rounding as an operand
+// moves it by 2^-12 (fp16) or 2^-9 (bf16).  In fp32 their buffers let one workgroup of four
+// wavefronts run on a CU, as fp16 two.
+template <typename T>
+using Score = std::conditional_t<sizeof(T) == 4, float, _Float16>;
 
 // Eight values of the accumulators of two blocks of 16 rows as an operand: element e < 4 is row
 // 4g + e of the first, e >= 4 row 4g + e - 4 of the second.
@@ -210,6 +247,19 @@ struct Stage {
     load(tokens.memory, [&](int, int r) {
       return r < ROWS && (wanted >> (r & 63)) & 1 ? (first + r) * tokens.stride : kNoRow;
     });
+  }
+  // Infinities and NaN in the rows whose bit of `suspect` is 1 become 0.
+  __device__ void make_finite(uint64_t suspect) {
+    typedef T Elements __attribute__((ext_vector_type(16 / sizeof(T))));
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      if (!((suspect >> (row(n) & 63)) & 1)) continue;
+      Elements x = __builtin_bit_cast(Elements, v[n]);
+#pragma unroll
+      for (int e = 0; e < kPer; ++e)
+        if (!(fabsf(static_cast<float>(x[e])) < INFINITY)) x[e] = static_cast<T>(0.0f);
+      v[n] = __builtin_bit_cast(u32x4_t, x);
+    }
   }
   // Row r goes to row place(r) of the tile.
   template <typename Place>
@@ -317,6 +367,19 @@ __device__ inline void kept_range(const uint64_t* words, int from, int to, int* 
   *last = to - 1;
 }
 
+// x[n][r] where bit 16 n + r is 1, else 0 (by its bits: one sign-extended field and one AND).
+template <int N>
+__device__ inline void drop(f32x4_t (&x)[N], uint64_t kept) {
+#pragma unroll
+  for (int n = 0; n < N; ++n)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const uint32_t word = static_cast<uint32_t>(kept >> (n / 2 * 32));
+      const int mask = __builtin_amdgcn_sbfe(static_cast<int>(word), n % 2 * 16 + r, 1);
+      x[n][r] = __builtin_bit_cast(float, __builtin_bit_cast(int, static_cast<float>(x[n][r])) & mask);
+    }
+}
+
 // ---- dropped places ---------------------------------------------------------------------
 
 // Bit j of row (b, h, i): the probability is dropped.  The element's place in the generator is its
@@ -344,43 +407,46 @@ __global__ __launch_bounds__(256) void dropped_bits_kernel(uint8_t* bits, int64_
 // A workgroup of NW wavefronts takes 16 NW queries and walks the keys in tiles of BK, the last
 // first (so that its windows move up).  Scores are computed transposed (a lane holds one query
 // and four keys of a block), so that the probabilities are the operand of O^T += V^T R^T as they are.
+// Padded queries have the score 0 for every key; only for them are the tiles without kept keys
+// walked.  Of V at padded keys, which a kept query multiplies by 0, what is not finite is taken as 0.
 template <typename T, int D, int NW, int BK>
 struct FwdLayout {
   static constexpr int BQ = 16 * NW, W = BQ + BK, LDC = BK + 20, LDP = BQ + 20;
   static constexpr int LD = kLd<T, D>;
   T k[BK * LD], v[BK * LD], pk[W * LD], pq[W * LD];
-  float c2p[BQ * LDC], p2c[BK * LDP];
+  Score<T> c2p[BQ * LDC], p2c[BK * LDP];
   uint64_t kept[kWords];
 };
 
 template <typename T, int D, int NW, int BK>
-__global__ __launch_bounds__(64 * NW) void attention_train_fwd_kernel(Params p) {
+__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(sizeof(T) == 2 ? 2 : 1)))
+void attention_train_fwd_kernel(Params p) {
   using Y = FwdLayout<T, D, NW, BK>;
   using F = typename Op<T>::frag;
   constexpr int BQ = Y::BQ, LD = Y::LD, LDC = Y::LDC, LDP = Y::LDP, NT = 64 * NW, KB = BK / 16;
+  constexpr uint64_t kBlock = BK == 64 ? ~uint64_t{0} : (uint64_t{1} << (BK % 64)) - 1;
   extern __shared__ __align__(16) unsigned char memory[];
   Y& s = *reinterpret_cast<Y*>(memory);
   const int blocks = (p.L + BQ - 1) / BQ;
   const int at = xcd_logical_block(blockIdx.x, gridDim.x);
   const int bh = at / blocks, i0 = at % blocks * BQ;
   const int b = bh / p.H, h = bh % p.H;
-  const bool uniform = blockIdx.y == 1;  // the block's padded queries, otherwise its kept ones
   const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, c = lane % 16, g = lane / 16;
   const int i = i0 + 16 * wave + c;
 
   read_mask(s.kept, p.mask, b, p.L);
   const int words = (p.L + 63) / 64;
-  bool any = false;
+  bool any_kept = false, any_padded = false;
   for (int at2 = i0; at2 < i0 + BQ && at2 < p.L; at2 += 16) {
-    const uint64_t kept = kept_from(s.kept, at2, p.L), inside = tokens_from(at2, p.L);
-    any |= ((uniform ? inside & ~kept : kept) & 0xFFFF) != 0;
+    const uint64_t kept = kept_from(s.kept, at2, p.L);
+    any_kept |= (kept & 0xFFFF) != 0;
+    any_padded |= (tokens_from(at2, p.L) & ~kept & 0xFFFF) != 0;
   }
-  int first = 0, last = words - 1;
-  if (!uniform) kept_range(s.kept, 0, words, &first, &last);
-  if (!any) return;
+  int first = 0, last = -1;  // blocks of 64 keys that are scored
+  if (any_kept) kept_range(s.kept, 0, words, &first, &last);
 
   const Tokens<T, D> q(p.q, p.sq, b, h, p.L), k(p.k, p.sk, b, h, p.L), v(p.v, p.sv, b, h, p.L);
-  const bool has_pk = p.pos_key && !uniform, has_pq = p.pos_query && !uniform;
+  const bool has_pk = p.pos_key, has_pq = p.pos_query;
   Window<T, D, Y::W, BK, NT> pk(static_cast<const T*>(p.pos_key) + h * p.pk_h, p.pk_s, p.lut, p.L,
                                 p.S);
   Window<T, D, Y::W, BK, NT> pq(static_cast<const T*>(p.pos_query) + h * p.pq_h, p.pq_s, p.lut,
@@ -399,53 +465,108 @@ __global__ __launch_bounds__(64 * NW) void attention_train_fwd_kernel(Params p) 
   const __amdgpu_buffer_rsrc_t bits = resource(
       p.bits ? p.bits + static_cast<int64_t>(bh) * p.L * p.bit_row : nullptr,
       p.bits ? p.L * p.bit_row : 0);
+  const uint32_t bits_at = i < p.L ? i * static_cast<uint32_t>(p.bit_row) : kNoRow;
 
-  auto taken_of = [&](int j0) {
-    constexpr uint64_t kBlock = BK == 64 ? ~uint64_t{0} : (uint64_t{1} << (BK % 64)) - 1;
-    return (uniform ? tokens_from(j0, p.L) : kept_from(s.kept, j0, p.L)) & kBlock;
-  };
   Stage<T, D, BK, NT> next_k, next_v;
-  auto read_tile = [&](int j0) {
-    const uint64_t taken = taken_of(j0);
-    next_v.load_tokens(v, j0, taken);
-    if (!uniform) next_k.load_tokens(k, j0, taken);
+  u32x2_t next_word;
+  // V of padded keys is needed where a query is padded.
+  auto read_v = [&](int j0) {
+    next_word = __builtin_amdgcn_raw_buffer_load_b64(bits, bits_at + j0 / 64 * 8, 0, 0);
+    next_v.load_tokens(v, j0,
+                       (any_padded ? tokens_from(j0, p.L) : kept_from(s.kept, j0, p.L)) & kBlock);
+  };
+  auto store_v = [&](int j0) {
+    const uint64_t padded = tokens_from(j0, p.L) & ~kept_from(s.kept, j0, p.L) & kBlock;
+    if (any_padded && padded) next_v.make_finite(padded);
+    next_v.store(s.v);
+  };
+  // The softmax of the scores x[kb][r] of key j0 + 16 kb + 4g + r so far, and the product with V.
+  auto add_tile = [&](f32x4_t (&x)[KB], int j0, u32x2_t word) {
+    const uint64_t taken =
+        (mine ? kept_from(s.kept, j0, p.L) : tokens_from(j0, p.L)) & kBlock;
+    if (!__all(taken == kBlock)) {
+      const uint64_t lane_taken = taken >> (4 * g);
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          x[kb][r] = (lane_taken >> (16 * kb + r)) & 1 ? x[kb][r] : -INFINITY;
+    }
+    float high = x[0][0];
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) high = fmaxf(high, x[kb][r]);
+    high = fmaxf(high, __shfl_xor(high, 16));
+    high = fmaxf(high, __shfl_xor(high, 32));
+    high = fmaxf(high, top);
+    const float base = high == -INFINITY ? 0.0f : high;  // (no key is taken so far)
+    const float shrink = __builtin_amdgcn_exp2f(top - base);
+    top = high;
+    sum *= shrink;
+#pragma unroll
+    for (int db = 0; db < D / 16; ++db) o[db] *= shrink;
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        x[kb][r] = __builtin_amdgcn_exp2f(x[kb][r] - base);
+        sum += x[kb][r];
+      }
+    if (p.bits) {
+      const uint64_t kept = ~((static_cast<uint64_t>(word[1]) << 32 | word[0]) >> (j0 % 64));
+      drop<KB>(x, kept >> (4 * g));
+    }
+    // (Rounded to T here, as the operand of the product: off by half a step of each probability.)
+#pragma unroll
+    for (int ks = 0; ks < KB / 2; ++ks) {
+      const F r = pack<T>(x[2 * ks], x[2 * ks + 1]);
+#pragma unroll
+      for (int db = 0; db < D / 16; ++db)
+        o[db] = Op<T>::run(
+            read_columns<T>(s.v + 16 * db, LD, 32 * ks + 4 * g, 32 * ks + 16 + 4 * g, c), r,
+            o[db]);
+    }
   };
 
-  const int stop = first * 64;
-  int j0 = last * 64 + 64 - BK;
-  read_tile(j0);
-  if (has_pk) {
-    pk.fill(s.pk, i0 - j0 - BK);
-    pk.read_slots(i0 - j0 - BK);
-  }
-  if (has_pq) {
-    pq.fill(s.pq, i0 - j0 - BK);
-    pq.read_slots(i0 - j0 - BK);
-  }
-  for (bool begun = false;; j0 -= BK, begun = true) {
-    lds_barrier();
-    next_v.store(s.v);
-    if (!uniform) next_k.store(s.k);
-    if (begun && has_pk) pk.advance(s.pk);
-    if (begun && has_pq) pq.advance(s.pq);
-    lds_barrier();
-    const uint64_t taken = taken_of(j0);
-    const u32x2_t word = __builtin_amdgcn_raw_buffer_load_b64(
-        bits, i < p.L ? i * static_cast<uint32_t>(p.bit_row) + j0 / 64 * 8 : kNoRow, 0, 0);
-    if (j0 > stop) {
-      read_tile(j0 - BK);
-      if (has_pk) {
-        pk.read_rows();
-        pk.read_slots(i0 - j0);
-      }
-      if (has_pq) {
-        pq.read_rows();
-        pq.read_slots(i0 - j0);
-      }
+  // The scored tiles.
+  if (first <= last) {
+    const int stop = first * 64;
+    int j0 = last * 64 + 64 - BK;
+    const bool wave_kept = __any(mine);
+    auto read_tile = [&](int j) {
+      read_v(j);
+      next_k.load_tokens(k, j, kept_from(s.kept, j, p.L) & kBlock);
+    };
+    read_tile(j0);
+    if (has_pk) {
+      pk.fill(s.pk, i0 - j0 - BK);
+      pk.read_slots(i0 - j0 - BK);
     }
+    if (has_pq) {
+      pq.fill(s.pq, i0 - j0 - BK);
+      pq.read_slots(i0 - j0 - BK);
+    }
+    for (bool begun = false;; j0 -= BK, begun = true) {
+      lds_barrier();
+      store_v(j0);
+      next_k.store(s.k);
+      if (begun && has_pk) pk.advance(s.pk);
+      if (begun && has_pq) pq.advance(s.pq);
+      lds_barrier();
+      const u32x2_t word = next_word;
+      if (j0 > stop) {
+        read_tile(j0 - BK);
+        if (has_pk) {
+          pk.read_rows();
+          pk.read_slots(i0 - j0);
+        }
+        if (has_pq) {
+          pq.read_rows();
+          pq.read_slots(i0 - j0);
+        }
+      }
 
-    f32x4_t x[KB] = {};  // x[kb][r]: key j0 + 16 kb + 4g + r
-    if (!uniform) {
       if (has_pq) {
         // Keys of block kb against deltas from i0 - j0 - 16 kb - 16.
 #pragma unroll
@@ -458,87 +579,77 @@ __global__ __launch_bounds__(64 * NW) void attention_train_fwd_kernel(Params p) 
             for (int ks = 0; ks < D / 32; ++ks)
               acc = Op<T>::run(read_row<T>(from + c * LD + 32 * ks, g),
                                read_row<T>(s.k + (16 * kb + c) * LD + 32 * ks, g), acc);
-            *reinterpret_cast<f32x4_t*>(s.p2c + (16 * kb + c) * LDP + 16 * wb + 4 * g) = acc;
+            store4(s.p2c + (16 * kb + c) * LDP + 16 * wb + 4 * g, acc * p.scale_log2);
           }
         }
       }
-      if (has_pk) {
-        // This wavefront's queries against deltas from i0 + 16 wave - j0 - BK.
+      f32x4_t x[KB] = {};
+      if (wave_kept) {
+        if (has_pk) {
+          // This wavefront's queries against deltas from i0 + 16 wave - j0 - BK.
 #pragma unroll
-        for (int wb = 0; wb < KB + 1; ++wb) {
-          const T* from = s.pk + pk.place(16 * wave + 16 * wb) * LD;
-          f32x4_t acc{};
+          for (int wb = 0; wb < KB + 1; ++wb) {
+            const T* from = s.pk + pk.place(16 * wave + 16 * wb) * LD;
+            f32x4_t acc{};
+#pragma unroll
+            for (int ks = 0; ks < D / 32; ++ks)
+              acc = Op<T>::run(read_row<T>(from + c * LD + 32 * ks, g), qf[ks], acc);
+            store4(s.c2p + (16 * wave + c) * LDC + 16 * wb + 4 * g, acc * p.scale_log2);
+          }
+        }
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
           for (int ks = 0; ks < D / 32; ++ks)
-            acc = Op<T>::run(read_row<T>(from + c * LD + 32 * ks, g), qf[ks], acc);
-          *reinterpret_cast<f32x4_t*>(s.c2p + (16 * wave + c) * LDC + 16 * wb + 4 * g) = acc;
+            x[kb] = Op<T>::run(read_row<T>(s.k + (16 * kb + c) * LD + 32 * ks, g), qf[ks], x[kb]);
+      }
+      if (has_pk || has_pq) lds_barrier();
+      if (wave_kept) {
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            x[kb][r] = fmaf(
+                x[kb][r], p.scale_log2,
+                has_pk ? static_cast<float>(
+                             s.c2p[(16 * wave + c) * LDC + BK + c - 16 * kb - 4 * g - r])
+                       : 0.0f);
+        if (has_pq) {
+#pragma unroll
+          for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+              x[kb][r] += static_cast<float>(
+                  s.p2c[(16 * kb + 4 * g + r) * LDP + 16 * wave + 16 + c - 4 * g - r]);
+        }
+        if (!__all(mine)) {
+#pragma unroll
+          for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) x[kb][r] = mine ? x[kb][r] : 0.0f;
         }
       }
-#pragma unroll
-      for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-        for (int ks = 0; ks < D / 32; ++ks)
-          x[kb] = Op<T>::run(read_row<T>(s.k + (16 * kb + c) * LD + 32 * ks, g), qf[ks], x[kb]);
+      add_tile(x, j0, word);
+      if (j0 <= stop) break;
+    }
+  }
+
+  // The tiles that only padded queries see.
+  if (any_padded) {
+    for (int j0 = 0; j0 < p.L; j0 += BK) {
+      if (j0 / 64 >= first && j0 / 64 <= last) continue;
+      read_v(j0);
       lds_barrier();
-      if (has_pk) {
-#pragma unroll
-        for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-          for (int r = 0; r < 4; ++r)
-            x[kb][r] += s.c2p[(16 * wave + c) * LDC + BK + c - 16 * kb - 4 * g - r];
-      }
-      if (has_pq) {
-#pragma unroll
-        for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-          for (int r = 0; r < 4; ++r)
-            x[kb][r] += s.p2c[(16 * kb + 4 * g + r) * LDP + 16 * wave + 16 + c - 4 * g - r];
-      }
+      store_v(j0);
+      lds_barrier();
+      f32x4_t x[KB] = {};
+      add_tile(x, j0, next_word);
     }
-    const uint64_t lane_taken = taken >> (4 * g);
-    float high = -INFINITY;
-#pragma unroll
-    for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        x[kb][r] = (lane_taken >> (16 * kb + r)) & 1 ? x[kb][r] * p.scale_log2 : -INFINITY;
-        high = fmaxf(high, x[kb][r]);
-      }
-    high = fmaxf(high, __shfl_xor(high, 16));
-    high = fmaxf(high, __shfl_xor(high, 32));
-    high = fmaxf(high, top);
-    const float base = high == -INFINITY ? 0.0f : high;  // (no key is taken so far)
-    const float shrink = __builtin_amdgcn_exp2f(top - base);
-    top = high;
-    sum *= shrink;
-#pragma unroll
-    for (int db = 0; db < D / 16; ++db) o[db] *= shrink;
-    const uint64_t dropped =
-        ((static_cast<uint64_t>(word[1]) << 32 | word[0]) >> (j0 % 64)) >> (4 * g);
-#pragma unroll
-    for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const float e = __builtin_amdgcn_exp2f(x[kb][r] - base);
-        sum += e;
-        x[kb][r] = (dropped >> (16 * kb + r)) & 1 ? 0.0f : e;
-      }
-    // (Rounded to T here, as the operand of the product: off by half a step of each probability.)
-#pragma unroll
-    for (int ks = 0; ks < KB / 2; ++ks) {
-      const F r = pack<T>(x[2 * ks], x[2 * ks + 1]);
-#pragma unroll
-      for (int db = 0; db < D / 16; ++db)
-        o[db] = Op<T>::run(
-            read_columns<T>(s.v + 16 * db, LD, 32 * ks + 4 * g, 32 * ks + 16 + 4 * g, c), r,
-            o[db]);
-    }
-    if (j0 <= stop) break;
   }
 
   sum += __shfl_xor(sum, 16);
   sum += __shfl_xor(sum, 32);
-  if (i >= p.L || mine == uniform) return;
+  if (i >= p.L) return;
   const float factor = p.keep_scale / sum;
   T* out = static_cast<T*>(p.out) + ((static_cast<int64_t>(b) * p.L + i) * p.H + h) * D;
 #pragma unroll
@@ -581,15 +692,14 @@ template <typename T, int D, int NW, int BQ>
 struct KeyLayout {
   static constexpr int BK = 16 * NW, WQ = BK + 16, WK = BQ + 16;
   static constexpr int LDC = WQ + 4, LDP = WK + 4;
-  static constexpr int KF = (WK + 31) / 32 * 32, LDF = KF + 16 / static_cast<int>(sizeof(T));
+  static constexpr int LDF = WK + 8;
   static constexpr int LD = kLd<T, D>;
-  // (dK's product reads KF rows of pq from row BK - 16 - 16 wave.)
-  static constexpr int PK = BQ + BK, PQ = BK - 16 + KF;
+  static constexpr int W = BQ + BK;
   static constexpr int kWide = BK < 64 ? 1 : BK / 64;  // words of dropped places a query
   // A wavefront's scores of its keys by delta, and after them G by delta.
-  static constexpr int kScores = 16 * LDP * 4, kSkew = 16 * LDF * static_cast<int>(sizeof(T));
-  T q[BQ * LD], dout[BQ * LD], pk[PK * LD], pq[PQ * LD];
-  float c2p[BQ * LDC];
+  static constexpr int kScores = 16 * LDP * static_cast<int>(sizeof(Score<T>)), kSkew = 16 * LDF * static_cast<int>(sizeof(T));
+  T q[BQ * LD], dout[BQ * LD], pk[W * LD], pq[W * LD];
+  Score<T> c2p[BQ * LDC];
   unsigned char own[NW * (kScores > kSkew ? kScores : kSkew)];
   float lse[BQ], delta[BQ];
   uint64_t dropped[BQ * kWide];
@@ -597,7 +707,8 @@ struct KeyLayout {
 };
 
 template <typename T, int D, int NW, int BQ>
-__global__ __launch_bounds__(64 * NW) void attention_train_key_kernel(Params p) {
+__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(sizeof(T) == 2 ? 2 : 1)))
+void attention_train_key_kernel(Params p) {
   using Y = KeyLayout<T, D, NW, BQ>;
   using F = typename Op<T>::frag;
   constexpr int BK = Y::BK, LD = Y::LD, LDC = Y::LDC, LDP = Y::LDP, LDF = Y::LDF, NT = 64 * NW;
@@ -613,7 +724,7 @@ __global__ __launch_bounds__(64 * NW) void attention_train_key_kernel(Params p) 
   const int64_t bh = static_cast<int64_t>(b) * p.H + h;
   const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, c = lane % 16, g = lane / 16;
   const int j = j0 + 16 * wave + c;
-  float* scores = reinterpret_cast<float*>(s.own + wave * (sizeof(s.own) / NW));
+  Score<T>* scores = reinterpret_cast<Score<T>*>(s.own + wave * (sizeof(s.own) / NW));
   T* skew = reinterpret_cast<T*>(scores);
 
   read_mask(s.kept, p.mask, b, p.L);
@@ -628,9 +739,9 @@ __global__ __launch_bounds__(64 * NW) void attention_train_key_kernel(Params p) 
   const int64_t row = static_cast<int64_t>(p.H) * D;
   const Tokens<T, D> dout(p.dout, Strides{p.L * row, D, row}, b, h, p.L);
   const bool has_pk = p.pos_key, has_pq = p.pos_query;
-  Window<T, D, Y::PK, BQ, NT> pk(static_cast<const T*>(p.pos_key) + h * p.pk_h, p.pk_s, p.lut, p.L,
+  Window<T, D, Y::W, BQ, NT> pk(static_cast<const T*>(p.pos_key) + h * p.pk_h, p.pk_s, p.lut, p.L,
                                  p.S);
-  Window<T, D, Y::PQ, BQ, NT> pq(static_cast<const T*>(p.pos_query) + h * p.pq_h, p.pq_s, p.lut,
+  Window<T, D, Y::W, BQ, NT> pq(static_cast<const T*>(p.pos_query) + h * p.pq_h, p.pq_s, p.lut,
                                  p.L, p.S);
   // Fragments of this pair: [16 keys][32 queries].
   const int q32 = 2 * words;
@@ -663,11 +774,14 @@ __global__ __launch_bounds__(64 * NW) void attention_train_key_kernel(Params p) 
     next_dout.store(s.dout);
     if (threadIdx.x < BQ * kWide) s.dropped[threadIdx.x] = next_dropped;
   };
-  // Place 4g + r of query block qb in the generator's bits, bit c.
+  // Place 4g + r of query block qb in the generator's bits, bit c: all ones where it is kept.
   const uint16_t* dropped16 =
       reinterpret_cast<const uint16_t*>(s.dropped) + j0 % 64 / 16 + wave + 4 * g * 4 * kWide;
-  auto factor_of = [&](int qb, int r) {
-    return (dropped16[(16 * qb + r) * 4 * kWide] >> c) & 1 ? 0.0f : p.keep_scale;
+  auto kept_mask = [&](int qb, int r) {
+    return ~__builtin_amdgcn_sbfe(dropped16[(16 * qb + r) * 4 * kWide], c, 1);
+  };
+  auto masked = [](float x, int mask) {
+    return __builtin_bit_cast(float, __builtin_bit_cast(int, x) & mask);
   };
   // dV += R^T dO of a tile, R as an operand.  (R is rounded to T: off by half a step of each.)
   auto add_dv = [&](const f32x4_t (&x)[QB]) {
@@ -739,7 +853,7 @@ __global__ __launch_bounds__(64 * NW) void attention_train_key_kernel(Params p) 
             for (int ks = 0; ks < D / 32; ++ks)
               acc = Op<T>::run(read_row<T>(from + c * LD + 32 * ks, g),
                                read_row<T>(s.q + (16 * qb + c) * LD + 32 * ks, g), acc);
-            *reinterpret_cast<f32x4_t*>(s.c2p + (16 * qb + c) * LDC + 16 * wb + 4 * g) = acc;
+            store4(s.c2p + (16 * qb + c) * LDC + 16 * wb + 4 * g, acc * p.scale_log2);
           }
         }
       }
@@ -752,7 +866,7 @@ __global__ __launch_bounds__(64 * NW) void attention_train_key_kernel(Params p) 
 #pragma unroll
           for (int ks = 0; ks < D / 32; ++ks)
             acc = Op<T>::run(read_row<T>(from + c * LD + 32 * ks, g), kf[ks], acc);
-          *reinterpret_cast<f32x4_t*>(scores + c * LDP + 16 * wb + 4 * g) = acc;
+          store4(scores + c * LDP + 16 * wb + 4 * g, acc * p.scale_log2);
         }
       }
 #pragma unroll
@@ -762,47 +876,56 @@ __global__ __launch_bounds__(64 * NW) void attention_train_key_kernel(Params p) 
           x[qb] = Op<T>::run(read_row<T>(s.q + (16 * qb + c) * LD + 32 * ks, g), kf[ks], x[qb]);
           y[qb] = Op<T>::run(read_row<T>(s.dout + (16 * qb + c) * LD + 32 * ks, g), vf[ks], y[qb]);
         }
-      lds_barrier();
-      if (has_pk) {
+      if (has_pk) lds_barrier();
 #pragma unroll
-        for (int qb = 0; qb < QB; ++qb)
+      for (int qb = 0; qb < QB; ++qb)
 #pragma unroll
-          for (int r = 0; r < 4; ++r)
-            x[qb][r] += s.c2p[(16 * qb + 4 * g + r) * LDC + 4 * g + r - c - 16 * wave + BK];
-      }
+        for (int r = 0; r < 4; ++r)
+          x[qb][r] = fmaf(
+              x[qb][r], p.scale_log2,
+              has_pk ? static_cast<float>(
+                           s.c2p[(16 * qb + 4 * g + r) * LDC + 4 * g + r - c - 16 * wave + BK])
+                     : 0.0f);
       if (has_pq) {
 #pragma unroll
         for (int qb = 0; qb < QB; ++qb)
 #pragma unroll
           for (int r = 0; r < 4; ++r)
-            x[qb][r] += scores[c * LDP + 16 * qb + 4 * g + r - c + 16];
+            x[qb][r] += static_cast<float>(scores[c * LDP + 16 * qb + 4 * g + r - c + 16]);
       }
-      const uint64_t kept = kept_from(s.kept, i0, p.L) >> (4 * g);
-      const uint64_t inside = tokens_from(i0, p.L) >> (4 * g);
+      // P, and P (M dP - D).
 #pragma unroll
       for (int qb = 0; qb < QB; ++qb) {
         const f32x4_t lse = *reinterpret_cast<const f32x4_t*>(s.lse + 16 * qb + 4 * g);
         const f32x4_t delta = *reinterpret_cast<const f32x4_t*>(s.delta + 16 * qb + 4 * g);
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          const bool live = (kept >> (16 * qb + r)) & 1;
-          const bool padded = ((inside >> (16 * qb + r)) & 1) && !live && j < p.L;
-          const float m = factor_of(qb, r);
-          const bool scored = live && mine;
-          const float prob =
-              scored ? __builtin_amdgcn_exp2f(x[qb][r] * p.scale_log2 - lse[r])
-                     : padded ? even : 0.0f;
-          // (One token has one probability, 1, and no gradient.)
-          y[qb][r] = scored && p.L > 1 ? prob * ((m == 0.0f ? 0.0f : y[qb][r] * m) - delta[r]) : 0.0f;
-          x[qb][r] = prob * m;
+          x[qb][r] = __builtin_amdgcn_exp2f(x[qb][r] - lse[r]);
+          const int mask = kept_mask(qb, r);
+          y[qb][r] = x[qb][r] * fmaf(masked(y[qb][r], mask), p.keep_scale, -delta[r]);
+          x[qb][r] = masked(x[qb][r], mask);
         }
+      }
+      const uint64_t kept = kept_from(s.kept, i0, p.L) & kBlock;
+      // (One token has one probability, 1, and no gradient.)
+      if (kept != kBlock || !__all(mine) || p.L == 1) {
+        const uint64_t live = kept >> (4 * g), inside = tokens_from(i0, p.L) >> (4 * g);
+#pragma unroll
+        for (int qb = 0; qb < QB; ++qb)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const bool scored = ((live >> (16 * qb + r)) & 1) && mine;
+            const bool padded = ((inside & ~live) >> (16 * qb + r)) & 1 && j < p.L;
+            if (!scored) x[qb][r] = padded ? masked(even, kept_mask(qb, r)) : 0.0f;
+            if (!scored || p.L == 1) y[qb][r] = 0.0f;
+          }
       }
       add_dv(x);
       asm volatile("" ::: "memory");  // (`skew` takes the place of `scores`)
       if (has_pq) {
-        // Places outside the band, which holds the 16 - c .. 15 - c + BQ of row c.
+        // Places outside the band, which is 16 - c .. 15 - c + BQ of row c.
         constexpr int kPer = 16 / static_cast<int>(sizeof(T));
-        constexpr int kLow = 16 / kPer, kChunks = kLow + (Y::KF - BQ) / kPer;
+        constexpr int kLow = 16 / kPer, kChunks = 2 * kLow;
         for (int n = lane; n < 16 * kChunks; n += 64) {
           const int chunk = n % kChunks;
           *reinterpret_cast<u32x4_t*>(skew + n / kChunks * LDF +
@@ -831,13 +954,18 @@ __global__ __launch_bounds__(64 * NW) void attention_train_key_kernel(Params p) 
       if (has_pq) {
         asm volatile("" ::: "memory");
 #pragma unroll
-        for (int ks = 0; ks < Y::KF / 32; ++ks) {
+        for (int ks = 0; ks < BQ / 32; ++ks) {
           const F sk = read_row<T>(skew + c * LDF + 32 * ks, g);
           const int lo = pq.place(BK - 16 - 16 * wave + 32 * ks + 16 * (g / 2)) + 8 * (g % 2);
 #pragma unroll
           for (int db = 0; db < D / 16; ++db)
             dk[db] = Op<T>::run(read_columns<T>(s.pq + 16 * db, LD, lo, lo + 4, c), sk, dk[db]);
         }
+        const auto sk = *reinterpret_cast<const Quad<T>*>(skew + c * LDF + BQ + 4 * g);
+        const int lo = pq.place(BK - 16 - 16 * wave + BQ) + 4 * g;
+#pragma unroll
+        for (int db = 0; db < D / 16; ++db)
+          dk[db] = Op<T>::run_half(read_columns_half<T>(s.pq + 16 * db, LD, lo, c), sk, dk[db]);
       }
       if (i0 >= stop) break;
     }
@@ -858,7 +986,7 @@ __global__ __launch_bounds__(64 * NW) void attention_train_key_kernel(Params p) 
     for (int qb = 0; qb < QB; ++qb)
 #pragma unroll
       for (int r = 0; r < 4; ++r)
-        x[qb][r] = (padded >> (16 * qb + 4 * g + r)) & 1 && j < p.L ? even * factor_of(qb, r) : 0.0f;
+        x[qb][r] = (padded >> (16 * qb + 4 * g + r)) & 1 && j < p.L ? masked(even, kept_mask(qb, r)) : 0.0f;
     add_dv(x);
   }
 
@@ -867,7 +995,7 @@ __global__ __launch_bounds__(64 * NW) void attention_train_key_kernel(Params p) 
 #pragma unroll
   for (int db = 0; db < D / 16; ++db) {
     store4(static_cast<T*>(p.dk) + base + 16 * db + 4 * g, dk[db] * p.scale);
-    store4(static_cast<T*>(p.dv) + base + 16 * db + 4 * g, dv[db]);
+    store4(static_cast<T*>(p.dv) + base + 16 * db + 4 * g, dv[db] * p.keep_scale);
   }
 }
 
@@ -875,8 +1003,8 @@ __global__ __launch_bounds__(64 * NW) void attention_train_key_kernel(Params p) 
 
 template <typename T, int D>
 struct QueryLayout {
-  static constexpr int LD = kLd<T, D>, LDG = kLd<T, 64>, LDE = kLd<T, 96>;
-  static constexpr int W = 144;
+  static constexpr int LD = kLd<T, D>, LDG = kLd<T, 64>, LDE = 80 + 8;
+  static constexpr int W = 128;
   T k[64 * LD], pk[W * LD];
   T g[64 * LDG];     // [key][query]
   T skew[64 * LDE];  // [query][delta]
@@ -966,13 +1094,18 @@ __global__ __launch_bounds__(256) void attention_train_query_kernel(Params p) {
       }
       if (has_pk) {
 #pragma unroll
-        for (int ks = 0; ks < 3; ++ks) {
+        for (int ks = 0; ks < 2; ++ks) {
           const F sk = read_row<T>(s.skew + (16 * wave + c) * LDE + 32 * ks, g);
           const int lo = pk.place(16 * wave + 32 * ks + 16 * (g / 2)) + 8 * (g % 2);
 #pragma unroll
           for (int db = 0; db < D / 16; ++db)
             dq[db] = Op<T>::run(read_columns<T>(s.pk + 16 * db, LD, lo, lo + 4, c), sk, dq[db]);
         }
+        const auto sk = *reinterpret_cast<const Quad<T>*>(s.skew + (16 * wave + c) * LDE + 64 + 4 * g);
+        const int lo = pk.place(16 * wave + 64) + 4 * g;
+#pragma unroll
+        for (int db = 0; db < D / 16; ++db)
+          dq[db] = Op<T>::run_half(read_columns_half<T>(s.pk + 16 * db, LD, lo, c), sk, dq[db]);
       }
       if (jb <= first) break;
     }
@@ -1167,13 +1300,13 @@ __global__ __launch_bounds__(256) void attention_train_slot_kernel(
 
 // ---- host -------------------------------------------------------------------------------------
 
-// What fits 160 KB of LDS.
+// Two workgroups a CU (80 KB of LDS each) of 16-bit rows of 32 or 64; one of the others.
 template <typename T, int D>
 struct Sizes {
   static constexpr bool kWord = sizeof(T) == 4;
-  static constexpr int kFwdWaves = !kWord ? (D == 128 ? 4 : 8) : D == 32 ? 8 : D == 64 ? 4 : 2;
-  static constexpr int kFwdKeys = kWord && D == 128 ? 32 : 64;
-  static constexpr int kKeyWaves = !kWord || D == 32 ? 8 : D == 64 ? 4 : 2;
+  static constexpr int kFwdWaves = !kWord ? (D == 128 ? 8 : 4) : D == 32 ? 8 : D == 64 ? 4 : 2;
+  static constexpr int kFwdKeys = D == 128 ? 32 : 64;
+  static constexpr int kKeyWaves = !kWord ? (D == 128 ? 8 : 4) : D == 32 ? 8 : D == 64 ? 4 : 2;
   static constexpr int kKeyQueries = kWord || D == 128 ? 32 : 64;
 };
 
@@ -1189,7 +1322,7 @@ int launch_forward(const Params& p, hipStream_t stream) {
   hipError_t e = ensure_dynamic_lds<&attention_train_fwd_kernel<T, D, NW, BK>>(sizeof(Y));
   if (e != hipSuccess) return hip_code(e);
   hipLaunchKernelGGL((attention_train_fwd_kernel<T, D, NW, BK>),
-                     dim3(static_cast<uint32_t>(blocks), p.mask ? 2 : 1), dim3(64 * NW), sizeof(Y),
+                     dim3(static_cast<uint32_t>(blocks)), dim3(64 * NW), sizeof(Y),
                      stream, p);
   return hip_code(hipGetLastError());
 }
@@ -1296,7 +1429,8 @@ bool off(const void* p, uintptr_t n) { return reinterpret_cast<uintptr_t>(p) % n
 
 int make_params(const dflash_attention_train* a, Params& p) {
   if (!a) return DFLASH_ERR_NULL;
-  if (a->B < 0 || a->H < 1 || a->L < 1 || a->S < 0 || !(a->p >= 0.0 && a->p <= 1.0))
+  if (a->B < 0 || a->H < 1 || a->L < 1 || a->S < 0 || !(a->p >= 0.0 && a->p <= 1.0) ||
+      !(a->scale > 0.0f && a->scale < INFINITY))
     return DFLASH_ERR_SHAPE;
   if (a->D != 32 && a->D != 64 && a->D != 128) return DFLASH_ERR_HEAD_DIM;
   if (a->dtype < DFLASH_DTYPE_FP16 || a->dtype > DFLASH_DTYPE_FP32) return DFLASH_ERR_DTYPE;

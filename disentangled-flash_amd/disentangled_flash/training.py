@@ -298,10 +298,12 @@ def attention(
     are) are read where they lie, others are copied.
     ``mask`` is a bool or uint8 ``[B, L]``, nonzero for tokens that are kept.  A kept query has
     the softmax over the kept keys, whatever the padded places hold; a padded query has ``1 / L``
-    for every key, as in Hugging Face's attention.  ``p``, ``rng`` and ``site`` as in
+    for every key, as in Hugging Face's attention (where a padded key's value is not finite it
+    counts as 0).  ``p``, ``rng`` and ``site`` as in
     :func:`dropout`, on the probabilities ``[B, H, L, L]``.
 
-    Scores and softmax are fp32; the probabilities, and in the backward pass the gradients of
+    Scores and softmax are fp32, but for the relative terms of 16-bit inputs, which are rounded to
+    fp16 after their products; the probabilities, and in the backward pass the gradients of
     the scores, are rounded to the dtype where they are multiplied.  One bit for each probability is kept for the
     backward pass, and no ``[L, L]`` tensor besides; the backward pass takes up to 2 GiB of
     memory for such a tensor at a time.
@@ -319,6 +321,8 @@ def attention(
         if tensor.shape != shape or tensor.dtype != dtype or tensor.get_device() != device:
             raise ValueError(f"{name} must match query: {tuple(shape)} {dtype} on {query.device}, "
                              f"got {tuple(tensor.shape)} {tensor.dtype} on {tensor.device}")
+    if not 0.0 < scale < float("inf"):
+        raise ValueError(f"scale must be positive and finite, got {scale}")
     slots = None
     for name, tensor in (("pos_key", pos_key), ("pos_query", pos_query)):
         if tensor is None:

@@ -9,6 +9,8 @@ off by at most n U sum|t|.
   largest of its scores' errors, a sum of at most L exponentials, and an exponential, a logarithm
   and a product of 2 U each (with the rounding of the base-2 exponent, U of at most 1.45 |s| and of the statistic):
   a probability is off by r = 2 max e_s + (L + 32) U + 4 U (max |s| + log L + 1) of itself.
+  Beside 16-bit inputs the two relative terms are rounded to fp16, scaled: 2^-12 of each in base
+  2, which is 2^-12 of it in base e too, or 2^-25.
 * Probabilities with their dropout factor (R) and score gradients (G) are rounded to the dtype as
   operands: u of each, or half the dtype's smallest subnormal (unnormalised in the forward pass, where
   the largest is 1, so of 1 / sum <= 1).
@@ -98,6 +100,12 @@ def attention(q, k, v, pk, pq, lut, scale, mask=None, mult=None, dout=None):
 
     s = scores(Q, K, PK, PQ)
     e_s = (d + 6) * U * scores(*map(absolute, (Q, K, PK, PQ))).abs()
+    if dtype in (torch.float16, torch.bfloat16):
+        none = torch.zeros_like(K)
+        if PK is not None:
+            e_s = e_s + 2.0 ** -12 * scores(Q, none, PK, None).abs() + 2.0 ** -25
+        if PQ is not None:
+            e_s = e_s + 2.0 ** -12 * scores(torch.zeros_like(Q), K, None, PQ).abs() + 2.0 ** -25
     s = torch.where(pair, s, torch.full_like(s, -1e300))
     s = torch.where(mask[:, None, :, None], s, torch.zeros_like(s))  # padded queries: all equal
     prob = torch.softmax(s, -1)
@@ -112,13 +120,10 @@ def attention(q, k, v, pk, pq, lut, scale, mask=None, mult=None, dout=None):
     sums = (2 * length + 16) * U
     # A padded query takes every key; of a kept one's excluded keys nothing arrives.
     taken = (pair | ~mask[:, None, :, None]).double()
-    finite_v = torch.where(torch.isfinite(V), V, torch.zeros_like(V))
-    whole = (~torch.isfinite(V)).any()
+    # (What is not finite at a padded key counts as 0.)
+    finite_v = torch.where(torch.isfinite(V) | mask[:, None, :, None], V, torch.zeros_like(V))
     out = kept @ finite_v
     e_out = (kept * (r + u + sums)) @ finite_v.abs() + floor * most * (taken @ finite_v.abs())
-    if whole:  # (only padded queries see what padded places hold)
-        bad = (~torch.isfinite(V)).double()
-        out = torch.where((kept * taken) @ bad > 0, torch.full_like(out, float("nan")), out)
     result = {"out": (out.transpose(1, 2),
                       (e_out + rounding(out, dtype)).transpose(1, 2))}
     if dout is None:

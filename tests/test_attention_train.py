@@ -130,6 +130,8 @@ def test_attention_refusals():
             (ValueError, "mask must be", {"mask": mask.float()}),
             (ValueError, "mask must be", {"mask": t(2, 8, 8, dtype=torch.bool)}),
             (ValueError, "mask is on", {"mask": t(2, 8, dtype=torch.bool, device="cpu")}),
+            (ValueError, "scale", {"scale": 0.0}), (ValueError, "scale", {"scale": float("nan")}),
+            (ValueError, "scale", {"scale": -1.0}), (ValueError, "scale", {"scale": float("inf")}),
             (ValueError, "probability", {"p": 1.5}),
             (ValueError, "needs rng", {"rng": None}),
             (ValueError, "int64", {"rng": rng.int()}),
@@ -169,6 +171,7 @@ def test_c_attention_refusals(lib):
         (null, {"query": None}), (null, {"value": None}), (null, {"delta_to_slot": None}),
         (null, {"S": 0}), (shape, {"B": -1}), (shape, {"H": 0}), (shape, {"L": 0}),
         (shape, {"S": -1}), (shape, {"p": 1.1}), (shape, {"p": float("nan")}),
+        (shape, {"scale": 0.0}), (shape, {"scale": float("nan")}), (shape, {"scale": float("inf")}),
         (head_dim, {"D": 48}), (dtype, {"dtype": 3}), (align, {"key": at + 8}),
         (align, {"pos_query": at + 2}), (align, {"delta_to_slot": at + 2}),
         (align, {"query_strides": strides}), (large, {"L": 16385}),
