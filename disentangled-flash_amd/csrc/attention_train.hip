@@ -68,6 +68,7 @@ struct Params {
   void *dq, *dk, *dv;     // [B, L, H, D]
   void* g;                // fragments
   float* partial;         // sums of dPK and dPQ by tile diagonal
+  uint64_t* words;        // [B][ceil(L / 64)]: the mask's bits
   int b0, h0, nb, nh;     // the (batch, head) pairs of this launch
   int B, H, L, S;
   float scale, scale_log2, keep_scale;
@@ -192,6 +193,19 @@ __device__ inline typename Op<T>::frag load_frag(__amdgpu_buffer_rsrc_t memory, 
 }
 
 template <typename T>
+__device__ inline void store_frag(__amdgpu_buffer_rsrc_t memory, uint32_t at,
+                                  typename Op<T>::frag f) {
+  if constexpr (sizeof(T) == 4) {
+    __builtin_amdgcn_raw_buffer_store_b128(
+        __builtin_bit_cast(u32x4_t, f32x4_t{f[0], f[1], f[2], f[3]}), memory, at, 0, 0);
+    __builtin_amdgcn_raw_buffer_store_b128(
+        __builtin_bit_cast(u32x4_t, f32x4_t{f[4], f[5], f[6], f[7]}), memory, at + 16, 0, 0);
+  } else {
+    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4_t, f), memory, at, 0, 0);
+  }
+}
+
+template <typename T>
 __device__ inline void store4(T* p, f32x4_t v) {
   Quad<T> q;
 #pragma unroll
@@ -276,16 +290,20 @@ struct Stage {
 
 // A window: ROWS position rows of successive deltas in LDS.  A step moves it STEP deltas on; the
 // rows form a ring, so that only the new ones are read.  They are read through the table of slots
-// two steps ahead of their use: first the slots, then the rows, then LDS.
+// two steps ahead of their use: first the slots, then the rows, then LDS.  Where the ring is two
+// steps long the loops are written out for both of its positions, PHASE, and every address
+// is a constant (one position at run time cost a quarter of the key kernel's time).
 template <typename T, int D, int ROWS, int STEP, int NT>
 struct Window {
   static_assert(ROWS % 16 == 0 && STEP % 16 == 0 && STEP <= ROWS, "blocks of 16 rows");
+  static_assert(ROWS != 2 * STEP || (STEP & (STEP - 1)) == 0, "a power of two");
   using First = Stage<T, D, ROWS, NT>;
   using Next = Stage<T, D, STEP, NT>;
   __amdgpu_buffer_rsrc_t table, lut;
   uint32_t stride;  // bytes
   int L, S;
-  int ring;  // the first row's place
+  static constexpr bool kTwo = ROWS == 2 * STEP;
+  int ring;  // the first row's place, where there are not two
   int slots[Next::N];
   Next rows;
 
@@ -294,15 +312,13 @@ struct Window {
         lut(resource(lut_, (2 * static_cast<int64_t>(L_) - 1) * 4)),
         stride(static_cast<uint32_t>(row_stride * sizeof(T))), L(L_), S(S_), ring(0) {}
 
+  __device__ bool inside(int delta) const { return delta > -L && delta < L; }
   __device__ int slot_of(int delta) const {
-    const int at = delta + L - 1;
-    const bool inside = at >= 0 && at <= 2 * L - 2;
-    const int slot = static_cast<int>(
-        __builtin_amdgcn_raw_buffer_load_b32(lut, inside ? 4 * at : kNoRow, 0, 0));
-    return inside ? slot : -1;
+    return static_cast<int>(__builtin_amdgcn_raw_buffer_load_b32(
+        lut, inside(delta) ? 4 * (delta + L - 1) : kNoRow, 0, 0));
   }
-  __device__ uint32_t offset_of(int slot) const {
-    return slot >= 0 && slot < S ? slot * stride : kNoRow;
+  __device__ uint32_t offset_of(int slot, int delta) const {
+    return inside(delta) && slot >= 0 && slot < S ? slot * stride : kNoRow;
   }
   // All rows, from the delta `first`.
   __device__ void fill(T* tile, int first) {
@@ -310,29 +326,51 @@ struct Window {
 #pragma unroll
     for (int n = 0; n < First::N; ++n) at[n] = slot_of(first + First::row(n));
     First all;
-    all.load(table, [&](int n, int) { return offset_of(at[n]); });
+    all.load(table, [&](int n, int r) { return offset_of(at[n], first + r); });
     all.store(tile);
     ring = 0;
   }
-  // The slots of the rows that come after those of the window from `first`.
+  // The slots of the rows that come after those of the window from `first`, and then those rows.
+  // (Nothing looks at a slot before: it would be waited for, and all other loads with it.)
   __device__ void read_slots(int first) {
 #pragma unroll
     for (int n = 0; n < Next::N; ++n) slots[n] = slot_of(first + ROWS + Next::row(n));
   }
-  __device__ void read_rows() {
-    rows.load(table, [&](int n, int) { return offset_of(slots[n]); });
+  __device__ void read_rows(int first) {
+    rows.load(table, [&](int n, int r) { return offset_of(slots[n], first + ROWS + r); });
+    asm volatile("" ::: "memory");  // (before slots are read into the same registers)
   }
+  // To the position PHASE.
+  template <int PHASE>
   __device__ void advance(T* tile) {
-    rows.store(tile, [&](int r) { return r + ring < ROWS ? r + ring : r + ring - ROWS; });
-    ring += STEP;
-    if (ring >= ROWS) ring -= ROWS;
+    if constexpr (kTwo) {
+      rows.store(tile, [](int r) { return r + (PHASE ? 0 : STEP); });
+    } else {
+      rows.store(tile, [&](int r) { return r + ring < ROWS ? r + ring : r + ring - ROWS; });
+      ring += STEP;
+      if (ring >= ROWS) ring -= ROWS;
+    }
   }
   // Where row r of the window lies; 16 rows from a multiple of 16 lie together.
+  template <int PHASE>
   __device__ int place(int r) const {
+    if constexpr (kTwo) return PHASE ? r ^ STEP : r;
     const int at = r + ring;
     return at < ROWS ? at : at - ROWS;
   }
 };
+// (r ^ STEP is r + STEP in a ring of 2 STEP rows, STEP a power of two.)
+
+// step(PHASE) until it returns false.
+template <bool TWO, typename Step>
+__device__ inline void alternate(const Step& step) {
+  for (;;) {
+    if (!step(std::integral_constant<int, 0>{})) break;
+    if constexpr (TWO) {
+      if (!step(std::integral_constant<int, 1>{})) break;
+    }
+  }
+}
 
 // Bit j % 64 of words[j / 64]: token j is kept (0 for j >= L).
 __device__ inline void read_mask(uint64_t* words, const uint8_t* mask, int b, int L) {
@@ -418,7 +456,7 @@ struct FwdLayout {
   uint64_t kept[kWords];
 };
 
-template <typename T, int D, int NW, int BK>
+template <typename T, int D, int NW, int BK, bool BOTH>
 __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(sizeof(T) == 2 ? 2 : 1)))
 void attention_train_fwd_kernel(Params p) {
   using Y = FwdLayout<T, D, NW, BK>;
@@ -431,7 +469,8 @@ void attention_train_fwd_kernel(Params p) {
   const int at = xcd_logical_block(blockIdx.x, gridDim.x);
   const int bh = at / blocks, i0 = at % blocks * BQ;
   const int b = bh / p.H, h = bh % p.H;
-  const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, c = lane % 16, g = lane / 16;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+  const int lane = threadIdx.x % 64, c = lane % 16, g = lane / 16;
   const int i = i0 + 16 * wave + c;
 
   read_mask(s.kept, p.mask, b, p.L);
@@ -446,7 +485,7 @@ void attention_train_fwd_kernel(Params p) {
   if (any_kept) kept_range(s.kept, 0, words, &first, &last);
 
   const Tokens<T, D> q(p.q, p.sq, b, h, p.L), k(p.k, p.sk, b, h, p.L), v(p.v, p.sv, b, h, p.L);
-  const bool has_pk = p.pos_key, has_pq = p.pos_query;
+  const bool has_pk = BOTH || p.pos_key, has_pq = BOTH || p.pos_query;
   Window<T, D, Y::W, BK, NT> pk(static_cast<const T*>(p.pos_key) + h * p.pk_h, p.pk_s, p.lut, p.L,
                                 p.S);
   Window<T, D, Y::W, BK, NT> pq(static_cast<const T*>(p.pos_query) + h * p.pq_h, p.pq_s, p.lut,
@@ -547,22 +586,24 @@ void attention_train_fwd_kernel(Params p) {
       pq.fill(s.pq, i0 - j0 - BK);
       pq.read_slots(i0 - j0 - BK);
     }
-    for (bool begun = false;; j0 -= BK, begun = true) {
+    bool begun = false;
+    alternate<decltype(pk)::kTwo>([&](auto phase) {
+      constexpr int kPhase = decltype(phase)::value;
       lds_barrier();
       store_v(j0);
       next_k.store(s.k);
-      if (begun && has_pk) pk.advance(s.pk);
-      if (begun && has_pq) pq.advance(s.pq);
+      if (begun && has_pk) pk.template advance<kPhase>(s.pk);
+      if (begun && has_pq) pq.template advance<kPhase>(s.pq);
       lds_barrier();
       const u32x2_t word = next_word;
       if (j0 > stop) {
         read_tile(j0 - BK);
         if (has_pk) {
-          pk.read_rows();
+          pk.read_rows(i0 - j0 - BK);
           pk.read_slots(i0 - j0);
         }
         if (has_pq) {
-          pq.read_rows();
+          pq.read_rows(i0 - j0 - BK);
           pq.read_slots(i0 - j0);
         }
       }
@@ -573,7 +614,7 @@ void attention_train_fwd_kernel(Params p) {
         for (int n = 0; n < (KB * (NW + 1) + NW - 1) / NW; ++n) {
           const int at2 = n * NW + wave, kb = at2 % KB, wb = at2 / KB;
           if (at2 < KB * (NW + 1)) {
-            const T* from = s.pq + pq.place(BK - 16 - 16 * kb + 16 * wb) * LD;
+            const T* from = s.pq + pq.template place<kPhase>(BK - 16 - 16 * kb + 16 * wb) * LD;
             f32x4_t acc{};
 #pragma unroll
             for (int ks = 0; ks < D / 32; ++ks)
@@ -589,7 +630,7 @@ void attention_train_fwd_kernel(Params p) {
           // This wavefront's queries against deltas from i0 + 16 wave - j0 - BK.
 #pragma unroll
           for (int wb = 0; wb < KB + 1; ++wb) {
-            const T* from = s.pk + pk.place(16 * wave + 16 * wb) * LD;
+            const T* from = s.pk + pk.template place<kPhase>(16 * wave + 16 * wb) * LD;
             f32x4_t acc{};
 #pragma unroll
             for (int ks = 0; ks < D / 32; ++ks)
@@ -630,20 +671,29 @@ void attention_train_fwd_kernel(Params p) {
         }
       }
       add_tile(x, j0, word);
-      if (j0 <= stop) break;
-    }
+      begun = true;
+      j0 -= BK;
+      return j0 >= stop;
+    });
   }
 
   // The tiles that only padded queries see.
   if (any_padded) {
-    for (int j0 = 0; j0 < p.L; j0 += BK) {
-      if (j0 / 64 >= first && j0 / 64 <= last) continue;
-      read_v(j0);
+    auto from = [&](int j0) {
+      return j0 / 64 >= first && j0 / 64 <= last ? (last + 1) * 64 : j0;
+    };
+    int j0 = from(0);
+    if (j0 < p.L) read_v(j0);
+    while (j0 < p.L) {
       lds_barrier();
       store_v(j0);
       lds_barrier();
+      const u32x2_t word = next_word;
+      const int next = from(j0 + BK);
+      if (next < p.L) read_v(next);
       f32x4_t x[KB] = {};
-      add_tile(x, j0, next_word);
+      add_tile(x, j0, word);
+      j0 = next;
     }
   }
 
@@ -695,18 +745,18 @@ struct KeyLayout {
   static constexpr int LDF = WK + 8;
   static constexpr int LD = kLd<T, D>;
   static constexpr int W = BQ + BK;
-  static constexpr int kWide = BK < 64 ? 1 : BK / 64;  // words of dropped places a query
+  static constexpr int kWide = BK < 64 ? 1 : BK / 64;  // words of the generator's bits a query
   // A wavefront's scores of its keys by delta, and after them G by delta.
   static constexpr int kScores = 16 * LDP * static_cast<int>(sizeof(Score<T>)), kSkew = 16 * LDF * static_cast<int>(sizeof(T));
   T q[BQ * LD], dout[BQ * LD], pk[W * LD], pq[W * LD];
   Score<T> c2p[BQ * LDC];
   unsigned char own[NW * (kScores > kSkew ? kScores : kSkew)];
   float lse[BQ], delta[BQ];
-  uint64_t dropped[BQ * kWide];
+  uint16_t places[NW][BQ];  // bit c of a wavefront's row: the place of key c is kept
   uint64_t kept[kWords];
 };
 
-template <typename T, int D, int NW, int BQ>
+template <typename T, int D, int NW, int BQ, bool BOTH>
 __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(sizeof(T) == 2 ? 2 : 1)))
 void attention_train_key_kernel(Params p) {
   using Y = KeyLayout<T, D, NW, BQ>;
@@ -722,12 +772,16 @@ void attention_train_key_kernel(Params p) {
   const int pair = at / blocks, j0 = at % blocks * BK;
   const int b = p.b0 + pair / p.nh, h = p.h0 + pair % p.nh;
   const int64_t bh = static_cast<int64_t>(b) * p.H + h;
-  const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, c = lane % 16, g = lane / 16;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+  const int lane = threadIdx.x % 64, c = lane % 16, g = lane / 16;
   const int j = j0 + 16 * wave + c;
   Score<T>* scores = reinterpret_cast<Score<T>*>(s.own + wave * (sizeof(s.own) / NW));
   T* skew = reinterpret_cast<T*>(scores);
 
   read_mask(s.kept, p.mask, b, p.L);
+  if (h == p.h0 && j0 == 0)
+    for (int n = threadIdx.x; n < words; n += NT)
+      p.words[static_cast<int64_t>(b) * words + n] = s.kept[n];
   const bool mine = j < p.L && bit_of(s.kept, j);
   const float even = 1.0f / static_cast<float>(p.L);
   // The queries' blocks that are scored; none where no key of the block is kept.
@@ -738,16 +792,21 @@ void attention_train_key_kernel(Params p) {
   const Tokens<T, D> q(p.q, p.sq, b, h, p.L), k(p.k, p.sk, b, h, p.L), v(p.v, p.sv, b, h, p.L);
   const int64_t row = static_cast<int64_t>(p.H) * D;
   const Tokens<T, D> dout(p.dout, Strides{p.L * row, D, row}, b, h, p.L);
-  const bool has_pk = p.pos_key, has_pq = p.pos_query;
+  const bool has_pk = BOTH || p.pos_key, has_pq = BOTH || p.pos_query;
   Window<T, D, Y::W, BQ, NT> pk(static_cast<const T*>(p.pos_key) + h * p.pk_h, p.pk_s, p.lut, p.L,
                                  p.S);
   Window<T, D, Y::W, BQ, NT> pq(static_cast<const T*>(p.pos_query) + h * p.pq_h, p.pq_s, p.lut,
                                  p.L, p.S);
   // Fragments of this pair: [16 keys][32 queries].
   const int q32 = 2 * words;
-  T* out_g = static_cast<T*>(p.g) +
-             (static_cast<int64_t>(pair) * (2 * q32) + j0 / 16 + wave) * q32 * kFragment + lane * 8;
-  const bool writes = j0 + 16 * wave < 64 * words;
+  const int64_t pair_bytes = static_cast<int64_t>(2 * q32) * q32 * kFragment * sizeof(T);
+  const __amdgpu_buffer_rsrc_t out_g =
+      resource(static_cast<const char*>(p.g) + pair * pair_bytes, pair_bytes);
+  // (Past the last keys' fragments nothing is written.)
+  const uint32_t g_at =
+      j0 + 16 * wave < 64 * words
+          ? static_cast<uint32_t>(((j0 / 16 + wave) * q32 * kFragment + lane * 8) * sizeof(T))
+          : kNoRow;
 
   F kf[D / 32], vf[D / 32];
 #pragma unroll
@@ -760,25 +819,36 @@ void attention_train_key_kernel(Params p) {
 
   Stage<T, D, BQ, NT> next_q, next_dout;
   float next_lse = 0, next_delta = 0;
-  uint64_t next_dropped = 0;
+  u32x2_t next_dropped{};
   static_assert(BQ * kWide <= NT, "one word of dropped places a thread");
-  const int64_t bit_words = p.bit_row / 8;
+  const __amdgpu_buffer_rsrc_t bits = resource(p.bits ? p.bits + bh * p.L * p.bit_row : nullptr,
+                                               p.bits ? p.L * p.bit_row : 0);
   auto read_rest = [&](int i0) {
     next_dout.load_tokens(dout, i0, tokens_from(i0, p.L));
     const int r = threadIdx.x / kWide, word = j0 / 64 + threadIdx.x % kWide;
-    if (p.bits && r < BQ && i0 + r < p.L && word < words)
-      next_dropped = reinterpret_cast<const uint64_t*>(
-          p.bits)[(bh * p.L + i0 + r) * bit_words + word];
+    next_dropped = __builtin_amdgcn_raw_buffer_load_b64(
+        bits,
+        r < BQ && word < words ? (i0 + r) * static_cast<uint32_t>(p.bit_row) + word * 8 : kNoRow, 0,
+        0);
   };
   auto store_rest = [&]() {
     next_dout.store(s.dout);
-    if (threadIdx.x < BQ * kWide) s.dropped[threadIdx.x] = next_dropped;
+    const int r = threadIdx.x / kWide, word = threadIdx.x % kWide;
+    if (r < BQ) {
+      uint64_t kept = ~(static_cast<uint64_t>(next_dropped[1]) << 32 | next_dropped[0]);
+      if (NW < 4) kept >>= j0 % 64;
+#pragma unroll
+      for (int n = 0; n < (NW < 4 ? NW : 4); ++n)
+        s.places[4 * word + n][r] = static_cast<uint16_t>(kept >> (16 * n));
+    }
   };
-  // Place 4g + r of query block qb in the generator's bits, bit c: all ones where it is kept.
-  const uint16_t* dropped16 =
-      reinterpret_cast<const uint16_t*>(s.dropped) + j0 % 64 / 16 + wave + 4 * g * 4 * kWide;
-  auto kept_mask = [&](int qb, int r) {
-    return ~__builtin_amdgcn_sbfe(dropped16[(16 * qb + r) * 4 * kWide], c, 1);
+  // Query 4g + r of block qb and this lane's key: all ones where the place is kept.
+  typedef uint32_t Kept __attribute__((ext_vector_type(2)));
+  auto kept_of = [&](int qb) {
+    return *reinterpret_cast<const Kept*>(&s.places[wave][16 * qb + 4 * g]);
+  };
+  auto mask_of = [&](Kept kept, int r) {
+    return __builtin_amdgcn_sbfe(static_cast<int>(kept[r / 2]), c + r % 2 * 16, 1);
   };
   auto masked = [](float x, int mask) {
     return __builtin_bit_cast(float, __builtin_bit_cast(int, x) & mask);
@@ -797,14 +867,14 @@ void attention_train_key_kernel(Params p) {
   };
 
   if (first <= last) {
+    const __amdgpu_buffer_rsrc_t lse = resource(p.lse + bh * p.L, 4 * static_cast<int64_t>(p.L));
+    const __amdgpu_buffer_rsrc_t delta = resource(p.delta + bh * p.L, 4 * static_cast<int64_t>(p.L));
     auto read_tile = [&](int i0) {
       read_rest(i0);
       next_q.load_tokens(q, i0, kept_from(s.kept, i0, p.L) & kBlock);
-      const int i = i0 + threadIdx.x;
-      if (threadIdx.x < BQ && i < p.L) {
-        next_lse = p.lse[bh * p.L + i];
-        next_delta = p.delta[bh * p.L + i];
-      }
+      const uint32_t at2 = threadIdx.x < BQ ? 4 * (i0 + threadIdx.x) : kNoRow;
+      next_lse = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(lse, at2, 0, 0));
+      next_delta = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(delta, at2, 0, 0));
     };
     const int stop = 64 * last + 64 - BQ;
     int i0 = 64 * first;
@@ -817,7 +887,9 @@ void attention_train_key_kernel(Params p) {
       pq.fill(s.pq, i0 - j0 - BK);
       pq.read_slots(i0 - j0 - BK);
     }
-    for (bool begun = false;; i0 += BQ, begun = true) {
+    bool begun = false;
+    alternate<decltype(pk)::kTwo>([&](auto phase) {
+      constexpr int kPhase = decltype(phase)::value;
       lds_barrier();
       store_rest();
       next_q.store(s.q);
@@ -825,17 +897,17 @@ void attention_train_key_kernel(Params p) {
         s.lse[threadIdx.x] = next_lse;
         s.delta[threadIdx.x] = next_delta;
       }
-      if (begun && has_pk) pk.advance(s.pk);
-      if (begun && has_pq) pq.advance(s.pq);
+      if (begun && has_pk) pk.template advance<kPhase>(s.pk);
+      if (begun && has_pq) pq.template advance<kPhase>(s.pq);
       lds_barrier();
       if (i0 < stop) {
         read_tile(i0 + BQ);
         if (has_pk) {
-          pk.read_rows();
+          pk.read_rows(i0 - j0 - BK);
           pk.read_slots(i0 + BQ - j0 - BK);
         }
         if (has_pq) {
-          pq.read_rows();
+          pq.read_rows(i0 - j0 - BK);
           pq.read_slots(i0 + BQ - j0 - BK);
         }
       }
@@ -847,7 +919,7 @@ void attention_train_key_kernel(Params p) {
         for (int n = 0; n < (QB * (NW + 1) + NW - 1) / NW; ++n) {
           const int at2 = n * NW + wave, qb = at2 % QB, wb = at2 / QB;
           if (at2 < QB * (NW + 1)) {
-            const T* from = s.pk + pk.place(16 * qb + 16 * wb) * LD;
+            const T* from = s.pk + pk.template place<kPhase>(16 * qb + 16 * wb) * LD;
             f32x4_t acc{};
 #pragma unroll
             for (int ks = 0; ks < D / 32; ++ks)
@@ -861,7 +933,7 @@ void attention_train_key_kernel(Params p) {
         // This wavefront's keys against deltas from i0 - j0 - 16 wave - 16.
 #pragma unroll
         for (int wb = 0; wb < QB + 1; ++wb) {
-          const T* from = s.pq + pq.place(BK - 16 - 16 * wave + 16 * wb) * LD;
+          const T* from = s.pq + pq.template place<kPhase>(BK - 16 - 16 * wave + 16 * wb) * LD;
           f32x4_t acc{};
 #pragma unroll
           for (int ks = 0; ks < D / 32; ++ks)
@@ -898,10 +970,11 @@ void attention_train_key_kernel(Params p) {
       for (int qb = 0; qb < QB; ++qb) {
         const f32x4_t lse = *reinterpret_cast<const f32x4_t*>(s.lse + 16 * qb + 4 * g);
         const f32x4_t delta = *reinterpret_cast<const f32x4_t*>(s.delta + 16 * qb + 4 * g);
+        const Kept kept = kept_of(qb);
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           x[qb][r] = __builtin_amdgcn_exp2f(x[qb][r] - lse[r]);
-          const int mask = kept_mask(qb, r);
+          const int mask = mask_of(kept, r);
           y[qb][r] = x[qb][r] * fmaf(masked(y[qb][r], mask), p.keep_scale, -delta[r]);
           x[qb][r] = masked(x[qb][r], mask);
         }
@@ -909,16 +982,27 @@ void attention_train_key_kernel(Params p) {
       const uint64_t kept = kept_from(s.kept, i0, p.L) & kBlock;
       // (One token has one probability, 1, and no gradient.)
       if (kept != kBlock || !__all(mine) || p.L == 1) {
-        const uint64_t live = kept >> (4 * g), inside = tokens_from(i0, p.L) >> (4 * g);
+        // By bits, which drops NaN too.
+        const uint64_t inside = tokens_from(i0, p.L);
+        const uint64_t live = mine ? kept >> (4 * g) : 0;
+        const uint64_t padded = j < p.L ? (inside & ~kept) >> (4 * g) : 0;
+        const int graded = p.L > 1 ? -1 : 0;
+        auto field = [](uint64_t bits, int at) {
+          return __builtin_amdgcn_sbfe(static_cast<int>(bits >> (at / 32 * 32)), at % 32, 1);
+        };
 #pragma unroll
-        for (int qb = 0; qb < QB; ++qb)
+        for (int qb = 0; qb < QB; ++qb) {
+          const Kept places = kept_of(qb);
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            const bool scored = ((live >> (16 * qb + r)) & 1) && mine;
-            const bool padded = ((inside & ~live) >> (16 * qb + r)) & 1 && j < p.L;
-            if (!scored) x[qb][r] = padded ? masked(even, kept_mask(qb, r)) : 0.0f;
-            if (!scored || p.L == 1) y[qb][r] = 0.0f;
+            const int scored = field(live, 16 * qb + r);
+            const int uniform = field(padded, 16 * qb + r) & mask_of(places, r);
+            x[qb][r] = __builtin_bit_cast(
+                float, (__builtin_bit_cast(int, static_cast<float>(x[qb][r])) & scored) |
+                           (__builtin_bit_cast(int, even) & uniform));
+            y[qb][r] = masked(y[qb][r], scored & graded);
           }
+        }
       }
       add_dv(x);
       asm volatile("" ::: "memory");  // (`skew` takes the place of `scores`)
@@ -938,8 +1022,8 @@ void attention_train_key_kernel(Params p) {
 #pragma unroll
       for (int ks = 0; ks < QB / 2; ++ks) {
         const F dg = pack<T>(y[2 * ks], y[2 * ks + 1]);
-        if (writes)
-          *reinterpret_cast<F*>(out_g + static_cast<int64_t>(i0 / 32 + ks) * kFragment) = dg;
+        store_frag<T>(out_g, g_at + (i0 / 32 + ks) * static_cast<uint32_t>(kFragment * sizeof(T)),
+                      dg);
 #pragma unroll
         for (int db = 0; db < D / 16; ++db)
           dk[db] = Op<T>::run(
@@ -956,37 +1040,48 @@ void attention_train_key_kernel(Params p) {
 #pragma unroll
         for (int ks = 0; ks < BQ / 32; ++ks) {
           const F sk = read_row<T>(skew + c * LDF + 32 * ks, g);
-          const int lo = pq.place(BK - 16 - 16 * wave + 32 * ks + 16 * (g / 2)) + 8 * (g % 2);
+          const int lo = pq.template place<kPhase>(BK - 16 - 16 * wave + 32 * ks + 16 * (g / 2)) + 8 * (g % 2);
 #pragma unroll
           for (int db = 0; db < D / 16; ++db)
             dk[db] = Op<T>::run(read_columns<T>(s.pq + 16 * db, LD, lo, lo + 4, c), sk, dk[db]);
         }
         const auto sk = *reinterpret_cast<const Quad<T>*>(skew + c * LDF + BQ + 4 * g);
-        const int lo = pq.place(BK - 16 - 16 * wave + BQ) + 4 * g;
+        const int lo = pq.template place<kPhase>(BK - 16 - 16 * wave + BQ) + 4 * g;
 #pragma unroll
         for (int db = 0; db < D / 16; ++db)
           dk[db] = Op<T>::run_half(read_columns_half<T>(s.pq + 16 * db, LD, lo, c), sk, dk[db]);
       }
-      if (i0 >= stop) break;
-    }
+      begun = true;
+      i0 += BQ;
+      return i0 <= stop;
+    });
   }
 
   // Padded queries of the tiles that are not scored: 1 / L for every key.
-  for (int i0 = 0; i0 < p.L; i0 += BQ) {
-    if (i0 / 64 >= first && i0 / 64 <= last) continue;
-    const uint64_t padded =
-        tokens_from(i0, p.L) & ~kept_from(s.kept, i0, p.L) & kBlock;
-    if (padded == 0) continue;
-    read_rest(i0);
+  auto padded_of = [&](int i0) {
+    return tokens_from(i0, p.L) & ~kept_from(s.kept, i0, p.L) & kBlock;
+  };
+  auto from = [&](int i0) {  // the first such tile from i0 on
+    while (i0 < p.L && ((i0 / 64 >= first && i0 / 64 <= last) || padded_of(i0) == 0)) i0 += BQ;
+    return i0;
+  };
+  int i0 = from(0);
+  if (i0 < p.L) read_rest(i0);
+  while (i0 < p.L) {
     lds_barrier();
     store_rest();
     lds_barrier();
+    const uint64_t padded = padded_of(i0) >> (4 * g);
+    i0 = from(i0 + BQ);
+    if (i0 < p.L) read_rest(i0);
     f32x4_t x[QB];
 #pragma unroll
-    for (int qb = 0; qb < QB; ++qb)
+    for (int qb = 0; qb < QB; ++qb) {
+      const Kept kept = kept_of(qb);
 #pragma unroll
       for (int r = 0; r < 4; ++r)
-        x[qb][r] = (padded >> (16 * qb + 4 * g + r)) & 1 && j < p.L ? masked(even, kept_mask(qb, r)) : 0.0f;
+        x[qb][r] = (padded >> (16 * qb + r)) & 1 && j < p.L ? masked(even, mask_of(kept, r)) : 0.0f;
+    }
     add_dv(x);
   }
 
@@ -1025,7 +1120,8 @@ __global__ __launch_bounds__(256) void attention_train_query_kernel(Params p) {
   const int at = xcd_logical_block(blockIdx.x, gridDim.x);
   const int pair = at / blocks, i0 = at % blocks * 64;
   const int b = p.b0 + pair / p.nh, h = p.h0 + pair % p.nh;
-  const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, c = lane % 16, g = lane / 16;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+  const int lane = threadIdx.x % 64, c = lane % 16, g = lane / 16;
   const int i = i0 + 16 * wave + c;
   read_mask(s.kept, p.mask, b, p.L);
   for (int n = threadIdx.x; n < 64 * LDE; n += 256) s.skew[n] = static_cast<T>(0.0f);
@@ -1063,7 +1159,9 @@ __global__ __launch_bounds__(256) void attention_train_query_kernel(Params p) {
       pk.fill(s.pk, i0 - 64 * jb - 64);
       pk.read_slots(i0 - 64 * jb - 64);
     }
-    for (bool begun = false;; --jb, begun = true) {
+    bool begun = false;
+    alternate<decltype(pk)::kTwo>([&](auto phase) {
+      constexpr int kPhase = decltype(phase)::value;
       lds_barrier();
       next_k.store(s.k);
       const int key = 16 * wave + c;
@@ -1075,12 +1173,12 @@ __global__ __launch_bounds__(256) void attention_train_query_kernel(Params p) {
           s.g[key * LDG + query] = next_g[n][e];
           if (has_pk) s.skew[query * LDE + query % 16 - key + 64] = next_g[n][e];
         }
-      if (begun && has_pk) pk.advance(s.pk);
+      if (begun && has_pk) pk.template advance<kPhase>(s.pk);
       lds_barrier();
       if (jb > first) {
         read_tile(jb - 1);
         if (has_pk) {
-          pk.read_rows();
+          pk.read_rows(i0 - 64 * jb - 64);
           pk.read_slots(i0 - 64 * jb);
         }
       }
@@ -1096,19 +1194,20 @@ __global__ __launch_bounds__(256) void attention_train_query_kernel(Params p) {
 #pragma unroll
         for (int ks = 0; ks < 2; ++ks) {
           const F sk = read_row<T>(s.skew + (16 * wave + c) * LDE + 32 * ks, g);
-          const int lo = pk.place(16 * wave + 32 * ks + 16 * (g / 2)) + 8 * (g % 2);
+          const int lo = pk.template place<kPhase>(16 * wave + 32 * ks + 16 * (g / 2)) + 8 * (g % 2);
 #pragma unroll
           for (int db = 0; db < D / 16; ++db)
             dq[db] = Op<T>::run(read_columns<T>(s.pk + 16 * db, LD, lo, lo + 4, c), sk, dq[db]);
         }
         const auto sk = *reinterpret_cast<const Quad<T>*>(s.skew + (16 * wave + c) * LDE + 64 + 4 * g);
-        const int lo = pk.place(16 * wave + 64) + 4 * g;
+        const int lo = pk.template place<kPhase>(16 * wave + 64) + 4 * g;
 #pragma unroll
         for (int db = 0; db < D / 16; ++db)
           dq[db] = Op<T>::run_half(read_columns_half<T>(s.pk + 16 * db, LD, lo, c), sk, dq[db]);
       }
-      if (jb <= first) break;
-    }
+      begun = true;
+      return --jb >= first;
+    });
   }
   if (i >= p.L) return;
   T* out = static_cast<T*>(p.dq) + ((static_cast<int64_t>(b) * p.L + i) * p.H + h) * D;
@@ -1157,7 +1256,8 @@ __global__ __launch_bounds__(256) void attention_train_position_kernel(Params p,
   const int m = Diagonals::nth(n);
   const int along = dg.blocks - (m < 0 ? -m : m);
   const int h = p.h0 + hh;
-  const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, c = lane % 16, g = lane / 16;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+  const int lane = threadIdx.x % 64, c = lane % 16, g = lane / 16;
   for (int x = threadIdx.x; x < 128 * LDX; x += 256) {
     s.by_query[x] = static_cast<T>(0.0f);
     s.by_key[x] = static_cast<T>(0.0f);
@@ -1173,12 +1273,8 @@ __global__ __launch_bounds__(256) void attention_train_position_kernel(Params p,
     for (; u < end; ++u) {
       const int bb = u / along, qt = u % along + (m > 0 ? m : 0), kt = qt - m;
       const int b = p.b0 + bb, i0 = 64 * qt, j0 = 64 * kt;
-      // (Every wavefront reads the masks of both blocks.)
-      auto kept_of = [&](int at) {
-        return __ballot(at + lane < p.L &&
-                        (!p.mask || p.mask[static_cast<int64_t>(b) * p.L + at + lane]));
-      };
-      const uint64_t kept_q = kept_of(i0), kept_k = kept_of(j0);
+      const uint64_t* words = p.words + static_cast<int64_t>(b) * dg.blocks;
+      const uint64_t kept_q = words[qt], kept_k = words[kt];
       if (kept_q == 0 || kept_k == 0) continue;
       const T* fragments =
           static_cast<const T*>(p.g) +
@@ -1248,54 +1344,99 @@ __global__ __launch_bounds__(256) void attention_train_position_kernel(Params p,
 
 // ---- dPK and dPQ by slot --------------------------------------------------------------------
 
-// One workgroup for a slot of a head: the sums of its deltas, each the parts of two diagonals.
+// The parts of a diagonal are added up in the place of its first.  256 threads take 1024 of its
+// 256 D sums.
+__global__ __launch_bounds__(256) void attention_train_parts_kernel(float* partial, int D,
+                                                                    Diagonals dg, int per_head) {
+  const int nth = blockIdx.y;
+  int first = 0;
+  for (int n = 0; n < nth; ++n) first += dg.parts(Diagonals::nth(n));
+  const int parts = dg.parts(Diagonals::nth(nth));
+  const int64_t step = 256 * D;
+  float* at = partial + (static_cast<int64_t>(blockIdx.z) * per_head + first) * step +
+              (blockIdx.x * 256 + threadIdx.x) * 4;
+  f32x4_t sum{};
+#pragma unroll 4
+  for (int n = 0; n < parts; ++n) sum += *reinterpret_cast<const f32x4_t*>(at + n * step);
+  *reinterpret_cast<f32x4_t*>(at) = sum;
+}
+
+// One workgroup for a slot of a head: the sums of its deltas, each of two diagonals.
 template <typename T, int D>
-__global__ __launch_bounds__(256) void attention_train_slot_kernel(
+__global__ __launch_bounds__(512) void attention_train_slot_kernel(
     const float* partial, const int32_t* lut, T* dpos_key, T* dpos_query, float* carry, int first,
     int last, int L, int S, int H, int h0, Diagonals dg, int per_head, float scale) {
-  constexpr int kLanes = D / 4, kGroups = 256 / kLanes;
-  __shared__ f32x4_t sums[2][256];
+  constexpr int kThreads = 512, kLanes = D / 4, kGroups = kThreads / kLanes;
+  constexpr int kSpan = 4096;  // deltas looked through at a time
+  __shared__ f32x4_t sums[2][kThreads];
+  __shared__ int16_t found[kSpan];
+  __shared__ int counts[kSpan / 64], starts[2 * kWords];
   const int slot = blockIdx.x, hh = blockIdx.y;
   const int lane = threadIdx.x % kLanes, group = threadIdx.x / kLanes;
+  const int wave = threadIdx.x / 64, bit = threadIdx.x % 64;
+  // Where the diagonal m = n - (blocks - 1) begins.
+  for (int n = threadIdx.x; n < 2 * dg.blocks - 1; n += kThreads) {
+    const int m = n - (dg.blocks - 1), order = m > 0 ? 2 * m - 1 : -2 * m;
+    int at = 0;
+    for (int x = 0; x < order; ++x) at += dg.parts(Diagonals::nth(x));
+    starts[n] = at;
+  }
   f32x4_t sum[2] = {};
   const float* base = partial + static_cast<int64_t>(hh) * per_head * 256 * D;
-  for (int at = group; at < 2 * L - 1; at += kGroups) {
-    if (lut[at] != slot) continue;
-    const int delta = at - (L - 1);
-    const int lower = delta >= 0 ? delta / 64 : -((63 - delta) / 64), place = delta - 64 * lower;
-    for (int n = 0, offset = 0, found = 0; n < 2 * dg.blocks - 1 && found < 2; ++n) {
-      const int m = Diagonals::nth(n), parts = dg.parts(m);
-      if (m == lower || m == lower + 1) {
-        ++found;
-        const int at2 = m == lower ? 64 + place : place;
-        for (int x = 0; x < parts; ++x) {
-          const float* from = base + static_cast<int64_t>(offset + x) * 256 * D + at2 * D + lane * 4;
-          sum[0] += *reinterpret_cast<const f32x4_t*>(from);
-          sum[1] += *reinterpret_cast<const f32x4_t*>(from + 128 * D);
-        }
+  for (int from = 0; from < 2 * L - 1; from += kSpan) {
+    // The deltas of this slot, in order: counted by 64, then listed.
+    __syncthreads();
+    const int until = min(from + kSpan, 2 * L - 1);
+    for (int n = wave; from + 64 * n < until; n += kThreads / 64) {
+      const int at = from + 64 * n + bit;
+      const uint64_t match = __ballot(at < until && lut[at] == slot);
+      if (bit == 0) counts[n] = __popcll(match);
+    }
+    __syncthreads();
+    int total = 0;
+    for (int n = 0; from + 64 * n < until; ++n) {
+      if (n % (kThreads / 64) == wave && counts[n]) {
+        const int at = from + 64 * n + bit;
+        const uint64_t match = __ballot(at < until && lut[at] == slot);
+        if ((match >> bit) & 1)
+          found[total + __popcll(match & ((uint64_t{1} << bit) - 1))] =
+              static_cast<int16_t>(64 * n + bit);
       }
-      offset += parts;
+      total += counts[n];
+    }
+    __syncthreads();
+#pragma unroll 4
+    for (int n = group; n < total; n += kGroups) {
+      // delta = 64 lower + place: place 64 + place of the diagonal `lower`, `place` of the next.
+      const int up = from + found[n] - (L - 1) + 64 * dg.blocks;
+      const int lower = up / 64 - dg.blocks, place = up % 64;
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        const int m = lower + x;
+        if (m <= -dg.blocks || m >= dg.blocks) continue;
+        const float* at = base + static_cast<int64_t>(starts[m + dg.blocks - 1]) * 256 * D +
+                          (x ? place : 64 + place) * D + lane * 4;
+        sum[0] += *reinterpret_cast<const f32x4_t*>(at);
+        sum[1] += *reinterpret_cast<const f32x4_t*>(at + 128 * D);
+      }
     }
   }
   sums[0][threadIdx.x] = sum[0];
   sums[1][threadIdx.x] = sum[1];
   __syncthreads();
-  if (group != 0) return;
+  if (group >= 2) return;
+  T* out = group ? dpos_query : dpos_key;
+  if (!out) return;
   const int64_t at = (static_cast<int64_t>(slot) * H + h0 + hh) * D + lane * 4;
-#pragma unroll
-  for (int x = 0; x < 2; ++x) {
-    T* out = x ? dpos_query : dpos_key;
-    if (!out) continue;
-    f32x4_t total{};
-    for (int n = 0; n < kGroups; ++n) total += sums[x][n * kLanes + lane];
-    // (Launches over parts of the batch add up in `carry`.)
-    f32x4_t* kept = reinterpret_cast<f32x4_t*>(carry + (x * static_cast<int64_t>(S) * H * D) + at);
-    if (!first) total += *kept;
-    if (last)
-      store4(out + at, total * scale);
-    else
-      *kept = total;
-  }
+  f32x4_t total{};
+  for (int n = 0; n < kGroups; ++n) total += sums[group][n * kLanes + lane];
+  // (Launches over parts of the batch add up in `carry`.)
+  f32x4_t* kept = reinterpret_cast<f32x4_t*>(carry + group * static_cast<int64_t>(S) * H * D + at);
+  if (!first) total += *kept;
+  if (last)
+    store4(out + at, total * scale);
+  else
+    *kept = total;
 }
 
 // ---- host -------------------------------------------------------------------------------------
@@ -1305,25 +1446,24 @@ template <typename T, int D>
 struct Sizes {
   static constexpr bool kWord = sizeof(T) == 4;
   static constexpr int kFwdWaves = !kWord ? (D == 128 ? 8 : 4) : D == 32 ? 8 : D == 64 ? 4 : 2;
-  static constexpr int kFwdKeys = D == 128 ? 32 : 64;
+  static constexpr int kFwdKeys = kWord && D != 128 ? 64 : 32;
   static constexpr int kKeyWaves = !kWord ? (D == 128 ? 8 : 4) : D == 32 ? 8 : D == 64 ? 4 : 2;
-  static constexpr int kKeyQueries = kWord || D == 128 ? 32 : 64;
+  static constexpr int kKeyQueries = 32;
 };
 
 int hip_code(hipError_t e) { return static_cast<int>(e); }
 
-template <typename T, int D>
+template <typename T, int D, bool BOTH>
 int launch_forward(const Params& p, hipStream_t stream) {
   constexpr int NW = Sizes<T, D>::kFwdWaves, BK = Sizes<T, D>::kFwdKeys;
   using Y = FwdLayout<T, D, NW, BK>;
   static_assert(sizeof(Y) <= 160 * 1024, "LDS");
   const int64_t blocks = static_cast<int64_t>((p.L + Y::BQ - 1) / Y::BQ) * p.B * p.H;
   if (blocks > kMaxBlocks256) return DFLASH_ERR_TOO_LARGE;
-  hipError_t e = ensure_dynamic_lds<&attention_train_fwd_kernel<T, D, NW, BK>>(sizeof(Y));
+  hipError_t e = ensure_dynamic_lds<&attention_train_fwd_kernel<T, D, NW, BK, BOTH>>(sizeof(Y));
   if (e != hipSuccess) return hip_code(e);
-  hipLaunchKernelGGL((attention_train_fwd_kernel<T, D, NW, BK>),
-                     dim3(static_cast<uint32_t>(blocks)), dim3(64 * NW), sizeof(Y),
-                     stream, p);
+  hipLaunchKernelGGL((attention_train_fwd_kernel<T, D, NW, BK, BOTH>),
+                     dim3(static_cast<uint32_t>(blocks)), dim3(64 * NW), sizeof(Y), stream, p);
   return hip_code(hipGetLastError());
 }
 
@@ -1331,7 +1471,7 @@ int launch_forward(const Params& p, hipStream_t stream) {
 struct Plan {
   int batch, heads;  // (batch, head) pairs of one launch: all heads, or some of one batch
   int blocks, tiles, per_head;
-  size_t g, partial, carry, delta, total;
+  size_t g, partial, carry, delta, words, total;
 };
 
 constexpr size_t kMostG = size_t{2} << 30;
@@ -1355,11 +1495,12 @@ Plan make_plan(int B, int H, int L, int S, int D, int esize) {
   x.partial = S > 0 ? round_up(static_cast<size_t>(x.heads) * x.per_head * 256 * D * 4) : 0;
   x.carry = S > 0 && x.batch < B ? round_up(static_cast<size_t>(2) * S * H * D * 4) : 0;
   x.delta = round_up(static_cast<size_t>(B) * H * L * 4);
-  x.total = x.g + x.partial + x.carry + x.delta;
+  x.words = round_up(static_cast<size_t>(B) * x.blocks * 8);
+  x.total = x.g + x.partial + x.carry + x.delta + x.words;
   return x;
 }
 
-template <typename T, int D>
+template <typename T, int D, bool BOTH>
 int launch_backward(Params p, const void* out, void* dpos_key, void* dpos_query, char* workspace,
                     hipStream_t stream) {
   constexpr int NW = Sizes<T, D>::kKeyWaves, BQ = Sizes<T, D>::kKeyQueries;
@@ -1374,7 +1515,8 @@ int launch_backward(Params p, const void* out, void* dpos_key, void* dpos_query,
   float* carry = reinterpret_cast<float*>(workspace + plan.g + plan.partial);
   float* delta = reinterpret_cast<float*>(workspace + plan.g + plan.partial + plan.carry);
   p.delta = delta;
-  hipError_t e = ensure_dynamic_lds<&attention_train_key_kernel<T, D, NW, BQ>>(sizeof(YK));
+  p.words = reinterpret_cast<uint64_t*>(workspace + plan.total - plan.words);
+  hipError_t e = ensure_dynamic_lds<&attention_train_key_kernel<T, D, NW, BQ, BOTH>>(sizeof(YK));
   if (e == hipSuccess) e = ensure_dynamic_lds<&attention_train_query_kernel<T, D>>(sizeof(YQ));
   if (e == hipSuccess) e = ensure_dynamic_lds<&attention_train_position_kernel<T, D>>(sizeof(YP));
   if (e != hipSuccess) return hip_code(e);
@@ -1392,7 +1534,7 @@ int launch_backward(Params p, const void* out, void* dpos_key, void* dpos_query,
       p.nb = p.B - b0 < plan.batch ? p.B - b0 : plan.batch;
       p.nh = p.H - h0 < plan.heads ? p.H - h0 : plan.heads;
       const int pairs = p.nb * p.nh;
-      hipLaunchKernelGGL((attention_train_key_kernel<T, D, NW, BQ>),
+      hipLaunchKernelGGL((attention_train_key_kernel<T, D, NW, BQ, BOTH>),
                          dim3(pairs * ((64 * plan.blocks + YK::BK - 1) / YK::BK)), dim3(64 * NW), sizeof(YK),
                          stream, p);
       hipLaunchKernelGGL((attention_train_query_kernel<T, D>), dim3(pairs * plan.blocks), dim3(256),
@@ -1402,7 +1544,9 @@ int launch_backward(Params p, const void* out, void* dpos_key, void* dpos_query,
         const int per_head = dg.total();
         hipLaunchKernelGGL((attention_train_position_kernel<T, D>), dim3(p.nh * per_head), dim3(256),
                            sizeof(YP), stream, p, dg, per_head);
-        hipLaunchKernelGGL((attention_train_slot_kernel<T, D>), dim3(p.S, p.nh), dim3(256), 0,
+        hipLaunchKernelGGL(attention_train_parts_kernel, dim3(D / 4, 2 * dg.blocks - 1, p.nh),
+                           dim3(256), 0, stream, p.partial, D, dg, per_head);
+        hipLaunchKernelGGL((attention_train_slot_kernel<T, D>), dim3(p.S, p.nh), dim3(512), 0,
                            stream, p.partial, p.lut, static_cast<T*>(dpos_key),
                            static_cast<T*>(dpos_query), carry, b0 == 0, b0 + p.nb == p.B, p.L, p.S,
                            p.H, h0, dg, per_head, p.scale);
@@ -1435,7 +1579,7 @@ int make_params(const dflash_attention_train* a, Params& p) {
   if (a->D != 32 && a->D != 64 && a->D != 128) return DFLASH_ERR_HEAD_DIM;
   if (a->dtype < DFLASH_DTYPE_FP16 || a->dtype > DFLASH_DTYPE_FP32) return DFLASH_ERR_DTYPE;
   if (a->L > kMaxLength || static_cast<int64_t>(a->B) * a->H > (1 << 20) ||
-      static_cast<int64_t>(a->S) * a->H >= (1 << 24) || a->H > 65535)
+      static_cast<int64_t>(a->S) * a->H >= (1 << 23) || a->H > 65535)
     return DFLASH_ERR_TOO_LARGE;
   const bool relative = a->pos_key || a->pos_query;
   if (!a->query || !a->key || !a->value || (relative && (!a->delta_to_slot || a->S < 1)))
@@ -1523,7 +1667,10 @@ int dflash_attention_train_fwd(const dflash_attention_train* a, const int64_t* r
   p.out = out;
   p.lse = lse;
   return by_type(a->dtype, a->D, [&](auto t, auto d) {
-    return launch_forward<decltype(t), decltype(d)::value>(p, s);
+    using T = decltype(t);
+    constexpr int D = decltype(d)::value;
+    return p.pos_key && p.pos_query ? launch_forward<T, D, true>(p, s)
+                                    : launch_forward<T, D, false>(p, s);
   });
 }
 
@@ -1556,9 +1703,12 @@ int dflash_attention_train_bwd(const dflash_attention_train* a, const void* out,
   p.dk = dkey;
   p.dv = dvalue;
   return by_type(a->dtype, a->D, [&](auto t, auto d) {
-    return launch_backward<decltype(t), decltype(d)::value>(p, out, dpos_key, dpos_query,
-                                                            static_cast<char*>(workspace),
-                                                            static_cast<hipStream_t>(stream));
+    using T = decltype(t);
+    constexpr int D = decltype(d)::value;
+    const auto call = p.pos_key && p.pos_query ? &launch_backward<T, D, true>
+                                               : &launch_backward<T, D, false>;
+    return call(p, out, dpos_key, dpos_query, static_cast<char*>(workspace),
+                static_cast<hipStream_t>(stream));
   });
 }
 
