@@ -1,0 +1,512 @@
+// Newton-Schulz iterations that bring a matrix's singular values near 1 (the update of the
+// Muon optimiser), for a batch of matrices of one shape.
+//
+//   X = G / (|G|_F + eps);  steps times:  A = X X^T,  B = b A + c A A,  X <- a X + B X
+//
+// on the side on which X has no more rows than columns (a tall G is transposed on its way in and out).
+//
+// Precision.  The products run on fp16 MFMA with fp32 sums.  X is kept in two fp16 parts, hi + lo
+// (22 bits), scaled by 2^8 (its entries are below 1 / sqrt(rows) on average, where fp16 would
+// lose bits); hi is the operand, and both enter a X, which alone carries the small
+// singular values, the ones that grow: with hi alone there a matrix of low rank beside noise is
+// 6e-3 off after five steps, with both 4e-4.  A is rounded to fp16 once, for b A as for A A: were
+// b A taken from its fp32 sums, the two would not cancel near 1 (normal 512 x 2048: 3.1e-3 off
+// against 1.7e-3).  bf16 operands are 1.3e-2 to 5e-2 off.  The result is bf16 (1.7e-3 by itself).
+//
+// One GEMM kernel, three forms.  All operands are zero-padded to whole 128 x 128 tiles in the
+// workspace, so that no access needs a bound.  A and B are symmetric: tiles below the diagonal
+// alone are computed and stored twice.  The loop is the projection GEMM's: slabs of 64 k copied
+// straight into LDS, fragments read a step ahead.  In B X the second operand is X's own rows, k by
+// columns, read with transposing reads, so that no transposed copy of X exists.
+//
+// Bound by the matrix unit and its feeding: 48 of 768 x 768 take MEASURED
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include <type_traits>
+
+#include "device_common.h"
+#include "dflash.h"
+#include "gemm_tile.h"
+#include "training.h"
+
+namespace dflash {
+namespace {
+
+constexpr int kTile = 128;
+constexpr float kScale = 256.0f;  // of X in its fp16 parts
+using Config = Cfg128x128;
+
+enum class Form { kGram, kPolynomial, kUpdate };
+
+typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
+typedef short s4_t __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s4_t lds_s4_t;
+
+struct Matrices {
+  _Float16* hi[2];  // [batch, rows, columns], the steps' in turn
+  _Float16* lo;
+  _Float16 *gram, *poly;  // [batch, rows, rows]
+  int rows, columns;      // padded
+  int batch;
+};
+
+// 16 bytes a lane from byte `off` + `scalar` of a buffer to LDS at `lds` + 16 * lane.
+__device__ inline void copy_to_lds(__amdgpu_buffer_rsrc_t r, uint32_t off, uint32_t scalar,
+                                   uint32_t lds) {
+  asm volatile(
+      "s_mov_b32 m0, %0\n\t"
+      "s_nop 0\n\t"
+      "buffer_load_dwordx4 %1, %2, %3 offen lds"
+      :
+      : "s"(lds), "v"(off), "s"(r), "s"(scalar)
+      : "memory");
+}
+
+// A buffer resource in scalar registers.
+__device__ inline __amdgpu_buffer_rsrc_t scalar_resource(const void* base, uint32_t bytes) {
+  const uint64_t at = reinterpret_cast<uintptr_t>(base);
+  const uint32_t lo = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(at));
+  const uint32_t hi = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(at >> 32));
+  return __builtin_amdgcn_make_buffer_rsrc(
+      reinterpret_cast<void*>(static_cast<uintptr_t>(hi) << 32 | lo), static_cast<short>(0),
+      static_cast<int>(__builtin_amdgcn_readfirstlane(bytes)), 0x00020000);
+}
+
+template <int N>
+__device__ inline void wait_copies() {
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+
+// Chunk (16 bytes) x of row r of a slab of rows of k, 128 columns each, lies at x ^ this: the four
+// rows that 16 lanes of a transposing read touch lie in different banks.
+__device__ inline int k_row_swizzle(int r) { return (r & 3) << 1; }
+
+// ---- |G|_F and the first X ---------------------------------------------------------------
+
+constexpr int kPartials = 256;  // partial sums of a matrix, at most
+
+// Sums of squares in fp64: no overflow and no underflow whatever the elements.
+template <typename T>
+__global__ __launch_bounds__(256) void norm_kernel(const T* g, double* partial, int64_t elements,
+                                                   int64_t block) {
+  __shared__ double sums[4];
+  const T* at = g + blockIdx.y * elements;
+  const int64_t first = blockIdx.x * block, end = min(first + block, elements);
+  double sum = 0;
+#pragma unroll 8
+  for (int64_t n = first + threadIdx.x; n < end; n += 256) {
+    const float x = static_cast<float>(at[n]);
+    sum += static_cast<double>(x) * x;
+  }
+  for (int step = 32; step; step /= 2) sum += __shfl_xor(sum, step);
+  if (threadIdx.x % 64 == 0) sums[threadIdx.x / 64] = sum;
+  __syncthreads();
+  if (threadIdx.x == 0)
+    partial[blockIdx.y * gridDim.x + blockIdx.x] = sums[0] + sums[1] + sums[2] + sums[3];
+}
+
+// A tile of 64 x 64 of X: rows and columns of X are those of G, or the other way round (`tall`).
+template <typename T>
+__global__ __launch_bounds__(256) void start_kernel(const T* g, const double* partial, int partials,
+                                                    Matrices x, int m, int n, int tall, float eps) {
+  __shared__ float tile[64][65];
+  const int b = blockIdx.z, r0 = blockIdx.y * 64, c0 = blockIdx.x * 64;
+  double square = 0;
+  for (int at = 0; at < partials; ++at) square += partial[b * partials + at];
+  const float factor = static_cast<float>(1.0 / (sqrt(square) + static_cast<double>(eps)));
+  // G's rows and columns of this tile.
+  const int gr = tall ? c0 : r0, gc = tall ? r0 : c0;
+  const T* from = g + static_cast<int64_t>(b) * m * n;
+  for (int at = threadIdx.x; at < 4096; at += 256) {
+    const int r = gr + at / 64, c = gc + at % 64;
+    tile[at / 64][at % 64] =
+        r < m && c < n ? static_cast<float>(from[static_cast<int64_t>(r) * n + c]) * factor : 0.0f;
+  }
+  __syncthreads();
+  const int64_t base = (static_cast<int64_t>(b) * x.rows + r0) * x.columns + c0;
+  for (int at = threadIdx.x; at < 2048; at += 256) {
+    const int r = at / 32, c = at % 32 * 2;
+    half2_t hi, lo;
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const float v = (tall ? tile[c + e][r] : tile[r][c + e]) * kScale;
+      hi[e] = static_cast<_Float16>(v);
+      lo[e] = static_cast<_Float16>(v - static_cast<float>(hi[e]));
+    }
+    *reinterpret_cast<half2_t*>(x.hi[0] + base + static_cast<int64_t>(r) * x.columns + c) = hi;
+    *reinterpret_cast<half2_t*>(x.lo + base + static_cast<int64_t>(r) * x.columns + c) = lo;
+  }
+}
+
+// ---- the products ----------------------------------------------------------------------------
+
+struct Step {
+  Matrices x;
+  int from;        // which of hi the step reads; it writes the other
+  float a, b, c;
+  int last;        // write `out` instead of X
+  __bf16* out;     // [batch, m, n]
+  int m, n, tall;  // of G
+};
+
+template <Form FORM>
+__global__ __launch_bounds__(Config::THREADS, Config::WGS) void product_kernel(Step p) {
+  using CF = Config;
+  constexpr int MB = CF::MB, NB = CF::NB, S = CF::STAGES;
+  constexpr bool kSquare = FORM != Form::kUpdate;  // symmetric, second operand by rows of k-runs
+  extern __shared__ __align__(16) unsigned char smem[];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int c = lane & 15, g = lane >> 4;
+  const int wm = wave % CF::WAVES_M, wn = wave / CF::WAVES_M;
+
+  // The tiles of a matrix lie on one XCD.
+  const int tiles_m = p.x.rows / kTile, tiles_n = (kSquare ? p.x.rows : p.x.columns) / kTile;
+  const int each = kSquare ? tiles_m * (tiles_m + 1) / 2 : tiles_m * tiles_n;
+  const int at = xcd_logical_block(blockIdx.x, gridDim.x);
+  const int batch = at / each;
+  int mt, nt;
+  if (kSquare) {  // the lower triangle, row by row
+    int rest = at % each;
+    for (mt = 0; rest > mt; ++mt) rest -= mt + 1;
+    nt = rest;
+  } else {
+    mt = at % each % tiles_m;
+    nt = at % each / tiles_m;
+  }
+  const int K = FORM == Form::kGram ? p.x.columns : p.x.rows;
+  const int64_t square = static_cast<int64_t>(p.x.rows) * p.x.rows;
+  const int64_t whole = static_cast<int64_t>(p.x.rows) * p.x.columns;
+  const _Float16* hi = p.x.hi[p.from] + batch * whole;
+  const _Float16* left = FORM == Form::kGram ? hi
+                         : FORM == Form::kPolynomial ? p.x.gram + batch * square
+                                                     : p.x.poly + batch * square;
+  const _Float16* X = left + static_cast<int64_t>(mt) * kTile * K;
+  const _Float16* W = kSquare ? left + static_cast<int64_t>(nt) * kTile * K : hi + nt * kTile;
+  const uint32_t x_row = static_cast<uint32_t>(K) * 2;
+  const uint32_t w_row_bytes = kSquare ? x_row : static_cast<uint32_t>(p.x.columns) * 2;
+  const int KT = K / kSlabK;
+
+  // Byte offsets of this lane's 16 bytes of each copy.
+  uint32_t xoff[CF::A_LOADS], woff[CF::B_LOADS];
+#pragma unroll
+  for (int j = 0; j < CF::A_LOADS; ++j) {
+    const int r = copy_row<CF>(j, wave, lane);
+    xoff[j] = r * x_row + copy_chunk(r, lane) * 16;
+  }
+#pragma unroll
+  for (int j = 0; j < CF::B_LOADS; ++j) {
+    if (kSquare) {
+      const int r = copy_row<CF>(j, wave, lane);
+      woff[j] = w_row(r) * w_row_bytes + copy_chunk(r, lane) * 16;
+    } else {  // four rows of k of 256 bytes
+      const int r = (j * CF::WAVES + wave) * 4 + (lane >> 4);
+      woff[j] = r * w_row_bytes + ((lane & 15) ^ k_row_swizzle(r)) * 16;
+    }
+  }
+  const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(smem));
+  // Past the last slab the copies fetch nothing (a size of 0), so that every slab has as many.
+  auto copy = [&](int j, int kt, uint32_t stage) {
+    const bool is_x = j < CF::A_LOADS;
+    const int jj = is_x ? j : j - CF::A_LOADS;
+    const uint32_t to = __builtin_amdgcn_readfirstlane(
+        lds0 + stage * CF::SLAB + (is_x ? 0 : CF::A_BYTES) + (jj * CF::WAVES + wave) * 1024);
+    const bool live = kt < KT;
+    if (is_x || kSquare) {
+      const auto memory = scalar_resource(is_x ? X : W, live ? kTile * x_row : 0);
+      copy_to_lds(memory, is_x ? xoff[is_x ? jj : 0] : woff[is_x ? 0 : jj],
+                  __builtin_amdgcn_readfirstlane(live ? kt * kSlabK * 2 : 0), to);
+    } else {  // a resource that begins at the slab's first row
+      const auto memory =
+          scalar_resource(W + static_cast<int64_t>(live ? kt : 0) * kSlabK * p.x.columns,
+                          live ? (kSlabK - 1) * w_row_bytes + kTile * 2 : 0);
+      copy_to_lds(memory, woff[is_x ? 0 : jj], 0, to);
+    }
+  };
+
+  using F = half8_t;
+  const int swz = slab_swizzle(c);
+  const int chunk[2] = {(g ^ swz) * 16, ((4 + g) ^ swz) * 16};
+  const int xrow = (wm * CF::WM + c) * (kSlabK * 2);
+  const int wrow = CF::A_BYTES + (wn * CF::WN + c) * (kSlabK * 2);
+  auto x_frag = [&](uint32_t base, int u, int i) {
+    return *static_cast<const F*>(
+        __builtin_assume_aligned(smem + base + xrow + chunk[u] + i * 16 * kSlabK * 2, 16));
+  };
+  auto w_frag = [&](uint32_t base, int u, int i) {
+    if constexpr (kSquare) {
+      return *static_cast<const F*>(
+          __builtin_assume_aligned(smem + base + wrow + chunk[u] + i * 16 * kSlabK * 2, 16));
+    } else {
+      // Columns 64 wn + 16 i + c of rows 32 u + 8g + 0..3 and + 4..7.
+      const int r = 32 * u + 8 * g + (c >> 2);
+      const int x = ((wn * CF::WN + 16 * i) / 8 + ((c & 3) >> 1)) ^ k_row_swizzle(r);
+      const unsigned char* p0 = smem + base + CF::A_BYTES + r * 256 + x * 16 + (c & 1) * 8;
+      const u32x2_t lo = __builtin_bit_cast(
+          u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4_t*)p0));
+      const u32x2_t up = __builtin_bit_cast(
+          u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4_t*)(p0 + 4 * 256)));
+      return __builtin_bit_cast(F, u32x4_t{lo[0], lo[1], up[0], up[1]});
+    }
+  };
+
+  f32x4_t acc[NB][MB] = {};
+  F xf[2][MB], wf[2][NB];
+#pragma unroll
+  for (int s = 0; s < S; ++s)
+#pragma unroll
+    for (int j = 0; j < CF::LOADS; ++j) copy(j, s, s);
+  wait_copies<(S - 1) * CF::LOADS>();
+  asm volatile("s_barrier" ::: "memory");
+#pragma unroll
+  for (int i = 0; i < NB; ++i) wf[0][i] = w_frag(0, 0, i);
+#pragma unroll
+  for (int i = 0; i < MB; ++i) xf[0][i] = x_frag(0, 0, i);
+
+  constexpr int kMfmas = MB * NB, kReads = MB + NB;
+  auto step = [&](auto parity, auto with_copies, uint32_t base, int kt, uint32_t stage) {
+    constexpr int P = decltype(parity)::value;
+    constexpr bool COPY = decltype(with_copies)::value;
+#pragma unroll
+    for (int q = 0; q < kMfmas; ++q) {
+      __builtin_amdgcn_sched_barrier(0);
+      acc[q % NB][q / NB] =
+          Mma<_Float16>::run(wf[P][q % NB], xf[P][q / NB], acc[q % NB][q / NB]);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int z = 0; z < kReads; ++z)
+        if (z * kMfmas * 3 / 4 / kReads == q) {
+          if (z < NB)
+            wf[P ^ 1][z] = w_frag(base, P ^ 1, z);
+          else
+            xf[P ^ 1][z - NB] = x_frag(base, P ^ 1, z - NB);
+        }
+      if constexpr (COPY) {
+#pragma unroll
+        for (int z = 0; z < CF::LOADS; ++z)
+          if (z * kMfmas * 3 / 4 / CF::LOADS == q) copy(z, kt, stage);
+      }
+    }
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  uint32_t stage = 0;
+  for (int kt = 0; kt < KT; ++kt) {
+    const uint32_t next = stage + 1 == S ? 0 : stage + 1;
+    step(std::integral_constant<int, 0>{}, std::false_type{}, stage * CF::SLAB, 0, 0);
+    wait_copies<(S - 2) * CF::LOADS>();
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    step(std::integral_constant<int, 1>{}, std::true_type{}, next * CF::SLAB, kt + S, stage);
+    stage = next;
+  }
+  wait_copies<0>();  // no copy may land in LDS any more
+
+  if constexpr (kSquare) {
+    // Eight consecutive elements of a row a lane and pair of blocks.
+    _Float16* out = (FORM == Form::kGram ? p.x.gram : p.x.poly) + batch * square;
+    const _Float16* gram = p.x.gram + batch * square;
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    // The mirrored tile, [column][row], rows of 128 + 8.
+    _Float16* mirror = reinterpret_cast<_Float16*>(smem);
+    constexpr int kLd = kTile + 8;
+    static_assert(kTile * kLd * 2 <= CF::LDS, "the mirrored tile");
+#pragma unroll
+    for (int j = 0; j < MB; ++j) {
+      const int row = wm * CF::WM + 16 * j + c;
+#pragma unroll
+      for (int i = 0; i < NB; i += 2) {
+        const int column = wn * CF::WN + 16 * i + 8 * g;
+        const int64_t to = static_cast<int64_t>(mt * kTile + row) * p.x.rows + nt * kTile + column;
+        half8_t v;
+        if constexpr (FORM == Form::kGram) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            v[e] = static_cast<_Float16>(acc[i + e / 4][j][e % 4] * (1.0f / (kScale * kScale)));
+        } else {
+          const half8_t a = *reinterpret_cast<const half8_t*>(gram + to);
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            v[e] = static_cast<_Float16>(p.b * static_cast<float>(a[e]) + p.c * acc[i + e / 4][j][e % 4]);
+        }
+        *reinterpret_cast<half8_t*>(out + to) = v;
+        if (mt != nt) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) mirror[(column + e) * kLd + row] = v[e];
+        }
+      }
+    }
+    if (mt != nt) {
+      __syncthreads();
+      for (int n = threadIdx.x; n < kTile * kTile / 8; n += CF::THREADS) {
+        const int r = n / (kTile / 8), k = n % (kTile / 8) * 8;
+        *reinterpret_cast<u32x4_t*>(out + static_cast<int64_t>(nt * kTile + r) * p.x.rows +
+                                    mt * kTile + k) =
+            *reinterpret_cast<const u32x4_t*>(mirror + r * kLd + k);
+      }
+    }
+  } else {
+    _Float16* next = p.x.hi[p.from ^ 1] + batch * whole;
+    _Float16* lo = p.x.lo + batch * whole;
+    __bf16* out = p.out + static_cast<int64_t>(batch) * p.m * p.n;
+#pragma unroll
+    for (int j = 0; j < MB; ++j) {
+      const int row = mt * kTile + wm * CF::WM + 16 * j + c;
+#pragma unroll
+      for (int i = 0; i < NB; ++i) {
+        const int column = nt * kTile + wn * CF::WN + 16 * i + 4 * g;
+        const int64_t to = static_cast<int64_t>(row) * p.x.columns + column;
+        const Quad<_Float16> h = *reinterpret_cast<const Quad<_Float16>*>(hi + to);
+        const Quad<_Float16> l = *reinterpret_cast<const Quad<_Float16>*>(lo + to);
+        f32x4_t v;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          v[e] = p.a * (static_cast<float>(h[e]) + static_cast<float>(l[e])) + acc[i][j][e];
+        if (!p.last) {
+          Quad<_Float16> nh, nl;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            nh[e] = static_cast<_Float16>(v[e]);
+            nl[e] = static_cast<_Float16>(v[e] - static_cast<float>(nh[e]));
+          }
+          *reinterpret_cast<Quad<_Float16>*>(next + to) = nh;
+          *reinterpret_cast<Quad<_Float16>*>(lo + to) = nl;
+          continue;
+        }
+        const int rows = p.tall ? p.n : p.m, columns = p.tall ? p.m : p.n;
+        if (row >= rows) continue;
+        Quad<__bf16> y;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) y[e] = static_cast<__bf16>(v[e] * (1.0f / kScale));
+        if (!p.tall && columns % 4 == 0) {
+          if (column < columns)
+            *reinterpret_cast<Quad<__bf16>*>(out + static_cast<int64_t>(row) * p.n + column) = y;
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (column + e < columns)
+              out[p.tall ? static_cast<int64_t>(column + e) * p.n + row
+                         : static_cast<int64_t>(row) * p.n + column + e] = y[e];
+        }
+      }
+    }
+  }
+}
+
+// ---- host --------------------------------------------------------------------------------------
+
+struct Plan {
+  int rows, columns, partials;
+  int64_t block;  // elements of a partial sum
+  size_t x, square, norm, total;
+};
+
+size_t round_up(size_t n) { return (n + 255) / 256 * 256; }
+
+Plan make_plan(int64_t batch, int64_t m, int64_t n) {
+  Plan p;
+  const int64_t small = m < n ? m : n, large = m < n ? n : m;
+  p.rows = static_cast<int>((small + kTile - 1) / kTile * kTile);
+  p.columns = static_cast<int>((large + kTile - 1) / kTile * kTile);
+  p.block = (m * n + kPartials - 1) / kPartials;
+  if (p.block < 8192) p.block = 8192;
+  p.partials = static_cast<int>((m * n + p.block - 1) / p.block);
+  p.x = round_up(static_cast<size_t>(batch) * p.rows * p.columns * 2);
+  p.square = round_up(static_cast<size_t>(batch) * p.rows * p.rows * 2);
+  p.norm = round_up(static_cast<size_t>(batch) * p.partials * 8);
+  p.total = 3 * p.x + 2 * p.square + p.norm;
+  return p;
+}
+
+int refuse(int64_t batch, int64_t m, int64_t n) {
+  if (batch < 0 || m < 1 || n < 1) return DFLASH_ERR_SHAPE;
+  // Grids, and a tile's rows within 31-bit byte offsets.
+  if (m > (1 << 20) || n > (1 << 20) || batch > 65535) return DFLASH_ERR_TOO_LARGE;
+  const int64_t small = m < n ? m : n, large = m < n ? n : m;
+  const int64_t rows = (small + kTile - 1) / kTile, columns = (large + kTile - 1) / kTile;
+  if (rows > 32767 || batch * rows * columns > (1 << 22)) return DFLASH_ERR_TOO_LARGE;
+  return DFLASH_OK;
+}
+
+template <typename T>
+int launch(const T* g, __bf16* out, int64_t batch, int m, int n, int steps, float a, float b,
+           float c, float eps, char* workspace, hipStream_t stream) {
+  const Plan plan = make_plan(batch, m, n);
+  Step p{};
+  p.x.hi[0] = reinterpret_cast<_Float16*>(workspace);
+  p.x.hi[1] = reinterpret_cast<_Float16*>(workspace + plan.x);
+  p.x.lo = reinterpret_cast<_Float16*>(workspace + 2 * plan.x);
+  p.x.gram = reinterpret_cast<_Float16*>(workspace + 3 * plan.x);
+  p.x.poly = reinterpret_cast<_Float16*>(workspace + 3 * plan.x + plan.square);
+  double* partial = reinterpret_cast<double*>(workspace + 3 * plan.x + 2 * plan.square);
+  p.x.rows = plan.rows;
+  p.x.columns = plan.columns;
+  p.x.batch = static_cast<int>(batch);
+  p.a = a;
+  p.b = b;
+  p.c = c;
+  p.out = out;
+  p.m = m;
+  p.n = n;
+  p.tall = m > n;
+  constexpr int kLds = Config::LDS;
+  hipError_t e = ensure_dynamic_lds<&product_kernel<Form::kGram>>(kLds);
+  if (e == hipSuccess) e = ensure_dynamic_lds<&product_kernel<Form::kPolynomial>>(kLds);
+  if (e == hipSuccess) e = ensure_dynamic_lds<&product_kernel<Form::kUpdate>>(kLds);
+  if (e != hipSuccess) return static_cast<int>(e);
+
+  const uint32_t count = static_cast<uint32_t>(batch);
+  hipLaunchKernelGGL((norm_kernel<T>), dim3(plan.partials, count), dim3(256), 0, stream, g, partial,
+                     static_cast<int64_t>(m) * n, plan.block);
+  hipLaunchKernelGGL((start_kernel<T>), dim3(plan.columns / 64, plan.rows / 64, count), dim3(256), 0,
+                     stream, g, partial, plan.partials, p.x, m, n, p.tall, eps);
+  const uint32_t rows = plan.rows / kTile, columns = plan.columns / kTile;
+  const dim3 triangle(count * (rows * (rows + 1) / 2)), all(count * rows * columns);
+  const dim3 threads(Config::THREADS);
+  for (int step = 0; step < steps; ++step) {
+    p.from = step % 2;
+    p.last = step + 1 == steps;
+    hipLaunchKernelGGL((product_kernel<Form::kGram>), triangle, threads, kLds, stream, p);
+    hipLaunchKernelGGL((product_kernel<Form::kPolynomial>), triangle, threads, kLds, stream, p);
+    hipLaunchKernelGGL((product_kernel<Form::kUpdate>), all, threads, kLds, stream, p);
+  }
+  return static_cast<int>(hipGetLastError());
+}
+
+}  // namespace
+}  // namespace dflash
+
+using namespace dflash;
+
+extern "C" {
+
+size_t dflash_orthogonalize_workspace_bytes(int64_t batch, int64_t m, int64_t n) {
+  if (batch < 1 || refuse(batch, m, n) != DFLASH_OK) return 0;
+  return make_plan(batch, m, n).total;
+}
+
+int dflash_orthogonalize(const void* update, void* out, int64_t batch, int64_t m, int64_t n,
+                         int steps, float a, float b, float c, float eps, int dtype,
+                         void* workspace, size_t workspace_bytes, void* stream) {
+  const int rc = refuse(batch, m, n);
+  if (rc != DFLASH_OK) return rc;
+  if (steps < 1 || !(eps >= 0.0f)) return DFLASH_ERR_SHAPE;
+  if (dtype < DFLASH_DTYPE_FP16 || dtype > DFLASH_DTYPE_FP32) return DFLASH_ERR_DTYPE;
+  if (batch == 0) return DFLASH_OK;
+  if (!update || !out || !workspace) return DFLASH_ERR_NULL;
+  const uintptr_t element = dtype == DFLASH_DTYPE_FP32 ? 4 : 2;
+  if (reinterpret_cast<uintptr_t>(update) % element != 0 ||
+      (reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(workspace)) % 16 != 0)
+    return DFLASH_ERR_ALIGN;
+  if (workspace_bytes < make_plan(batch, m, n).total) return DFLASH_ERR_WORKSPACE;
+  auto call = [&](auto t) {
+    using T = decltype(t);
+    return launch(static_cast<const T*>(update), static_cast<__bf16*>(out), batch,
+                  static_cast<int>(m), static_cast<int>(n), steps, a, b, c, eps,
+                  static_cast<char*>(workspace), static_cast<hipStream_t>(stream));
+  };
+  if (dtype == DFLASH_DTYPE_FP16) return call(_Float16{});
+  if (dtype == DFLASH_DTYPE_BF16) return call(__bf16{});
+  return call(float{});
+}
+
+}  // extern "C"

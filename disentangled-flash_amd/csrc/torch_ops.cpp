@@ -45,6 +45,8 @@ struct Library {
   decltype(&dflash_attention_train_fwd) attention_fwd;
   decltype(&dflash_attention_train_bwd) attention_bwd;
   decltype(&dflash_attention_train_bwd_workspace_bytes) attention_bwd_workspace_bytes;
+  decltype(&dflash_orthogonalize) orthogonalize;
+  decltype(&dflash_orthogonalize_workspace_bytes) orthogonalize_workspace_bytes;
   decltype(&dflash_error_string) error_string;
 } lib;
 
@@ -69,6 +71,8 @@ void bind_library(std::string path) {
   find(handle, "dflash_attention_train_fwd", lib.attention_fwd);
   find(handle, "dflash_attention_train_bwd", lib.attention_bwd);
   find(handle, "dflash_attention_train_bwd_workspace_bytes", lib.attention_bwd_workspace_bytes);
+  find(handle, "dflash_orthogonalize", lib.orthogonalize);
+  find(handle, "dflash_orthogonalize_workspace_bytes", lib.orthogonalize_workspace_bytes);
   find(handle, "dflash_error_string", lib.error_string);
 }
 
@@ -415,6 +419,23 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> attention_backward(
   return {dq, dk, dv, dpk, dpq};
 }
 
+Tensor orthogonalize(const Tensor& update, int64_t steps, double a, double b, double c,
+                     double eps) {
+  expect(update.is_contiguous() && update.dim() == 3 && update.size(1) >= 1 && update.size(2) >= 1,
+         "update");
+  expect(steps >= 1 && steps <= INT32_MAX, "steps");
+  Tensor out = fresh(update.sizes(), at::kBFloat16, update);
+  if (update.numel() == 0) return out;
+  const int64_t batch = update.size(0), m = update.size(1), n = update.size(2);
+  const size_t bytes = lib.orthogonalize_workspace_bytes(batch, m, n);
+  Tensor workspace = fresh({static_cast<int64_t>(bytes)}, at::kByte, update);
+  On on(update);
+  check(lib.orthogonalize(data(update), data(out), batch, m, n, steps, a, b, c, eps,
+                          code_of(update), data(workspace), bytes, on.stream),
+        "dflash_orthogonalize");
+  return out;
+}
+
 // ---- autograd ------------------------------------------------------------------------
 
 template <typename F>
@@ -683,6 +704,8 @@ TORCH_LIBRARY_FRAGMENT(disentangled_flash, m) {
       "Tensor key, Tensor value, Tensor? pos_key, Tensor? pos_query, Tensor delta_to_slot, "
       "Tensor? mask, float scale, float p, bool want_pos_key, bool want_pos_query) -> (Tensor, "
       "Tensor, Tensor, Tensor, Tensor)");
+  m.def(
+      "orthogonalize(Tensor update, int steps, float a, float b, float c, float eps) -> Tensor");
 }
 
 TORCH_LIBRARY_IMPL(disentangled_flash, CUDA, m) {
@@ -695,6 +718,7 @@ TORCH_LIBRARY_IMPL(disentangled_flash, CUDA, m) {
   m.impl("attention", &attention);
   m.impl("attention_train", &attention_train);
   m.impl("attention_backward", &attention_backward);
+  m.impl("orthogonalize", &orthogonalize);
 }
 
 TORCH_LIBRARY_IMPL(disentangled_flash, Autograd, m) {

@@ -210,6 +210,14 @@ def _bind(lib: ctypes.CDLL) -> None:
         _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p,   # dq, dk, dv, dpos_key, dpos_query
         _c_void_p, ctypes.c_size_t, _c_void_p,                   # workspace, bytes, stream
     ]
+    lib.dflash_orthogonalize_workspace_bytes.restype = ctypes.c_size_t
+    lib.dflash_orthogonalize_workspace_bytes.argtypes = [_c_int64, _c_int64, _c_int64]
+    lib.dflash_orthogonalize.restype = _c_int
+    lib.dflash_orthogonalize.argtypes = [
+        _c_void_p, _c_void_p, _c_int64, _c_int64, _c_int64,      # update, out, batch, m, n
+        _c_int, _c_float, _c_float, _c_float, _c_float, _c_int,  # steps, a, b, c, eps, dtype
+        _c_void_p, ctypes.c_size_t, _c_void_p,                   # workspace, bytes, stream
+    ]
     lib.dflash_error_string.restype = ctypes.c_char_p
     lib.dflash_error_string.argtypes = [_c_int]
     lib.dflash_abi_version.restype = _c_int

@@ -464,6 +464,23 @@ DFLASH_API int dflash_attention_train_bwd(const dflash_attention_train* attentio
                                           void* dpos_query, void* workspace,
                                           size_t workspace_bytes, void* stream);
 
+/*
+ * Newton-Schulz iterations (the update of the Muon optimiser; no counterpart in the reference):
+ *   X = G / (|G|_F + eps);  steps times:  A = X X^T,  X <- a X + (b A + c A A) X
+ * on the side on which X has no more rows than columns, for a batch of matrices.
+ *   update    : G, [batch, m, n] contiguous, `dtype`; m and n at most 2^20
+ *   out       : bf16 [batch, m, n], 16-byte aligned
+ *   workspace : dflash_orthogonalize_workspace_bytes(batch, m, n) bytes, 16-byte aligned (0:
+ *               sizes the call refuses)
+ * Products of fp16 operands with fp32 sums; the coefficients must keep X's singular values
+ * below 128.
+ */
+DFLASH_API size_t dflash_orthogonalize_workspace_bytes(int64_t batch, int64_t m, int64_t n);
+DFLASH_API int dflash_orthogonalize(const void* update, void* out, int64_t batch, int64_t m,
+                                    int64_t n, int steps, float a, float b, float c, float eps,
+                                    int dtype, void* workspace, size_t workspace_bytes,
+                                    void* stream);
+
 /* Text for a return code of any dflash_* entry point. */
 DFLASH_API const char* dflash_error_string(int code);
 
