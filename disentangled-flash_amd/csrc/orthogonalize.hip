@@ -36,9 +36,8 @@ namespace {
 
 constexpr int kTile = 128;
 constexpr float kScale = 256.0f;  // of X in its fp16 parts
-using Config = Cfg128x128;
 
-enum class Form { kGram, kPolynomial, kUpdate };
+enum class Form { kGram, kPolynomial, kUpdate, kResult };  // kResult: the last kUpdate
 
 typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
 typedef short s4_t __attribute__((ext_vector_type(4)));
@@ -110,33 +109,75 @@ __global__ __launch_bounds__(256) void norm_kernel(const T* g, double* partial, 
 // A tile of 64 x 64 of X: rows and columns of X are those of G, or the other way round (`tall`).
 template <typename T>
 __global__ __launch_bounds__(256) void start_kernel(const T* g, const double* partial, int partials,
-                                                    Matrices x, int m, int n, int tall, float eps) {
+                                                    Matrices x, int m, int n, int tall, int whole,
+                                                    float eps) {
   __shared__ float tile[64][65];
   const int b = blockIdx.z, r0 = blockIdx.y * 64, c0 = blockIdx.x * 64;
-  double square = 0;
-  for (int at = 0; at < partials; ++at) square += partial[b * partials + at];
-  const float factor = static_cast<float>(1.0 / (sqrt(square) + static_cast<double>(eps)));
+  __shared__ double sums[4];
+  static_assert(kPartials == 256, "one a thread");
+  double square = threadIdx.x < partials ? partial[b * partials + threadIdx.x] : 0.0;
+  for (int step = 32; step; step /= 2) square += __shfl_xor(square, step);
+  if (threadIdx.x % 64 == 0) sums[threadIdx.x / 64] = square;
+  __syncthreads();
+  square = sums[0] + sums[1] + sums[2] + sums[3];
+  // (The scale is a power of two: it rounds nothing.)
+  const float factor =
+      static_cast<float>(1.0 / (sqrt(square) + static_cast<double>(eps))) * kScale;
   // G's rows and columns of this tile.
   const int gr = tall ? c0 : r0, gc = tall ? r0 : c0;
   const T* from = g + static_cast<int64_t>(b) * m * n;
-  for (int at = threadIdx.x; at < 4096; at += 256) {
-    const int r = gr + at / 64, c = gc + at % 64;
-    tile[at / 64][at % 64] =
-        r < m && c < n ? static_cast<float>(from[static_cast<int64_t>(r) * n + c]) * factor : 0.0f;
+  const int64_t base = (static_cast<int64_t>(b) * x.rows + r0) * x.columns + c0;
+  auto put = [&](int r, int c, const float (&v)[8]) {
+    half8_t hi, lo;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      hi[e] = static_cast<_Float16>(v[e]);
+      lo[e] = static_cast<_Float16>(v[e] - static_cast<float>(hi[e]));
+    }
+    *reinterpret_cast<half8_t*>(x.hi[0] + base + static_cast<int64_t>(r) * x.columns + c) = hi;
+    *reinterpret_cast<half8_t*>(x.lo + base + static_cast<int64_t>(r) * x.columns + c) = lo;
+  };
+  if (!tall) {
+#pragma unroll
+    for (int at = 0; at < 2; ++at) {
+      const int r = (at * 256 + threadIdx.x) / 8, c = threadIdx.x % 8 * 8;
+      const T* row = from + static_cast<int64_t>(gr + r) * n + gc + c;
+      float v[8] = {};
+      if (whole) {  // rows of whole 16-byte chunks, on 16-byte boundaries
+        constexpr int N = Chunk<T>::N;
+        if (gr + r < m && gc + c < n) {
+#pragma unroll
+          for (int e = 0; e < 8; e += N) {
+            float part[N];
+            load_floats<T, N>(row + e, part);
+#pragma unroll
+            for (int x = 0; x < N; ++x) v[e + x] = part[x] * factor;
+          }
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          v[e] = gr + r < m && gc + c + e < n ? static_cast<float>(row[e]) * factor : 0.0f;
+      }
+      put(r, c, v);
+    }
+    return;
+  }
+#pragma unroll
+  for (int at = 0; at < 16; ++at) {
+    const int r = at * 4 + threadIdx.x / 64, c = threadIdx.x % 64;
+    tile[r][c] = gr + r < m && gc + c < n
+                     ? static_cast<float>(from[static_cast<int64_t>(gr + r) * n + gc + c]) * factor
+                     : 0.0f;
   }
   __syncthreads();
-  const int64_t base = (static_cast<int64_t>(b) * x.rows + r0) * x.columns + c0;
-  for (int at = threadIdx.x; at < 2048; at += 256) {
-    const int r = at / 32, c = at % 32 * 2;
-    half2_t hi, lo;
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const float v = (tall ? tile[c + e][r] : tile[r][c + e]) * kScale;
-      hi[e] = static_cast<_Float16>(v);
-      lo[e] = static_cast<_Float16>(v - static_cast<float>(hi[e]));
-    }
-    *reinterpret_cast<half2_t*>(x.hi[0] + base + static_cast<int64_t>(r) * x.columns + c) = hi;
-    *reinterpret_cast<half2_t*>(x.lo + base + static_cast<int64_t>(r) * x.columns + c) = lo;
+  for (int at = 0; at < 2; ++at) {
+    const int r = (at * 256 + threadIdx.x) % 64, c = (at * 256 + threadIdx.x) / 64 * 8;
+    float v[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = tile[c + e][r];
+    put(r, c, v);
   }
 }
 
@@ -146,23 +187,24 @@ struct Step {
   Matrices x;
   int from;        // which of hi the step reads; it writes the other
   float a, b, c;
-  int last;        // write `out` instead of X
-  __bf16* out;     // [batch, m, n]
+  int read_lo, write_lo;
+  __bf16* out;     // [batch, m, n]: kResult writes it instead of X
   int m, n, tall;  // of G
 };
 
-template <Form FORM>
-__global__ __launch_bounds__(Config::THREADS, Config::WGS) void product_kernel(Step p) {
-  using CF = Config;
+template <Form FORM, typename CF>
+__global__ __launch_bounds__(CF::THREADS, CF::WGS) void product_kernel(Step p) {
+  constexpr int BM = CF::BM, BN = CF::BN;
   constexpr int MB = CF::MB, NB = CF::NB, S = CF::STAGES;
-  constexpr bool kSquare = FORM != Form::kUpdate;  // symmetric, second operand by rows of k-runs
+  constexpr bool kSquare = FORM == Form::kGram || FORM == Form::kPolynomial;  // symmetric, second operand by rows of k-runs
   extern __shared__ __align__(16) unsigned char smem[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int c = lane & 15, g = lane >> 4;
   const int wm = wave % CF::WAVES_M, wn = wave / CF::WAVES_M;
 
   // The tiles of a matrix lie on one XCD.
-  const int tiles_m = p.x.rows / kTile, tiles_n = (kSquare ? p.x.rows : p.x.columns) / kTile;
+  static_assert(!kSquare || BM == BN, "tiles on both sides of the diagonal");
+  const int tiles_m = p.x.rows / BM, tiles_n = (kSquare ? p.x.rows : p.x.columns) / BN;
   const int each = kSquare ? tiles_m * (tiles_m + 1) / 2 : tiles_m * tiles_n;
   const int at = xcd_logical_block(blockIdx.x, gridDim.x);
   const int batch = at / each;
@@ -182,12 +224,13 @@ __global__ __launch_bounds__(Config::THREADS, Config::WGS) void product_kernel(S
   const _Float16* left = FORM == Form::kGram ? hi
                          : FORM == Form::kPolynomial ? p.x.gram + batch * square
                                                      : p.x.poly + batch * square;
-  const _Float16* X = left + static_cast<int64_t>(mt) * kTile * K;
-  const _Float16* W = kSquare ? left + static_cast<int64_t>(nt) * kTile * K : hi + nt * kTile;
+  const _Float16* X = left + static_cast<int64_t>(mt) * BM * K;
+  const _Float16* W = kSquare ? left + static_cast<int64_t>(nt) * BN * K : hi + nt * BN;
   const uint32_t x_row = static_cast<uint32_t>(K) * 2;
   const uint32_t w_row_bytes = kSquare ? x_row : static_cast<uint32_t>(p.x.columns) * 2;
   const int KT = K / kSlabK;
 
+  constexpr int kChunks = BN / 8;  // of a row of k
   // Byte offsets of this lane's 16 bytes of each copy.
   uint32_t xoff[CF::A_LOADS], woff[CF::B_LOADS];
 #pragma unroll
@@ -200,9 +243,9 @@ __global__ __launch_bounds__(Config::THREADS, Config::WGS) void product_kernel(S
     if (kSquare) {
       const int r = copy_row<CF>(j, wave, lane);
       woff[j] = w_row(r) * w_row_bytes + copy_chunk(r, lane) * 16;
-    } else {  // four rows of k of 256 bytes
-      const int r = (j * CF::WAVES + wave) * 4 + (lane >> 4);
-      woff[j] = r * w_row_bytes + ((lane & 15) ^ k_row_swizzle(r)) * 16;
+    } else {  // rows of k, BN columns each
+      const int r = ((j * CF::WAVES + wave) * 64 + lane) / kChunks;
+      woff[j] = r * w_row_bytes + (lane % kChunks ^ k_row_swizzle(r)) * 16;
     }
   }
   const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(smem));
@@ -214,13 +257,13 @@ __global__ __launch_bounds__(Config::THREADS, Config::WGS) void product_kernel(S
         lds0 + stage * CF::SLAB + (is_x ? 0 : CF::A_BYTES) + (jj * CF::WAVES + wave) * 1024);
     const bool live = kt < KT;
     if (is_x || kSquare) {
-      const auto memory = scalar_resource(is_x ? X : W, live ? kTile * x_row : 0);
+      const auto memory = scalar_resource(is_x ? X : W, live ? (is_x ? BM : BN) * x_row : 0);
       copy_to_lds(memory, is_x ? xoff[is_x ? jj : 0] : woff[is_x ? 0 : jj],
                   __builtin_amdgcn_readfirstlane(live ? kt * kSlabK * 2 : 0), to);
     } else {  // a resource that begins at the slab's first row
       const auto memory =
           scalar_resource(W + static_cast<int64_t>(live ? kt : 0) * kSlabK * p.x.columns,
-                          live ? (kSlabK - 1) * w_row_bytes + kTile * 2 : 0);
+                          live ? (kSlabK - 1) * w_row_bytes + BN * 2 : 0);
       copy_to_lds(memory, woff[is_x ? 0 : jj], 0, to);
     }
   };
@@ -239,17 +282,40 @@ __global__ __launch_bounds__(Config::THREADS, Config::WGS) void product_kernel(S
       return *static_cast<const F*>(
           __builtin_assume_aligned(smem + base + wrow + chunk[u] + i * 16 * kSlabK * 2, 16));
     } else {
-      // Columns 64 wn + 16 i + c of rows 32 u + 8g + 0..3 and + 4..7.
+      // Columns wn WN + 16 i + c of rows 32 u + 8g + 0..3 and + 4..7.
       const int r = 32 * u + 8 * g + (c >> 2);
       const int x = ((wn * CF::WN + 16 * i) / 8 + ((c & 3) >> 1)) ^ k_row_swizzle(r);
-      const unsigned char* p0 = smem + base + CF::A_BYTES + r * 256 + x * 16 + (c & 1) * 8;
+      const unsigned char* p0 = smem + base + CF::A_BYTES + r * (BN * 2) + x * 16 + (c & 1) * 8;
       const u32x2_t lo = __builtin_bit_cast(
           u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4_t*)p0));
       const u32x2_t up = __builtin_bit_cast(
-          u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4_t*)(p0 + 4 * 256)));
+          u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4_t*)(p0 + 4 * BN * 2)));
       return __builtin_bit_cast(F, u32x4_t{lo[0], lo[1], up[0], up[1]});
     }
   };
+
+  // X of this tile, for a X: read with the first slabs, a thread's rows and chunks of eight
+  // columns as it will write them.
+  constexpr int kRows = BM * BN / 8 / CF::THREADS;  // chunks a thread
+  _Float16* lo = p.x.lo + batch * whole;
+  half8_t h[kSquare ? 1 : kRows], l[kSquare ? 1 : kRows];
+  auto place = [&](int n) {  // row and column of a thread's n-th chunk
+    const int at2 = n * CF::THREADS + threadIdx.x;
+    return int2{at2 / (BN / 8), at2 % (BN / 8) * 8};
+  };
+  auto address = [&](int2 rc) {
+    return static_cast<int64_t>(mt * BM + rc.x) * p.x.columns + nt * BN + rc.y;
+  };
+  if constexpr (!kSquare) {
+#pragma unroll
+    for (int n = 0; n < kRows; ++n) {
+      const int64_t to = address(place(n));
+      h[n] = *reinterpret_cast<const half8_t*>(hi + to);
+      l[n] = half8_t{};
+      if (p.read_lo) l[n] = *reinterpret_cast<const half8_t*>(lo + to);
+    }
+    asm volatile("" ::: "memory");
+  }
 
   f32x4_t acc[NB][MB] = {};
   F xf[2][MB], wf[2][NB];
@@ -299,7 +365,9 @@ __global__ __launch_bounds__(Config::THREADS, Config::WGS) void product_kernel(S
     step(std::integral_constant<int, 1>{}, std::true_type{}, next * CF::SLAB, kt + S, stage);
     stage = next;
   }
-  wait_copies<0>();  // no copy may land in LDS any more
+  // No copy may land in LDS any more (and the compiler knows that no load is left).
+  __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
+  asm volatile("" ::: "memory");
 
   if constexpr (kSquare) {
     // Eight consecutive elements of a row a lane and pair of blocks.
@@ -308,15 +376,15 @@ __global__ __launch_bounds__(Config::THREADS, Config::WGS) void product_kernel(S
     asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
     // The mirrored tile, [column][row], rows of 128 + 8.
     _Float16* mirror = reinterpret_cast<_Float16*>(smem);
-    constexpr int kLd = kTile + 8;
-    static_assert(kTile * kLd * 2 <= CF::LDS, "the mirrored tile");
+    constexpr int kLd = BM + 8;
+    static_assert(BN * kLd * 2 <= CF::LDS, "the mirrored tile");
 #pragma unroll
     for (int j = 0; j < MB; ++j) {
       const int row = wm * CF::WM + 16 * j + c;
 #pragma unroll
       for (int i = 0; i < NB; i += 2) {
         const int column = wn * CF::WN + 16 * i + 8 * g;
-        const int64_t to = static_cast<int64_t>(mt * kTile + row) * p.x.rows + nt * kTile + column;
+        const int64_t to = static_cast<int64_t>(mt * BM + row) * p.x.rows + nt * BN + column;
         half8_t v;
         if constexpr (FORM == Form::kGram) {
 #pragma unroll
@@ -337,52 +405,64 @@ __global__ __launch_bounds__(Config::THREADS, Config::WGS) void product_kernel(S
     }
     if (mt != nt) {
       __syncthreads();
-      for (int n = threadIdx.x; n < kTile * kTile / 8; n += CF::THREADS) {
-        const int r = n / (kTile / 8), k = n % (kTile / 8) * 8;
-        *reinterpret_cast<u32x4_t*>(out + static_cast<int64_t>(nt * kTile + r) * p.x.rows +
-                                    mt * kTile + k) =
+      for (int n = threadIdx.x; n < BN * BM / 8; n += CF::THREADS) {
+        const int r = n / (BM / 8), k = n % (BM / 8) * 8;
+        *reinterpret_cast<u32x4_t*>(out + static_cast<int64_t>(nt * BN + r) * p.x.rows +
+                                    mt * BM + k) =
             *reinterpret_cast<const u32x4_t*>(mirror + r * kLd + k);
       }
     }
   } else {
-    _Float16* next = p.x.hi[p.from ^ 1] + batch * whole;
-    _Float16* lo = p.x.lo + batch * whole;
-    __bf16* out = p.out + static_cast<int64_t>(batch) * p.m * p.n;
+    // Through LDS, so that rows are read and written 256 bytes at a time (straight from the
+    // accumulators, 8 bytes a lane in 16 rows, X's accesses took 69 of 114 us of a step of 48 of
+    // 768 x 768).  Chunk (four columns) x of row r lies at x ^ (r % 8).
+    static_assert(BM * BN * 4 <= CF::LDS, "the tile");
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    f32x4_t* tile = reinterpret_cast<f32x4_t*>(smem);
 #pragma unroll
-    for (int j = 0; j < MB; ++j) {
-      const int row = mt * kTile + wm * CF::WM + 16 * j + c;
+    for (int j = 0; j < MB; ++j)
 #pragma unroll
       for (int i = 0; i < NB; ++i) {
-        const int column = nt * kTile + wn * CF::WN + 16 * i + 4 * g;
-        const int64_t to = static_cast<int64_t>(row) * p.x.columns + column;
-        const Quad<_Float16> h = *reinterpret_cast<const Quad<_Float16>*>(hi + to);
-        const Quad<_Float16> l = *reinterpret_cast<const Quad<_Float16>*>(lo + to);
-        f32x4_t v;
+        const int r = wm * CF::WM + 16 * j + c, x = (wn * CF::WN + 16 * i) / 4 + g;
+        tile[r * (BN / 4) + (x ^ (r & 7))] = acc[i][j];
+      }
+    __syncthreads();
+    _Float16* next = p.x.hi[p.from ^ 1] + batch * whole;
+    __bf16* out = p.out + static_cast<int64_t>(batch) * p.m * p.n;
+    const int rows = p.tall ? p.n : p.m, columns = p.tall ? p.m : p.n;
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          v[e] = p.a * (static_cast<float>(h[e]) + static_cast<float>(l[e])) + acc[i][j][e];
-        if (!p.last) {
-          Quad<_Float16> nh, nl;
+    for (int n = 0; n < kRows; ++n) {
+      const int2 rc = place(n);
+      float v[8];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            nh[e] = static_cast<_Float16>(v[e]);
-            nl[e] = static_cast<_Float16>(v[e] - static_cast<float>(nh[e]));
-          }
-          *reinterpret_cast<Quad<_Float16>*>(next + to) = nh;
-          *reinterpret_cast<Quad<_Float16>*>(lo + to) = nl;
-          continue;
+      for (int half = 0; half < 2; ++half) {
+        const f32x4_t sum = tile[rc.x * (BN / 4) + ((rc.y / 4 + half) ^ (rc.x & 7))];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int at2 = 4 * half + e;
+          v[at2] = p.a * (static_cast<float>(h[n][at2]) + static_cast<float>(l[n][at2])) + sum[e];
         }
-        const int rows = p.tall ? p.n : p.m, columns = p.tall ? p.m : p.n;
-        if (row >= rows) continue;
-        Quad<__bf16> y;
+      }
+      if constexpr (FORM == Form::kUpdate) {
+        half8_t nh, nl;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) y[e] = static_cast<__bf16>(v[e] * (1.0f / kScale));
-        if (!p.tall && columns % 4 == 0) {
-          if (column < columns)
-            *reinterpret_cast<Quad<__bf16>*>(out + static_cast<int64_t>(row) * p.n + column) = y;
+        for (int e = 0; e < 8; ++e) {
+          nh[e] = static_cast<_Float16>(v[e]);
+          nl[e] = static_cast<_Float16>(v[e] - static_cast<float>(nh[e]));
+        }
+        *reinterpret_cast<half8_t*>(next + address(rc)) = nh;
+        if (p.write_lo) *reinterpret_cast<half8_t*>(lo + address(rc)) = nl;
+      } else {
+        const int row = mt * BM + rc.x, column = nt * BN + rc.y;
+        if (row >= rows || column >= columns) continue;
+        bf16x8_t y;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) y[e] = static_cast<__bf16>(v[e] * (1.0f / kScale));
+        if (!p.tall && columns % 8 == 0) {
+          *reinterpret_cast<bf16x8_t*>(out + static_cast<int64_t>(row) * p.n + column) = y;
         } else {
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
+          for (int e = 0; e < 8; ++e)
             if (column + e < columns)
               out[p.tall ? static_cast<int64_t>(column + e) * p.n + row
                          : static_cast<int64_t>(row) * p.n + column + e] = y[e];
@@ -405,8 +485,9 @@ size_t round_up(size_t n) { return (n + 255) / 256 * 256; }
 Plan make_plan(int64_t batch, int64_t m, int64_t n) {
   Plan p;
   const int64_t small = m < n ? m : n, large = m < n ? n : m;
-  p.rows = static_cast<int>((small + kTile - 1) / kTile * kTile);
-  p.columns = static_cast<int>((large + kTile - 1) / kTile * kTile);
+  const int64_t tile = kTile;
+  p.rows = static_cast<int>((small + tile - 1) / tile * tile);
+  p.columns = static_cast<int>((large + tile - 1) / tile * tile);
   p.block = (m * n + kPartials - 1) / kPartials;
   if (p.block < 8192) p.block = 8192;
   p.partials = static_cast<int>((m * n + p.block - 1) / p.block);
@@ -425,6 +506,29 @@ int refuse(int64_t batch, int64_t m, int64_t n) {
   const int64_t rows = (small + kTile - 1) / kTile, columns = (large + kTile - 1) / kTile;
   if (rows > 32767 || batch * rows * columns > (1 << 22)) return DFLASH_ERR_TOO_LARGE;
   return DFLASH_OK;
+}
+
+template <Form FORM, typename CF>
+int launch_config(const Step& p, hipStream_t stream) {
+  const uint32_t m = p.x.rows / CF::BM, n = p.x.columns / CF::BN;
+  const uint32_t tiles = FORM == Form::kGram || FORM == Form::kPolynomial ? m * (m + 1) / 2 : m * n;
+  const hipError_t e = ensure_dynamic_lds<&product_kernel<FORM, CF>>(CF::LDS);
+  if (e != hipSuccess) return static_cast<int>(e);
+  hipLaunchKernelGGL((product_kernel<FORM, CF>), dim3(p.x.batch * tiles), dim3(CF::THREADS),
+                     CF::LDS, stream, p);
+  return static_cast<int>(hipGetLastError());
+}
+
+// Up to one tile a CU: eight wavefronts and five slabs in flight; more: two workgroups of four a CU,
+// two slabs.  us a step, deep / two: Gram of 6144 x 1536 (78 tiles) 44 / 67, of four (312) 105 / 96,
+// of 48 of 768 x 768 (1008) 51 / 42; update of 256 x 256 (4) 7.5 / 9.
+template <Form FORM>
+int launch_product(const Step& p, hipStream_t stream) {
+  constexpr bool kSquare = FORM == Form::kGram || FORM == Form::kPolynomial;
+  const int m = p.x.rows / kTile, n = p.x.columns / kTile;
+  const int64_t tiles = static_cast<int64_t>(p.x.batch) * (kSquare ? m * (m + 1) / 2 : m * n);
+  return tiles <= 256 ? launch_config<FORM, Cfg128x128Deep>(p, stream)
+                      : launch_config<FORM, Cfg128x128>(p, stream);
 }
 
 template <typename T>
@@ -448,26 +552,23 @@ int launch(const T* g, __bf16* out, int64_t batch, int m, int n, int steps, floa
   p.m = m;
   p.n = n;
   p.tall = m > n;
-  constexpr int kLds = Config::LDS;
-  hipError_t e = ensure_dynamic_lds<&product_kernel<Form::kGram>>(kLds);
-  if (e == hipSuccess) e = ensure_dynamic_lds<&product_kernel<Form::kPolynomial>>(kLds);
-  if (e == hipSuccess) e = ensure_dynamic_lds<&product_kernel<Form::kUpdate>>(kLds);
-  if (e != hipSuccess) return static_cast<int>(e);
-
   const uint32_t count = static_cast<uint32_t>(batch);
   hipLaunchKernelGGL((norm_kernel<T>), dim3(plan.partials, count), dim3(256), 0, stream, g, partial,
                      static_cast<int64_t>(m) * n, plan.block);
   hipLaunchKernelGGL((start_kernel<T>), dim3(plan.columns / 64, plan.rows / 64, count), dim3(256), 0,
-                     stream, g, partial, plan.partials, p.x, m, n, p.tall, eps);
-  const uint32_t rows = plan.rows / kTile, columns = plan.columns / kTile;
-  const dim3 triangle(count * (rows * (rows + 1) / 2)), all(count * rows * columns);
-  const dim3 threads(Config::THREADS);
+                     stream, g, partial, plan.partials, p.x, m, n, p.tall,
+                     n % 8 == 0 && reinterpret_cast<uintptr_t>(g) % 16 == 0, eps);
   for (int step = 0; step < steps; ++step) {
     p.from = step % 2;
-    p.last = step + 1 == steps;
-    hipLaunchKernelGGL((product_kernel<Form::kGram>), triangle, threads, kLds, stream, p);
-    hipLaunchKernelGGL((product_kernel<Form::kPolynomial>), triangle, threads, kLds, stream, p);
-    hipLaunchKernelGGL((product_kernel<Form::kUpdate>), all, threads, kLds, stream, p);
+    // (The last step's X, whose small singular values grow no more, has hi alone.)
+    p.read_lo = step == 0 || step + 1 < steps;
+    p.write_lo = step + 2 < steps;
+    int rc = launch_product<Form::kGram>(p, stream);
+    if (rc == DFLASH_OK) rc = launch_product<Form::kPolynomial>(p, stream);
+    if (rc == DFLASH_OK)
+      rc = step + 1 < steps ? launch_product<Form::kUpdate>(p, stream)
+                            : launch_product<Form::kResult>(p, stream);
+    if (rc != DFLASH_OK) return rc;
   }
   return static_cast<int>(hipGetLastError());
 }

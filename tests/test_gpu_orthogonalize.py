@@ -43,9 +43,10 @@ def _emulate(update, steps=5, coefficients=COEFFICIENTS, eps=1e-7):
     x = x.mT if x.shape[-2] > x.shape[-1] else x
     norm = update.double().square().sum((-2, -1), keepdim=True).sqrt() + eps
     x = (x.double() / norm).float()
-    for _ in range(steps):
+    for step in range(steps):
         high = half(x * 256) / 256
-        x = high + half((x - high) * 256) / 256
+        rest = half((x - high) * 256) / 256
+        x = high + rest if step == 0 or step + 1 < steps else high
         s = half(high @ high.mT.contiguous())
         x = a * x + half(b * s + c * (s @ s)) @ high
     return x.mT if update.shape[-2] > update.shape[-1] else x
