@@ -8,8 +8,13 @@ The operators, on a GPU in fp16, bf16 and fp32, with their gradients:
   without residual and dropout a plain LayerNorm.
 * :func:`dropout` - dropout whose mask comes from a counter-based generator and is drawn
   again in the backward pass instead of being stored.
+* :func:`attention` - disentangled attention with learned rows for the log buckets of the relative
+  distance and with dropout on its probabilities, without an ``[L, L]`` tensor of scores.
 * :func:`embedding` - the table lookup with a scale, and the dense gradient of the table,
   summed in an order that depends on the ids alone (the same bits on every call).
+
+* :func:`orthogonalize` - the Newton-Schulz iterations of the Muon optimiser for a batch of matrices;
+  :class:`Muon` is that optimiser.
 
 :func:`enable_deberta_training` puts them into a Hugging Face DeBERTa-v2/v3 backbone;
 ``optimize_deberta`` takes the same model afterwards for inference.
@@ -34,9 +39,10 @@ those that do not start on a 16-byte boundary.
 from __future__ import annotations
 
 import itertools
+import math
 import threading
 from collections import OrderedDict
-from collections.abc import Mapping
+from collections.abc import Iterable, Mapping
 from typing import Any
 
 import torch
@@ -44,6 +50,7 @@ from torch import nn
 from torch.nn.modules import module as torch_module
 
 from . import _lib
+from .position import SharedPositionPlanCache
 
 MAX_HIDDEN = 8192  # widest row of layer_norm
 ATTENTION_WIDTHS = (32, 64, 128)  # head widths of attention
@@ -697,6 +704,172 @@ class OutputBlock(nn.Module):
                           site=drop.site)
 
 
+class _PositionPlans:
+    """Slots and places of relative distances for each length, and whether the slots in use are
+    successive rows of the table (then they are a view of it)."""
+
+    def __init__(self, attention: nn.Module) -> None:
+        self.cache = SharedPositionPlanCache(
+            position_buckets=attention.position_buckets,
+            max_relative_positions=attention.max_relative_positions,
+            position_embedding_size=attention.pos_ebd_size)
+        self.ranges: dict[int, tuple[int, int] | None] = {}
+
+    def of(self, length: int, device: torch.device) -> tuple[Any, tuple[int, int] | None]:
+        if length not in self.ranges:
+            slots = self.cache.compact(length, "cpu").active_slots
+            first, last = int(slots[0]), int(slots[-1])
+            self.ranges[length] = (first, last + 1) if last - first + 1 == len(slots) else None
+        return self.cache.compact(length, device), self.ranges[length]
+
+
+def _is_factorized(mask: Any, batch: int, length: int) -> bool:
+    """The form in which :class:`_EncoderParts` hands a padding mask on: ``[B, 1, L, 1]``."""
+
+    return isinstance(mask, torch.Tensor) and mask.shape == (batch, 1, length, 1)
+
+
+class _Attention:
+    """The forward of a Hugging Face ``DisentangledSelfAttention`` on :func:`attention`.
+
+    Its projections and its dropouts stay the modules that they are.  What the operator lacks (the
+    CPU, other dtypes and head widths, attention probabilities as an output, masks of pairs, relative
+    positions given by the caller) and children that were replaced or have hooks go to the
+    original's forward.
+    """
+
+    def forward(self, hidden_states, attention_mask, output_attentions=False, query_states=None,
+                relative_pos=None, rel_embeddings=None):
+        batch, length = hidden_states.shape[:2]
+        factorized = _is_factorized(attention_mask, batch, length)
+        if factorized and relative_pos is None and not output_attentions:
+            out = self._fused(hidden_states, attention_mask[:, 0, :, 0],
+                              hidden_states if query_states is None else query_states,
+                              rel_embeddings)
+            if out is not None:
+                return out, None
+        if factorized:
+            mask = attention_mask[:, 0, :, 0]
+            attention_mask = mask[:, None, None, :] * mask[:, None, :, None]
+        return super().forward(hidden_states, attention_mask, output_attentions,
+                               query_states=query_states, relative_pos=relative_pos,
+                               rel_embeddings=rel_embeddings)
+
+    def _fused(self, hidden_states, mask, query_states, rel_embeddings):
+        drop = self.dropout
+        terms = [m for m in ("c2p", "p2c") if m in self.pos_att_type]  # (the scale counts them)
+        modes = terms if self.relative_attention else []
+        if not (_on_gpu(hidden_states) and self.attention_head_size in ATTENTION_WIDTHS
+                and 1 <= hidden_states.shape[1] <= MAX_LENGTH
+                and query_states.shape == hidden_states.shape
+                and _dropout_fits(drop) and not _hooks_on_all_modules()
+                and (not modes or (rel_embeddings is not None
+                                   and rel_embeddings.shape[0] >= 2 * self.pos_ebd_size))):
+            return None
+        batch, length = hidden_states.shape[:2]
+        shape = (batch, length, self.num_attention_heads, self.attention_head_size)
+        query, key, value = (projection(x).view(shape) for projection, x in (
+            (self.query_proj, query_states), (self.key_proj, hidden_states),
+            (self.value_proj, hidden_states)))
+        pos_key = pos_query = None
+        if modes:
+            plan, rows = self._plans.of(length, hidden_states.device)
+            used = self.pos_dropout(rel_embeddings)
+            used = used[rows[0]:rows[1]] if rows else used.index_select(0, plan.active_slots)
+            shared = self.share_att_key
+
+            def table(projection):
+                return projection(used).view(-1, *shape[2:]).transpose(0, 1)
+
+            if "c2p" in modes:
+                pos_key = table(self.key_proj if shared else self.pos_key_proj)
+            if "p2c" in modes:
+                pos_query = table(self.query_proj if shared else self.pos_query_proj)
+            places = plan.delta_to_local
+        else:
+            places = self._no_places(length, hidden_states.device)
+        tensors = [t for t in (query, key, value, pos_key, pos_query) if t is not None]
+        dtype = query.dtype
+        if dtype not in _lib.DTYPE_CODES or any(t.dtype != dtype for t in tensors):
+            return None
+        dropping = drop.training and drop.p > 0
+        out = attention(query, key, value, pos_key, pos_query, places,
+                        1 / math.sqrt(self.attention_head_size * (1 + len(terms))),
+                        mask=mask.bool(), p=drop.p if dropping else 0.0,
+                        rng=drop.state.rng if dropping else None, site=drop.site)
+        return out.view(batch, length, -1)
+
+    @staticmethod
+    def _no_places(length, device):
+        return torch.zeros(2 * length - 1, dtype=torch.int32, device=device)
+
+
+class _EncoderParts:
+    """Stands for ``get_attention_mask`` or ``get_rel_pos`` of a Hugging Face encoder whose
+    attention is :class:`_Attention`: a padding mask stays ``[B, L]`` values (as ``[B, 1, L, 1]``), and the
+    relative positions are left to the attention.  Anything else is the encoder's own."""
+
+    def __init__(self, encoder: nn.Module, name: str) -> None:
+        self.encoder, self.name = encoder, name
+
+    def __call__(self, *args: Any, **kwargs: Any) -> Any:
+        encoder = self.encoder
+        own = getattr(type(encoder), self.name)
+        if not all(isinstance(layer.attention.self, _Attention) for layer in encoder.layer):
+            return own(encoder, *args, **kwargs)
+        given = [*args, *kwargs.values()]
+        if self.name == "get_attention_mask":
+            mask = given[0]
+            if isinstance(mask, torch.Tensor) and mask.dim() == 2:
+                return mask[:, None, :, None]
+        elif len(given) < 3 or given[2] is None:
+            return None
+        return own(encoder, *args, **kwargs)
+
+
+_attention_class: type | None = None
+
+
+def __getattr__(name: str) -> Any:
+    """``DisentangledSelfAttention``: Hugging Face's with the forward of :class:`_Attention` (made when
+    first asked for: this module does without transformers)."""
+
+    global _attention_class
+    if name != "DisentangledSelfAttention":
+        raise AttributeError(f"module {__name__!r} has no attribute {name!r}")
+    if _attention_class is None:
+        from transformers.models.deberta_v2.modeling_deberta_v2 import DisentangledSelfAttention
+
+        _attention_class = type("DisentangledSelfAttention", (_Attention, DisentangledSelfAttention),
+                                {"__module__": __name__, "__doc__": _Attention.__doc__})
+    return _attention_class
+
+
+def _is_attention(module: nn.Module) -> bool:
+    kind = type(module)
+    return (kind.__name__ == "DisentangledSelfAttention" and kind.__module__ == _OUTPUT_BLOCKS_FROM
+            and kind.forward.__module__ == _OUTPUT_BLOCKS_FROM)
+
+
+def _fuse_attention(encoder: nn.Module) -> None:
+    """Gives every attention of the encoder the fused forward, in place; none of them where one
+    is not Hugging Face's own, or has hooks."""
+
+    modules = [layer.attention.self for layer in encoder.layer]
+    if not modules or not all(_is_attention(m) and not _has_hooks(m) for m in modules):
+        raise TypeError("the encoder's attention is not transformers' DisentangledSelfAttention")
+    if type(encoder).__module__ != _OUTPUT_BLOCKS_FROM:
+        raise TypeError("the encoder is not transformers' DebertaV2Encoder")
+    plans = None
+    for module in modules:
+        if module.relative_attention and plans is None:
+            plans = _PositionPlans(module)
+        module.__class__ = __getattr__("DisentangledSelfAttention")
+        module.__dict__["_plans"] = plans
+    for name in ("get_attention_mask", "get_rel_pos"):
+        encoder.__dict__[name] = _EncoderParts(encoder, name)
+
+
 _OUTPUT_BLOCKS = ("DebertaV2SelfOutput", "DebertaV2Output")
 _OUTPUT_BLOCKS_FROM = "transformers.models.deberta_v2.modeling_deberta_v2"
 
@@ -774,7 +947,9 @@ def _keep_state(model: nn.Module, args: Any, outputs: Any) -> None:
         state.keep_for(outputs)
 
 
-def enable_deberta_training(model: nn.Module, *, seed: int = 0) -> nn.Module:
+def enable_deberta_training(
+    model: nn.Module, *, seed: int = 0, attention: str = "torch"
+) -> nn.Module:
     """Put the training operators into a HF DeBERTa-v2/v3 backbone, in place.
 
     ``model`` is the Hugging Face backbone (the module with ``embeddings`` and ``encoder``), as
@@ -788,9 +963,13 @@ def enable_deberta_training(model: nn.Module, *, seed: int = 0) -> nn.Module:
     its backward pass has the same step again, so what is checkpointed (a layer, or the whole
     backbone) recomputes what it computed.  A forward of a backbone in eval mode advances where a dropout in training mode first drops (Monte Carlo dropout, a few
     layers in training).
+
+    ``attention="hip"`` runs the backbone's attention on :func:`attention` too (its projections stay
+    torch's products): no ``[L, L]`` tensor of scores or probabilities is made, and the same
+    probabilities are dropped as with ``"torch"``, which leaves the attention as it is.
     """
 
-    from .deberta import DebertaV2InferenceEncoder
+    from .deberta import DebertaV2InferenceEncoder, resolve_backend
 
     if not (hasattr(model, "encoder") and hasattr(model, "embeddings")):
         raise TypeError("model must be a Hugging Face DeBERTa-v2/v3 backbone")
@@ -798,6 +977,8 @@ def enable_deberta_training(model: nn.Module, *, seed: int = 0) -> nn.Module:
         raise TypeError("the model's encoder is inference-only (DebertaV2InferenceEncoder)")
     if hasattr(model, "dropout_state"):
         raise TypeError("the model already uses the training operators")
+    if resolve_backend(attention) == "hip":
+        _fuse_attention(model.encoder)
     state = DropoutState(seed, next(model.parameters()).device)
     sites = iter(range(1 << 32))
     places: list[nn.Module] = [model]
@@ -814,11 +995,96 @@ def enable_deberta_training(model: nn.Module, *, seed: int = 0) -> nn.Module:
     return model
 
 
+# ---- optimiser ---------------------------------------------------------------------------
+
+
+def split_parameters(model: nn.Module) -> tuple[list[nn.Parameter], list[nn.Parameter]]:
+    """(the weights of the encoder's ``nn.Linear`` layers, all other parameters), those that require a
+    gradient: the former for :class:`Muon`, the latter for another optimiser."""
+
+    encoder = getattr(model, "encoder", model)
+    matrices = {id(m.weight): m.weight for m in encoder.modules()
+                if isinstance(m, nn.Linear) and m.weight.requires_grad}
+    rest = [p for p in model.parameters() if p.requires_grad and id(p) not in matrices]
+    return list(matrices.values()), rest
+
+
+class Muon(torch.optim.Optimizer):
+    """Muon on :func:`orthogonalize`, for matrices: ``B <- momentum B + g``; the update is ``g + momentum
+    B`` (``B`` without ``nesterov``), orthogonalised; ``p <- (1 - lr weight_decay) p - lr r update``.
+
+    Names and defaults are those of ``torch.optim.Muon``.  ``adjust_lr_fn`` chooses ``r`` for ``[m, n]``:
+    ``"original"`` (the default) ``sqrt(max(1, m / n))``, ``"match_rms_adamw"`` ``0.2 sqrt(max(m,
+    n))``.  Parameters of one shape, dtype and device are orthogonalised by one call.  They must be on
+    a GPU, in fp16, bf16 or fp32; the momentum is kept in the parameter's dtype.
+    """
+
+    def __init__(self, params: Iterable[Any], lr: float = 1e-3, weight_decay: float = 0.1,
+                 momentum: float = 0.95, nesterov: bool = True,
+                 ns_coefficients: tuple[float, float, float] = NEWTON_SCHULZ, eps: float = 1e-7,
+                 ns_steps: int = 5, adjust_lr_fn: str | None = None) -> None:
+        if not lr >= 0.0:
+            raise ValueError(f"lr must not be negative, got {lr}")
+        if not 0.0 <= momentum < 1.0:
+            raise ValueError(f"momentum must be in [0, 1), got {momentum}")
+        if not weight_decay >= 0.0:
+            raise ValueError(f"weight_decay must not be negative, got {weight_decay}")
+        if adjust_lr_fn not in (None, "original", "match_rms_adamw"):
+            raise ValueError(f"adjust_lr_fn must be 'original' or 'match_rms_adamw', got "
+                             f"{adjust_lr_fn!r}")
+        super().__init__(params, dict(lr=lr, weight_decay=weight_decay, momentum=momentum,
+                                      nesterov=nesterov, ns_coefficients=ns_coefficients, eps=eps,
+                                      ns_steps=ns_steps, adjust_lr_fn=adjust_lr_fn))
+        for group in self.param_groups:
+            for p in group["params"]:
+                if p.dim() != 2:
+                    raise ValueError(f"parameters must be matrices, got {tuple(p.shape)}")
+
+    @torch.no_grad()
+    def step(self, closure: Any = None) -> Any:
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        for group in self.param_groups:
+            alike: dict[Any, list[nn.Parameter]] = {}
+            for p in group["params"]:
+                if p.grad is not None:
+                    if p.grad.is_sparse:
+                        raise RuntimeError("sparse gradients are not supported")
+                    alike.setdefault((p.shape, p.dtype, p.device), []).append(p)
+            for (shape, dtype, _), params in alike.items():
+                self._update(group, shape, dtype, params)
+        return loss
+
+    def _update(self, group: dict[str, Any], shape: torch.Size, dtype: torch.dtype,
+                params: list[nn.Parameter]) -> None:
+        grads = [p.grad for p in params]
+        for p in params:
+            if "momentum_buffer" not in self.state[p]:
+                self.state[p]["momentum_buffer"] = torch.zeros_like(p)
+        buffers = [self.state[p]["momentum_buffer"] for p in params]
+        torch._foreach_mul_(buffers, group["momentum"])
+        torch._foreach_add_(buffers, grads)
+        updates = torch._foreach_add(grads, buffers, alpha=group["momentum"]) \
+            if group["nesterov"] else buffers
+        rows, columns = shape
+        if group["adjust_lr_fn"] == "match_rms_adamw":
+            ratio = 0.2 * math.sqrt(max(rows, columns))
+        else:
+            ratio = math.sqrt(max(1.0, rows / columns))
+        turned = orthogonalize(torch.stack(updates), group["ns_steps"], group["ns_coefficients"],
+                               group["eps"]).to(dtype)
+        torch._foreach_mul_(params, 1.0 - group["lr"] * group["weight_decay"])
+        torch._foreach_add_(params, list(turned.unbind()), alpha=-group["lr"] * ratio)
+
+
 __all__ = [
     "Dropout",
     "DropoutState",
     "Embedding",
     "LayerNorm",
+    "Muon",
     "OutputBlock",
     "attention",
     "dropout",
@@ -826,4 +1092,5 @@ __all__ = [
     "enable_deberta_training",
     "layer_norm",
     "orthogonalize",
+    "split_parameters",
 ]
