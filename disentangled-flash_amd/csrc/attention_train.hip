@@ -1218,20 +1218,23 @@ __global__ __launch_bounds__(256) void attention_train_query_kernel(Params p) {
 // ---- dPK and dPQ by delta -------------------------------------------------------------------
 
 // The tiles of 64 x 64 with (query block) - (key block) = m, of all sequences of one head, share
-// their deltas, 64 m - 63 .. 64 m + 63: place 64 + (i - j) - 64 m of 128.  `tiles` of them are one
-// workgroup's; the parts of a diagonal are added up by the next kernel.
+// their deltas, 64 m - 63 .. 64 m + 63: place 64 + (i - j) - 64 m of 128.  2^`shift` of them are one
+// workgroup's; the parts of a diagonal are added up by the next kernel.  Every diagonal has the
+// room of the longest, m = 0.
 struct Diagonals {
-  int blocks, batch, tiles;
+  int blocks, batch, shift;
+  __host__ __device__ int count() const { return 2 * blocks - 1; }
+  __host__ __device__ int tiles(int m) const { return batch * (blocks - (m < 0 ? -m : m)); }
   __host__ __device__ int parts(int m) const {
-    const int n = batch * (blocks - (m < 0 ? -m : m));
-    return (n + tiles - 1) / tiles;
+    return (tiles(m) + (1 << shift) - 1) >> shift;
   }
   // Diagonals in the order 0, 1, -1, 2, -2, ..: the longest first.
   __host__ __device__ static int nth(int n) { return n % 2 ? (n + 1) / 2 : -(n / 2); }
-  __host__ __device__ int total() const {
-    int sum = 0;
-    for (int n = 0; n < 2 * blocks - 1; ++n) sum += parts(nth(n));
-    return sum;
+  __host__ __device__ static int order(int m) { return m > 0 ? 2 * m - 1 : -2 * m; }
+  __host__ __device__ int per_head() const { return count() * parts(0); }
+  // The first part of diagonal m.
+  __host__ __device__ int64_t first(int head, int m) const {
+    return static_cast<int64_t>(head) * per_head() + order(m) * parts(0);
   }
 };
 
@@ -1243,17 +1246,16 @@ struct PositionLayout {
 };
 
 template <typename T, int D>
-__global__ __launch_bounds__(256) void attention_train_position_kernel(Params p, Diagonals dg,
-                                                                       int per_head) {
+__global__ __launch_bounds__(256) void attention_train_position_kernel(Params p, Diagonals dg) {
   using Y = PositionLayout<T, D>;
   using F = typename Op<T>::frag;
   constexpr int LD = Y::LD, LDX = Y::LDX;
   extern __shared__ __align__(16) unsigned char memory[];
   Y& s = *reinterpret_cast<Y*>(memory);
-  const int hh = blockIdx.x % p.nh, rest = blockIdx.x / p.nh;  // (heads first: longest first)
-  int n = 0, part = rest;
-  for (; part >= dg.parts(Diagonals::nth(n)); ++n) part -= dg.parts(Diagonals::nth(n));
-  const int m = Diagonals::nth(n);
+  // Heads first, then parts: the long diagonals start first.
+  const int hh = blockIdx.x % p.nh, part = blockIdx.x / p.nh % dg.parts(0);
+  const int m = Diagonals::nth(blockIdx.x / p.nh / dg.parts(0));
+  if (part >= dg.parts(m)) return;
   const int along = dg.blocks - (m < 0 ? -m : m);
   const int h = p.h0 + hh;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
@@ -1265,7 +1267,7 @@ __global__ __launch_bounds__(256) void attention_train_position_kernel(Params p,
   const int q32 = 2 * dg.blocks;
   const bool pk = p.pos_key != nullptr, pq = p.pos_query != nullptr;
   f32x4_t dpk[2][D / 16] = {}, dpq[2][D / 16] = {};
-  const int end = min((part + 1) * dg.tiles, dg.batch * along);
+  const int end = min((part + 1) << dg.shift, dg.tiles(m));
   Stage<T, D, 64, 256> next_q, next_k;
   F next_g[2];
   // Reads the tile `u` or the first after it that has kept queries and keys.
@@ -1290,7 +1292,7 @@ __global__ __launch_bounds__(256) void attention_train_position_kernel(Params p,
     }
     return u;
   };
-  for (int u = read_tile(part * dg.tiles); u < end;) {
+  for (int u = read_tile(part << dg.shift); u < end;) {
     lds_barrier();
     if (pk) next_q.store(s.q);
     if (pq) next_k.store(s.k);
@@ -1330,7 +1332,7 @@ __global__ __launch_bounds__(256) void attention_train_position_kernel(Params p,
       }
     }
   }
-  float* out = p.partial + (static_cast<int64_t>(hh) * per_head + rest) * 2 * 128 * D;
+  float* out = p.partial + (dg.first(hh, m) + part) * 256 * D;
 #pragma unroll
   for (int half = 0; half < 2; ++half) {
     float* to = out + (16 * (wave + 4 * half) + c) * D + 4 * g;
@@ -1347,14 +1349,10 @@ __global__ __launch_bounds__(256) void attention_train_position_kernel(Params p,
 // The parts of a diagonal are added up in the place of its first.  256 threads take 1024 of its
 // 256 D sums.
 __global__ __launch_bounds__(256) void attention_train_parts_kernel(float* partial, int D,
-                                                                    Diagonals dg, int per_head) {
-  const int nth = blockIdx.y;
-  int first = 0;
-  for (int n = 0; n < nth; ++n) first += dg.parts(Diagonals::nth(n));
-  const int parts = dg.parts(Diagonals::nth(nth));
+                                                                    Diagonals dg) {
+  const int m = Diagonals::nth(blockIdx.y), parts = dg.parts(m);
   const int64_t step = 256 * D;
-  float* at = partial + (static_cast<int64_t>(blockIdx.z) * per_head + first) * step +
-              (blockIdx.x * 256 + threadIdx.x) * 4;
+  float* at = partial + dg.first(blockIdx.z, m) * step + (blockIdx.x * 256 + threadIdx.x) * 4;
   f32x4_t sum{};
 #pragma unroll 4
   for (int n = 0; n < parts; ++n) sum += *reinterpret_cast<const f32x4_t*>(at + n * step);
@@ -1363,62 +1361,69 @@ __global__ __launch_bounds__(256) void attention_train_parts_kernel(float* parti
 
 // One workgroup for a slot of a head: the sums of its deltas, each of two diagonals.
 template <typename T, int D>
-__global__ __launch_bounds__(512) void attention_train_slot_kernel(
+__global__ __launch_bounds__(256) void attention_train_slot_kernel(
     const float* partial, const int32_t* lut, T* dpos_key, T* dpos_query, float* carry, int first,
-    int last, int L, int S, int H, int h0, Diagonals dg, int per_head, float scale) {
-  constexpr int kThreads = 512, kLanes = D / 4, kGroups = kThreads / kLanes;
+    int last, int L, int S, int H, int h0, Diagonals dg, float scale) {
+  constexpr int kThreads = 256, kLanes = D / 4, kGroups = kThreads / kLanes;
   constexpr int kSpan = 4096;  // deltas looked through at a time
   __shared__ f32x4_t sums[2][kThreads];
   __shared__ int16_t found[kSpan];
-  __shared__ int counts[kSpan / 64], starts[2 * kWords];
+  __shared__ int counts[kThreads / 64];
   const int slot = blockIdx.x, hh = blockIdx.y;
   const int lane = threadIdx.x % kLanes, group = threadIdx.x / kLanes;
   const int wave = threadIdx.x / 64, bit = threadIdx.x % 64;
-  // Where the diagonal m = n - (blocks - 1) begins.
-  for (int n = threadIdx.x; n < 2 * dg.blocks - 1; n += kThreads) {
-    const int m = n - (dg.blocks - 1), order = m > 0 ? 2 * m - 1 : -2 * m;
-    int at = 0;
-    for (int x = 0; x < order; ++x) at += dg.parts(Diagonals::nth(x));
-    starts[n] = at;
-  }
   f32x4_t sum[2] = {};
-  const float* base = partial + static_cast<int64_t>(hh) * per_head * 256 * D;
+  const __amdgpu_buffer_rsrc_t table = resource(lut, (2 * static_cast<int64_t>(L) - 1) * 4);
   for (int from = 0; from < 2 * L - 1; from += kSpan) {
-    // The deltas of this slot, in order: counted by 64, then listed.
-    __syncthreads();
-    const int until = min(from + kSpan, 2 * L - 1);
-    for (int n = wave; from + 64 * n < until; n += kThreads / 64) {
-      const int at = from + 64 * n + bit;
-      const uint64_t match = __ballot(at < until && lut[at] == slot);
-      if (bit == 0) counts[n] = __popcll(match);
-    }
-    __syncthreads();
-    int total = 0;
-    for (int n = 0; from + 64 * n < until; ++n) {
-      if (n % (kThreads / 64) == wave && counts[n]) {
-        const int at = from + 64 * n + bit;
-        const uint64_t match = __ballot(at < until && lut[at] == slot);
-        if ((match >> bit) & 1)
-          found[total + __popcll(match & ((uint64_t{1} << bit) - 1))] =
-              static_cast<int16_t>(64 * n + bit);
+    // The deltas of this slot are listed, each wavefront's 1024 in an order of its own: four loads of
+    // four places a lane, all in flight together.
+    constexpr int kLoads = kSpan / kThreads / 4;
+    u32x4_t places[kLoads];
+#pragma unroll
+    for (int n = 0; n < kLoads; ++n)
+      places[n] = __builtin_amdgcn_raw_buffer_load_b128(
+          table, 4 * (from + (wave * kLoads + n) * 256 + 4 * bit), 0, 0);
+    uint64_t match[kLoads][4];
+    int mine = 0;
+#pragma unroll
+    for (int n = 0; n < kLoads; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int at = from + (wave * kLoads + n) * 256 + 4 * bit + e;
+        match[n][e] = __ballot(at < 2 * L - 1 && static_cast<int>(places[n][e]) == slot);
+        mine += __popcll(match[n][e]);
       }
+    __syncthreads();
+    if (bit == 0) counts[wave] = mine;
+    __syncthreads();
+    int total = 0, to = 0;
+#pragma unroll
+    for (int n = 0; n < kThreads / 64; ++n) {
+      if (n == wave) to = total;
       total += counts[n];
     }
-    __syncthreads();
-#pragma unroll 4
-    for (int n = group; n < total; n += kGroups) {
-      // delta = 64 lower + place: place 64 + place of the diagonal `lower`, `place` of the next.
-      const int up = from + found[n] - (L - 1) + 64 * dg.blocks;
-      const int lower = up / 64 - dg.blocks, place = up % 64;
 #pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        const int m = lower + x;
-        if (m <= -dg.blocks || m >= dg.blocks) continue;
-        const float* at = base + static_cast<int64_t>(starts[m + dg.blocks - 1]) * 256 * D +
-                          (x ? place : 64 + place) * D + lane * 4;
-        sum[0] += *reinterpret_cast<const f32x4_t*>(at);
-        sum[1] += *reinterpret_cast<const f32x4_t*>(at + 128 * D);
+    for (int n = 0; n < kLoads; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if ((match[n][e] >> bit) & 1)
+          found[to + __popcll(match[n][e] & ((uint64_t{1} << bit) - 1))] =
+              static_cast<int16_t>((wave * kLoads + n) * 256 + 4 * bit + e);
+        to += __popcll(match[n][e]);
       }
+    __syncthreads();
+    // Twice each: delta = 64 lower + place is place 64 + place of the diagonal `lower` and `place` of
+    // the next.  (Without branches, so that eight are in flight.  Where there is no such diagonal
+    // place 0 is read, which no delta has.)
+#pragma unroll 8
+    for (int n = group; n < 2 * total; n += kGroups) {
+      const int x = n & 1, up = from + found[n >> 1] - (L - 1) + 64 * dg.blocks;
+      const int m = up / 64 - dg.blocks + x;
+      const bool none = m <= -dg.blocks || m >= dg.blocks;
+      const float* at = partial + dg.first(hh, none ? 0 : m) * 256 * D +
+                        (none ? 0 : 64 - 64 * x + up % 64) * D + lane * 4;
+      sum[0] += *reinterpret_cast<const f32x4_t*>(at);
+      sum[1] += *reinterpret_cast<const f32x4_t*>(at + 128 * D);
     }
   }
   sums[0][threadIdx.x] = sum[0];
@@ -1470,7 +1475,7 @@ int launch_forward(const Params& p, hipStream_t stream) {
 // How the backward pass divides its work.
 struct Plan {
   int batch, heads;  // (batch, head) pairs of one launch: all heads, or some of one batch
-  int blocks, tiles, per_head;
+  int blocks, shift;
   size_t g, partial, carry, delta, words, total;
 };
 
@@ -1487,12 +1492,11 @@ Plan make_plan(int B, int H, int L, int S, int D, int esize) {
   x.batch = x.heads == H ? static_cast<int>(fit / H) : 1;
   if (x.batch > B) x.batch = B;
   const int64_t all = static_cast<int64_t>(x.batch) * x.heads * x.blocks * x.blocks;
-  // About 1024 workgroups, of 64 tiles at most.
-  int64_t tiles = (all + 1023) / 1024;
-  x.tiles = static_cast<int>(tiles < 1 ? 1 : tiles > 64 ? 64 : tiles);
-  x.per_head = Diagonals{x.blocks, x.batch, x.tiles}.total();
+  // From 512 to 1024 workgroups, of 64 tiles at most.
+  while (x.shift < 6 && all >> x.shift > 1024) ++x.shift;
+  const int per_head = Diagonals{x.blocks, x.batch, x.shift}.per_head();
   x.g = round_up(each * x.batch * x.heads);
-  x.partial = S > 0 ? round_up(static_cast<size_t>(x.heads) * x.per_head * 256 * D * 4) : 0;
+  x.partial = S > 0 ? round_up(static_cast<size_t>(x.heads) * per_head * 256 * D * 4) : 0;
   x.carry = S > 0 && x.batch < B ? round_up(static_cast<size_t>(2) * S * H * D * 4) : 0;
   x.delta = round_up(static_cast<size_t>(B) * H * L * 4);
   x.words = round_up(static_cast<size_t>(B) * x.blocks * 8);
@@ -1540,16 +1544,16 @@ int launch_backward(Params p, const void* out, void* dpos_key, void* dpos_query,
       hipLaunchKernelGGL((attention_train_query_kernel<T, D>), dim3(pairs * plan.blocks), dim3(256),
                          sizeof(YQ), stream, p);
       if (dpos_key || dpos_query) {
-        const Diagonals dg{plan.blocks, p.nb, plan.tiles};
-        const int per_head = dg.total();
-        hipLaunchKernelGGL((attention_train_position_kernel<T, D>), dim3(p.nh * per_head), dim3(256),
-                           sizeof(YP), stream, p, dg, per_head);
-        hipLaunchKernelGGL(attention_train_parts_kernel, dim3(D / 4, 2 * dg.blocks - 1, p.nh),
-                           dim3(256), 0, stream, p.partial, D, dg, per_head);
-        hipLaunchKernelGGL((attention_train_slot_kernel<T, D>), dim3(p.S, p.nh), dim3(512), 0,
-                           stream, p.partial, p.lut, static_cast<T*>(dpos_key),
+        const Diagonals dg{plan.blocks, p.nb, plan.shift};
+        hipLaunchKernelGGL((attention_train_position_kernel<T, D>), dim3(p.nh * dg.per_head()), dim3(256),
+                           sizeof(YP), stream, p, dg);
+        if (dg.parts(0) > 1)
+          hipLaunchKernelGGL(attention_train_parts_kernel, dim3(D / 4, dg.count(), p.nh), dim3(256), 0,
+                             stream, p.partial, D, dg);
+        hipLaunchKernelGGL((attention_train_slot_kernel<T, D>), dim3(p.S, p.nh), dim3(256), 0, stream,
+                           p.partial, p.lut, static_cast<T*>(dpos_key),
                            static_cast<T*>(dpos_query), carry, b0 == 0, b0 + p.nb == p.B, p.L, p.S,
-                           p.H, h0, dg, per_head, p.scale);
+                           p.H, h0, dg, p.scale);
       }
     }
   }
@@ -1579,7 +1583,7 @@ int make_params(const dflash_attention_train* a, Params& p) {
   if (a->D != 32 && a->D != 64 && a->D != 128) return DFLASH_ERR_HEAD_DIM;
   if (a->dtype < DFLASH_DTYPE_FP16 || a->dtype > DFLASH_DTYPE_FP32) return DFLASH_ERR_DTYPE;
   if (a->L > kMaxLength || static_cast<int64_t>(a->B) * a->H > (1 << 20) ||
-      static_cast<int64_t>(a->S) * a->H >= (1 << 23) || a->H > 65535)
+      static_cast<int64_t>(a->S) * a->H >= (1 << 22) || a->H > 65535)
     return DFLASH_ERR_TOO_LARGE;
   const bool relative = a->pos_key || a->pos_query;
   if (!a->query || !a->key || !a->value || (relative && (!a->delta_to_slot || a->S < 1)))

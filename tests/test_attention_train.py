@@ -175,7 +175,7 @@ def test_c_attention_refusals(lib):
         (head_dim, {"D": 48}), (dtype, {"dtype": 3}), (align, {"key": at + 8}),
         (align, {"pos_query": at + 2}), (align, {"delta_to_slot": at + 2}),
         (align, {"query_strides": strides}), (large, {"L": 16385}),
-        (large, {"B": 1 << 20}), (large, {"S": 1 << 22}),
+        (large, {"B": 1 << 20}), (large, {"S": 1 << 21}),
     ):
         a = _struct(**changed)
         assert lib.dflash_attention_train_fwd(a, None, 0, at, None, None, None) == code, changed
