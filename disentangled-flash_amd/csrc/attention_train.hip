@@ -62,6 +62,7 @@ struct Params {
   const uint8_t* bits;    // dropped places, rows of `bit_row` bytes; NULL: no dropout
   int64_t bit_row;
   void* out;              // [B, L, H, D]
+  void* low;              // what `out`'s rounding left off, may be NULL
   float* lse;             // [B, H, L], base 2
   const void* dout;       // [B, L, H, D]
   const float* delta;     // [B, H, L]: D_i
@@ -155,12 +156,15 @@ __device__ inline typename Op<T>::half read_columns_half(const T* p, int ld, int
   }
 }
 
-// Scores by delta, scaled, in LDS.  Beside 16-bit inputs they are fp16: off by at most half a step, 2^-12
-// of their size, which moves a probability by 2^-12 |score| of itself where its rounding as an operand
-// moves it by 2^-12 (fp16) or 2^-9 (bf16).  In fp32 their buffers let one workgroup of four
-// wavefronts run on a CU, as fp16 two.
+// Scores by delta, scaled, in LDS: fp32, but for the forward pass of bf16 inputs.  fp16 is off by up to
+// half a step, 2^-12 of a score, and a probability by that times the score.  Beside fp16 operands
+// that was the largest error: the gradients of 16 x 384 tokens, heads of 32, were off by 4.0e-4 of their
+// size, with fp32 by 3.0e-4.  Probabilities of bf16 are rounded to 2^-9 of themselves, beside which
+// it is little; the backward pass has fp32 all the same (279 us for 268 at 32 x 512 tokens), as all that
+// a gradient is off by adds up there, and the forward pass fp16 (190 us, 246 with fp32).
 template <typename T>
-using Score = std::conditional_t<sizeof(T) == 4, float, _Float16>;
+using FwdScore = std::conditional_t<std::is_same_v<T, __bf16>, _Float16, float>;
+using KeyScore = float;
 
 // Eight values of the accumulators of two blocks of 16 rows as an operand: element e < 4 is row
 // 4g + e of the first, e >= 4 row 4g + e - 4 of the second.
@@ -172,6 +176,14 @@ __device__ inline typename Op<T>::frag pack(f32x4_t a, f32x4_t b) {
 #pragma unroll
   for (int e = 0; e < 4; ++e) f[4 + e] = static_cast<T>(b[e]);
   return f;
+}
+
+// What rounding to T left off.
+template <typename T>
+__device__ inline f32x4_t left(f32x4_t x) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e) x[e] -= static_cast<float>(static_cast<T>(x[e]));
+  return x;
 }
 
 // The same from global memory; `from`: byte offset of the eight.
@@ -452,7 +464,7 @@ struct FwdLayout {
   static constexpr int BQ = 16 * NW, W = BQ + BK, LDC = BK + 20, LDP = BQ + 20;
   static constexpr int LD = kLd<T, D>;
   T k[BK * LD], v[BK * LD], pk[W * LD], pq[W * LD];
-  Score<T> c2p[BQ * LDC], p2c[BK * LDP];
+  FwdScore<T> c2p[BQ * LDC], p2c[BK * LDP];
   uint64_t kept[kWords];
 };
 
@@ -556,15 +568,23 @@ void attention_train_fwd_kernel(Params p) {
       const uint64_t kept = ~((static_cast<uint64_t>(word[1]) << 32 | word[0]) >> (j0 % 64));
       drop<KB>(x, kept >> (4 * g));
     }
-    // (Rounded to T here, as the operand of the product: off by half a step of each probability.)
+    // A probability of 16 bits is the operand in two parts, itself rounded and what that left off.
+    // Rounded alone it puts an error into D_i = dO_i.O_i that all gradients of a query share, and
+    // that weighs more where many deltas have one slot.  Over 2000 tokens in bf16 the gradients were off by
+    // 2.7e-3 of their size, with both parts and with `low` by 2.5e-3, and outputs of fp16 by 2.7e-4 and
+    // 2.1e-4, their own rounding.  At 32 x 512 tokens it takes 198 us instead of 186.
 #pragma unroll
     for (int ks = 0; ks < KB / 2; ++ks) {
       const F r = pack<T>(x[2 * ks], x[2 * ks + 1]);
+      F rest;
+      if constexpr (sizeof(T) == 2) rest = pack<T>(left<T>(x[2 * ks]), left<T>(x[2 * ks + 1]));
 #pragma unroll
-      for (int db = 0; db < D / 16; ++db)
-        o[db] = Op<T>::run(
-            read_columns<T>(s.v + 16 * db, LD, 32 * ks + 4 * g, 32 * ks + 16 + 4 * g, c), r,
-            o[db]);
+      for (int db = 0; db < D / 16; ++db) {
+        const F values =
+            read_columns<T>(s.v + 16 * db, LD, 32 * ks + 4 * g, 32 * ks + 16 + 4 * g, c);
+        if constexpr (sizeof(T) == 2) o[db] = Op<T>::run(values, rest, o[db]);
+        o[db] = Op<T>::run(values, r, o[db]);
+      }
     }
   };
 
@@ -701,9 +721,19 @@ void attention_train_fwd_kernel(Params p) {
   sum += __shfl_xor(sum, 32);
   if (i >= p.L) return;
   const float factor = p.keep_scale / sum;
-  T* out = static_cast<T*>(p.out) + ((static_cast<int64_t>(b) * p.L + i) * p.H + h) * D;
+  const int64_t to = ((static_cast<int64_t>(b) * p.L + i) * p.H + h) * D + 4 * g;
 #pragma unroll
-  for (int db = 0; db < D / 16; ++db) store4(out + 16 * db + 4 * g, o[db] * factor);
+  for (int db = 0; db < D / 16; ++db) {
+    o[db] *= factor;
+    store4(static_cast<T*>(p.out) + to + 16 * db, o[db]);
+  }
+  if constexpr (sizeof(T) == 2) {
+    if (p.low) {
+#pragma unroll
+      for (int db = 0; db < D / 16; ++db)
+        store4(static_cast<T*>(p.low) + to + 16 * db, left<T>(o[db]));
+    }
+  }
   if (p.lse && g == 0) p.lse[static_cast<int64_t>(bh) * p.L + i] = top + log2f(sum);
 }
 
@@ -711,7 +741,7 @@ void attention_train_fwd_kernel(Params p) {
 
 template <typename T, int D>
 __global__ __launch_bounds__(256) void attention_delta_kernel(const T* dout, const T* out,
-                                                              float* delta, int64_t rows, int H,
+                                                              const T* low, float* delta, int64_t rows, int H,
                                                               int L) {
   constexpr int N = Chunk<T>::N, kLanes = D / N;
   const int64_t at = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) / kLanes;
@@ -723,6 +753,11 @@ __global__ __launch_bounds__(256) void attention_delta_kernel(const T* dout, con
     load_floats<T, N>(out + at * D + lane * N, y);
 #pragma unroll
     for (int e = 0; e < N; ++e) sum += x[e] * y[e];
+    if (low) {
+      load_floats<T, N>(low + at * D + lane * N, y);
+#pragma unroll
+      for (int e = 0; e < N; ++e) sum += x[e] * y[e];
+    }
   }
 #pragma unroll
   for (int step = 1; step < kLanes; step *= 2) sum += __shfl_xor(sum, step);
@@ -747,9 +782,10 @@ struct KeyLayout {
   static constexpr int W = BQ + BK;
   static constexpr int kWide = BK < 64 ? 1 : BK / 64;  // words of the generator's bits a query
   // A wavefront's scores of its keys by delta, and after them G by delta.
-  static constexpr int kScores = 16 * LDP * static_cast<int>(sizeof(Score<T>)), kSkew = 16 * LDF * static_cast<int>(sizeof(T));
+  static constexpr int kScores = 16 * LDP * static_cast<int>(sizeof(KeyScore));
+  static constexpr int kSkew = 16 * LDF * static_cast<int>(sizeof(T));
   T q[BQ * LD], dout[BQ * LD], pk[W * LD], pq[W * LD];
-  Score<T> c2p[BQ * LDC];
+  KeyScore c2p[BQ * LDC];
   unsigned char own[NW * (kScores > kSkew ? kScores : kSkew)];
   float lse[BQ], delta[BQ];
   uint16_t places[NW][BQ];  // bit c of a wavefront's row: the place of key c is kept
@@ -775,7 +811,7 @@ void attention_train_key_kernel(Params p) {
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
   const int lane = threadIdx.x % 64, c = lane % 16, g = lane / 16;
   const int j = j0 + 16 * wave + c;
-  Score<T>* scores = reinterpret_cast<Score<T>*>(s.own + wave * (sizeof(s.own) / NW));
+  KeyScore* scores = reinterpret_cast<KeyScore*>(s.own + wave * (sizeof(s.own) / NW));
   T* skew = reinterpret_cast<T*>(scores);
 
   read_mask(s.kept, p.mask, b, p.L);
@@ -1505,7 +1541,7 @@ Plan make_plan(int B, int H, int L, int S, int D, int esize) {
 }
 
 template <typename T, int D, bool BOTH>
-int launch_backward(Params p, const void* out, void* dpos_key, void* dpos_query, char* workspace,
+int launch_backward(Params p, const void* out, const void* low, void* dpos_key, void* dpos_query, char* workspace,
                     hipStream_t stream) {
   constexpr int NW = Sizes<T, D>::kKeyWaves, BQ = Sizes<T, D>::kKeyQueries;
   using YK = KeyLayout<T, D, NW, BQ>;
@@ -1529,8 +1565,8 @@ int launch_backward(Params p, const void* out, void* dpos_key, void* dpos_query,
   constexpr int kRows = 256 / (D / Chunk<T>::N);
   hipLaunchKernelGGL((attention_delta_kernel<T, D>),
                      dim3(static_cast<uint32_t>((rows + kRows - 1) / kRows)), dim3(256), 0, stream,
-                     static_cast<const T*>(p.dout), static_cast<const T*>(out), delta, rows, p.H,
-                     p.L);
+                     static_cast<const T*>(p.dout), static_cast<const T*>(out),
+                     sizeof(T) == 2 ? static_cast<const T*>(low) : nullptr, delta, rows, p.H, p.L);
   for (int b0 = 0; b0 < p.B; b0 += plan.batch) {
     for (int h0 = 0; h0 < p.H; h0 += plan.heads) {
       p.b0 = b0;
@@ -1650,13 +1686,13 @@ size_t dflash_attention_train_bits_bytes(int B, int H, int L) {
 }
 
 int dflash_attention_train_fwd(const dflash_attention_train* a, const int64_t* rng, uint32_t site,
-                               void* out, float* lse, void* bits, void* stream) {
+                               void* out, void* out_low, float* lse, void* bits, void* stream) {
   Params p;
   const int rc = make_params(a, p);
   if (rc != DFLASH_OK) return rc;
   if (a->B == 0) return DFLASH_OK;
   if (!out || (a->p > 0 && (!rng || !bits))) return DFLASH_ERR_NULL;
-  if (off(out, 16) || off(lse, 4) || off(bits, 8) || off(rng, 8)) return DFLASH_ERR_ALIGN;
+  if (off(out, 16) || off(out_low, 16) || off(lse, 4) || off(bits, 8) || off(rng, 8)) return DFLASH_ERR_ALIGN;
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (a->p > 0) {
     Dropout d;
@@ -1669,6 +1705,7 @@ int dflash_attention_train_fwd(const dflash_attention_train* a, const int64_t* r
     p.bits = static_cast<const uint8_t*>(bits);
   }
   p.out = out;
+  p.low = out_low;
   p.lse = lse;
   return by_type(a->dtype, a->D, [&](auto t, auto d) {
     using T = decltype(t);
@@ -1684,18 +1721,21 @@ size_t dflash_attention_train_bwd_workspace_bytes(const dflash_attention_train* 
   return make_plan(p.B, p.H, p.L, p.S, a->D, a->dtype == DFLASH_DTYPE_FP32 ? 4 : 2).total;
 }
 
-int dflash_attention_train_bwd(const dflash_attention_train* a, const void* out, const float* lse,
-                               const void* bits, const void* dout, void* dquery, void* dkey,
+int dflash_attention_train_bwd(const dflash_attention_train* a, const void* out,
+                               const void* out_low, const float* lse, const void* bits,
+                               const void* dout, void* dquery, void* dkey,
                                void* dvalue, void* dpos_key, void* dpos_query, void* workspace,
                                size_t workspace_bytes, void* stream) {
   Params p;
   const int rc = make_params(a, p);
   if (rc != DFLASH_OK) return rc;
   if (a->B == 0) return DFLASH_OK;
-  if (!out || !lse || !dout || !dquery || !dkey || !dvalue || !workspace || (a->p > 0 && !bits) ||
+  const bool halves = a->dtype != DFLASH_DTYPE_FP32;
+  if (!out || (halves && !out_low) || !lse || !dout || !dquery || !dkey || !dvalue || !workspace || (a->p > 0 && !bits) ||
       (dpos_key && !a->pos_key) || (dpos_query && !a->pos_query))
     return DFLASH_ERR_NULL;
-  const void* tensors[] = {out, dout, dquery, dkey, dvalue, dpos_key, dpos_query, workspace};
+  const void* tensors[] = {out,  out_low, dout,     dquery,    dkey,
+                           dvalue, dpos_key, dpos_query, workspace};
   for (const void* t : tensors)
     if (off(t, 16)) return DFLASH_ERR_ALIGN;
   if (off(lse, 4) || off(bits, 8)) return DFLASH_ERR_ALIGN;
@@ -1711,7 +1751,7 @@ int dflash_attention_train_bwd(const dflash_attention_train* a, const void* out,
     constexpr int D = decltype(d)::value;
     const auto call = p.pos_key && p.pos_query ? &launch_backward<T, D, true>
                                                : &launch_backward<T, D, false>;
-    return call(p, out, dpos_key, dpos_query, static_cast<char*>(workspace),
+    return call(p, out, out_low, dpos_key, dpos_query, static_cast<char*>(workspace),
                 static_cast<hipStream_t>(stream));
   });
 }

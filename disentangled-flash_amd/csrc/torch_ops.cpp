@@ -334,8 +334,9 @@ dflash_attention_train attention_of(const Tensor& q, const Tensor& k, const Tens
   return a;
 }
 
-// (out, lse, bits); without `statistics` the last two are empty.
-std::tuple<Tensor, Tensor, Tensor> attention_forward(
+// (out, what its 16 bits left off, lse, bits); without `statistics` the middle two are empty, and in
+// fp32 the second.
+std::tuple<Tensor, Tensor, Tensor, Tensor> attention_forward(
     const Tensor& given_q, const Tensor& given_k, const Tensor& given_v,
     const MaybeTensor& given_pk, const MaybeTensor& given_pq, const Tensor& places,
     const MaybeTensor& mask, const MaybeTensor& rng, double scale, double p, int64_t site,
@@ -347,17 +348,19 @@ std::tuple<Tensor, Tensor, Tensor> attention_forward(
   expect(p == 0 || rng, "rng");
   Tensor out = fresh(q.sizes(), q.scalar_type(), q);
   const bool any = q.numel() > 0;
+  const bool halves = statistics && q.scalar_type() != at::kFloat;
+  Tensor low = halves ? fresh(q.sizes(), q.scalar_type(), q) : fresh({0}, q.scalar_type(), q);
   Tensor lse = fresh({statistics ? a.B : 0, a.H, a.L}, at::kFloat, q);
   const size_t bytes = p > 0 && any ? lib.attention_bits_bytes(a.B, a.H, a.L) : 0;
   Tensor bits = fresh({static_cast<int64_t>(bytes)}, at::kByte, q);
   if (any) {
     On on(q);
-    check(lib.attention_fwd(&a, words(rng), site, data(out),
+    check(lib.attention_fwd(&a, words(rng), site, data(out), halves ? data(low) : nullptr,
                             statistics ? static_cast<float*>(data(lse)) : nullptr,
                             bytes ? data(bits) : nullptr, on.stream),
           "dflash_attention_train_fwd");
   }
-  return {out, lse, bits};
+  return {out, low, lse, bits};
 }
 
 Tensor attention(const Tensor& q, const Tensor& k, const Tensor& v, const MaybeTensor& pk,
@@ -367,7 +370,7 @@ Tensor attention(const Tensor& q, const Tensor& k, const Tensor& v, const MaybeT
       attention_forward(q, k, v, pk, pq, places, mask, rng, scale, p, site, false));
 }
 
-std::tuple<Tensor, Tensor, Tensor> attention_train(
+std::tuple<Tensor, Tensor, Tensor, Tensor> attention_train(
     const Tensor& q, const Tensor& k, const Tensor& v, const MaybeTensor& pk,
     const MaybeTensor& pq, const Tensor& places, const MaybeTensor& mask, const MaybeTensor& rng,
     double scale, double p, int64_t site) {
@@ -376,8 +379,8 @@ std::tuple<Tensor, Tensor, Tensor> attention_train(
 
 // (dquery, dkey, dvalue, dpos_key, dpos_query); the tables' [S, H, D], empty where not wanted.
 std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> attention_backward(
-    const Tensor& given_dout, const Tensor& out, const Tensor& lse, const Tensor& bits,
-    const Tensor& given_q, const Tensor& given_k, const Tensor& given_v,
+    const Tensor& given_dout, const Tensor& out, const Tensor& low, const Tensor& lse,
+    const Tensor& bits, const Tensor& given_q, const Tensor& given_k, const Tensor& given_v,
     const MaybeTensor& given_pk, const MaybeTensor& given_pq, const Tensor& places,
     const MaybeTensor& mask, double scale, double p, bool want_pk, bool want_pq) {
   const Tensor q = with_rows(given_q), k = with_rows(given_k), v = with_rows(given_v);
@@ -387,6 +390,8 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> attention_backward(
              given_dout.scalar_type() == q.scalar_type() && given_dout.device() == q.device(),
          "dout");
   expect(same_form(out, given_dout), "out");
+  const bool halves = q.scalar_type() != at::kFloat;
+  expect(halves ? same_form(low, out) : fits(low, q), "low");
   const bool any = q.numel() > 0;
   expect(fits(lse, q) && lse.scalar_type() == at::kFloat &&
              lse.numel() == static_cast<int64_t>(a.B) * a.H * a.L,
@@ -411,8 +416,8 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> attention_backward(
   const size_t bytes = lib.attention_bwd_workspace_bytes(&a);
   Tensor workspace = fresh({static_cast<int64_t>(bytes)}, at::kByte, q);
   On on(q);
-  check(lib.attention_bwd(&a, data(out), static_cast<const float*>(data(lse)),
-                          p > 0 ? data(bits) : nullptr, data(dout), data(dq), data(dk), data(dv),
+  check(lib.attention_bwd(&a, data(out), halves ? data(low) : nullptr,
+                          static_cast<const float*>(data(lse)), p > 0 ? data(bits) : nullptr, data(dout), data(dq), data(dk), data(dv),
                           want_pk ? data(dpk) : nullptr, want_pq ? data(dpq) : nullptr,
                           data(workspace), bytes, on.stream),
         "dflash_attention_train_bwd");
@@ -601,10 +606,10 @@ struct AttentionNode : Function<AttentionNode> {
                         const MaybeTensor& mask, const MaybeTensor& rng, double scale, double p,
                         int64_t site) {
     at::AutoDispatchBelowADInplaceOrView below;
-    auto [out, lse, bits] =
+    auto [out, low, lse, bits] =
         attention_train_op().call(q, k, v, pk, pq, places, mask, rng, scale, p, site);
-    ctx->save_for_backward({out, lse, bits, q, k, v, pk.value_or(Tensor()), pq.value_or(Tensor()),
-                            places, mask.value_or(Tensor())});
+    ctx->save_for_backward({out, low, lse, bits, q, k, v, pk.value_or(Tensor()),
+                            pq.value_or(Tensor()), places, mask.value_or(Tensor())});
     ctx->saved_data["scale"] = scale;
     ctx->saved_data["p"] = p;
     ctx->saved_data["wanted"] = static_cast<int64_t>(
@@ -621,7 +626,7 @@ struct AttentionNode : Function<AttentionNode> {
       at::AutoDispatchBelowADInplaceOrView below;
       std::tie(all[0], all[1], all[2], all[3], all[4]) = attention_backward_op().call(
           grads[0].contiguous(), saved[0], saved[1], saved[2], saved[3], saved[4], saved[5],
-          maybe(saved[6]), maybe(saved[7]), saved[8], maybe(saved[9]),
+          saved[6], maybe(saved[7]), maybe(saved[8]), saved[9], maybe(saved[10]),
           ctx->saved_data["scale"].toDouble(), ctx->saved_data["p"].toDouble(), wanted & 8,
           wanted & 16);
       for (int n : {3, 4})
@@ -698,10 +703,10 @@ TORCH_LIBRARY_FRAGMENT(disentangled_flash, m) {
   m.def(
       "attention_train(Tensor query, Tensor key, Tensor value, Tensor? pos_key, "
       "Tensor? pos_query, Tensor delta_to_slot, Tensor? mask, Tensor? rng, float scale, float p, "
-      "int site) -> (Tensor, Tensor, Tensor)");
+      "int site) -> (Tensor, Tensor, Tensor, Tensor)");
   m.def(
-      "attention_backward(Tensor dout, Tensor out, Tensor lse, Tensor bits, Tensor query, "
-      "Tensor key, Tensor value, Tensor? pos_key, Tensor? pos_query, Tensor delta_to_slot, "
+      "attention_backward(Tensor dout, Tensor out, Tensor low, Tensor lse, Tensor bits, "
+      "Tensor query, Tensor key, Tensor value, Tensor? pos_key, Tensor? pos_query, Tensor delta_to_slot, "
       "Tensor? mask, float scale, float p, bool want_pos_key, bool want_pos_query) -> (Tensor, "
       "Tensor, Tensor, Tensor, Tensor)");
   m.def(

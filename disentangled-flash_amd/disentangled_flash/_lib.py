@@ -199,13 +199,13 @@ def _bind(lib: ctypes.CDLL) -> None:
     lib.dflash_attention_train_fwd.restype = _c_int
     lib.dflash_attention_train_fwd.argtypes = [
         ctypes.POINTER(AttentionTrain), _c_void_p, _c_uint32,    # attention, rng, site
-        _c_void_p, _c_void_p, _c_void_p, _c_void_p,              # out, lse, bits, stream
+        _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p,   # out, out_low, lse, bits, stream
     ]
     lib.dflash_attention_train_bwd_workspace_bytes.restype = ctypes.c_size_t
     lib.dflash_attention_train_bwd_workspace_bytes.argtypes = [ctypes.POINTER(AttentionTrain)]
     lib.dflash_attention_train_bwd.restype = _c_int
     lib.dflash_attention_train_bwd.argtypes = [
-        ctypes.POINTER(AttentionTrain), _c_void_p, _c_void_p,    # attention, out, lse
+        ctypes.POINTER(AttentionTrain), _c_void_p, _c_void_p, _c_void_p,  # attention, out, out_low, lse
         _c_void_p, _c_void_p,                                    # bits, dout
         _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p,   # dq, dk, dv, dpos_key, dpos_query
         _c_void_p, ctypes.c_size_t, _c_void_p,                   # workspace, bytes, stream

@@ -134,12 +134,14 @@ def _register_fakes() -> None:
         batch, length, heads, _ = query.shape
         row = (length + 63) // 64 * 8
         bits = batch * heads * length * row if p > 0 else 0
-        return (contiguous(query), query.new_empty((batch, heads, length), dtype=torch.float32),
+        low = query.new_empty(0) if query.dtype == torch.float32 else contiguous(query)
+        return (contiguous(query), low,
+                query.new_empty((batch, heads, length), dtype=torch.float32),
                 query.new_empty(bits, dtype=torch.uint8))
 
     @fake("disentangled_flash::attention_backward")
-    def _(dout, out, lse, bits, query, key, value, pos_key, pos_query, delta_to_slot, mask, scale,
-          p, want_pos_key, want_pos_query):
+    def _(dout, out, low, lse, bits, query, key, value, pos_key, pos_query, delta_to_slot, mask,
+          scale, p, want_pos_key, want_pos_query):
         def table(t, wanted):
             if t is None or not wanted:
                 return query.new_empty(0)

@@ -439,14 +439,16 @@ typedef struct dflash_attention_train {
 
 /*
  *   out  : [B, L, H, D] contiguous
+ *   out_low : of the type and shape of out, what its rounding to 16 bits left off, kept for the
+ *          backward pass; may be NULL, not written in fp32
  *   lse  : fp32 [B, H, L], kept for the backward pass; may be NULL
  *   bits : dflash_attention_train_bits_bytes(B, H, L) bytes, 8-byte aligned: the dropped places,
  *          one bit each, kept for the backward pass; may be NULL when p is 0
  */
 DFLASH_API size_t dflash_attention_train_bits_bytes(int B, int H, int L);
 DFLASH_API int dflash_attention_train_fwd(const dflash_attention_train* attention,
-                                          const int64_t* rng, uint32_t site, void* out, float* lse,
-                                          void* bits, void* stream);
+                                          const int64_t* rng, uint32_t site, void* out,
+                                          void* out_low, float* lse, void* bits, void* stream);
 
 /*
  * Its backward pass, from the same inputs and what the forward pass wrote.
@@ -459,9 +461,9 @@ DFLASH_API int dflash_attention_train_fwd(const dflash_attention_train* attentio
 DFLASH_API size_t dflash_attention_train_bwd_workspace_bytes(
     const dflash_attention_train* attention);
 DFLASH_API int dflash_attention_train_bwd(const dflash_attention_train* attention, const void* out,
-                                          const float* lse, const void* bits, const void* dout,
-                                          void* dquery, void* dkey, void* dvalue, void* dpos_key,
-                                          void* dpos_query, void* workspace,
+                                          const void* out_low, const float* lse, const void* bits,
+                                          const void* dout, void* dquery, void* dkey, void* dvalue,
+                                          void* dpos_key, void* dpos_query, void* workspace,
                                           size_t workspace_bytes, void* stream);
 
 /*

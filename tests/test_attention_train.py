@@ -178,30 +178,32 @@ def test_c_attention_refusals(lib):
         (large, {"B": 1 << 20}), (large, {"S": 1 << 21}),
     ):
         a = _struct(**changed)
-        assert lib.dflash_attention_train_fwd(a, None, 0, at, None, None, None) == code, changed
+        assert lib.dflash_attention_train_fwd(a, None, 0, at, None, None, None, None) == code, changed
         assert lib.dflash_attention_train_bwd_workspace_bytes(a) == 0, changed
-        assert lib.dflash_attention_train_bwd(a, at, at, None, at, at, at, at, None, None, at,
+        assert lib.dflash_attention_train_bwd(a, at, at, at, None, at, at, at, at, None, None, at,
                                               1 << 40, None) == code, changed
     a = _struct()
     fwd, bwd = lib.dflash_attention_train_fwd, lib.dflash_attention_train_bwd
-    assert fwd(a, None, 0, None, None, None, None) == null
-    assert fwd(a, None, 0, at + 8, None, None, None) == align
+    assert fwd(a, None, 0, None, None, None, None, None) == null
+    assert fwd(a, None, 0, at + 8, None, None, None, None) == align
+    assert fwd(a, None, 0, at, at + 8, None, None, None) == align
     dropping = _struct(p=0.1)
-    assert fwd(dropping, None, 0, at, None, at, None) == null
-    assert fwd(dropping, at, 0, at, None, None, None) == null
-    assert fwd(dropping, at, 0, at, None, at + 4, None) == align
+    assert fwd(dropping, None, 0, at, None, None, at, None) == null
+    assert fwd(dropping, at, 0, at, None, None, None, None) == null
+    assert fwd(dropping, at, 0, at, None, None, at + 4, None) == align
     size = lib.dflash_attention_train_bwd_workspace_bytes(a)
     assert size > 0
-    good = [at] * 2 + [None] + [at] * 7 + [size, None]
-    for n, value, code in ((0, None, null), (1, None, null), (3, None, null), (5, None, null),
-                           (0, at + 8, align), (1, at + 2, align), (8, at + 4, align),
-                           (9, None, null), (10, size - 1, -7)):
+    good = [at] * 3 + [None] + [at] * 7 + [size, None]
+    for n, value, code in ((0, None, null), (1, None, null), (2, None, null), (4, None, null),
+                           (6, None, null), (0, at + 8, align), (1, at + 8, align),
+                           (2, at + 2, align), (9, at + 4, align), (10, None, null),
+                           (11, size - 1, -7)):
         args = list(good)
         args[n] = value
         assert bwd(a, *args) == code, n
     args = list(good)
     assert bwd(dropping, *args) == null  # the bits
     assert bwd(_struct(pos_key=None), *args) == null  # a gradient of no table
-    assert fwd(_struct(B=0), None, 0, None, None, None, None) == 0
+    assert fwd(_struct(B=0), None, 0, None, None, None, None, None) == 0
     assert lib.dflash_attention_train_bits_bytes(2, 3, 65) == 2 * 3 * 65 * 16
     assert lib.dflash_attention_train_bits_bytes(0, 3, 65) == 0

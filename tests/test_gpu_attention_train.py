@@ -143,3 +143,24 @@ def test_a_long_sequence(dtype):
     used, lut = compact_position_plan(1100, position_buckets=256, max_relative_positions=512,
                                       position_embedding_size=256)
     _check(_case(13, 1, 1100, 2, 64, dtype, slots=(used.numel(), lut.cuda())), p=0.1)
+
+
+@pytest.mark.parametrize("half,length", [(torch.float16, 17), (torch.bfloat16, 1500)])
+def test_gradients_are_off_by_little_more_than_their_roundings(half, length):
+    """G is rounded once and a gradient once, independently: sqrt(2) of one rounding, by root mean
+    squares.  The rows of G add up to 0, so that on shared slots the sums are smaller than their terms
+    and G's share is larger: 1.47 by a model of the roundings in 64 bits.  An output that was
+    rounded before D, or of rounded probabilities, made it 1.54 (17 tokens) and 1.63."""
+
+    from disentangled_flash.training import attention
+
+    args, dout = _case(23, 1, length, 12 if length < 100 else 2, 64, half, mask="none",
+                       slots=_lut(length, 256, 512))
+    y = attention(*args, p=0.1, rng=_rng(), site=SITE)
+    shape = (1, args[0].shape[2], length, length)
+    want = ref.attention(*args, mult=common.factor(shape, 0.1, _rng(), SITE), dout=dout)
+    for name, value in {"out": y.detach(), **_gradients(y, args[:5], dout)}.items():
+        exact = want[name][0].double().to(value.device)
+        error = (value.double() - exact).square().sum().sqrt()
+        rounding = (exact.to(half).double() - exact).square().sum().sqrt()
+        assert error < (1.2 if name == "out" else 1.52) * rounding, (name, error / rounding)
