@@ -107,10 +107,15 @@ struct Op<float> {
   }
 };
 
-// A row of D elements in LDS is padded by 16 bytes, so that the 16 rows that a fragment read
-// touches lie in different banks.
+// Rows in LDS are padded by 16 bytes: the 16 rows that a fragment read touches lie in different banks.
+// Padded by 32, so do the rows 8g + 0..3 of a transposing read of 16-bit elements, which is worth it where no
+// workgroup less fits a CU for it: in the key kernel (321 -> 288 us at 32 x 512 full tokens, heads of 128
+// 228 -> 207) and in the forward pass with fp32 scores (fp16: 272 -> 263, heads of 128 195 -> 183);
+// the forward pass in bf16 would lose its third workgroup (220 -> 290), as the query kernel (91 -> 109).
 template <typename T, int D>
 constexpr int kLd = D + 16 / static_cast<int>(sizeof(T));
+template <typename T, int D>
+constexpr int kLdWide = sizeof(T) == 2 ? D + 16 : kLd<T, D>;
 
 // Lane (c, g): elements 8g .. 8g+7 of the row of `p` (p: the row, at the k-step's start).
 template <typename T>
@@ -250,7 +255,7 @@ struct Tokens {
 };
 
 // ROWS rows of D elements on their way into LDS, in the registers of NT threads.
-template <typename T, int D, int ROWS, int NT>
+template <typename T, int D, int ROWS, int NT, int LD = kLd<T, D>>
 struct Stage {
   static constexpr int kChunks = D * static_cast<int>(sizeof(T)) / 16;
   static constexpr int kPer = 16 / static_cast<int>(sizeof(T));
@@ -293,7 +298,7 @@ struct Stage {
 #pragma unroll
     for (int n = 0; n < N; ++n)
       if (inside(n))
-        *reinterpret_cast<u32x4_t*>(tile + place(row(n)) * kLd<T, D> + chunk(n) * kPer) = v[n];
+        *reinterpret_cast<u32x4_t*>(tile + place(row(n)) * LD + chunk(n) * kPer) = v[n];
   }
   __device__ void store(T* tile) const {
     store(tile, [](int r) { return r; });
@@ -305,12 +310,12 @@ struct Stage {
 // two steps ahead of their use: first the slots, then the rows, then LDS.  Where the ring is two
 // steps long the loops are written out for both of its positions, PHASE, and every address
 // is a constant (one position at run time cost a quarter of the key kernel's time).
-template <typename T, int D, int ROWS, int STEP, int NT>
+template <typename T, int D, int ROWS, int STEP, int NT, int LD = kLd<T, D>>
 struct Window {
   static_assert(ROWS % 16 == 0 && STEP % 16 == 0 && STEP <= ROWS, "blocks of 16 rows");
   static_assert(ROWS != 2 * STEP || (STEP & (STEP - 1)) == 0, "a power of two");
-  using First = Stage<T, D, ROWS, NT>;
-  using Next = Stage<T, D, STEP, NT>;
+  using First = Stage<T, D, ROWS, NT, LD>;
+  using Next = Stage<T, D, STEP, NT, LD>;
   __amdgpu_buffer_rsrc_t table, lut;
   uint32_t stride;  // bytes
   int L, S;
@@ -462,7 +467,8 @@ __global__ __launch_bounds__(256) void dropped_bits_kernel(uint8_t* bits, int64_
 template <typename T, int D, int NW, int BK>
 struct FwdLayout {
   static constexpr int BQ = 16 * NW, W = BQ + BK, LDC = BK + 20, LDP = BQ + 20;
-  static constexpr int LD = kLd<T, D>;
+  static constexpr int LD =
+      sizeof(FwdScore<T>) == 4 || D == 128 ? kLdWide<T, D> : kLd<T, D>;
   T k[BK * LD], v[BK * LD], pk[W * LD], pq[W * LD];
   FwdScore<T> c2p[BQ * LDC], p2c[BK * LDP];
   uint64_t kept[kWords];
@@ -498,9 +504,9 @@ void attention_train_fwd_kernel(Params p) {
 
   const Tokens<T, D> q(p.q, p.sq, b, h, p.L), k(p.k, p.sk, b, h, p.L), v(p.v, p.sv, b, h, p.L);
   const bool has_pk = BOTH || p.pos_key, has_pq = BOTH || p.pos_query;
-  Window<T, D, Y::W, BK, NT> pk(static_cast<const T*>(p.pos_key) + h * p.pk_h, p.pk_s, p.lut, p.L,
+  Window<T, D, Y::W, BK, NT, LD> pk(static_cast<const T*>(p.pos_key) + h * p.pk_h, p.pk_s, p.lut, p.L,
                                 p.S);
-  Window<T, D, Y::W, BK, NT> pq(static_cast<const T*>(p.pos_query) + h * p.pq_h, p.pq_s, p.lut,
+  Window<T, D, Y::W, BK, NT, LD> pq(static_cast<const T*>(p.pos_query) + h * p.pq_h, p.pq_s, p.lut,
                                 p.L, p.S);
   const bool mine = i < p.L && bit_of(s.kept, i);
 
@@ -518,7 +524,7 @@ void attention_train_fwd_kernel(Params p) {
       p.bits ? p.L * p.bit_row : 0);
   const uint32_t bits_at = i < p.L ? i * static_cast<uint32_t>(p.bit_row) : kNoRow;
 
-  Stage<T, D, BK, NT> next_k, next_v;
+  Stage<T, D, BK, NT, LD> next_k, next_v;
   u32x2_t next_word;
   // V of padded keys is needed where a query is padded.
   auto read_v = [&](int j0) {
@@ -778,7 +784,7 @@ struct KeyLayout {
   static constexpr int BK = 16 * NW, WQ = BK + 16, WK = BQ + 16;
   static constexpr int LDC = WQ + 4, LDP = WK + 4;
   static constexpr int LDF = WK + 8;
-  static constexpr int LD = kLd<T, D>;
+  static constexpr int LD = kLdWide<T, D>;
   static constexpr int W = BQ + BK;
   static constexpr int kWide = BK < 64 ? 1 : BK / 64;  // words of the generator's bits a query
   // A wavefront's scores of its keys by delta, and after them G by delta.
@@ -829,9 +835,9 @@ void attention_train_key_kernel(Params p) {
   const int64_t row = static_cast<int64_t>(p.H) * D;
   const Tokens<T, D> dout(p.dout, Strides{p.L * row, D, row}, b, h, p.L);
   const bool has_pk = BOTH || p.pos_key, has_pq = BOTH || p.pos_query;
-  Window<T, D, Y::W, BQ, NT> pk(static_cast<const T*>(p.pos_key) + h * p.pk_h, p.pk_s, p.lut, p.L,
+  Window<T, D, Y::W, BQ, NT, LD> pk(static_cast<const T*>(p.pos_key) + h * p.pk_h, p.pk_s, p.lut, p.L,
                                  p.S);
-  Window<T, D, Y::W, BQ, NT> pq(static_cast<const T*>(p.pos_query) + h * p.pq_h, p.pq_s, p.lut,
+  Window<T, D, Y::W, BQ, NT, LD> pq(static_cast<const T*>(p.pos_query) + h * p.pq_h, p.pq_s, p.lut,
                                  p.L, p.S);
   // Fragments of this pair: [16 keys][32 queries].
   const int q32 = 2 * words;
@@ -853,7 +859,7 @@ void attention_train_key_kernel(Params p) {
   }
   f32x4_t dk[D / 16] = {}, dv[D / 16] = {};
 
-  Stage<T, D, BQ, NT> next_q, next_dout;
+  Stage<T, D, BQ, NT, LD> next_q, next_dout;
   float next_lse = 0, next_delta = 0;
   u32x2_t next_dropped{};
   static_assert(BQ * kWide <= NT, "one word of dropped places a thread");
@@ -1202,11 +1208,17 @@ __global__ __launch_bounds__(256) void attention_train_query_kernel(Params p) {
       next_k.store(s.k);
       const int key = 16 * wave + c;
 #pragma unroll
+      for (int n = 0; n < 4; ++n) {
+        Quad<T> four;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) four[e] = next_g[n / 2][4 * (n % 2) + e];
+        *reinterpret_cast<Quad<T>*>(s.g + key * LDG + 16 * n + 4 * g) = four;
+      }
+#pragma unroll
       for (int n = 0; n < 2; ++n)
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           const int query = 32 * n + query_of(g, e);
-          s.g[key * LDG + query] = next_g[n][e];
           if (has_pk) s.skew[query * LDE + query % 16 - key + 64] = next_g[n][e];
         }
       if (begun && has_pk) pk.template advance<kPhase>(s.pk);
@@ -1276,9 +1288,14 @@ struct Diagonals {
 
 template <typename T, int D>
 struct PositionLayout {
-  static constexpr int LD = kLd<T, D>, LDX = kLd<T, 64>;
+  static constexpr int LD = kLd<T, D>, LDX = kLd<T, 32>;
   T q[64 * LD], k[64 * LD];
-  T by_query[128 * LDX], by_key[128 * LDX];  // [delta][query], [delta][key]
+  // [half][place][query or key]: 32 queries meet 96 of the 128 places, from 0 or 32 on, and
+  // 32 keys from 32 or 0 on.  (All 128 left room for two workgroups of heads of 64 a CU, not three: 112 us
+  // instead of 98 at 32 x 512 padded tokens.)
+  T by_query[2 * 96 * LDX], by_key[2 * 96 * LDX];
+  uint64_t kept[64][2];                      // of the part's tiles: the queries' and the keys' bits,
+  int at[64][2];                             // sequence and block of queries
 };
 
 template <typename T, int D>
@@ -1296,39 +1313,58 @@ __global__ __launch_bounds__(256) void attention_train_position_kernel(Params p,
   const int h = p.h0 + hh;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
   const int lane = threadIdx.x % 64, c = lane % 16, g = lane / 16;
-  for (int x = threadIdx.x; x < 128 * LDX; x += 256) {
+  for (int x = threadIdx.x; x < 2 * 96 * LDX; x += 256) {
     s.by_query[x] = static_cast<T>(0.0f);
     s.by_key[x] = static_cast<T>(0.0f);
   }
   const int q32 = 2 * dg.blocks;
   const bool pk = p.pos_key != nullptr, pq = p.pos_query != nullptr;
   f32x4_t dpk[2][D / 16] = {}, dpq[2][D / 16] = {};
-  const int end = min((part + 1) << dg.shift, dg.tiles(m));
+  // The part's tiles are looked up together, one a lane, and those with kept queries and keys remembered
+  // as bits (looked up one by one, with a
+  // division each, 24576 tiles took 164 us instead of 162).
+  const int begin = part << dg.shift, end = min((part + 1) << dg.shift, dg.tiles(m));
+  uint64_t live;
+  {
+    const int u = begin + lane, bb = u / along, qt = u % along + (m > 0 ? m : 0);
+    uint64_t kept[2] = {0, 0};
+    if (u < end) {
+      const uint64_t* words = p.words + static_cast<int64_t>(p.b0 + bb) * dg.blocks;
+      kept[0] = words[qt];
+      kept[1] = words[qt - m];
+    }
+    live = __ballot(kept[0] != 0 && kept[1] != 0);
+    if (wave == 0) {
+      s.kept[lane][0] = kept[0];
+      s.kept[lane][1] = kept[1];
+      s.at[lane][0] = bb;
+      s.at[lane][1] = qt;
+    }
+  }
+  __syncthreads();
   Stage<T, D, 64, 256> next_q, next_k;
   F next_g[2];
-  // Reads the tile `u` or the first after it that has kept queries and keys.
-  auto read_tile = [&](int u) {
-    for (; u < end; ++u) {
-      const int bb = u / along, qt = u % along + (m > 0 ? m : 0), kt = qt - m;
-      const int b = p.b0 + bb, i0 = 64 * qt, j0 = 64 * kt;
-      const uint64_t* words = p.words + static_cast<int64_t>(b) * dg.blocks;
-      const uint64_t kept_q = words[qt], kept_k = words[kt];
-      if (kept_q == 0 || kept_k == 0) continue;
-      const T* fragments =
-          static_cast<const T*>(p.g) +
-          ((static_cast<int64_t>(bb * p.nh + hh) * 2 * q32 + j0 / 16 + wave) * q32 + i0 / 32) *
-              kFragment +
-          lane * 8;
+  // Reads the next live tile.
+  auto read_tile = [&]() {
+    const int u = __builtin_ctzll(live);
+    live &= live - 1;
+    const int bb = __builtin_amdgcn_readfirstlane(s.at[u][0]);
+    const int qt = __builtin_amdgcn_readfirstlane(s.at[u][1]), kt = qt - m;
+    const T* fragments =
+        static_cast<const T*>(p.g) +
+        ((static_cast<int64_t>(bb * p.nh + hh) * 2 * q32 + 4 * kt + wave) * q32 + 2 * qt) *
+            kFragment +
+        lane * 8;
 #pragma unroll
-      for (int x = 0; x < 2; ++x)
-        next_g[x] = *reinterpret_cast<const F*>(fragments + x * kFragment);
-      if (pk) next_q.load_tokens(Tokens<T, D>(p.q, p.sq, b, h, p.L), i0, kept_q);
-      if (pq) next_k.load_tokens(Tokens<T, D>(p.k, p.sk, b, h, p.L), j0, kept_k);
-      break;
-    }
-    return u;
+    for (int x = 0; x < 2; ++x)
+      next_g[x] = *reinterpret_cast<const F*>(fragments + x * kFragment);
+    const int b = p.b0 + bb;
+    if (pk) next_q.load_tokens(Tokens<T, D>(p.q, p.sq, b, h, p.L), 64 * qt, s.kept[u][0]);
+    if (pq) next_k.load_tokens(Tokens<T, D>(p.k, p.sk, b, h, p.L), 64 * kt, s.kept[u][1]);
   };
-  for (int u = read_tile(part << dg.shift); u < end;) {
+  bool more = live != 0;
+  if (more) read_tile();
+  while (more) {
     lds_barrier();
     if (pk) next_q.store(s.q);
     if (pq) next_k.store(s.k);
@@ -1337,12 +1373,13 @@ __global__ __launch_bounds__(256) void attention_train_position_kernel(Params p,
     for (int x = 0; x < 2; ++x)
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const int query = 32 * x + query_of(g, e), place = 64 + query - key;
-        if (pk) s.by_query[place * LDX + query] = next_g[x][e];
-        if (pq) s.by_key[place * LDX + key] = next_g[x][e];
+        const int query = query_of(g, e), place = 64 + 32 * x + query - key;
+        if (pk) s.by_query[(64 * x + place) * LDX + query] = next_g[x][e];
+        if (pq) s.by_key[(128 * (wave / 2) - 32 + place) * LDX + key % 32] = next_g[x][e];
       }
     lds_barrier();
-    u = read_tile(u + 1);
+    more = live != 0;
+    if (more) read_tile();
     // Blocks of 16 places `wave` and `wave` + 4; those that a step of 32 queries or keys does not
     // reach are left out.
 #pragma unroll
@@ -1352,14 +1389,14 @@ __global__ __launch_bounds__(256) void attention_train_position_kernel(Params p,
       for (int half = 0; half < 2; ++half) {
         const int wb = wave + 4 * half;
         if (pk && (ks == 0 ? wb < 6 : wb >= 2)) {
-          const F x = read_row<T>(s.by_query + (16 * wb + c) * LDX + 32 * ks, g);
+          const F x = read_row<T>(s.by_query + (64 * ks + 16 * wb + c) * LDX, g);
 #pragma unroll
           for (int db = 0; db < D / 16; ++db)
             dpk[half][db] = Op<T>::run(read_columns<T>(s.q + 16 * db, LD, lo, lo + 4, c), x,
                                        dpk[half][db]);
         }
         if (pq && (ks == 0 ? wb >= 2 : wb < 6)) {
-          const F x = read_row<T>(s.by_key + (16 * wb + c) * LDX + 32 * ks, g);
+          const F x = read_row<T>(s.by_key + (128 * ks - 32 + 16 * wb + c) * LDX, g);
 #pragma unroll
           for (int db = 0; db < D / 16; ++db)
             dpq[half][db] = Op<T>::run(read_columns<T>(s.k + 16 * db, LD, lo, lo + 4, c), x,
@@ -1528,7 +1565,7 @@ Plan make_plan(int B, int H, int L, int S, int D, int esize) {
   x.batch = x.heads == H ? static_cast<int>(fit / H) : 1;
   if (x.batch > B) x.batch = B;
   const int64_t all = static_cast<int64_t>(x.batch) * x.heads * x.blocks * x.blocks;
-  // From 512 to 1024 workgroups, of 64 tiles at most.
+  // From 512 to 1024 workgroups, of 64 tiles at most, which a wavefront looks up together.
   while (x.shift < 6 && all >> x.shift > 1024) ++x.shift;
   const int per_head = Diagonals{x.blocks, x.batch, x.shift}.per_head();
   x.g = round_up(each * x.batch * x.heads);
