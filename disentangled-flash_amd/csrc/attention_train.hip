@@ -15,10 +15,19 @@
 // [row][i - j], whose places outside the band stay 0, and that buffer is the operand of the
 // products with PK, PQ (dQ, dK) and, transposed, with Q, K (dPK, dPQ).
 //
-// Five kernels for the backward pass.  D_i; then one over blocks of keys, which computes P and G,
-// sums dV and dK in registers and writes G once; one over blocks of queries, which sums dQ from
-// G; one over diagonals of tiles, which sums dPK and dPQ from G by delta; and one that adds
-// up the deltas of each slot.  No atomics: every sum has an order of its own.
+// The backward pass: D_i; then a kernel over blocks of keys, which computes P and G, sums dV and dK
+// in registers and writes G once; one over blocks of queries, which sums dQ from G; one over
+// diagonals of tiles, which sums dPK and dPQ from G by delta; one that adds up a diagonal's parts; and
+// one that adds up the deltas of each slot.  No atomics: every sum has an order of its own.
+//
+// Measured (us; heads of 64 in bf16, dropout 0.1, both terms, padded batches):
+//                  dropped places   forward   D    dV dK G   dQ   by delta   parts   by slot
+//   32 x 512 x 12 heads       35       202    14       264   77         97      12        16
+//   2 x 2000 x 12 heads       34       216     6       311   79        101      19        59
+// Of the forward and the dV dK G kernel no part stands out: with the window products, the skewed reads, the
+// skewed buffer and dK, the store of G, the loads of the windows or dV taken out, the latter lost
+// 14 to 28 % each.  Their instructions beside the MFMA (skewed reads of 2 and 4 bytes, conversions, masks)
+// bound them, at two or three wavefronts a SIMD.
 //
 // G is kept in fragments: 16 keys x 32 queries are 512 elements in the order in which the
 // lanes of a wavefront hold them, so that they are written and read 16 bytes a lane.
@@ -234,7 +243,7 @@ __device__ inline void store4(T* p, f32x4_t v) {
 
 // Rows are read through buffer resources: an offset past the size gives zeros, so that rows
 // that are not to be read cost no branch, and all loads of a tile are in flight together
-// (behind a branch for each of them a tile took 11 us).
+// (behind a branch for each of them a tile of the first kernels took 11 us, most of it waiting).
 constexpr uint32_t kNoRow = 0x80000000u;  // past every resource's size
 constexpr int kBufferFlags = 0x00020000;  // raw buffer, gfx9 family descriptor word 3
 
@@ -309,7 +318,7 @@ struct Stage {
 // rows form a ring, so that only the new ones are read.  They are read through the table of slots
 // two steps ahead of their use: first the slots, then the rows, then LDS.  Where the ring is two
 // steps long the loops are written out for both of its positions, PHASE, and every address
-// is a constant (one position at run time cost a quarter of the key kernel's time).
+// is a constant; a longer one has its position in a scalar register.
 template <typename T, int D, int ROWS, int STEP, int NT, int LD = kLd<T, D>>
 struct Window {
   static_assert(ROWS % 16 == 0 && STEP % 16 == 0 && STEP <= ROWS, "blocks of 16 rows");
@@ -1082,7 +1091,8 @@ void attention_train_key_kernel(Params p) {
 #pragma unroll
         for (int ks = 0; ks < BQ / 32; ++ks) {
           const F sk = read_row<T>(skew + c * LDF + 32 * ks, g);
-          const int lo = pq.template place<kPhase>(BK - 16 - 16 * wave + 32 * ks + 16 * (g / 2)) + 8 * (g % 2);
+          const int lo =
+              pq.template place<kPhase>(BK - 16 - 16 * wave + 32 * ks + 16 * (g / 2)) + 8 * (g % 2);
 #pragma unroll
           for (int db = 0; db < D / 16; ++db)
             dk[db] = Op<T>::run(read_columns<T>(s.pq + 16 * db, LD, lo, lo + 4, c), sk, dk[db]);
@@ -1291,8 +1301,8 @@ struct PositionLayout {
   static constexpr int LD = kLd<T, D>, LDX = kLd<T, 32>;
   T q[64 * LD], k[64 * LD];
   // [half][place][query or key]: 32 queries meet 96 of the 128 places, from 0 or 32 on, and
-  // 32 keys from 32 or 0 on.  (All 128 left room for two workgroups of heads of 64 a CU, not three: 112 us
-  // instead of 98 at 32 x 512 padded tokens.)
+  // 32 keys from 32 or 0 on.  (All 128 left room for two workgroups of heads of 64 a CU, not
+  // three: 112 us instead of 97 at 32 x 512 padded tokens.)
   T by_query[2 * 96 * LDX], by_key[2 * 96 * LDX];
   uint64_t kept[64][2];                      // of the part's tiles: the queries' and the keys' bits,
   int at[64][2];                             // sequence and block of queries
@@ -1320,8 +1330,8 @@ __global__ __launch_bounds__(256) void attention_train_position_kernel(Params p,
   const int q32 = 2 * dg.blocks;
   const bool pk = p.pos_key != nullptr, pq = p.pos_query != nullptr;
   f32x4_t dpk[2][D / 16] = {}, dpq[2][D / 16] = {};
-  // The part's tiles are looked up together, one a lane, and those with kept queries and keys remembered
-  // as bits (looked up one by one, with a
+  // The part's tiles are looked up together, one a lane, and those with kept queries and keys are
+  // remembered as bits (looked up one by one, with a
   // division each, 24576 tiles took 164 us instead of 162).
   const int begin = part << dg.shift, end = min((part + 1) << dg.shift, dg.tiles(m));
   uint64_t live;
@@ -1519,7 +1529,11 @@ __global__ __launch_bounds__(256) void attention_train_slot_kernel(
 
 // ---- host -------------------------------------------------------------------------------------
 
-// Two workgroups a CU (80 KB of LDS each) of 16-bit rows of 32 or 64; one of the others.
+// Of 16-bit rows of 32 or 64 elements workgroups of four wavefronts, two to four to a CU by their LDS
+// (34 to 67 KB); of eight, whose windows serve twice the rows, the kernels took 10 % longer there (key
+// kernel 321 -> 353 us, forward 220 -> 249 at 32 x 512 tokens).  Rows of 128 have room for one
+// workgroup, of eight.  In fp32 as many wavefronts as fit.  Tiles are of 32 tokens (64 in fp32, where one
+// workgroup fits a CU either way): with 64 the key kernel spilled registers.
 template <typename T, int D>
 struct Sizes {
   static constexpr bool kWord = sizeof(T) == 4;
@@ -1578,8 +1592,8 @@ Plan make_plan(int B, int H, int L, int S, int D, int esize) {
 }
 
 template <typename T, int D, bool BOTH>
-int launch_backward(Params p, const void* out, const void* low, void* dpos_key, void* dpos_query, char* workspace,
-                    hipStream_t stream) {
+int launch_backward(Params p, const void* out, const void* low, void* dpos_key, void* dpos_query,
+                    char* workspace, hipStream_t stream) {
   constexpr int NW = Sizes<T, D>::kKeyWaves, BQ = Sizes<T, D>::kKeyQueries;
   using YK = KeyLayout<T, D, NW, BQ>;
   using YQ = QueryLayout<T, D>;
@@ -1612,14 +1626,14 @@ int launch_backward(Params p, const void* out, const void* low, void* dpos_key, 
       p.nh = p.H - h0 < plan.heads ? p.H - h0 : plan.heads;
       const int pairs = p.nb * p.nh;
       hipLaunchKernelGGL((attention_train_key_kernel<T, D, NW, BQ, BOTH>),
-                         dim3(pairs * ((64 * plan.blocks + YK::BK - 1) / YK::BK)), dim3(64 * NW), sizeof(YK),
-                         stream, p);
+                         dim3(pairs * ((64 * plan.blocks + YK::BK - 1) / YK::BK)), dim3(64 * NW),
+                         sizeof(YK), stream, p);
       hipLaunchKernelGGL((attention_train_query_kernel<T, D>), dim3(pairs * plan.blocks), dim3(256),
                          sizeof(YQ), stream, p);
       if (dpos_key || dpos_query) {
         const Diagonals dg{plan.blocks, p.nb, plan.shift};
-        hipLaunchKernelGGL((attention_train_position_kernel<T, D>), dim3(p.nh * dg.per_head()), dim3(256),
-                           sizeof(YP), stream, p, dg);
+        hipLaunchKernelGGL((attention_train_position_kernel<T, D>), dim3(p.nh * dg.per_head()),
+                           dim3(256), sizeof(YP), stream, p, dg);
         if (dg.parts(0) > 1)
           hipLaunchKernelGGL(attention_train_parts_kernel, dim3(D / 4, dg.count(), p.nh), dim3(256), 0,
                              stream, p.partial, D, dg);
@@ -1729,7 +1743,8 @@ int dflash_attention_train_fwd(const dflash_attention_train* a, const int64_t* r
   if (rc != DFLASH_OK) return rc;
   if (a->B == 0) return DFLASH_OK;
   if (!out || (a->p > 0 && (!rng || !bits))) return DFLASH_ERR_NULL;
-  if (off(out, 16) || off(out_low, 16) || off(lse, 4) || off(bits, 8) || off(rng, 8)) return DFLASH_ERR_ALIGN;
+  if (off(out, 16) || off(out_low, 16) || off(lse, 4) || off(bits, 8) || off(rng, 8))
+    return DFLASH_ERR_ALIGN;
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (a->p > 0) {
     Dropout d;
@@ -1768,8 +1783,8 @@ int dflash_attention_train_bwd(const dflash_attention_train* a, const void* out,
   if (rc != DFLASH_OK) return rc;
   if (a->B == 0) return DFLASH_OK;
   const bool halves = a->dtype != DFLASH_DTYPE_FP32;
-  if (!out || (halves && !out_low) || !lse || !dout || !dquery || !dkey || !dvalue || !workspace || (a->p > 0 && !bits) ||
-      (dpos_key && !a->pos_key) || (dpos_query && !a->pos_query))
+  if (!out || (halves && !out_low) || !lse || !dout || !dquery || !dkey || !dvalue ||
+      !workspace || (a->p > 0 && !bits) || (dpos_key && !a->pos_key) || (dpos_query && !a->pos_query))
     return DFLASH_ERR_NULL;
   const void* tensors[] = {out,  out_low, dout,     dquery,    dkey,
                            dvalue, dpos_key, dpos_query, workspace};

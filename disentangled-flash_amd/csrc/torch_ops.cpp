@@ -417,7 +417,8 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> attention_backward(
   Tensor workspace = fresh({static_cast<int64_t>(bytes)}, at::kByte, q);
   On on(q);
   check(lib.attention_bwd(&a, data(out), halves ? data(low) : nullptr,
-                          static_cast<const float*>(data(lse)), p > 0 ? data(bits) : nullptr, data(dout), data(dq), data(dk), data(dv),
+                          static_cast<const float*>(data(lse)), p > 0 ? data(bits) : nullptr,
+                          data(dout), data(dq), data(dk), data(dv),
                           want_pk ? data(dpk) : nullptr, want_pq ? data(dpq) : nullptr,
                           data(workspace), bytes, on.stream),
         "dflash_attention_train_bwd");
@@ -706,7 +707,8 @@ TORCH_LIBRARY_FRAGMENT(disentangled_flash, m) {
       "int site) -> (Tensor, Tensor, Tensor, Tensor)");
   m.def(
       "attention_backward(Tensor dout, Tensor out, Tensor low, Tensor lse, Tensor bits, "
-      "Tensor query, Tensor key, Tensor value, Tensor? pos_key, Tensor? pos_query, Tensor delta_to_slot, "
+      "Tensor query, Tensor key, Tensor value, Tensor? pos_key, Tensor? pos_query, "
+      "Tensor delta_to_slot, "
       "Tensor? mask, float scale, float p, bool want_pos_key, bool want_pos_query) -> (Tensor, "
       "Tensor, Tensor, Tensor, Tensor)");
   m.def(

@@ -316,11 +316,12 @@ def attention(
     counts as 0).  ``p``, ``rng`` and ``site`` as in
     :func:`dropout`, on the probabilities ``[B, H, L, L]``.
 
-    Scores and softmax are fp32, but for the relative terms of 16-bit inputs, which are rounded to
-    fp16 after their products; the probabilities, and in the backward pass the gradients of
-    the scores, are rounded to the dtype where they are multiplied.  One bit for each probability is kept for the
-    backward pass, and no ``[L, L]`` tensor besides; the backward pass takes up to 2 GiB of
-    memory for such a tensor at a time.
+    Scores, softmax and sums are fp32, but that the forward pass of bf16 inputs rounds the relative terms
+    to fp16.  Its output is that of unrounded probabilities, rounded once; the backward pass
+    rounds probabilities and the scores' gradients to the dtype where they are multiplied.
+    Kept for it are the inputs, the output, in 16 bits also what its rounding left off, a
+    statistic for each row and with dropout one bit for each probability; it takes up to 2 GiB of
+    memory at a time for the scores' gradients.
     """
 
     p, site, scale = float(p), int(site), float(scale)
@@ -389,8 +390,8 @@ def orthogonalize(
     """The matrices ``update`` ``[..., m, n]`` with their singular values brought near 1, bf16.
 
     ``X = update / (|update|_F + eps)``, then ``steps`` times ``X <- a X + (b A + c A A) X`` with
-    ``A = X X^T`` (transposed where ``m > n``), as the Muon optimiser takes it: with the usual coefficients and
-    five steps, singular values above 1e-3 of the norm come to lie between 0.7 and 1.2.  All matrices
+    ``A = X X^T`` (transposed where ``m > n``), as the Muon optimiser takes it: with the usual
+    coefficients and five steps, singular values above 1e-3 of the norm come to lie between 0.7 and 1.2.  All matrices
     of a call go through the same launches.  The products take fp16 operands and fp32
     sums (2e-3 from the formula's result, which bf16 rounds by as much); the coefficients must
     keep singular values below 128.  Not differentiable: the result has no gradient.
