@@ -24,10 +24,12 @@
 //                  dropped places   forward   D    dV dK G   dQ   by delta   parts   by slot
 //   32 x 512 x 12 heads       35       202    14       264   77         97      12        16
 //   2 x 2000 x 12 heads       34       216     6       311   79        101      19        59
-// Of the forward and the dV dK G kernel no part stands out: with the window products, the skewed reads, the
-// skewed buffer and dK, the store of G, the loads of the windows or dV taken out, the latter lost
-// 14 to 28 % each.  Their instructions beside the MFMA (skewed reads of 2 and 4 bytes, conversions, masks)
-// bound them, at two or three wavefronts a SIMD.
+// No unit bounds the forward and the dV dK G kernel: the matrix unit is busy 11 and 12 % of the time,
+// the vector unit 40 and 25 %, LDS 35 % in either; a wavefront waits at barriers and for loads 40 and 37 % of its
+// time and for its turn to issue 22 %.  It is the chain of products, LDS, skewed reads, exponentials
+// and products again, at three and two wavefronts a SIMD.  Nor does a part stand out: without the
+// window products, the skewed reads, the skewed buffer and dK, the store of G, the loads of the windows
+// or dV, the latter kernel lost 14 to 28 % each.
 //
 // G is kept in fragments: 16 keys x 32 queries are 512 elements in the order in which the
 // lanes of a wavefront hold them, so that they are written and read 16 bytes a lane.

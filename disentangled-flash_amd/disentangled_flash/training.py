@@ -964,8 +964,8 @@ def enable_deberta_training(
 
     Every training forward of the backbone starts with ``model.dropout_state.advance()``, and
     its backward pass has the same step again, so what is checkpointed (a layer, or the whole
-    backbone) recomputes what it computed.  A forward of a backbone in eval mode advances where a dropout in training mode first drops (Monte Carlo dropout, a few
-    layers in training).
+    backbone) recomputes what it computed.  A forward of a backbone in eval mode advances where a
+    dropout in training mode first drops (Monte Carlo dropout, a few layers in training).
 
     ``attention="hip"`` runs the backbone's attention on :func:`attention` too (its projections stay
     torch's products): no ``[L, L]`` tensor of scores or probabilities is made, and the same
@@ -1013,12 +1013,13 @@ def split_parameters(model: nn.Module) -> tuple[list[nn.Parameter], list[nn.Para
 
 
 class Muon(torch.optim.Optimizer):
-    """Muon on :func:`orthogonalize`, for matrices: ``B <- momentum B + g``; the update is ``g + momentum
-    B`` (``B`` without ``nesterov``), orthogonalised; ``p <- (1 - lr weight_decay) p - lr r update``.
+    """Muon on :func:`orthogonalize`, for matrices: ``B <- momentum B + g``; the update is
+    ``g + momentum B`` (``B`` without ``nesterov``), orthogonalised;
+    ``p <- (1 - lr weight_decay) p - lr r update``.
 
-    Names and defaults are those of ``torch.optim.Muon``.  ``adjust_lr_fn`` chooses ``r`` for ``[m, n]``:
-    ``"original"`` (the default) ``sqrt(max(1, m / n))``, ``"match_rms_adamw"`` ``0.2 sqrt(max(m,
-    n))``.  Parameters of one shape, dtype and device are orthogonalised by one call.  They must be on
+    Names and defaults are those of ``torch.optim.Muon``.  ``adjust_lr_fn`` chooses ``r`` for
+    ``[m, n]``: ``"original"`` (the default) ``sqrt(max(1, m / n))``, ``"match_rms_adamw"``
+    ``0.2 sqrt(max(m, n))``.  Parameters of one shape, dtype and device are orthogonalised by one call.  They must be on
     a GPU, in fp16, bf16 or fp32; the momentum is kept in the parameter's dtype.
     """
 
@@ -1038,10 +1039,13 @@ class Muon(torch.optim.Optimizer):
         super().__init__(params, dict(lr=lr, weight_decay=weight_decay, momentum=momentum,
                                       nesterov=nesterov, ns_coefficients=ns_coefficients, eps=eps,
                                       ns_steps=ns_steps, adjust_lr_fn=adjust_lr_fn))
-        for group in self.param_groups:
-            for p in group["params"]:
-                if p.dim() != 2:
-                    raise ValueError(f"parameters must be matrices, got {tuple(p.shape)}")
+
+    def add_param_group(self, param_group: dict[str, Any]) -> None:
+        super().add_param_group(param_group)
+        for p in self.param_groups[-1]["params"]:
+            if p.dim() != 2 or p.numel() == 0:
+                del self.param_groups[-1]
+                raise ValueError(f"parameters must be matrices, got {tuple(p.shape)}")
 
     @torch.no_grad()
     def step(self, closure: Any = None) -> Any:
@@ -1055,6 +1059,7 @@ class Muon(torch.optim.Optimizer):
                 if p.grad is not None:
                     if p.grad.is_sparse:
                         raise RuntimeError("sparse gradients are not supported")
+                    _check_floating("parameters", p)  # (before any momentum changes)
                     alike.setdefault((p.shape, p.dtype, p.device), []).append(p)
             for (shape, dtype, _), params in alike.items():
                 self._update(group, shape, dtype, params)
@@ -1071,15 +1076,15 @@ class Muon(torch.optim.Optimizer):
         torch._foreach_add_(buffers, grads)
         updates = torch._foreach_add(grads, buffers, alpha=group["momentum"]) \
             if group["nesterov"] else buffers
-        rows, columns = shape
+        rows, columns, lr = *shape, float(group["lr"])
         if group["adjust_lr_fn"] == "match_rms_adamw":
             ratio = 0.2 * math.sqrt(max(rows, columns))
         else:
             ratio = math.sqrt(max(1.0, rows / columns))
         turned = orthogonalize(torch.stack(updates), group["ns_steps"], group["ns_coefficients"],
                                group["eps"]).to(dtype)
-        torch._foreach_mul_(params, 1.0 - group["lr"] * group["weight_decay"])
-        torch._foreach_add_(params, list(turned.unbind()), alpha=-group["lr"] * ratio)
+        torch._foreach_mul_(params, 1.0 - lr * group["weight_decay"])
+        torch._foreach_add_(params, list(turned.unbind()), alpha=-lr * ratio)
 
 
 __all__ = [

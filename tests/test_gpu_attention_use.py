@@ -514,3 +514,48 @@ def test_trained_model_goes_on_to_inference():
         got = model(ids, attention_mask=mask).last_hidden_state
     kept = mask.bool()
     assert float((got - want)[kept].abs().max()) < 1e-4 * float(want.abs().max())
+
+
+def test_transforms():
+    """vmap over calls, with an rng for every sample; no transforms that differentiate."""
+
+    from disentangled_flash.training import attention
+
+    args, dout = _case(31, 4, 33, 2, 32, torch.bfloat16, mask="none")
+    q, k, v, pk, pq = [t.detach() for t in args[:5]]
+    lut, scale = args[5:7]
+    rngs = torch.stack([_rng() + i for i in range(4)])
+
+    def one(q, k, v, r):
+        return attention(q[None], k[None], v[None], pk, pq, lut, scale, p=0.3, rng=r, site=SITE)[0]
+
+    got = torch.func.vmap(one)(q, k, v, rngs)
+    for i in range(4):
+        assert torch.equal(got[i], one(q[i], k[i], v[i], rngs[i]))
+    with pytest.raises(ValueError, match="rng"):
+        torch.func.vmap(lambda t: one(t, k[0], v[0], rngs[0]))(q)
+
+    def loss(q, pk):
+        return (attention(q, k, v, pk, pq, lut, scale) * dout).float().sum()
+
+    with pytest.raises(RuntimeError):
+        torch.func.grad(loss, argnums=(0, 1))(q, pk)
+    with pytest.raises(RuntimeError):
+        torch.func.jvp(lambda t: attention(t, k, v, pk, pq, lut, scale), (q,), (q,))
+    with torch.inference_mode():
+        assert torch.equal(attention(q, k, v, pk, pq, lut, scale),
+                           attention(q.clone().requires_grad_(), k, v, pk, pq, lut, scale))
+
+
+def test_muon_takes_a_rate_that_is_a_tensor():
+    from disentangled_flash import training
+
+    values = torch.randn(24, 40, device="cuda")
+    found = []
+    for lr in (0.1, torch.tensor(0.1)):
+        p = torch.nn.Parameter(values.clone())
+        p.grad = torch.ones_like(p).cumsum(0).cumsum(1)
+        training.Muon([p], lr=lr).step()
+        found.append(p.detach())
+    assert torch.allclose(found[0], found[1], rtol=1e-6, atol=1e-7)  # 0.1 in 32 bits
+    assert not torch.equal(found[0], values)

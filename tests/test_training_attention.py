@@ -201,6 +201,7 @@ def test_muon_steps(monkeypatch, nesterov, adjust):
         return _exact(update, steps, coefficients, eps)
 
     monkeypatch.setattr(training, "orthogonalize", orthogonalize)
+    monkeypatch.setattr(training, "_check_floating", lambda *a: None)  # on the CPU, in 64 bits
     gen = torch.Generator().manual_seed(0)
 
     def normal(*shape):
@@ -246,9 +247,14 @@ def test_muon_refusals():
     with pytest.raises(ValueError, match="matrices"):
         training.Muon([nn.Parameter(torch.zeros(3))])
     optimizer = training.Muon([matrix])
+    for bad in (torch.zeros(3), torch.zeros(2, 3, 4), torch.zeros(0, 4)):
+        with pytest.raises(ValueError, match="matrices"):
+            optimizer.add_param_group({"params": [nn.Parameter(bad)]})
+    assert len(optimizer.param_groups) == 1
     matrix.grad = torch.ones(3, 4)
     with pytest.raises(RuntimeError, match="GPU"):
         optimizer.step()
+    assert not optimizer.state and torch.equal(matrix, torch.zeros(3, 4))
 
 
 def test_split_parameters():
