@@ -17,7 +17,8 @@
 // workspace, so that no access needs a bound.  A and B are symmetric: tiles below the diagonal
 // alone are computed and stored twice.  The loop is the projection GEMM's: slabs of 64 k copied
 // straight into LDS, fragments read a step ahead.  In B X the second operand is X's own rows, k by
-// columns, read with transposing reads, so that no transposed copy of X exists.
+// columns, read with transposing reads, so that no transposed copy of X exists.  Of up to 128 rows B X
+// takes both operands in two parts.
 //
 // Bound by feeding the matrix unit: a step's products reach 520 to 570 TFLOP/s for 48 of 768 x 768
 // (A 45 us, B 46, B X 84) and 640 to 700 for 4 of 1536 x 6144 (98, 32 and 165 us), where the card's large
@@ -50,6 +51,7 @@ struct Matrices {
   _Float16* hi[2];  // [batch, rows, columns], the steps' in turn
   _Float16* lo;
   _Float16 *gram, *poly;  // [batch, rows, rows]
+  _Float16* poly_lo;      // what B's rounding left off, where it is an operand
   int rows, columns;      // padded
   int batch;
 };
@@ -195,7 +197,10 @@ struct Step {
   int m, n, tall;  // of G
 };
 
-template <Form FORM, typename CF>
+// PARTS: B and X are operands of B X in two parts, as one product of three times the length,
+// B_hi X_hi + B_hi X_lo + B_lo X_hi.  For X of one tile of rows: then a workgroup alone reads the low parts
+// of its columns, and writes them when its wavefronts have read them.
+template <Form FORM, typename CF, bool PARTS>
 __global__ __launch_bounds__(CF::THREADS, CF::WGS) void product_kernel(Step p) {
   constexpr int BM = CF::BM, BN = CF::BN;
   constexpr int MB = CF::MB, NB = CF::NB, S = CF::STAGES;
@@ -230,9 +235,12 @@ __global__ __launch_bounds__(CF::THREADS, CF::WGS) void product_kernel(Step p) {
                                                      : p.x.poly + batch * square;
   const _Float16* X = left + static_cast<int64_t>(mt) * BM * K;
   const _Float16* W = kSquare ? left + static_cast<int64_t>(nt) * BN * K : hi + nt * BN;
+  constexpr bool kThree = PARTS && !kSquare;
+  const _Float16* X_lo = kThree ? p.x.poly_lo + batch * square + static_cast<int64_t>(mt) * BM * K : X;
+  const _Float16* W_lo = kThree ? p.x.lo + batch * whole + nt * BN : W;
   const uint32_t x_row = static_cast<uint32_t>(K) * 2;
   const uint32_t w_row_bytes = kSquare ? x_row : static_cast<uint32_t>(p.x.columns) * 2;
-  const int KT = K / kSlabK;
+  const int slabs = K / kSlabK, KT = kThree ? 3 * slabs : slabs;
 
   constexpr int kChunks = BN / 8;  // of a row of k
   // Byte offsets of this lane's 16 bytes of each copy.
@@ -260,13 +268,17 @@ __global__ __launch_bounds__(CF::THREADS, CF::WGS) void product_kernel(Step p) {
     const uint32_t to = __builtin_amdgcn_readfirstlane(
         lds0 + stage * CF::SLAB + (is_x ? 0 : CF::A_BYTES) + (jj * CF::WAVES + wave) * 1024);
     const bool live = kt < KT;
+    const int part = kThree ? kt >= 2 * slabs ? 2 : kt >= slabs ? 1 : 0 : 0;
+    kt -= part * slabs;
     if (is_x || kSquare) {
-      const auto memory = scalar_resource(is_x ? X : W, live ? (is_x ? BM : BN) * x_row : 0);
+      const auto memory = scalar_resource(is_x ? (part == 2 ? X_lo : X) : W,
+                                          live ? (is_x ? BM : BN) * x_row : 0);
       copy_to_lds(memory, is_x ? xoff[is_x ? jj : 0] : woff[is_x ? 0 : jj],
                   __builtin_amdgcn_readfirstlane(live ? kt * kSlabK * 2 : 0), to);
     } else {  // a resource that begins at the slab's first row
       const auto memory =
-          scalar_resource(W + static_cast<int64_t>(live ? kt : 0) * kSlabK * p.x.columns,
+          scalar_resource((part == 1 ? W_lo : W) +
+                              static_cast<int64_t>(live ? kt : 0) * kSlabK * p.x.columns,
                           live ? (kSlabK - 1) * w_row_bytes + BN * 2 : 0);
       copy_to_lds(memory, woff[is_x ? 0 : jj], 0, to);
     }
@@ -380,8 +392,10 @@ __global__ __launch_bounds__(CF::THREADS, CF::WGS) void product_kernel(Step p) {
     asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
     // The mirrored tile, [column][row], rows of 128 + 8.
     _Float16* mirror = reinterpret_cast<_Float16*>(smem);
+    constexpr bool kRest = PARTS && FORM == Form::kPolynomial;
     constexpr int kLd = BM + 8;
     static_assert(BN * kLd * 2 <= CF::LDS, "the mirrored tile");
+    _Float16* out_lo = kRest ? p.x.poly_lo + batch * square : nullptr;
 #pragma unroll
     for (int j = 0; j < MB; ++j) {
       const int row = wm * CF::WM + 16 * j + c;
@@ -389,7 +403,7 @@ __global__ __launch_bounds__(CF::THREADS, CF::WGS) void product_kernel(Step p) {
       for (int i = 0; i < NB; i += 2) {
         const int column = wn * CF::WN + 16 * i + 8 * g;
         const int64_t to = static_cast<int64_t>(mt * BM + row) * p.x.rows + nt * BN + column;
-        half8_t v;
+        half8_t v, rest;
         if constexpr (FORM == Form::kGram) {
 #pragma unroll
           for (int e = 0; e < 8; ++e)
@@ -397,11 +411,14 @@ __global__ __launch_bounds__(CF::THREADS, CF::WGS) void product_kernel(Step p) {
         } else {
           const half8_t a = *reinterpret_cast<const half8_t*>(gram + to);
 #pragma unroll
-          for (int e = 0; e < 8; ++e)
-            v[e] = static_cast<_Float16>(p.b * static_cast<float>(a[e]) +
-                                         p.c * acc[i + e / 4][j][e % 4]);
+          for (int e = 0; e < 8; ++e) {
+            const float x = p.b * static_cast<float>(a[e]) + p.c * acc[i + e / 4][j][e % 4];
+            v[e] = static_cast<_Float16>(x);
+            rest[e] = static_cast<_Float16>(x - static_cast<float>(v[e]));
+          }
         }
         *reinterpret_cast<half8_t*>(out + to) = v;
+        if constexpr (kRest) *reinterpret_cast<half8_t*>(out_lo + to) = rest;
         if (mt != nt) {
 #pragma unroll
           for (int e = 0; e < 8; ++e) mirror[(column + e) * kLd + row] = v[e];
@@ -482,6 +499,11 @@ __global__ __launch_bounds__(CF::THREADS, CF::WGS) void product_kernel(Step p) {
 struct Plan {
   int rows, columns, partials;
   int64_t block;  // elements of a partial sum
+  // B X of operands in two parts, for one tile of rows.  The fewer rows, the more of the result is what
+  // their roundings make: it was off by 1.35 times its own rounding with 256 rows, 1.42 with 128, 1.52
+  // with 64, 1.79 with 8; in parts by 1.14, 1.17 and 1.37.  They cost 3 us a step of 128 x 128 (98 us
+  // instead of 83 for five); two tiles of rows would take 139 us instead of 111 (150 x 140).
+  bool parts;
   size_t x, square, norm, total;
 };
 
@@ -499,7 +521,8 @@ Plan make_plan(int64_t batch, int64_t m, int64_t n) {
   p.x = round_up(static_cast<size_t>(batch) * p.rows * p.columns * 2);
   p.square = round_up(static_cast<size_t>(batch) * p.rows * p.rows * 2);
   p.norm = round_up(static_cast<size_t>(batch) * p.partials * 8);
-  p.total = 3 * p.x + 2 * p.square + p.norm;
+  p.parts = p.rows == kTile;
+  p.total = 3 * p.x + (p.parts ? 3 : 2) * p.square + p.norm;
   return p;
 }
 
@@ -513,13 +536,13 @@ int refuse(int64_t batch, int64_t m, int64_t n) {
   return DFLASH_OK;
 }
 
-template <Form FORM, typename CF>
+template <Form FORM, typename CF, bool PARTS>
 int launch_config(const Step& p, hipStream_t stream) {
   const uint32_t m = p.x.rows / CF::BM, n = p.x.columns / CF::BN;
   const uint32_t tiles = FORM == Form::kGram || FORM == Form::kPolynomial ? m * (m + 1) / 2 : m * n;
-  const hipError_t e = ensure_dynamic_lds<&product_kernel<FORM, CF>>(CF::LDS);
+  const hipError_t e = ensure_dynamic_lds<&product_kernel<FORM, CF, PARTS>>(CF::LDS);
   if (e != hipSuccess) return static_cast<int>(e);
-  hipLaunchKernelGGL((product_kernel<FORM, CF>), dim3(p.x.batch * tiles), dim3(CF::THREADS),
+  hipLaunchKernelGGL((product_kernel<FORM, CF, PARTS>), dim3(p.x.batch * tiles), dim3(CF::THREADS),
                      CF::LDS, stream, p);
   return static_cast<int>(hipGetLastError());
 }
@@ -527,13 +550,23 @@ int launch_config(const Step& p, hipStream_t stream) {
 // Up to one tile a CU: eight wavefronts and five slabs in flight; more: two workgroups of four a CU,
 // two slabs.  us a step, deep / two: Gram of 6144 x 1536 (78 tiles) 44 / 67, of four (312) 105 / 96,
 // of 48 of 768 x 768 (1008) 51 / 42; update of 256 x 256 (4) 7.5 / 9.
-template <Form FORM>
+template <Form FORM, bool PARTS>
 int launch_product(const Step& p, hipStream_t stream) {
   constexpr bool kSquare = FORM == Form::kGram || FORM == Form::kPolynomial;
   const int m = p.x.rows / kTile, n = p.x.columns / kTile;
   const int64_t tiles = static_cast<int64_t>(p.x.batch) * (kSquare ? m * (m + 1) / 2 : m * n);
-  return tiles <= 256 ? launch_config<FORM, Cfg128x128Deep>(p, stream)
-                      : launch_config<FORM, Cfg128x128>(p, stream);
+  return tiles <= 256 ? launch_config<FORM, Cfg128x128Deep, PARTS>(p, stream)
+                      : launch_config<FORM, Cfg128x128, PARTS>(p, stream);
+}
+
+// A step from X of `from` to that of `from` ^ 1, or to the result.
+template <bool PARTS>
+int launch_step(const Step& p, bool last, hipStream_t stream) {
+  int rc = launch_product<Form::kGram, false>(p, stream);
+  if (rc == DFLASH_OK) rc = launch_product<Form::kPolynomial, PARTS>(p, stream);
+  if (rc != DFLASH_OK) return rc;
+  return last ? launch_product<Form::kResult, PARTS>(p, stream)
+              : launch_product<Form::kUpdate, PARTS>(p, stream);
 }
 
 template <typename T>
@@ -544,9 +577,11 @@ int launch(const T* g, __bf16* out, int64_t batch, int m, int n, int steps, floa
   p.x.hi[0] = reinterpret_cast<_Float16*>(workspace);
   p.x.hi[1] = reinterpret_cast<_Float16*>(workspace + plan.x);
   p.x.lo = reinterpret_cast<_Float16*>(workspace + 2 * plan.x);
-  p.x.gram = reinterpret_cast<_Float16*>(workspace + 3 * plan.x);
-  p.x.poly = reinterpret_cast<_Float16*>(workspace + 3 * plan.x + plan.square);
-  double* partial = reinterpret_cast<double*>(workspace + 3 * plan.x + 2 * plan.square);
+  char* squares = workspace + 3 * plan.x;
+  p.x.gram = reinterpret_cast<_Float16*>(squares);
+  p.x.poly = reinterpret_cast<_Float16*>(squares + plan.square);
+  p.x.poly_lo = plan.parts ? reinterpret_cast<_Float16*>(squares + 2 * plan.square) : nullptr;
+  double* partial = reinterpret_cast<double*>(workspace + plan.total - plan.norm);
   p.x.rows = plan.rows;
   p.x.columns = plan.columns;
   p.x.batch = static_cast<int>(batch);
@@ -565,14 +600,12 @@ int launch(const T* g, __bf16* out, int64_t batch, int m, int n, int steps, floa
                      n % 8 == 0 && reinterpret_cast<uintptr_t>(g) % 16 == 0, eps);
   for (int step = 0; step < steps; ++step) {
     p.from = step % 2;
-    // (The last step's X, whose small singular values grow no more, has hi alone.)
-    p.read_lo = step == 0 || step + 1 < steps;
-    p.write_lo = step + 2 < steps;
-    int rc = launch_product<Form::kGram>(p, stream);
-    if (rc == DFLASH_OK) rc = launch_product<Form::kPolynomial>(p, stream);
-    if (rc == DFLASH_OK)
-      rc = step + 1 < steps ? launch_product<Form::kUpdate>(p, stream)
-                            : launch_product<Form::kResult>(p, stream);
+    const bool last = step + 1 == steps;
+    // (The last step's X, whose small singular values grow no more, has hi alone, but in parts.)
+    p.read_lo = step == 0 || !last || plan.parts;
+    p.write_lo = step + 2 < steps || plan.parts;
+    const int rc = plan.parts ? launch_step<true>(p, last, stream)
+                              : launch_step<false>(p, last, stream);
     if (rc != DFLASH_OK) return rc;
   }
   return static_cast<int>(hipGetLastError());
