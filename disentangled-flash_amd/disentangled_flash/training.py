@@ -313,7 +313,7 @@ def attention(
     ``mask`` is a bool or uint8 ``[B, L]``, nonzero for tokens that are kept.  A kept query has
     the softmax over the kept keys, whatever the padded places hold; a padded query has ``1 / L``
     for every key, as in Hugging Face's attention (where a padded key's value is not finite it
-    counts as 0).  ``p``, ``rng`` and ``site`` as in
+    counts as 0; a kept key's makes the rows that see it NaN).  ``p``, ``rng`` and ``site`` as in
     :func:`dropout`, on the probabilities ``[B, H, L, L]``.
 
     Scores, softmax and sums are fp32, but that the forward pass of bf16 inputs rounds the relative terms

@@ -451,7 +451,7 @@ DFLASH_API int dflash_attention_train_fwd(const dflash_attention_train* attentio
                                           void* out_low, float* lse, void* bits, void* stream);
 
 /*
- * Its backward pass, from the same inputs and what the forward pass wrote.
+ * Its backward pass, from the same inputs and what the forward pass wrote (out_low too, but in fp32).
  *   dout, dquery, dkey, dvalue : [B, L, H, D] contiguous
  *   dpos_key, dpos_query       : [S, H, D] contiguous; either may be NULL
  *   workspace                  : dflash_attention_train_bwd_workspace_bytes(attention) bytes,
