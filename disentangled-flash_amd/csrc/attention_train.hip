@@ -121,8 +121,8 @@ struct Op<float> {
 // Rows in LDS are padded by 16 bytes: the 16 rows that a fragment read touches lie in different banks.
 // Padded by 32, so do the rows 8g + 0..3 of a transposing read of 16-bit elements, which is worth it where no
 // workgroup less fits a CU for it: in the key kernel (321 -> 288 us at 32 x 512 full tokens, heads of 128
-// 228 -> 207) and in the forward pass with fp32 scores (fp16: 272 -> 263, heads of 128 195 -> 183);
-// the forward pass in bf16 would lose its third workgroup (220 -> 290), as the query kernel (91 -> 109).
+// 228 -> 207) and in the forward pass (fp16: 272 -> 263, heads of 128 195 -> 183); the query kernel would
+// lose one (91 -> 109).
 template <typename T, int D>
 constexpr int kLd = D + 16 / static_cast<int>(sizeof(T));
 template <typename T, int D>
@@ -172,15 +172,12 @@ __device__ inline typename Op<T>::half read_columns_half(const T* p, int ld, int
   }
 }
 
-// Scores by delta, scaled, in LDS: fp32, but for the forward pass of bf16 inputs.  fp16 is off by up to
-// half a step, 2^-12 of a score, and a probability by that times the score.  Beside fp16 operands
-// that was the largest error: the gradients of 16 x 384 tokens, heads of 32, were off by 4.0e-4 of their
-// size, with fp32 by 3.0e-4.  Probabilities of bf16 are rounded to 2^-9 of themselves, beside which
-// it is little; the backward pass has fp32 all the same (279 us for 268 at 32 x 512 tokens), as all that
-// a gradient is off by adds up there, and the forward pass fp16 (190 us, 246 with fp32).
-template <typename T>
-using FwdScore = std::conditional_t<std::is_same_v<T, __bf16>, _Float16, float>;
-using KeyScore = float;
+// Scores by delta are fp32 in LDS, scaled, as the backward pass computes them again: its probabilities
+// are those of the forward pass only if their rounding is the same, and fp16 would have neither
+// the range of bf16 inputs (a score past 65504) nor their sums (a row of probabilities of scores of
+// some hundreds adds up to 0.92 .. 1.09 beside a statistic of rounded ones).  Beside fp16 operands scores in
+// fp16 were the largest error: the gradients of 16 x 384 tokens, heads of 32, were off by 4.0e-4 of their
+// size, with fp32 by 3.0e-4.
 
 // Eight values of the accumulators of two blocks of 16 rows as an operand: element e < 4 is row
 // 4g + e of the first, e >= 4 row 4g + e - 4 of the second.
@@ -478,10 +475,9 @@ __global__ __launch_bounds__(256) void dropped_bits_kernel(uint8_t* bits, int64_
 template <typename T, int D, int NW, int BK>
 struct FwdLayout {
   static constexpr int BQ = 16 * NW, W = BQ + BK, LDC = BK + 20, LDP = BQ + 20;
-  static constexpr int LD =
-      sizeof(FwdScore<T>) == 4 || D == 128 ? kLdWide<T, D> : kLd<T, D>;
+  static constexpr int LD = kLdWide<T, D>;
   T k[BK * LD], v[BK * LD], pk[W * LD], pq[W * LD];
-  FwdScore<T> c2p[BQ * LDC], p2c[BK * LDP];
+  float c2p[BQ * LDC], p2c[BK * LDP];
   uint64_t kept[kWords];
 };
 
@@ -689,16 +685,13 @@ void attention_train_fwd_kernel(Params p) {
           for (int r = 0; r < 4; ++r)
             x[kb][r] = fmaf(
                 x[kb][r], p.scale_log2,
-                has_pk ? static_cast<float>(
-                             s.c2p[(16 * wave + c) * LDC + BK + c - 16 * kb - 4 * g - r])
-                       : 0.0f);
+                has_pk ? s.c2p[(16 * wave + c) * LDC + BK + c - 16 * kb - 4 * g - r] : 0.0f);
         if (has_pq) {
 #pragma unroll
           for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
             for (int r = 0; r < 4; ++r)
-              x[kb][r] += static_cast<float>(
-                  s.p2c[(16 * kb + 4 * g + r) * LDP + 16 * wave + 16 + c - 4 * g - r]);
+              x[kb][r] += s.p2c[(16 * kb + 4 * g + r) * LDP + 16 * wave + 16 + c - 4 * g - r];
         }
         if (!__all(mine)) {
 #pragma unroll
@@ -799,10 +792,10 @@ struct KeyLayout {
   static constexpr int W = BQ + BK;
   static constexpr int kWide = BK < 64 ? 1 : BK / 64;  // words of the generator's bits a query
   // A wavefront's scores of its keys by delta, and after them G by delta.
-  static constexpr int kScores = 16 * LDP * static_cast<int>(sizeof(KeyScore));
+  static constexpr int kScores = 16 * LDP * static_cast<int>(sizeof(float));
   static constexpr int kSkew = 16 * LDF * static_cast<int>(sizeof(T));
   T q[BQ * LD], dout[BQ * LD], pk[W * LD], pq[W * LD];
-  KeyScore c2p[BQ * LDC];
+  float c2p[BQ * LDC];
   unsigned char own[NW * (kScores > kSkew ? kScores : kSkew)];
   float lse[BQ], delta[BQ];
   uint16_t places[NW][BQ];  // bit c of a wavefront's row: the place of key c is kept
@@ -828,7 +821,7 @@ void attention_train_key_kernel(Params p) {
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
   const int lane = threadIdx.x % 64, c = lane % 16, g = lane / 16;
   const int j = j0 + 16 * wave + c;
-  KeyScore* scores = reinterpret_cast<KeyScore*>(s.own + wave * (sizeof(s.own) / NW));
+  float* scores = reinterpret_cast<float*>(s.own + wave * (sizeof(s.own) / NW));
   T* skew = reinterpret_cast<T*>(scores);
 
   read_mask(s.kept, p.mask, b, p.L);
@@ -1008,15 +1001,13 @@ void attention_train_key_kernel(Params p) {
         for (int r = 0; r < 4; ++r)
           x[qb][r] = fmaf(
               x[qb][r], p.scale_log2,
-              has_pk ? static_cast<float>(
-                           s.c2p[(16 * qb + 4 * g + r) * LDC + 4 * g + r - c - 16 * wave + BK])
-                     : 0.0f);
+              has_pk ? s.c2p[(16 * qb + 4 * g + r) * LDC + 4 * g + r - c - 16 * wave + BK] : 0.0f);
       if (has_pq) {
 #pragma unroll
         for (int qb = 0; qb < QB; ++qb)
 #pragma unroll
           for (int r = 0; r < 4; ++r)
-            x[qb][r] += static_cast<float>(scores[c * LDP + 16 * qb + 4 * g + r - c + 16]);
+            x[qb][r] += scores[c * LDP + 16 * qb + 4 * g + r - c + 16];
       }
       // P, and P (M dP - D).
 #pragma unroll
