@@ -88,7 +88,11 @@ def compact_position_plan(
 
 
 class SharedPositionPlanCache:
-    """Per-(length, device) cache of immutable position index tensors."""
+    """Per-(length, device) cache of immutable position index tensors.
+
+    Tables serve later calls in other modes, so none is made an inference tensor (which no backward
+    pass could save).
+    """
 
     def __init__(
         self,
@@ -116,28 +120,27 @@ class SharedPositionPlanCache:
         resolved = torch.device(device)
         return sequence_length, str(resolved), resolved
 
-    @torch.no_grad()
     def compact(self, sequence_length: int, device: torch.device | str) -> SharedPositionIndexPlan:
         length, name, resolved = self._key(sequence_length, device)
         hit = self._compact.get((length, name))
         if hit is not None:
             return hit
-        active, lookup = compact_position_plan(
-            length,
-            position_buckets=self.position_buckets,
-            max_relative_positions=self.max_relative_positions,
-            position_embedding_size=self.position_embedding_size,
-            uses_position_bias=self.uses_position_bias,
-        )
-        plan = SharedPositionIndexPlan(
-            sequence_length=length,
-            active_slots=active.to(device=resolved),
-            delta_to_local=lookup.to(device=resolved),
-        )
+        with torch.inference_mode(False), torch.no_grad():
+            active, lookup = compact_position_plan(
+                length,
+                position_buckets=self.position_buckets,
+                max_relative_positions=self.max_relative_positions,
+                position_embedding_size=self.position_embedding_size,
+                uses_position_bias=self.uses_position_bias,
+            )
+            plan = SharedPositionIndexPlan(
+                sequence_length=length,
+                active_slots=active.to(device=resolved),
+                delta_to_local=lookup.to(device=resolved),
+            )
         self._compact[(length, name)] = plan
         return plan
 
-    @torch.no_grad()
     def dense(
         self, sequence_length: int, device: torch.device | str
     ) -> SharedDensePositionIndexPlan:
@@ -146,10 +149,11 @@ class SharedPositionPlanCache:
         if hit is not None:
             return hit
         compact = self.compact(length, resolved)
-        positions = torch.arange(length, dtype=torch.long)
-        delta_index = positions[:, None] - positions[None, :] + (length - 1)
-        pair = compact.delta_to_local.cpu()[delta_index].to(device=resolved, dtype=torch.long)
-        plan = SharedDensePositionIndexPlan(compact=compact, pair_to_local=pair[None, None])
+        with torch.inference_mode(False), torch.no_grad():
+            positions = torch.arange(length, dtype=torch.long)
+            delta_index = positions[:, None] - positions[None, :] + (length - 1)
+            pair = compact.delta_to_local.cpu()[delta_index].to(device=resolved, dtype=torch.long)
+            plan = SharedDensePositionIndexPlan(compact=compact, pair_to_local=pair[None, None])
         self._dense[(length, name)] = plan
         return plan
 

@@ -1,0 +1,66 @@
+"""CPU tests of the tables of relative distances that calls of one length share."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from disentangled_flash import enable_deberta_training, training
+from disentangled_flash.position import SharedPositionPlanCache
+
+transformers = pytest.importorskip("transformers")
+
+from test_training_attention import _inputs, _model, calls  # noqa: E402, F401 (tests/ is on the path)
+
+
+def _cache():
+    return SharedPositionPlanCache(position_buckets=8, max_relative_positions=40,
+                                   position_embedding_size=8)
+
+
+class _Saves(torch.autograd.Function):
+    """Saves a table for its backward pass, as the attention's node does."""
+
+    @staticmethod
+    def forward(ctx, x, table):
+        ctx.save_for_backward(table)
+        return x * 1
+
+    @staticmethod
+    def backward(ctx, grad):
+        assert ctx.saved_tensors[0] is not None
+        return grad, None
+
+
+def test_tables_made_in_inference_mode_serve_a_backward_pass():
+    cache = _cache()
+    with torch.inference_mode():
+        dense = cache.dense(9, "cpu")
+        compact = cache.compact(11, "cpu")
+    x = torch.ones(3, requires_grad=True)
+    for table in (dense.pair_to_local, dense.active_slots, dense.compact.delta_to_local,
+                  compact.active_slots, compact.delta_to_local):
+        assert not table.is_inference()
+        _Saves.apply(x, table).sum().backward()
+    assert cache.compact(9, "cpu") is dense.compact
+
+
+def test_training_after_a_validation_in_inference_mode(calls, monkeypatch):  # noqa: F811
+    """The first forward of a length runs in inference mode, the next one trains."""
+
+    stand_in = training.attention
+
+    def attention(query, key, value, pos_key, pos_query, places, *args, **settings):
+        out = stand_in(query, key, value, pos_key, pos_query, places, *args, **settings)
+        return _Saves.apply(out, places) if out.requires_grad else out
+
+    monkeypatch.setattr(training, "attention", attention)
+    model = enable_deberta_training(_model(), attention="hip")
+    ids, mask = _inputs()
+    model.eval()
+    with torch.inference_mode():
+        model(ids, attention_mask=mask)
+    model.train()
+    model(ids, attention_mask=mask).last_hidden_state.sum().backward()
+    assert len(calls) == 4
+    assert model.encoder.rel_embeddings.weight.grad is not None
