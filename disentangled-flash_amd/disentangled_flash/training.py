@@ -534,8 +534,14 @@ class DropoutState(nn.Module):
         if self._phase.unknown:
             raise RuntimeError(_UNKNOWN_STEP)
         if self._rng is None or self._rng.device != self.counter.device:
-            self._rng = self.counter.clone()
+            self._rng = self._copy()
         return self._rng
+
+    def _copy(self) -> torch.Tensor:
+        """The counter's values; not an inference tensor, since a training forward may come to it."""
+
+        with torch.inference_mode(False):
+            return self.counter.clone()
 
     def begin(self) -> None:
         self._phase.begun = self._phase.inside = True
@@ -567,7 +573,7 @@ class DropoutState(nn.Module):
             phase.unknown = self._rng is None  # (an error where masks are drawn)
             return
         self.counter[1:].add_(1)
-        self._rng = self.counter.clone()
+        self._rng = self._copy()
         _remember(place, self._rng)
 
     def keep_for(self, outputs: Any) -> None:

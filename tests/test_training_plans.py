@@ -1,4 +1,4 @@
-"""CPU tests of the tables of relative distances that calls of one length share."""
+"""CPU tests of what calls share: the tables of relative distances, the steps of a dropout state."""
 
 from __future__ import annotations
 
@@ -64,3 +64,21 @@ def test_training_after_a_validation_in_inference_mode(calls, monkeypatch):  # n
     model(ids, attention_mask=mask).last_hidden_state.sum().backward()
     assert len(calls) == 4
     assert model.encoder.rel_embeddings.weight.grad is not None
+
+
+@pytest.mark.parametrize("how", ["first read", "advance", "begin"])
+def test_a_step_drawn_in_inference_mode_serves_a_backward_pass(how):
+    state = training.DropoutState(5)
+    with torch.inference_mode():
+        if how == "advance":
+            state.advance()
+        elif how == "begin":
+            state.begin()
+        state.rng  # noqa: B018
+        state.end()
+    assert not state.rng.is_inference() and not state.counter.is_inference()
+    assert state.rng.tolist() == [5, 0 if how == "first read" else 1]
+    x = torch.ones(3, requires_grad=True)
+    _Saves.apply(x, state.rng).sum().backward()
+    state.advance()
+    assert state.rng.tolist() == [5, 1 if how == "first read" else 2]
