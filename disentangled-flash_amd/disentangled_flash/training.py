@@ -732,10 +732,11 @@ class _PositionPlans:
         return self.cache.compact(length, device), self.ranges[length]
 
 
-def _is_factorized(mask: Any, batch: int, length: int) -> bool:
-    """The form in which :class:`_EncoderParts` hands a padding mask on: ``[B, 1, L, 1]``."""
+def _is_factorized(mask: Any) -> bool:
+    """The form in which :class:`_EncoderParts` hands a padding mask on: ``[B, 1, L, 1, 1]``, of a
+    dimension more than any mask that an attention takes."""
 
-    return isinstance(mask, torch.Tensor) and mask.shape == (batch, 1, length, 1)
+    return isinstance(mask, torch.Tensor) and mask.dim() == 5
 
 
 class _Attention:
@@ -749,16 +750,14 @@ class _Attention:
 
     def forward(self, hidden_states, attention_mask, output_attentions=False, query_states=None,
                 relative_pos=None, rel_embeddings=None):
-        batch, length = hidden_states.shape[:2]
-        factorized = _is_factorized(attention_mask, batch, length)
-        if factorized and relative_pos is None and not output_attentions:
-            out = self._fused(hidden_states, attention_mask[:, 0, :, 0],
-                              hidden_states if query_states is None else query_states,
-                              rel_embeddings)
-            if out is not None:
-                return out, None
-        if factorized:
-            mask = attention_mask[:, 0, :, 0]
+        if _is_factorized(attention_mask):
+            mask = attention_mask[:, 0, :, 0, 0]
+            if relative_pos is None and not output_attentions:
+                out = self._fused(hidden_states, mask,
+                                  hidden_states if query_states is None else query_states,
+                                  rel_embeddings)
+                if out is not None:
+                    return out, None
             attention_mask = mask[:, None, None, :] * mask[:, None, :, None]
         return super().forward(hidden_states, attention_mask, output_attentions,
                                query_states=query_states, relative_pos=relative_pos,
@@ -771,6 +770,7 @@ class _Attention:
         if not (_on_gpu(hidden_states) and self.attention_head_size in ATTENTION_WIDTHS
                 and 1 <= hidden_states.shape[1] <= MAX_LENGTH
                 and query_states.shape == hidden_states.shape
+                and all(n in (1, m) for n, m in zip(mask.shape, hidden_states.shape))
                 and _dropout_fits(drop) and not _hooks_on_all_modules()
                 and (not modes or (rel_embeddings is not None
                                    and rel_embeddings.shape[0] >= 2 * self.pos_ebd_size))):
@@ -804,7 +804,7 @@ class _Attention:
         dropping = drop.training and drop.p > 0
         out = attention(query, key, value, pos_key, pos_query, places,
                         1 / math.sqrt(self.attention_head_size * (1 + len(terms))),
-                        mask=mask.bool(), p=drop.p if dropping else 0.0,
+                        mask=mask.bool().expand(batch, length), p=drop.p if dropping else 0.0,
                         rng=drop.state.rng if dropping else None, site=drop.site)
         return out.view(batch, length, -1)
 
@@ -815,7 +815,7 @@ class _Attention:
 
 class _EncoderParts:
     """Stands for ``get_attention_mask`` or ``get_rel_pos`` of a Hugging Face encoder whose
-    attention is :class:`_Attention`: a padding mask stays ``[B, L]`` values (as ``[B, 1, L, 1]``), and the
+    attention is :class:`_Attention`: a padding mask stays ``[B, L]`` values, and the
     relative positions are left to the attention.  Anything else is the encoder's own."""
 
     def __init__(self, encoder: nn.Module, name: str) -> None:
@@ -830,7 +830,7 @@ class _EncoderParts:
         if self.name == "get_attention_mask":
             mask = given[0]
             if isinstance(mask, torch.Tensor) and mask.dim() == 2:
-                return mask[:, None, :, None]
+                return mask[:, None, :, None, None]
         elif len(given) < 3 or given[2] is None:
             return None
         return own(encoder, *args, **kwargs)

@@ -30,3 +30,23 @@ def test_training_after_a_validation_in_inference_mode(changed):
     for name, g in grads.items():
         w = want_grads[name]
         assert float((g - w).abs().max()) <= 1e-4 * float(w.abs().max()) + 1e-6, name
+
+
+@pytest.mark.parametrize("kind", ["one row for all", "one value a sequence", "queries", "keys"])
+def test_masks_that_are_broadcast(kind):
+    """Against torch's attention: both in fp32, so 1e-4 of the largest (rows of kept queries, and all rows
+    of masks that name queries or keys)."""
+
+    ids, mask = _batch()
+    given = {"one row for all": mask[1:2], "one value a sequence": mask[:, 60:61],
+             "queries": mask[:, None, :, None], "keys": mask[:, None, None, :]}[kind]
+    gen = torch.Generator(device="cuda").manual_seed(6)
+    hidden = torch.randn(*ids.shape, 128, device="cuda", generator=gen)
+    found = []
+    for attention in ("torch", "hip"):
+        model = _model(attention=attention, conv_kernel_size=0).eval()
+        with torch.no_grad():
+            found.append(model.encoder(hidden, given).last_hidden_state)
+    kept = given.bool().expand(ids.shape) if given.dim() == 2 else torch.ones_like(ids).bool()
+    want, got = (x[kept] for x in found)
+    assert float((got - want).abs().max()) < 1e-4 * float(want.abs().max())
