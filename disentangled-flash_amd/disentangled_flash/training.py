@@ -826,12 +826,11 @@ class _EncoderParts:
         own = getattr(type(encoder), self.name)
         if not all(isinstance(layer.attention.self, _Attention) for layer in encoder.layer):
             return own(encoder, *args, **kwargs)
-        given = [*args, *kwargs.values()]
         if self.name == "get_attention_mask":
-            mask = given[0]
+            mask = args[0] if args else kwargs.get("attention_mask")
             if isinstance(mask, torch.Tensor) and mask.dim() == 2:
                 return mask[:, None, :, None, None]
-        elif len(given) < 3 or given[2] is None:
+        elif (args[2] if len(args) > 2 else kwargs.get("relative_pos")) is None:
             return None
         return own(encoder, *args, **kwargs)
 

@@ -76,3 +76,20 @@ def test_a_layer_called_by_itself():
     fused = enable_deberta_training(model, attention="hip").eval()
     got = fused.encoder.layer[0].attention(_hidden(), mask, rel_embeddings=table)[0]
     assert torch.equal(got, want)
+
+
+def test_relative_positions_by_name():
+    """The encoder's methods take their arguments by name too."""
+
+    model = enable_deberta_training(_model(), attention="hip")
+    hidden = _hidden()
+    places = torch.ones(1, 11, 11, dtype=torch.long)
+    assert model.encoder.get_rel_pos(hidden, relative_pos=places) is places
+    assert model.encoder.get_rel_pos(hidden, None, places) is places
+    assert model.encoder.get_rel_pos(hidden_states=hidden, query_states=None,
+                                     relative_pos=places) is places
+    assert model.encoder.get_rel_pos(hidden, query_states=hidden) is None
+    mask = model.encoder.get_attention_mask(attention_mask=PADDING)
+    assert torch.equal(mask.flatten(1), PADDING)
+    pairs = model.encoder.get_attention_mask(attention_mask=MASKS["3-D"])
+    assert torch.equal(pairs, MASKS["3-D"][:, None])
