@@ -87,11 +87,19 @@ def compact_position_plan(
     return active, lookup
 
 
+def _lies_on(tensor: torch.Tensor, device: torch.device) -> bool:
+    """Whether ``device``, which may lack an index, is the tensor's."""
+
+    at = tensor.device
+    return at == device or (at.type == device.type and None in (at.index, device.index))
+
+
 class SharedPositionPlanCache:
     """Per-(length, device) cache of immutable position index tensors.
 
     Tables serve later calls in other modes, so none is made an inference tensor (which no backward
-    pass could save).
+    pass could save).  A cache that was pickled may hold tables which its loading has moved: they are
+    made again.
     """
 
     def __init__(
@@ -123,7 +131,7 @@ class SharedPositionPlanCache:
     def compact(self, sequence_length: int, device: torch.device | str) -> SharedPositionIndexPlan:
         length, name, resolved = self._key(sequence_length, device)
         hit = self._compact.get((length, name))
-        if hit is not None:
+        if hit is not None and _lies_on(hit.delta_to_local, resolved):
             return hit
         with torch.inference_mode(False), torch.no_grad():
             active, lookup = compact_position_plan(
@@ -146,7 +154,7 @@ class SharedPositionPlanCache:
     ) -> SharedDensePositionIndexPlan:
         length, name, resolved = self._key(sequence_length, device)
         hit = self._dense.get((length, name))
-        if hit is not None:
+        if hit is not None and _lies_on(hit.pair_to_local, resolved):
             return hit
         compact = self.compact(length, resolved)
         with torch.inference_mode(False), torch.no_grad():

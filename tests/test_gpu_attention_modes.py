@@ -3,6 +3,8 @@ masks, moved and copied models."""
 
 from __future__ import annotations
 
+import io
+
 import pytest
 import torch
 
@@ -50,3 +52,23 @@ def test_masks_that_are_broadcast(kind):
     kept = given.bool().expand(ids.shape) if given.dim() == 2 else torch.ones_like(ids).bool()
     want, got = (x[kept] for x in found)
     assert float((got - want).abs().max()) < 1e-4 * float(want.abs().max())
+
+
+def test_a_model_saved_on_the_gpu_and_loaded_on_the_cpu():
+    """And brought back: its tables of relative distances are made again."""
+
+    ids, mask = _batch()
+    model = _model()
+    want, want_grads = _grads(model, ids, mask)
+    store = io.BytesIO()
+    model.zero_grad()
+    torch.save(model, store)
+    store.seek(0)
+    loaded = torch.load(store, weights_only=False, map_location="cpu")
+    assert not any(p.is_cuda for p in loaded.parameters())
+    got, grads = _grads(loaded.cuda(), ids, mask)
+    assert float((got - want).abs().max()) < 1e-5 * float(want.abs().max())
+    assert set(grads) == set(want_grads)
+    for name, g in grads.items():
+        w = want_grads[name]
+        assert float((g - w).abs().max()) <= 1e-4 * float(w.abs().max()) + 1e-6, name

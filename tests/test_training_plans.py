@@ -2,6 +2,8 @@
 
 from __future__ import annotations
 
+import io
+
 import pytest
 import torch
 
@@ -82,3 +84,37 @@ def test_a_step_drawn_in_inference_mode_serves_a_backward_pass(how):
     _Saves.apply(x, state.rng).sum().backward()
     state.advance()
     assert state.rng.tolist() == [5, 1 if how == "first read" else 2]
+
+
+def test_tables_of_a_cache_that_was_moved_are_made_again():
+    """Loading to another device moves the tables, not the names under which they are kept."""
+
+    cache = _cache()
+    want = cache.dense(9, "cpu"), cache.compact(11, "cpu")
+    store = io.BytesIO()
+    torch.save(cache, store)
+    store.seek(0)
+    moved = torch.load(store, weights_only=False, map_location="meta")
+    got = moved.dense(9, "cpu"), moved.compact(11, "cpu")
+    assert torch.equal(got[0].pair_to_local, want[0].pair_to_local)
+    for a, b in ((got[0].compact, want[0].compact), (got[1], want[1])):
+        assert torch.equal(a.active_slots, b.active_slots)
+        assert torch.equal(a.delta_to_local, b.delta_to_local)
+    assert moved.dense(9, "cpu") is got[0] and moved.compact(11, "cpu") is got[1]
+    assert cache.compact(11, torch.device("cpu", 0)).delta_to_local.device.type == "cpu"
+    named = cache.compact(11, torch.device("cpu", 0))
+    assert cache.compact(11, torch.device("cpu", 0)) is named
+
+
+def test_a_backbone_that_was_saved_on_another_device(calls):  # noqa: F811
+    model = enable_deberta_training(_model(), attention="hip").eval()
+    ids, mask = _inputs()
+    want = model(ids, attention_mask=mask).last_hidden_state
+    plans = model.encoder.layer[0].attention.self._plans
+    store = io.BytesIO()
+    torch.save(plans, store)
+    store.seek(0)
+    moved = torch.load(store, weights_only=False, map_location="meta")
+    for layer in model.encoder.layer:
+        layer.attention.self.__dict__["_plans"] = moved
+    assert torch.equal(model(ids, attention_mask=mask).last_hidden_state, want)
