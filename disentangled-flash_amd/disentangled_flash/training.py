@@ -1022,16 +1022,26 @@ class Muon(torch.optim.Optimizer):
     ``g + momentum B`` (``B`` without ``nesterov``), orthogonalised;
     ``p <- (1 - lr weight_decay) p - lr r update``.
 
-    Names and defaults are those of ``torch.optim.Muon``.  ``adjust_lr_fn`` chooses ``r`` for
+    ``adjust_lr_fn`` chooses ``r`` for
     ``[m, n]``: ``"original"`` (the default) ``sqrt(max(1, m / n))``, ``"match_rms_adamw"``
     ``0.2 sqrt(max(m, n))``.  Parameters of one shape, dtype and device are orthogonalised by one call.  They must be on
     a GPU, in fp16, bf16 or fp32; the momentum is kept in the parameter's dtype.
+
+    Names and defaults are those of ``torch.optim.Muon``, whose ``momentum_buffer`` however is an average:
+    ``B <- momentum B + (1 - momentum) g``, and the update ``(1 - momentum) g + momentum B``.
+    ``average=True`` takes that rule.  While ``momentum`` stays what it is both rules take the same steps, but for
+    ``eps``, since an update's length does not count; where it changes they differ.  States are interchangeable
+    with torch's under ``average=True`` alone: one that does not say which of the two it holds is
+    refused.  A sum of steady gradients is ``1 / (1 - momentum)`` times as large as they are, which in fp16 may
+    pass 65504; an average never does.  Unlike torch's, ``momentum`` must be below 1, and ``eps`` is added
+    to an update's norm.
     """
 
     def __init__(self, params: Iterable[Any], lr: float = 1e-3, weight_decay: float = 0.1,
                  momentum: float = 0.95, nesterov: bool = True,
                  ns_coefficients: tuple[float, float, float] = NEWTON_SCHULZ, eps: float = 1e-7,
-                 ns_steps: int = 5, adjust_lr_fn: str | None = None) -> None:
+                 ns_steps: int = 5, adjust_lr_fn: str | None = None,
+                 average: bool = False) -> None:
         if not lr >= 0.0:
             raise ValueError(f"lr must not be negative, got {lr}")
         if not 0.0 <= momentum < 1.0:
@@ -1043,7 +1053,21 @@ class Muon(torch.optim.Optimizer):
                              f"{adjust_lr_fn!r}")
         super().__init__(params, dict(lr=lr, weight_decay=weight_decay, momentum=momentum,
                                       nesterov=nesterov, ns_coefficients=ns_coefficients, eps=eps,
-                                      ns_steps=ns_steps, adjust_lr_fn=adjust_lr_fn))
+                                      ns_steps=ns_steps, adjust_lr_fn=adjust_lr_fn,
+                                      average=bool(average)))
+
+    def __setstate__(self, state: dict[str, Any]) -> None:
+        super().__setstate__(state)
+        for group in self.param_groups:
+            group.setdefault("average", False)
+
+    def load_state_dict(self, state_dict: dict[str, Any]) -> None:
+        for group in state_dict["param_groups"]:
+            if "average" not in group:
+                raise ValueError(
+                    "the state does not say what its momentum_buffer holds: set 'average' in each of its "
+                    "param_groups, to True for a state of torch.optim.Muon and to False for a sum of gradients")
+        super().load_state_dict(state_dict)
 
     def add_param_group(self, param_group: dict[str, Any]) -> None:
         super().add_param_group(param_group)
@@ -1077,10 +1101,16 @@ class Muon(torch.optim.Optimizer):
             if "momentum_buffer" not in self.state[p]:
                 self.state[p]["momentum_buffer"] = torch.zeros_like(p)
         buffers = [self.state[p]["momentum_buffer"] for p in params]
-        torch._foreach_mul_(buffers, group["momentum"])
-        torch._foreach_add_(buffers, grads)
-        updates = torch._foreach_add(grads, buffers, alpha=group["momentum"]) \
-            if group["nesterov"] else buffers
+        momentum, updates = group["momentum"], buffers
+        if group["average"]:
+            torch._foreach_lerp_(buffers, grads, 1.0 - momentum)
+            if group["nesterov"]:
+                updates = torch._foreach_lerp(grads, buffers, momentum)
+        else:
+            torch._foreach_mul_(buffers, momentum)
+            torch._foreach_add_(buffers, grads)
+            if group["nesterov"]:
+                updates = torch._foreach_add(grads, buffers, alpha=momentum)
         rows, columns, lr = *shape, float(group["lr"])
         if group["adjust_lr_fn"] == "match_rms_adamw":
             ratio = 0.2 * math.sqrt(max(rows, columns))
