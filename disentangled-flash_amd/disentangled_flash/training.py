@@ -379,6 +379,17 @@ def attention(
 
 
 NEWTON_SCHULZ = (3.4445, -4.775, 2.0315)  # the quintic's coefficients that are in common use
+_TILE = 128  # of orthogonalize's products
+
+
+def _check_iterations(batch: int, m: int, n: int, steps: int, eps: float) -> None:
+    if steps < 1:
+        raise ValueError(f"steps must be at least 1, got {steps}")
+    if not eps >= 0.0:
+        raise ValueError(f"eps must not be negative, got {eps}")
+    if batch > 65535 or max(m, n) > 1 << 20 or batch * -(-m // _TILE) * -(-n // _TILE) > 1 << 22:
+        raise ValueError(f"at most 65535 matrices of at most 2^20 rows and columns and 2^22 tiles of "
+                         f"{_TILE} x {_TILE} in all, got {batch} of {m} x {n}")
 
 
 def orthogonalize(
@@ -392,7 +403,8 @@ def orthogonalize(
     ``X = update / (|update|_F + eps)``, then ``steps`` times ``X <- a X + (b A + c A A) X`` with
     ``A = X X^T`` (transposed where ``m > n``), as the Muon optimiser takes it: with the usual
     coefficients and five steps, singular values above 1e-3 of the norm come to lie between 0.7 and 1.2.  All matrices
-    of a call go through the same launches.  The products take fp16 operands and fp32
+    of a call go through the same launches: at most 65535, of at most 2^20 rows and columns, 2^22 tiles of
+    128 x 128 in all.  The products take fp16 operands and fp32
     sums (2e-3 from the formula's result, which bf16 rounds by as much); the coefficients must
     keep singular values below 128.  Not differentiable: the result has no gradient.
     """
@@ -402,11 +414,8 @@ def orthogonalize(
     _check_floating("update", update)
     if update.dim() < 2 or update.shape[-1] < 1 or update.shape[-2] < 1:
         raise ValueError(f"update must be [..., m, n], got {tuple(update.shape)}")
-    if steps < 1:
-        raise ValueError(f"steps must be at least 1, got {steps}")
-    if not eps >= 0.0:
-        raise ValueError(f"eps must not be negative, got {eps}")
     shape = update.shape
+    _check_iterations(update.numel() // (shape[-2] * shape[-1]), shape[-2], shape[-1], steps, eps)
     rows = update.detach().reshape(-1, shape[-2], shape[-1]).contiguous()
     return _ops.orthogonalize(rows, steps, a, b, c, eps).view(shape)
 
@@ -1082,16 +1091,20 @@ class Muon(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        for group in self.param_groups:
-            alike: dict[Any, list[nn.Parameter]] = {}
+        alike: dict[Any, list[nn.Parameter]] = {}
+        for n, group in enumerate(self.param_groups):
             for p in group["params"]:
                 if p.grad is not None:
                     if p.grad.is_sparse:
                         raise RuntimeError("sparse gradients are not supported")
-                    _check_floating("parameters", p)  # (before any momentum changes)
-                    alike.setdefault((p.shape, p.dtype, p.device), []).append(p)
-            for (shape, dtype, _), params in alike.items():
-                self._update(group, shape, dtype, params)
+                    _check_floating("parameters", p)
+                    alike.setdefault((n, p.shape, p.dtype, p.device), []).append(p)
+        for (n, shape, *_), params in alike.items():
+            group = self.param_groups[n]
+            _check_iterations(len(params), *shape, int(group["ns_steps"]), float(group["eps"]))
+        # (What is refused is refused before any group's momentum or weights change.)
+        for (n, shape, dtype, _), params in alike.items():
+            self._update(self.param_groups[n], shape, dtype, params)
         return loss
 
     def _update(self, group: dict[str, Any], shape: torch.Size, dtype: torch.dtype,

@@ -470,7 +470,8 @@ DFLASH_API int dflash_attention_train_bwd(const dflash_attention_train* attentio
  * Newton-Schulz iterations (the update of the Muon optimiser; no counterpart in the reference):
  *   X = G / (|G|_F + eps);  steps times:  A = X X^T,  X <- a X + (b A + c A A) X
  * on the side on which X has no more rows than columns, for a batch of matrices.
- *   update    : G, [batch, m, n] contiguous, `dtype`; m and n at most 2^20
+ *   update    : G, [batch, m, n] contiguous, `dtype`; at most 65535 matrices, m and n at most 2^20,
+ *               and 2^22 tiles of 128 x 128 in all
  *   out       : bf16 [batch, m, n], 16-byte aligned
  *   workspace : dflash_orthogonalize_workspace_bytes(batch, m, n) bytes, 16-byte aligned (0:
  *               sizes the call refuses)

@@ -127,3 +127,80 @@ def test_averages_stay_in_the_range_of_their_gradients():
         assert bool(torch.isfinite(buffer).all()) == average
         if average:
             assert bool((buffer <= 6000).all()) and bool(torch.isfinite(p).all())
+
+
+def _two_groups(bad, **settings):
+    good = nn.Parameter(torch.ones(3, 4))
+    optimizer = training.Muon([{"params": [good]}, {"params": [bad], **settings}], lr=0.1)
+    good.grad, bad.grad = torch.ones_like(good), torch.ones_like(bad)
+    return optimizer, good
+
+
+def _unchanged(optimizer, good):
+    return not optimizer.state and torch.equal(good, torch.ones(3, 4))
+
+
+@pytest.mark.parametrize("settings", [{"ns_steps": 0}, {"eps": -1.0}, {"eps": float("nan")}], ids=str)
+def test_a_refused_step_changes_no_group(settings):
+    optimizer, good = _two_groups(nn.Parameter(torch.ones(2, 2)), **settings)
+    with pytest.raises(ValueError):
+        optimizer.step()
+    assert _unchanged(optimizer, good)
+    optimizer.param_groups[1].update(ns_steps=5, eps=1e-7)
+    optimizer.step()
+    assert len(optimizer.state) == 2 and not _unchanged(optimizer, good)
+
+
+def test_a_refused_parameter_changes_no_group(monkeypatch):
+    def check(name, tensor):
+        if tensor.shape == (2, 2):
+            raise RuntimeError("must be on a GPU")
+
+    monkeypatch.setattr(training, "_check_floating", check)
+    optimizer, good = _two_groups(nn.Parameter(torch.ones(2, 2)))
+    with pytest.raises(RuntimeError, match="GPU"):
+        optimizer.step()
+    assert _unchanged(optimizer, good)
+    optimizer, good = _two_groups(nn.Parameter(torch.ones(2, 3)))
+    optimizer.param_groups[1]["params"][0].grad = torch.ones(2, 3).to_sparse()
+    with pytest.raises(RuntimeError, match="sparse"):
+        optimizer.step()
+    assert _unchanged(optimizer, good)
+
+
+def test_sizes_that_are_refused(monkeypatch):
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    monkeypatch.undo()
+    with FakeTensorMode():
+        for shape in ((65536, 2, 3), (2, 2 ** 20 + 1, 2), (3, 2 ** 19, 2 ** 18)):
+            with pytest.raises(ValueError, match="at most"):
+                training.orthogonalize(torch.empty(shape, device="cuda"))
+        assert training.orthogonalize(torch.empty(65535, 2, 3, device="cuda")).shape[0] == 65535
+    with FakeTensorMode():
+        many = [nn.Parameter(torch.empty(2 ** 20 + 1, 1, device="cuda"))]
+        optimizer = training.Muon(many)
+        many[0].grad = torch.empty_like(many[0])
+        with pytest.raises(ValueError, match="at most"):
+            optimizer.step()
+        assert not optimizer.state
+
+
+def test_groups_of_a_shape_keep_their_settings():
+    """Parameters of one shape in two groups: each group's own rate and momentum."""
+
+    def steps(optimizer, params):
+        gen = torch.Generator().manual_seed(7)
+        for _ in range(3):
+            for p in params:
+                p.grad = torch.randn(p.shape, generator=gen)
+            optimizer.step()
+        return [p.detach() for p in params]
+
+    a = [nn.Parameter(torch.ones(3, 4)) for _ in range(2)]
+    both = steps(training.Muon([{"params": a[:1], "lr": 0.1}, {"params": a[1:], "lr": 0.2,
+                                                               "momentum": 0.5}]), a)
+    for n, settings in ((0, {"lr": 0.1}), (1, {"lr": 0.2, "momentum": 0.5})):
+        b = [nn.Parameter(torch.ones(3, 4)) for _ in range(2)]
+        alone = steps(training.Muon(b, **settings), b)
+        assert torch.equal(alone[n], both[n])
