@@ -125,9 +125,12 @@ __global__ __launch_bounds__(256) void start_kernel(const T* g, const double* pa
   if (threadIdx.x % 64 == 0) sums[threadIdx.x / 64] = square;
   __syncthreads();
   square = sums[0] + sums[1] + sums[2] + sums[3];
-  // (The scale is a power of two: it rounds nothing.)
-  const float factor =
-      static_cast<float>(1.0 / (sqrt(square) + static_cast<double>(eps))) * kScale;
+  // In two factors, the first a power of two: one alone would pass fp32's range for norms below 2^-120
+  // and be subnormal for those above 2^134.
+  const double factor = kScale / (sqrt(square) + static_cast<double>(eps));
+  const float shift = factor > 0x1p+100 ? 0x1p+64f : factor < 0x1p-100 ? 0x1p-64f : 1.0f;
+  const float rest = static_cast<float>(factor / static_cast<double>(shift));
+  auto scaled = [=](float x) { return x * shift * rest; };
   // G's rows and columns of this tile.
   const int gr = tall ? c0 : r0, gc = tall ? r0 : c0;
   const T* from = g + static_cast<int64_t>(b) * m * n;
@@ -156,13 +159,13 @@ __global__ __launch_bounds__(256) void start_kernel(const T* g, const double* pa
             float part[N];
             load_floats<T, N>(row + e, part);
 #pragma unroll
-            for (int x = 0; x < N; ++x) v[e + x] = part[x] * factor;
+            for (int x = 0; x < N; ++x) v[e + x] = scaled(part[x]);
           }
         }
       } else {
 #pragma unroll
         for (int e = 0; e < 8; ++e)
-          v[e] = gr + r < m && gc + c + e < n ? static_cast<float>(row[e]) * factor : 0.0f;
+          v[e] = gr + r < m && gc + c + e < n ? scaled(static_cast<float>(row[e])) : 0.0f;
       }
       put(r, c, v);
     }
@@ -172,7 +175,7 @@ __global__ __launch_bounds__(256) void start_kernel(const T* g, const double* pa
   for (int at = 0; at < 16; ++at) {
     const int r = at * 4 + threadIdx.x / 64, c = threadIdx.x % 64;
     tile[r][c] = gr + r < m && gc + c < n
-                     ? static_cast<float>(from[static_cast<int64_t>(gr + r) * n + gc + c]) * factor
+                     ? scaled(static_cast<float>(from[static_cast<int64_t>(gr + r) * n + gc + c]))
                      : 0.0f;
   }
   __syncthreads();
