@@ -12,6 +12,11 @@
 // 6e-3 off after five steps, with both 4e-4.  A is rounded to fp16 once, for b A as for A A: were
 // b A taken from its fp32 sums, the two would not cancel near 1 (normal 512 x 2048: 3.1e-3 off
 // against 1.7e-3).  bf16 operands are 1.3e-2 to 5e-2 off.  The result is bf16 (1.7e-3 by itself).
+// fp16 holds 2^8 X for singular values below 255, A then too, and B while |b s^2 + c s^4| is below 65504.
+// In the last step hi alone enters a X too, above 128 rows: the roundings of X in a X and in B X
+// then are one and the same, which p(s) nearly cancels where s is near 1.  By emulation of 768 x 768 a normal
+// matrix is 1.3e-3 off before the result's rounding instead of 1.4e-3 with both parts, one of rank 20 beside noise
+// 5.8e-4 instead of 2.4e-4 (2.1e-3, 2.2e-3, 1.76e-3 and 1.68e-3 with it); X's low part is not read again.
 //
 // One GEMM kernel, three forms.  All operands are zero-padded to whole 128 x 128 tiles in the
 // workspace, so that no access needs a bound.  A and B are symmetric: tiles below the diagonal
@@ -604,7 +609,7 @@ int launch(const T* g, __bf16* out, int64_t batch, int m, int n, int steps, floa
   for (int step = 0; step < steps; ++step) {
     p.from = step % 2;
     const bool last = step + 1 == steps;
-    // (The last step's X, whose small singular values grow no more, has hi alone, but in parts.)
+    // (The last step's X has hi alone, but in parts.)
     p.read_lo = step == 0 || !last || plan.parts;
     p.write_lo = step + 2 < steps || plan.parts;
     const int rc = plan.parts ? launch_step<true>(p, last, stream)

@@ -405,8 +405,9 @@ def orthogonalize(
     coefficients and five steps, singular values above 1e-3 of the norm come to lie between 0.7 and 1.2.  All matrices
     of a call go through the same launches: at most 65535, of at most 2^20 rows and columns, 2^22 tiles of
     128 x 128 in all.  The products take fp16 operands and fp32
-    sums (2e-3 from the formula's result, which bf16 rounds by as much); the coefficients must
-    keep singular values below 128.  Not differentiable: the result has no gradient.
+    sums (2e-3 from the formula's result, which bf16 rounds by as much); at every step each singular value
+    ``s`` of ``X`` must be below 255 and ``|b s^2 + c s^4|`` below 65504 (with the usual coefficients, which keep
+    ``s`` near 1, below 13.4), or the result is not finite.  Not differentiable: the result has no gradient.
     """
 
     steps, eps = int(steps), float(eps)

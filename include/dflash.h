@@ -475,8 +475,9 @@ DFLASH_API int dflash_attention_train_bwd(const dflash_attention_train* attentio
  *   out       : bf16 [batch, m, n], 16-byte aligned
  *   workspace : dflash_orthogonalize_workspace_bytes(batch, m, n) bytes, 16-byte aligned (0:
  *               sizes the call refuses)
- * Products of fp16 operands with fp32 sums; the coefficients must keep X's singular values
- * below 128.
+ * Products of fp16 operands with fp32 sums.  At every step each singular value s of X must be
+ * below 255 and |b s^2 + c s^4| below 65504 (with 3.4445, -4.775, 2.0315: s below 13.4), or the
+ * result is not finite.
  */
 DFLASH_API size_t dflash_orthogonalize_workspace_bytes(int64_t batch, int64_t m, int64_t n);
 DFLASH_API int dflash_orthogonalize(const void* update, void* out, int64_t batch, int64_t m,
