@@ -268,8 +268,14 @@ bool has_rows(const Tensor& t) {
   for (int64_t n = 0; n + 1 < t.dim(); ++n) every |= t.size(n) > 1 ? t.stride(n) : 0;
   return t.stride(-1) == 1 && every * t.element_size() % 16 == 0 && is_aligned(t);
 }
+// [B, L, H, D] or [H, S, D]: rows of one head within the kernels' 31-bit byte offsets.
+bool spans_little(const Tensor& t) {
+  return t.numel() == 0 ||
+         ((t.size(1) - 1) * t.stride(1) + t.size(-1)) * t.element_size() < int64_t{1} << 31;
+}
 Tensor with_rows(const Tensor& t) {
-  return has_rows(t) ? t : t.is_contiguous() ? t.clone() : t.contiguous();
+  if (!t.is_contiguous()) return has_rows(t) && spans_little(t) ? t : t.contiguous();
+  return has_rows(t) ? t : t.clone();
 }
 MaybeTensor with_rows(const MaybeTensor& t) { return t ? MaybeTensor(with_rows(*t)) : t; }
 

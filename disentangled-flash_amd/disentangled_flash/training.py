@@ -308,8 +308,8 @@ def attention(
 
     ``query``, ``key`` and ``value`` are ``[B, L, H, d]`` with ``d`` 32, 64 or 128 and at most
     16384 tokens, ``pos_key`` and ``pos_query`` ``[H, S, d]`` (``None``: no such term), all of one
-    dtype; views whose rows of ``d`` start on 16-byte boundaries (the projections' outputs
-    are) are read where they lie, others are copied.
+    dtype; views whose rows of ``d`` start on 16-byte boundaries and, of one head, lie within 2 GiB (the
+    projections' outputs do) are read where they lie, others are copied.
     ``mask`` is a bool or uint8 ``[B, L]``, nonzero for tokens that are kept.  A kept query has
     the softmax over the kept keys, whatever the padded places hold; a padded query has ``1 / L``
     for every key, as in Hugging Face's attention (where a padded key's value is not finite it

@@ -72,3 +72,28 @@ def test_a_model_saved_on_the_gpu_and_loaded_on_the_cpu():
     for name, g in grads.items():
         w = want_grads[name]
         assert float((g - w).abs().max()) <= 1e-4 * float(w.abs().max()) + 1e-6, name
+
+
+def test_rows_of_a_head_that_lie_more_than_2_gib_apart():
+    """Tokens outermost, in a tensor of more than 2 GiB: the rows are copied."""
+
+    from disentangled_flash.training import attention
+
+    length, width = 600, 2_000_000
+    store = torch.zeros(length, width, dtype=torch.float16, device="cuda")
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    q, k, v, dout = (torch.randn(1, length, 2, 32, device="cuda", generator=gen).half()
+                     for _ in range(4))
+    pk = torch.randn(2, 9, 32, device="cuda", generator=gen).half()
+    lut = torch.randint(0, 9, (2 * length - 1,), device="cuda", dtype=torch.int32, generator=gen)
+    views = []
+    for n, t in enumerate((q, k, v)):
+        store[:, 64 * n:64 * n + 64] = t[0].flatten(1)
+        views.append(store[:, 64 * n:64 * n + 64].view(1, length, 2, 32))
+    found = []
+    for tensors in ((q, k, v), views):
+        leaves = [t.detach().requires_grad_() for t in (*tensors, pk)]
+        out = attention(*leaves, None, lut, 0.1)
+        found.append([out.detach(), *torch.autograd.grad(out, leaves, dout)])
+    assert views[0].stride(1) * 2 * (length - 1) > 1 << 31
+    assert all(map(torch.equal, *found))
