@@ -8,7 +8,8 @@ import io
 import pytest
 import torch
 
-from test_gpu_attention_use import _batch, _grads, _model  # noqa: E402 (tests/ is on the path)
+from test_gpu_attention_train import _case, _rng  # noqa: E402 (tests/ is on the path)
+from test_gpu_attention_use import _batch, _grads, _model
 
 pytestmark = pytest.mark.gpu
 
@@ -96,4 +97,40 @@ def test_rows_of_a_head_that_lie_more_than_2_gib_apart():
         out = attention(*leaves, None, lut, 0.1)
         found.append([out.detach(), *torch.autograd.grad(out, leaves, dout)])
     assert views[0].stride(1) * 2 * (length - 1) > 1 << 31
+    assert all(map(torch.equal, *found))
+
+
+def test_backbone_compiled_ahead_of_time():
+    """Through torch.compile's joint graph of forward and backward, two lengths one after the other (the
+    second may be traced with symbolic sizes)."""
+
+    plain, model = (_model(dropout=0.1) for _ in range(2))
+    torch._dynamo.reset()
+    model.compile(backend="aot_eager")
+    ids, mask = _batch()
+    for length in (90, 50):
+        given = ids[:, :length], mask[:, :length]
+        want, want_grads = _grads(plain, *given)
+        got, grads = _grads(model, *given)
+        assert float((got - want).abs().max()) < 1e-5 * float(want.abs().max())
+        assert set(grads) == set(want_grads)
+        for name, g in grads.items():
+            w = want_grads[name]
+            assert float((g - w).abs().max()) <= 1e-4 * float(w.abs().max()) + 1e-6, name
+
+
+def test_operator_compiled_ahead_of_time():
+    from disentangled_flash.training import attention
+
+    args, dout = _case(1, 2, 100, 2, 64, torch.bfloat16)
+    rng = _rng()
+
+    def twice(*args):
+        return attention(*args, p=0.1, rng=rng, site=3) * 2
+
+    torch._dynamo.reset()
+    found = []
+    for call in (twice, torch.compile(twice, backend="aot_eager", fullgraph=True)):
+        y = call(*args)
+        found.append([y.detach(), *torch.autograd.grad(y, args[:5], dout)])
     assert all(map(torch.equal, *found))

@@ -40,3 +40,13 @@ def test_singular_values_near_the_most_that_fp16_holds(rows, value, coefficients
     update = torch.linalg.qr(torch.randn(rows + 60, rows, device="cuda", generator=gen))[0]
     assert abs(b * value ** 2 + c * value ** 4) < 65504 and value < 255
     _check(update, steps=2, coefficients=(a, b, c), eps=0.0)
+
+
+@pytest.mark.parametrize("shape", [(5, 64, 96), (3, 300, 200), (2, 513, 1025)], ids=str)
+def test_calls_are_repeatable(shape):
+    from disentangled_flash.training import orthogonalize
+
+    update = _normal(5, shape, torch.bfloat16, rank=9)
+    want = orthogonalize(update)
+    for _ in range(3):
+        assert torch.equal(orthogonalize(update), want)
