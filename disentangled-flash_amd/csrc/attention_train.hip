@@ -22,14 +22,16 @@
 //
 // Measured (us; heads of 64 in bf16, dropout 0.1, both terms, padded batches):
 //                  dropped places   forward   D    dV dK G   dQ   by delta   parts   by slot
-//   32 x 512 x 12 heads       35       202    14       264   77         97      12        16
-//   2 x 2000 x 12 heads       34       216     6       311   79        101      19        59
-// No unit bounds the forward and the dV dK G kernel: the matrix unit is busy 11 and 12 % of the time,
-// the vector unit 40 and 25 %, LDS 35 % in either; a wavefront waits at barriers and for loads 40 and 37 % of its
-// time and for its turn to issue 22 %.  It is the chain of products, LDS, skewed reads, exponentials
-// and products again, at three and two wavefronts a SIMD.  Nor does a part stand out: without the
+//   32 x 512 x 12 heads       34       247    14       264   77         96      11        16
+//   2 x 2000 x 12 heads       33       283     6       301   77         98      19        58
+// No unit bounds the forward and the dV dK G kernel: the matrix unit is busy 9 and 12 % of the time,
+// the vector unit 32 and 25 %, LDS 23 and 34 %; a wavefront waits at barriers and for loads 42 and 37 % of its
+// time and for its turn to issue 15 and 23 %.  It is the chain of products, LDS, skewed reads, exponentials
+// and products again, at two wavefronts a SIMD: latency, and no limit of the card (the inference kernel computes
+// the same scores, softmax and product, over all pairs, in 87).  Nor does a part stand out: without the
 // window products, the skewed reads, the skewed buffer and dK, the store of G, the loads of the windows
-// or dV, the latter kernel lost 14 to 28 % each.
+// or dV, the latter kernel lost 14 to 28 % each.  (Comments below give both sides of a choice as measured together,
+// some of them by earlier builds, whose times differ from these.)
 //
 // G is kept in fragments: 16 keys x 32 queries are 512 elements in the order in which the
 // lanes of a wavefront hold them, so that they are written and read 16 bytes a lane.
@@ -121,8 +123,8 @@ struct Op<float> {
 // Rows in LDS are padded by 16 bytes: the 16 rows that a fragment read touches lie in different banks.
 // Padded by 32, so do the rows 8g + 0..3 of a transposing read of 16-bit elements, which is worth it where no
 // workgroup less fits a CU for it: in the key kernel (321 -> 288 us at 32 x 512 full tokens, heads of 128
-// 228 -> 207) and in the forward pass (fp16: 272 -> 263, heads of 128 195 -> 183); the query kernel would
-// lose one (91 -> 109).
+// 228 -> 207) and in the forward pass (251 -> 247 at 32 x 512 padded tokens, heads of 128 45 -> 43 at 7 x 437); the
+// query kernel would lose one (91 -> 109 at 32 x 512 full tokens).
 template <typename T, int D>
 constexpr int kLd = D + 16 / static_cast<int>(sizeof(T));
 template <typename T, int D>
@@ -585,7 +587,7 @@ void attention_train_fwd_kernel(Params p) {
     // Rounded alone it puts an error into D_i = dO_i.O_i that all gradients of a query share, and
     // that weighs more where many deltas have one slot.  Over 2000 tokens in bf16 the gradients were off by
     // 2.7e-3 of their size, with both parts and with `low` by 2.5e-3, and outputs of fp16 by 2.7e-4 and
-    // 2.1e-4, their own rounding.  At 32 x 512 tokens it takes 198 us instead of 186.
+    // 2.1e-4, their own rounding.  At 32 x 512 padded tokens it takes 247 us instead of 235.
 #pragma unroll
     for (int ks = 0; ks < KB / 2; ++ks) {
       const F r = pack<T>(x[2 * ks], x[2 * ks + 1]);
@@ -1524,7 +1526,8 @@ __global__ __launch_bounds__(256) void attention_train_slot_kernel(
 
 // Of 16-bit rows of 32 or 64 elements workgroups of four wavefronts, two to four to a CU by their LDS
 // (34 to 67 KB); of eight, whose windows serve twice the rows, the kernels took 10 % longer there (key
-// kernel 321 -> 353 us, forward 220 -> 249 at 32 x 512 tokens).  Rows of 128 have room for one
+// kernel 321 -> 353 us, forward, by an earlier build with scores in fp16, 220 -> 249
+// at 32 x 512 full tokens).  Rows of 128 have room for one
 // workgroup, of eight.  In fp32 as many wavefronts as fit.  Tiles are of 32 tokens (64 in fp32, where one
 // workgroup fits a CU either way): with 64 the key kernel spilled registers.
 template <typename T, int D>

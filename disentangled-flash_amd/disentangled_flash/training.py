@@ -316,12 +316,15 @@ def attention(
     counts as 0; a kept key's makes the rows that see it NaN).  ``p``, ``rng`` and ``site`` as in
     :func:`dropout`, on the probabilities ``[B, H, L, L]``.
 
-    Scores, softmax and sums are fp32, but that the forward pass of bf16 inputs rounds the relative terms
-    to fp16.  Its output is that of unrounded probabilities, rounded once; the backward pass
+    Scores, softmax and sums are fp32, the same in both passes.  The output is that of unrounded
+    probabilities, rounded once; the backward pass
     rounds probabilities and the scores' gradients to the dtype where they are multiplied.
     Kept for it are the inputs, the output, in 16 bits also what its rounding left off, a
-    statistic for each row and with dropout one bit for each probability; it takes up to 2 GiB of
-    memory at a time for the scores' gradients.
+    statistic for each row and with dropout one bit for each probability.  It takes memory for the
+    scores' gradients, ``[B, H, L, L]`` of the dtype in parts of up to 2 GiB, and for the sums of the tables'
+    gradients by distance, up to ``16 d`` MiB in 16 bits and half of that in fp32.
+
+    ``B H`` is at most 2^20, ``H`` 65535 and ``H S`` below 2^22.
     """
 
     p, site, scale = float(p), int(site), float(scale)

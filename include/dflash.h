@@ -423,7 +423,8 @@ DFLASH_API int dflash_embedding_bwd(const void* ids, const void* dout, void* dta
  *   delta_to_slot      : int32 [2L - 1]; an entry outside [0, S) stands for a row of zeros
  *                        that takes no gradient
  *   mask               : uint8 [B, L], nonzero: kept; NULL: all kept
- * Tensors and strides are multiples of 16 bytes.  L is at most 16384, B H at most 2^20.
+ * Tensors and strides are multiples of 16 bytes, rows of one head lie within 2 GiB.  L is at most
+ * 16384, B H at most 2^20, H 65535, H S below 2^22.
  */
 typedef struct dflash_attention_train {
   const void *query, *key, *value;
