@@ -1118,7 +1118,7 @@ class Muon(torch.optim.Optimizer):
             if "momentum_buffer" not in self.state[p]:
                 self.state[p]["momentum_buffer"] = torch.zeros_like(p)
         buffers = [self.state[p]["momentum_buffer"] for p in params]
-        momentum, updates = group["momentum"], buffers
+        momentum, updates = float(group["momentum"]), buffers
         if group["average"]:
             torch._foreach_lerp_(buffers, grads, 1.0 - momentum)
             if group["nesterov"]:

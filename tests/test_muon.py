@@ -204,3 +204,14 @@ def test_groups_of_a_shape_keep_their_settings():
         b = [nn.Parameter(torch.ones(3, 4)) for _ in range(2)]
         alone = steps(training.Muon(b, **settings), b)
         assert torch.equal(alone[n], both[n])
+
+
+@pytest.mark.parametrize("average", [True, False])
+def test_a_momentum_that_is_a_tensor(average):
+    found = []
+    for momentum in (0.75, torch.tensor(0.75)):
+        params = _params()
+        optimizer = training.Muon(params, average=average)
+        _steps([optimizer], 3, seed=4, momenta=[momentum] * 3)
+        found.append([p.detach() for p in params] + _buffers(optimizer))
+    assert all(map(torch.equal, *found))
