@@ -108,3 +108,25 @@ def test_probabilities_of_the_backward_pass_add_up_to_1(dtype, d, scores):
     allowed = 2 * u + 2 * length * info.tiny * info.eps \
         + U * (8 * scores * 1.4427 + 2 * length + 16)
     assert float((rows - 1).abs().max()) <= allowed, ((rows - 1).abs().max().item(), allowed)
+
+
+@pytest.mark.parametrize("size", [1.0, 30.0])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32], ids=str)
+@pytest.mark.parametrize("d", [32, 64, 128])
+def test_statistics_are_those_of_fp32_scores(d, dtype, size):
+    """A row's log2 of the sum of its exponentials is off by the largest error of its scores, (d + 6) U sum|t|,
+    by (L + 32) U of a sum of L exponentials, and by the roundings of the result, its parts and its base, 4 U
+    of its size and of 1."""
+
+    from disentangled_flash import training
+
+    length = 90
+    args, _ = _inputs(2, length, 3, d, dtype, size, 2)
+    q, k, v, pk, pq, lut, scale = args
+    training._load()
+    lse = torch.ops.disentangled_flash.attention_train(q, k, v, pk, pq, lut, None, None, scale, 0.0,
+                                                       0)[2]
+    s, sums = _scores(q, k, pk, pq, lut, scale)
+    want = torch.logsumexp(s, -1) / math.log(2)
+    allowed = 1.4427 * ((d + 6) * U * sums.amax(-1) + (length + 32) * U) + 4 * U * (want.abs() + 1)
+    assert bool(((lse.double() - want).abs() <= allowed).all())
