@@ -134,3 +134,44 @@ def test_operator_compiled_ahead_of_time():
         y = call(*args)
         found.append([y.detach(), *torch.autograd.grad(y, args[:5], dout)])
     assert all(map(torch.equal, *found))
+
+
+def test_captured_step_of_a_backbone():
+    """Every replay drops other places and equals the eager step of another model with that counter.  (No
+    convolution; gradients of matrices only: torch's own sums record memsets, which replays do not
+    repeat reliably.)"""
+
+    ids, mask = _batch()
+    model, eager = (_model(torch.bfloat16, dropout=0.2, conv_kernel_size=0) for _ in range(2))
+    gen = torch.Generator(device="cuda").manual_seed(5)
+    direction = torch.randn(*ids.shape, 128, device="cuda", generator=gen).bfloat16() * mask[..., None]
+
+    def step(model):
+        matrices = [p for n, p in model.named_parameters() if "proj.weight" in n]
+        hidden = model(ids, attention_mask=mask).last_hidden_state
+        return [hidden.detach(), *torch.autograd.grad(hidden, matrices, direction)]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            step(model)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            outputs = step(model)
+    torch.cuda.current_stream().wait_stream(side)
+    model.dropout_state.counter[1] = 30
+    seen = []
+    for n in range(4):
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [t.clone() for t in outputs]
+        eager.dropout_state.counter[1] = 30 + n
+        want = step(eager)
+        torch.cuda.synchronize()
+        for a, b in zip(got, want):
+            # (torch's products may be other ones in a capture: sums of bf16 in another order.)
+            assert float((a.float() - b.float()).norm()) < 2e-2 * float(b.float().norm())
+        seen.append(got[0])
+    for n in range(4):
+        assert all(not torch.equal(seen[n], seen[m]) for m in range(n))
